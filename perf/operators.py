@@ -352,7 +352,7 @@ def _exact_append(case, s):
         for name, rows in (("k", x[b, :n, H:H + kv]), ("v", x[b, :n, H + kv:])):
             if case["fp8"]:
                 mant, e = torch.frexp(rows.abs().amax(-1) / 448.0)
-                e = torch.where(mant == 0.5, e - 1, e).clamp(min=-126)
+                e = torch.where(mant == 0.5, e - 1, torch.where(mant == 0, -126, e)).clamp(min=-126)
                 unit = torch.pow(torch.tensor(2.0, dtype=torch.float64, device="cuda"), e.double())
                 out[name + "s"][page, :, j % P] = unit
                 rows = (rows / unit[..., None]).float().to(torch.float8_e4m3fn).double()
