@@ -36,6 +36,25 @@ class CdkGemmEpilogue(C.Structure):
     ]
 
 
+class CdkPagedCache(C.Structure):
+    _fields_ = [
+        ("k", _vp),
+        ("v", _vp),
+        ("k_scale", _vp),
+        ("v_scale", _vp),
+        ("table", _vp),
+        ("ldt", _i64),
+        ("width", _i64),
+        ("num_pages", _i64),
+        ("ld_page", _i64),
+        ("ld_scale", _i64),
+        ("kv_heads", _i32),
+        ("page_size", _i32),
+        ("dtype", _i32),
+        ("reserved", _i32),
+    ]
+
+
 # name -> (restype, argtypes); mirrors include/cdk.h
 SIGNATURES = {
     "cdk_version": (_int, []),
@@ -103,6 +122,13 @@ SIGNATURES = {
     "cdk_swiglu_f32": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _vp]),
     "cdk_head_select": (_int, [_vp, _i64, _i64, _i64, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
     "cdk_mish_bf16": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _vp]),
+    "cdk_paged_append": (_int, [_vp, _i64, _int, _vp, _vp, _i64, _i64, _i64, _i64, C.POINTER(CdkPagedCache), _vp, _vp,
+                                _vp, _i64, _vp]),
+    "cdk_paged_gather": (_int, [C.POINTER(CdkPagedCache), _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp]),
+    "cdk_paged_attn_workspace": (_i64, [_i64, _i64, _i64]),
+    "cdk_paged_attn": (_int, [_vp, _i64, C.POINTER(CdkPagedCache), _i64, _i64, _vp, _vp, _i64, _f32, _vp, _i64, _vp]),
+    "cdk_token_logprobs": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "cdk_token_logprobs_bwd": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
 }
 
 _lib = None

@@ -638,3 +638,252 @@ def mish_bf16(z, a):
     rows, cols = z.shape
     _check(lib().cdk_mish_bf16(_p(z), z.stride(0), rows, cols, _p(a), a.stride(0), _stream()), "mish_bf16")
     _count(1)
+
+
+# ---------------------------------------------------------------------------
+# Paged KV cache (csrc/paged.cu)
+# ---------------------------------------------------------------------------
+def _refuse(op, why):
+    raise RuntimeError(f"cdk op {op}: {why}")
+
+
+def _call(op, fn, dev, *args):
+    """fn(*args, stream) on `dev`'s current stream, with `dev` the current
+    device for the launch (a caller's tensors may live on another one)."""
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, C.c_void_p(torch.cuda.current_stream(dev).cuda_stream))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, C.c_void_p(torch.cuda.current_stream(dev).cuda_stream))
+    if rc:
+        _check(rc, op)
+
+
+def _on(op, dev, *ts):
+    """Every tensor on CUDA device `dev`."""
+    for t in ts:
+        if t is not None and t.device != dev:
+            _refuse(op, f"tensors on {dev} and {t.device}")
+    if dev.type != "cuda":
+        raise RuntimeError("chessdecoder_b200 ops need CUDA tensors (no CPU implementation exists)")
+
+
+def _vec(op, name, t, dtype, n):
+    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+        _refuse(op, f"{name} must be a contiguous {dtype} [{n}]")
+
+
+def _rows16(op, name, t, dtypes, rows, cols):
+    """2-D rows with unit inner stride (the row pitch is free)."""
+    if t.dtype not in dtypes or t.dim() != 2 or t.shape[0] != rows or t.shape[1] < cols or t.stride(1) != 1:
+        _refuse(op, f"{name} must be {' or '.join(map(str, dtypes))} [{rows}, >= {cols}] with unit inner stride")
+
+
+def _pages(op, k, v, table, k_scale, v_scale, B):
+    """CdkPagedCache of one layer's pools (see include/cdk.h)."""
+    if k.dim() != 4 or k.shape[3] != 64 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride():
+        _refuse(op, "k_pages and v_pages must be alike, [num_pages, kv_heads, page_size, 64]")
+    n, h, p, _ = k.shape
+    if k.stride(3) != 1 or (p > 1 and k.stride(2) != 64) or (h > 1 and k.stride(1) != 64 * p):
+        _refuse(op, "the rows of a page must be contiguous")
+    c = _lib.CdkPagedCache()
+    if k.dtype == torch.float8_e4m3fn:
+        if k_scale is None or v_scale is None:
+            _refuse(op, "e4m3 pages need k_scale and v_scale")
+        for s in (k_scale, v_scale):
+            if s.dtype not in (torch.float8_e8m0fnu, torch.uint8) or s.shape != (n, h, p) \
+                    or s.stride() != k_scale.stride() or (p > 1 and s.stride(2) != 1) or (h > 1 and s.stride(1) != p):
+                _refuse(op, f"scales must be float8_e8m0fnu (or uint8) [{n}, {h}, {p}], contiguous in a page")
+        c.k_scale, c.v_scale, c.dtype = k_scale.data_ptr(), v_scale.data_ptr(), 1
+        c.ld_scale = k_scale.stride(0) if n > 1 else h * p
+    elif k.dtype == torch.bfloat16:
+        if k_scale is not None or v_scale is not None:
+            _refuse(op, "bf16 pages have no scales")
+    else:
+        _refuse(op, "pages must be bfloat16 or float8_e4m3fn")
+    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != B or (table.shape[1] > 1
+                                                                                 and table.stride(1) != 1):
+        _refuse(op, f"table must be int32 [{B}, pages per sequence] with unit inner stride")
+    c.k, c.v, c.table = k.data_ptr(), v.data_ptr(), table.data_ptr()
+    c.width = table.shape[1]
+    c.ldt = table.stride(0) if B > 1 else table.shape[1]
+    c.num_pages, c.kv_heads, c.page_size = n, h, p
+    c.ld_page = k.stride(0) if n > 1 else h * p * 64
+    return c
+
+
+@_timed("paged_append")
+def paged_append(qkv, B, S_new, H, k_pages, v_pages, table, start, *, num_new=None, k_scale=None, v_scale=None,
+                 pos=None, rope=None, q_out=None):
+    """S_new new tokens of each of B sequences into the paged cache: rows
+    t = b * S_new + s of qkv (fp32 or bf16, q | k | v heads of 64) go to cache
+    row start[b] + s.  rope (fp32 [n, 32, 2]) with pos (int32 [T]) rotates q and
+    k first; q_out (bf16) receives q.  Pages are bf16, or float8_e4m3fn with one
+    power-of-two scale a row in k_scale / v_scale.  num_new (int32 [B]): only the
+    first num_new[b] tokens of a sequence are real; nothing is written for the
+    others.  The rows of one call must be distinct."""
+    op = "paged_append"
+    c = _pages(op, k_pages, v_pages, table, k_scale, v_scale, B)
+    T, Hkv = B * S_new, k_pages.shape[1]
+    _rows16(op, "qkv", qkv, (torch.float32, torch.bfloat16), T, (H + 2 * Hkv) * 64)
+    _vec(op, "start", start, torch.int32, B)
+    if num_new is not None:
+        _vec(op, "num_new", num_new, torch.int32, B)
+    if (rope is None) != (pos is None):
+        _refuse(op, "pos and rope go together")
+    if rope is not None:
+        _vec(op, "pos", pos, torch.int32, T)
+        if rope.dtype != torch.float32 or rope.dim() != 3 or rope.shape[1:] != (32, 2) or not rope.is_contiguous():
+            _refuse(op, "rope must be contiguous fp32 [positions, 32, 2]")
+    if q_out is not None:
+        _rows16(op, "q_out", q_out, (torch.bfloat16,), T, H * 64)
+    _on(op, k_pages.device, v_pages, table, k_scale, v_scale, qkv, start, num_new, pos, rope, q_out)
+    if T == 0:
+        return
+    _call(op, lib().cdk_paged_append, k_pages.device, qkv.data_ptr(), qkv.stride(0) if T > 1 else qkv.shape[1],
+          int(qkv.dtype == torch.float32), _p(pos), _p(rope), 0 if rope is None else rope.shape[0], B, S_new, H,
+          C.byref(c), start.data_ptr(), _p(num_new), _p(q_out),
+          0 if q_out is None else (q_out.stride(0) if T > 1 else q_out.shape[1]))
+    _count(1)
+
+
+@_timed("paged_gather")
+def paged_gather(k_pages, v_pages, table, lens, k_out, v_out, *, k_scale=None, v_scale=None):
+    """Rows [0, lens[b]) of every sequence's paged keys and values as bf16 into
+    k_out / v_out [B, kv_heads, S, 64] (any strides but the last); the rows
+    behind a sequence's length are left as they were."""
+    op = "paged_gather"
+    B = table.shape[0] if table.dim() == 2 else -1
+    c = _pages(op, k_pages, v_pages, table, k_scale, v_scale, B)
+    _vec(op, "lens", lens, torch.int32, B)
+    for o in (k_out, v_out):
+        if o.dtype != torch.bfloat16 or o.dim() != 4 or o.shape != k_out.shape or o.stride() != k_out.stride() \
+                or o.shape[0] != B or o.shape[1] != k_pages.shape[1] or o.shape[3] != 64 or o.stride(3) != 1:
+            _refuse(op, f"k_out and v_out must be alike, bf16 [{B}, {k_pages.shape[1]}, rows, 64] with unit inner stride")
+    sb, sh, ss, _ = (s if n > 1 else 0 for s, n in zip(k_out.stride(), k_out.shape))
+    span = 64
+    for s, n in sorted((s, n) for s, n in zip((sb, sh, ss), k_out.shape) if n > 1):
+        if s < span:
+            _refuse(op, "the rows of k_out and v_out must not overlap")
+        span = s * n
+    _on(op, k_pages.device, v_pages, table, k_scale, v_scale, lens, k_out, v_out)
+    if k_out.numel() == 0:
+        return
+    _call(op, lib().cdk_paged_gather, k_pages.device, C.byref(c), B, lens.data_ptr(), k_out.data_ptr(),
+          v_out.data_ptr(), sb, sh, ss, k_out.shape[2])
+    _count(1)
+
+
+def paged_attn_workspace(B, H, kv_heads):
+    """Bytes of workspace that paged_attn needs."""
+    n = int(lib().cdk_paged_attn_workspace(B, H, kv_heads))
+    if n < 0:
+        _refuse("paged_attn", f"B={B}, H={H}, kv_heads={kv_heads}: at most 16384 sequences, H a multiple of kv_heads "
+                "with at most 16 query heads each")
+    return n
+
+
+@_timed("paged_attn")
+def paged_attn(q, k_pages, v_pages, table, lens, out, *, k_scale=None, v_scale=None, scale=0.125, workspace=None):
+    """Attention of one new token per sequence over its first lens[b] cached
+    rows: q, out bf16 [B, H * 64]; H may be a multiple of the cache's kv_heads
+    (grouped queries).  A sequence of length 0 gets zeros.  workspace (uint8,
+    paged_attn_workspace bytes): allocated here when not given; a given one must
+    not be shared by calls that can overlap."""
+    op = "paged_attn"
+    B = table.shape[0] if table.dim() == 2 else -1
+    c = _pages(op, k_pages, v_pages, table, k_scale, v_scale, B)
+    if out.dim() != 2 or out.shape[1] % 64 or out.shape[1] == 0:
+        _refuse(op, "out must be [B, H * 64]")
+    H = out.shape[1] // 64
+    _rows16(op, "out", out, (torch.bfloat16,), B, H * 64)
+    _rows16(op, "q", q, (torch.bfloat16,), B, H * 64)
+    if q.shape[1] != H * 64:
+        _refuse(op, "q and out must have the same heads")
+    _vec(op, "lens", lens, torch.int32, B)
+    need = paged_attn_workspace(B, H, k_pages.shape[1])
+    if workspace is not None and (workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need):
+        _refuse(op, f"workspace must be contiguous uint8 of at least {need} bytes")
+    _on(op, k_pages.device, v_pages, table, k_scale, v_scale, q, lens, out, workspace)
+    if B == 0:
+        return
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=k_pages.device)
+    _call(op, lib().cdk_paged_attn, k_pages.device, q.data_ptr(), q.stride(0) if B > 1 else H * 64, C.byref(c), B, H,
+          lens.data_ptr(), out.data_ptr(), out.stride(0) if B > 1 else H * 64, float(scale), workspace.data_ptr(),
+          workspace.numel())
+    _count(1)
+
+
+# ---------------------------------------------------------------------------
+# Token statistics (csrc/token_stats.cu)
+# ---------------------------------------------------------------------------
+MAX_TOP = 32
+
+
+def _logits(op, logits, target32, ncls):
+    if logits.dtype not in (torch.float32, torch.bfloat16) or logits.dim() != 2 or (logits.shape[1] > 1
+                                                                                    and logits.stride(1) != 1):
+        _refuse(op, "logits must be fp32 or bf16 [rows, classes] with unit inner stride")
+    rows, cols = logits.shape
+    ncls = cols if ncls is None else ncls
+    if not 0 < ncls <= cols:
+        _refuse(op, f"ncls {ncls} of {cols} columns")
+    if rows > 1 and logits.stride(0) < ncls:
+        _refuse(op, "the rows of logits overlap")
+    _vec(op, "target32", target32, torch.int32, rows)
+    return rows, ncls
+
+
+@_timed("token_logprobs")
+def token_logprobs(logits, target32, lp, *, entropy=None, lse=None, top_ids=None, top_lp=None, ncls=None):
+    """Per row: lp = log_softmax(logits)[target] (0 for a target outside
+    [0, ncls)), and where given the entropy, the log-sum-exp and the k best
+    classes (top_ids int32 [rows, k], top_lp fp32 [rows, k], k <= 32; equal
+    logits in order of their index).  fp32 outputs."""
+    op = "token_logprobs"
+    rows, ncls = _logits(op, logits, target32, ncls)
+    for name, t in (("lp", lp), ("entropy", entropy), ("lse", lse)):
+        if t is not None:
+            _vec(op, name, t, torch.float32, rows)
+    if (top_ids is None) != (top_lp is None):
+        _refuse(op, "top_ids and top_lp go together")
+    k = 0
+    if top_ids is not None:
+        k = top_ids.shape[1] if top_ids.dim() == 2 else -1
+        if not 0 <= k <= min(MAX_TOP, ncls) or top_ids.shape != (rows, k) or top_lp.shape != (rows, k) \
+                or top_ids.dtype != torch.int32 or top_lp.dtype != torch.float32 \
+                or not (top_ids.is_contiguous() and top_lp.is_contiguous()):
+            _refuse(op, f"top_ids / top_lp must be contiguous int32 / fp32 [{rows}, k], k <= min({MAX_TOP}, classes)")
+    _on(op, logits.device, target32, lp, entropy, lse, top_ids, top_lp)
+    if rows == 0:
+        return
+    _call(op, lib().cdk_token_logprobs, logits.device, logits.data_ptr(), int(logits.dtype == torch.bfloat16),
+          logits.stride(0) if rows > 1 else logits.shape[1], rows, ncls, target32.data_ptr(), lp.data_ptr(),
+          _p(entropy), _p(lse), _p(top_ids) if k else None, _p(top_lp) if k else None, k)
+    _count(1)
+
+
+@_timed("token_logprobs_bwd")
+def token_logprobs_bwd(logits, target32, lse, entropy, dlp, dentropy, dlogits, *, ncls=None):
+    """dlogits = dlp * (onehot(target) - p) - dentropy * p * (log p + entropy)
+    from the forward's lse and entropy; dlp / dentropy fp32 [rows], either may be
+    None (zero; entropy is then not needed for dentropy None).  dlogits has the
+    logits' type and may be the same tensor."""
+    op = "token_logprobs_bwd"
+    rows, ncls = _logits(op, logits, target32, ncls)
+    if dentropy is not None and entropy is None:
+        _refuse(op, "dentropy needs the forward's entropy")
+    for name, t in (("lse", lse), ("entropy", entropy), ("dlp", dlp), ("dentropy", dentropy)):
+        if t is not None:
+            _vec(op, name, t, torch.float32, rows)
+    _rows16(op, "dlogits", dlogits, (logits.dtype,), rows, ncls)
+    if rows > 1 and dlogits.stride(0) < ncls:
+        _refuse(op, "the rows of dlogits overlap")
+    _on(op, logits.device, target32, lse, entropy, dlp, dentropy, dlogits)
+    if rows == 0:
+        return
+    _call(op, lib().cdk_token_logprobs_bwd, logits.device, logits.data_ptr(), int(logits.dtype == torch.bfloat16),
+          logits.stride(0) if rows > 1 else logits.shape[1], rows, ncls, target32.data_ptr(), lse.data_ptr(),
+          _p(entropy), _p(dlp), _p(dentropy), dlogits.data_ptr(), dlogits.stride(0) if rows > 1 else dlogits.shape[1])
+    _count(1)

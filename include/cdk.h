@@ -407,6 +407,96 @@ int cdk_head_select(const float* logits, int64_t ldl, int64_t rows, int64_t ncol
  * step's hidden states (evalWlHead / evalDHead, batched_engine.cpp:151-180). */
 int cdk_mish_bf16(const float* z, int64_t ldz, int64_t rows, int64_t cols, void* a, int64_t lda, void* stream);
 
+/* ---- paged KV cache (no counterpart in the reference, whose decoder keeps one
+ *      dense cache of one length for the whole batch,
+ *      chessdecoder/cpp/decoder/batched_backbone.hpp:17-94) ------------------
+ * Key / value rows of 64 live in pages of page_size (a power of two) rows:
+ *   k, v      bf16 (dtype 0) or e4m3 (dtype 1)
+ *             [num_pages][kv_heads][page_size][64], ld_page elements from page
+ *             to page (a multiple of 8 for bf16, 16 for e4m3; 16-byte aligned
+ *             base)
+ *   k_scale, v_scale   dtype 1: one byte e per row, [num_pages][kv_heads]
+ *             [page_size], ld_scale bytes from page to page; the row stands for
+ *             code * 2^(e - 127).  dtype 0: unused.
+ *   table     int32 [B][width], row pitch ldt: row j of sequence b is row
+ *             j % page_size of page table[b][j / page_size].
+ * A table entry outside [0, num_pages) that a call has to follow, or a row at or
+ * past width * page_size, sets the index error bit and the row is skipped
+ * (append: not written; read-back: left as it was; attention: masked).  Pages
+ * may be shared for reading.  An append must be given distinct rows: two tokens
+ * that one call sends to the same row leave it undefined. */
+typedef struct CdkPagedCache {
+  void* k;
+  void* v;
+  uint8_t* k_scale;
+  uint8_t* v_scale;
+  const int32_t* table;
+  int64_t ldt;
+  int64_t width;
+  int64_t num_pages;
+  int64_t ld_page;
+  int64_t ld_scale;
+  int32_t kv_heads;
+  int32_t page_size;
+  int32_t dtype;
+  int32_t reserved;
+} CdkPagedCache;
+
+/* cdk_paged_append: rows t = b * S_new + s of qkv (fp32 or bf16; q | k | v with
+ * H, kv_heads and kv_heads heads of 64, pitch ldq elements, 16-byte aligned
+ * rows).  With rope ([rope_len][32][2] = (cos, sin)), q and k are rotated at
+ * positions pos[t].  q goes to q_out (bf16, pitch ldo; NULL: not wanted), k and
+ * v to row start[b] + s of sequence b, as bf16 or quantised: with a = max|x| of
+ * the 64 values, e = the least integer >= -126 with a <= 448 * 2^e, code =
+ * e4m3(x * 2^-e) (round to nearest even), scale byte e + 127.  Scaling by a
+ * power of two is exact, so the only rounding is the code's.  A row holding an
+ * infinity keeps it (as code 448 at the largest scale) and loses the others; a
+ * NaN stays a NaN.  num_new (int32 [B], NULL = S_new everywhere): tokens
+ * s >= num_new[b] are padding: neither q_out nor the cache is touched for them. */
+int cdk_paged_append(const void* qkv, int64_t ldq, int qkv_f32, const int32_t* pos, const float* rope,
+                     int64_t rope_len, int64_t B, int64_t S_new, int64_t H, const CdkPagedCache* cache,
+                     const int32_t* start, const int32_t* num_new, void* q_out, int64_t ldo, void* stream);
+/* cdk_paged_gather: rows [0, lens[b]) of every sequence as bf16 into k_out and
+ * v_out at element offset b * sb + h * sh + j * ss (+ 0..63; strides multiples
+ * of 8, 16-byte aligned bases).  Other rows are left as they were.  lens[b] > S
+ * (the rows that the outputs have) sets the index error bit and is cut to S. */
+int cdk_paged_gather(const CdkPagedCache* cache, int64_t B, const int32_t* lens, void* k_out, void* v_out, int64_t sb,
+                     int64_t sh, int64_t ss, int64_t S, void* stream);
+/* cdk_paged_attn: one new token per sequence, out[b, h] = sum_j p_j v_j with
+ * p = softmax(scale * q[b, h] . k_j) over rows j < lens[b] of kv head
+ * h / (H / kv_heads) (H a multiple of kv_heads, at most 16 query heads each).
+ * q, out bf16 [B, H * 64] with pitches ldq, ldo (multiples of 8, 16-byte aligned
+ * bases).  lens[b] == 0 gives zeros.  B <= 16384.  workspace:
+ * cdk_paged_attn_workspace bytes, 16-byte aligned, not shared by calls that can
+ * overlap; nothing in it needs clearing or is kept between calls. */
+int64_t cdk_paged_attn_workspace(int64_t B, int64_t H, int64_t kv_heads);
+int cdk_paged_attn(const void* q, int64_t ldq, const CdkPagedCache* cache, int64_t B, int64_t H, const int32_t* lens,
+                   void* out, int64_t ldo, float scale, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- token statistics (log_softmax + gather of chessdecoder/rl/log_probs.py:
+ *      58-101 with the entropy and the best alternatives in the same pass) ----
+ * Per row of logits (dtype 0 fp32, 1 bf16; pitch ldl): L = logsumexp(x),
+ *   lp = x[target] - L (0 for a target outside [0, ncls), as in padded rows)
+ *   entropy = L - sum_j p_j x_j, a class of probability 0 (logit -inf: a move
+ *             that is not legal) adding 0
+ *   top_ids / top_lp [rows][k] = the k best classes (k <= 32, k <= ncls), equal
+ *             logits in order of their index, and their log-probabilities.
+ * entropy, lse, top_ids with top_lp may be NULL.  A row whose logits are all
+ * -inf has lse -inf, entropy 0 and every log-probability -inf; a row with a NaN
+ * or +inf has lse, lp, entropy and top_lp NaN (NaN ranks above every number).
+ * ncls < 2^31 - 32.
+ *
+ * Backward: dlogits_j = g (1[j = target] - p_j) - h p_j (log p_j + entropy) with
+ * g = dlp[r] (taken as 0 for a target outside [0, ncls)), h = dentropy[r];
+ * either may be NULL (= 0).  Rows whose lse is -inf get zeros.  dlogits has the
+ * logits' type and may alias them; every element of [rows][ncls] is written. */
+int cdk_token_logprobs(const void* logits, int dtype, int64_t ldl, int64_t rows, int64_t ncls, const int32_t* target,
+                       float* lp, float* entropy, float* lse, int32_t* top_ids, float* top_lp, int64_t k,
+                       void* stream);
+int cdk_token_logprobs_bwd(const void* logits, int dtype, int64_t ldl, int64_t rows, int64_t ncls,
+                           const int32_t* target, const float* lse, const float* entropy, const float* dlp,
+                           const float* dentropy, void* dlogits, int64_t ldd, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
