@@ -14,6 +14,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "cdk.h"
 #include "cdk_common.cuh"
 
@@ -212,67 +214,560 @@ __global__ void __launch_bounds__(256)
 }
 
 // ---------------------------------------------------------------------------
-// One new token per sequence.  One block per (query head, sequence): each warp
-// takes every fourth key, lane l dims 2l and 2l + 1; a running maximum and sum
-// per warp, merged through shared memory.
+// One new token per sequence.
+//
+// o = sum_j p_j v_j / sum_j p_j with p_j = 2^(s_j - m), s = scale log2(e) q . k,
+// m the running maximum: one pass over the cached rows, which is what bounds it
+// (HBM; the products are a few percent of the tensor pipe even for one query).
+//
+// Work.  The keys of one (sequence, kv head) item are cut into tiles of 32; the
+// tiles of all items, in the order (sequence, head, tile), are dealt to the
+// grid's warps in equal contiguous runs, whatever the lengths.  A warp that
+// holds a whole item writes its output; the others leave partial results (m, l,
+// O) in the workspace, two per warp at most (the item it ends, the item it
+// begins), which paged_attn_join_kernel adds up in a fixed order.  Warps never
+// wait for one another.
+//
+// Tile.  Scores are taken transposed, S^T = K Q^T, with mma.sync m16n8k16: 16
+// keys by 8 queries, so a group of up to 8 query heads costs what one costs.
+// Operands come from HBM straight into registers: the sum over dims may run in
+// any order, so a lane takes 16 contiguous bytes of a key row as its share of
+// the k index (and of q alike).  O^T = V^T P^T takes 8 contiguous dims of a value
+// row per lane; pairs of keys are interleaved by byte permutes, and P^T is
+// turned from the accumulator's layout into the operand's by movmatrix.  No
+// shared memory, no barrier in the loop: the loads of the next tile's keys are
+// issued before this tile's softmax, those of its values after its products.
+//
+// bf16 pages: the weights are split into two bf16 (p = hi + lo, 2^-17 of p) so
+// that they add no error beside the output's rounding.  e4m3 pages: codes are
+// exact in fp16; q is scaled to fp16 by a power of two per head; the value scales
+// 2^e_j enter the exponent of the weights, w_j = 2^(s_j + e_j - m'), with their
+// own maximum m', so that a weight is at most 1 whatever the scales are; they are
+// rounded to fp16 (2^-11).
 // ---------------------------------------------------------------------------
-template <bool FP8>
-__global__ void __launch_bounds__(128)
-    paged_attn_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, Pages pg, int group,
-                      const int32_t* __restrict__ lens, __nv_bfloat16* __restrict__ out, long long ldo, float scale) {
-  const long long b = blockIdx.y;
-  const int h = blockIdx.x, kvh = h / group;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long len = max(lens[b], 0);
-  if (len > (pg.width << pg.log_page)) {
-    if (threadIdx.x == 0) report_error(kErrIndex);
-    len = pg.width << pg.log_page;
+constexpr int kTK = 32;             // keys per tile
+constexpr int kAttnThreads = 128;   // 4 warps; 128 registers: 4 blocks per SM
+constexpr int kAttnBlocks = 148 * 4;
+constexpr int kAttnWarps = kAttnBlocks * kAttnThreads / 32;
+constexpr int kSlots = 2 * kAttnWarps;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T>
+__device__ __forceinline__ T ld_once(const char* p);  // read once: no place in L1
+template <>
+__device__ __forceinline__ uint4 ld_once<uint4>(const char* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+template <>
+__device__ __forceinline__ uint2 ld_once<uint2>(const char* p) {
+  uint2 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t e4m3x2_h(uint32_t w) {  // low 16 bits: two codes -> two fp16 (exact)
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
+  return (uint32_t)h.x | ((uint32_t)h.y << 16);
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+struct AttnArgs {
+  const __nv_bfloat16* q;
+  long long ldq;
+  Pages pg;
+  int B, group;
+  const int32_t* lens;
+  __nv_bfloat16* out;
+  long long ldo;
+  float scale_log2;
+  int32_t* prefix;  // workspace: [B + 1] tiles before each sequence, per kv head
+  float4* stat;     // workspace: [kSlots][group] (m, l, m', -)
+  float* part;      // workspace: [kSlots][group][64]
+};
+
+__device__ __forceinline__ int tiles_of(const AttnArgs& a, int b, int* len_out, bool report) {
+  long long len = max(a.lens[b], 0);
+  const long long cap = a.pg.width << a.pg.log_page;
+  if (len > cap) {
+    if (report) report_error(kErrIndex);
+    len = cap;
   }
-  const float2 qf = bf2f(*reinterpret_cast<const uint32_t*>(q + b * ldq + h * kHD + 2 * lane));
-  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (long long j = warp; j < len; j += 4) {
-    const int page = page_of(pg, b, j);
-    if (page < 0) continue;
-    const long long r = ((long long)kvh << pg.log_page) + (j & ((1ll << pg.log_page) - 1));
-    const long long row = page * pg.ld_page + r * (kHD * (FP8 ? 1 : 2)), srow = page * pg.ld_scale + r;
-    float2 kf, vf;
-    if (FP8) {
-      kf = e4m3x2_f(*reinterpret_cast<const uint16_t*>(pg.k + row + 2 * lane));
-      vf = e4m3x2_f(*reinterpret_cast<const uint16_t*>(pg.v + row + 2 * lane));
-      const float a = scale_of(pg.ks[srow]), c = scale_of(pg.vs[srow]);
-      kf.x *= a; kf.y *= a;
-      vf.x *= c; vf.y *= c;
-    } else {
-      kf = bf2f(*reinterpret_cast<const uint32_t*>(pg.k + row + 4 * lane));
-      vf = bf2f(*reinterpret_cast<const uint32_t*>(pg.v + row + 4 * lane));
+  if (len_out) *len_out = (int)len;
+  return (int)((len + kTK - 1) / kTK);
+}
+
+// Writes `out` of one (sequence, head): 8 dims per lane.
+__device__ __forceinline__ void store_out8(const AttnArgs& a, int b, int h, int d, const float (&o)[8], float f) {
+  *reinterpret_cast<uint4*>(a.out + (long long)b * a.ldo + h * kHD + d) =
+      make_uint4(pack_bf16(o[0] * f, o[1] * f), pack_bf16(o[2] * f, o[3] * f), pack_bf16(o[4] * f, o[5] * f),
+                 pack_bf16(o[6] * f, o[7] * f));
+}
+
+template <bool FP8, int NT>
+__global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 3) paged_attn_kernel(const AttnArgs a) {
+  extern __shared__ int32_t prefix[];  // [B + 1]
+  __shared__ int warp_sum_[kAttnThreads / 32];
+  constexpr int kRow = FP8 ? kHD : 2 * kHD;  // bytes of a cached row
+  constexpr int kKC = FP8 ? 1 : 2;           // 16-byte chunks of a key row per lane
+  using VT = typename std::conditional<FP8, uint2, uint4>::type;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int g = lane >> 2, t4 = lane & 3;
+  const Pages& pg = a.pg;
+
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may be set up; it waits for this grid
+  {  // tiles before each sequence: thread i takes a contiguous run of sequences
+    const int per = (a.B + kAttnThreads - 1) / kAttnThreads;
+    const int b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
+    int sum = 0;
+    for (int b = b0; b < b1; ++b) sum += tiles_of(a, b, nullptr, blockIdx.x == 0);
+    int scan = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, scan, o);
+      if (lane >= o) scan += v;
     }
-    const float sc = warp_sum(qf.x * kf.x + qf.y * kf.y) * scale;
-    const float mn = fmaxf(m, sc);
-    const float al = m == -INFINITY ? 0.f : __expf(m - mn), p = __expf(sc - mn);
-    l = l * al + p;
-    o0 = o0 * al + p * vf.x;
-    o1 = o1 * al + p * vf.y;
-    m = mn;
+    if (lane == 31) warp_sum_[warp] = scan;
+    __syncthreads();
+    int at = scan - sum;
+    for (int w = 0; w < warp; ++w) at += warp_sum_[w];
+    for (int b = b0; b < b1; ++b) {
+      prefix[b] = at;
+      if (blockIdx.x == 0) a.prefix[b] = at;
+      at += tiles_of(a, b, nullptr, false);
+    }
+    if (tid == kAttnThreads - 1) {
+      prefix[a.B] = at;
+      if (blockIdx.x == 0) a.prefix[a.B] = at;
+    }
+    __syncthreads();
   }
-  __shared__ float sm[4][66];
-  sm[warp][2 * lane] = o0;
-  sm[warp][2 * lane + 1] = o1;
-  if (lane == 0) {
-    sm[warp][64] = m;
-    sm[warp][65] = l;
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x)  // sequences without keys
+    if (prefix[b] == prefix[b + 1])
+      for (int i = tid; i < pg.kv_heads * a.group * (kHD / 8); i += kAttnThreads)
+        *reinterpret_cast<uint4*>(a.out + (long long)b * a.ldo + i * 8) = make_uint4(0u, 0u, 0u, 0u);
+
+  const long long total = (long long)prefix[a.B] * pg.kv_heads;
+  const long long n_warps = (long long)gridDim.x * (kAttnThreads / 32);
+  const long long chunk = (total + n_warps - 1) / n_warps;
+  const long long w = (long long)blockIdx.x * (kAttnThreads / 32) + warp;
+  long long f = w * chunk;
+  const long long f_end = min(f + chunk, total);
+  if (f >= f_end) return;
+
+  int b;  // the sequence of flat tile f: last b with prefix[b] * kv_heads <= f
+  {
+    int lo = 0, hi = a.B;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if ((long long)prefix[mid] * pg.kv_heads <= f) lo = mid;
+      else hi = mid;
+    }
+    b = lo;
   }
+  while (f < f_end) {
+    while ((long long)prefix[b + 1] * pg.kv_heads <= f) ++b;
+    const int tiles = prefix[b + 1] - prefix[b];
+    const long long first = (long long)prefix[b] * pg.kv_heads;
+    const int kvh = (int)((f - first) / tiles);
+    const long long item = first + (long long)kvh * tiles;  // flat tile where the item begins
+    const int ta = (int)(f - item);
+    const int tb = (int)min((long long)tiles, f_end - item);
+    int len;
+    tiles_of(a, b, &len, false);
+    const int32_t* trow = pg.table + (long long)b * pg.ldt;
+
+    // page of this lane's key (tile * 32 + lane), -1 where there is none
+    auto page_at = [&](int tile) -> int {
+      const int key = tile * kTK + lane;
+      return tile < tb && key < len ? __ldg(trow + (key >> pg.log_page)) : -1;
+    };
+    auto mask_of = [&](int tile, int page) -> uint32_t {
+      const bool in = tile * kTK + lane < len;
+      const bool ok = in && page >= 0 && page < pg.num_pages;
+      if (in && !ok) report_error(kErrIndex);
+      return __ballot_sync(0xffffffffu, ok);
+    };
+    const long long head_row = (long long)kvh << pg.log_page;
+    const int pmask = (1 << pg.log_page) - 1;
+    uint4 kr[4][kKC];
+    VT vr[2][4];
+    uint32_t sc = 0;  // e4m3: this lane's key's scale bytes, key | value << 8
+
+    // rows of a tile: row x of the tile is in page shfl(page, x)
+    auto load_k = [&](int tile, int page, uint32_t mask) {
+      const int t0 = tile * kTK;
+      if (FP8) {
+        sc = 0;
+        if ((mask >> lane) & 1) {
+          const long long r = (long long)page * pg.ld_scale + head_row + ((t0 + lane) & pmask);
+          sc = (uint32_t)__ldg(pg.ks + r) | ((uint32_t)__ldg(pg.vs + r) << 8);
+        }
+      }
+      if (pg.log_page >= 5 && mask == 0xffffffffu) {
+        const long long p0 = __shfl_sync(0xffffffffu, page, 0);
+        const char* base = pg.k + p0 * pg.ld_page + (head_row + (t0 & pmask) + g) * kRow + t4 * 16;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int c = 0; c < kKC; ++c) kr[r][c] = ld_once<uint4>(base + r * 8 * kRow + c * 64);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int x = g + 8 * r;
+          const long long p = __shfl_sync(0xffffffffu, page, x);
+          const char* base = pg.k + p * pg.ld_page + (head_row + ((t0 + x) & pmask)) * kRow + t4 * 16;
+#pragma unroll
+          for (int c = 0; c < kKC; ++c)
+            kr[r][c] = (mask >> x) & 1 ? ld_once<uint4>(base + c * 64) : make_uint4(0u, 0u, 0u, 0u);
+        }
+      }
+    };
+    auto load_v = [&](int tile, int page, uint32_t mask) {
+      const int t0 = tile * kTK;
+      if (pg.log_page >= 5 && mask == 0xffffffffu) {
+        const long long p0 = __shfl_sync(0xffffffffu, page, 0);
+        const char* base = pg.v + p0 * pg.ld_page + (head_row + (t0 & pmask) + 2 * t4) * kRow + g * (kRow / 8);
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) vr[jj][i] = ld_once<VT>(base + (16 * jj + (i & 1) + (i >> 1) * 8) * kRow);
+      } else {
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int x = 16 * jj + 2 * t4 + (i & 1) + (i >> 1) * 8;
+            const long long p = __shfl_sync(0xffffffffu, page, x);
+            const char* base = pg.v + p * pg.ld_page + (head_row + ((t0 + x) & pmask)) * kRow + g * (kRow / 8);
+            vr[jj][i] = (mask >> x) & 1 ? ld_once<VT>(base) : VT{};
+          }
+      }
+    };
+
+    int page = page_at(ta);
+    int page_next = page_at(ta + 1);
+    uint32_t mask = mask_of(ta, page);
+    load_k(ta, page, mask);
+    load_v(ta, page, mask);
+
+    // queries of the group as the B operand: head n * 8 + g, 8 (bf16) or 16 (e4m3) dims per chunk and lane
+    uint32_t qf[NT][8];
+    float qs[NT][2];  // factor of the scores of heads n * 8 + 2 t4, + 1
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int hq = n * 8 + g;
+      const __nv_bfloat16* qrow = a.q + (long long)b * a.ldq + (kvh * a.group + hq) * kHD;
+      uint4 x = make_uint4(0u, 0u, 0u, 0u), y = x;
+      if (hq < a.group) {
+        x = *reinterpret_cast<const uint4*>(qrow + (FP8 ? 16 : 8) * t4);
+        y = *reinterpret_cast<const uint4*>(qrow + (FP8 ? 16 * t4 + 8 : 32 + 8 * t4));
+      }
+      const uint32_t raw[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+      if (!FP8) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) qf[n][i] = raw[i];
+        qs[n][0] = qs[n][1] = a.scale_log2;
+      } else {
+        uint32_t top = 0;  // the row's largest magnitude, as bf16 bits
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, max(raw[i] & 0x7fffu, (raw[i] >> 16) & 0x7fffu));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // largest in [2^14, 2^15): fp16 then holds all 8 bits of whatever is above 2^-38 of it
+        const int e = min(max((int)(top >> 7), 15), 250);  // exponent field; the factor 2^(141 - e) is a normal number
+        const float up = __uint_as_float((uint32_t)(127 + 141 - e) << 23);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float2 v = bf2f(raw[i]);
+          qf[n][i] = pack_f16(v.x * up, v.y * up);
+        }
+        // lanes (g, *) hold head g's factor; this lane's score columns are heads 2 t4, 2 t4 + 1
+        qs[n][0] = a.scale_log2 / __shfl_sync(0xffffffffu, up, 8 * t4);
+        qs[n][1] = a.scale_log2 / __shfl_sync(0xffffffffu, up, 8 * t4 + 4);
+      }
+    }
+
+    float o[NT][4][4];
+    float m[NT][2], l[NT][2], mv[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+      m[n][0] = m[n][1] = mv[n][0] = mv[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
+    }
+
+    for (int tile = ta; tile < tb; ++tile) {
+      // S^T: keys g + 8 r by heads 2 t4 + c -> s[n][r][c]
+      float s[NT][4][2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float acc[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+        if (FP8) {
+          const uint4 u = kr[2 * i][0], w4 = kr[2 * i + 1][0];
+          const uint32_t lo[4] = {u.x, u.y, u.z, u.w}, hi[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t af[4] = {e4m3x2_h(lo[j]), e4m3x2_h(hi[j]), e4m3x2_h(lo[j] >> 16), e4m3x2_h(hi[j] >> 16)};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_f16_16816(acc[n], af, qf[n][2 * j], qf[n][2 * j + 1]);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < kKC; ++c) {
+            const uint4 u = kr[2 * i][c], w4 = kr[2 * i + 1][c];
+            const uint32_t a0[4] = {u.x, w4.x, u.y, w4.y}, a1[4] = {u.z, w4.z, u.w, w4.w};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              mma_bf16_16816(acc[n], a0, qf[n][4 * c], qf[n][4 * c + 1]);
+              mma_bf16_16816(acc[n], a1, qf[n][4 * c + 2], qf[n][4 * c + 3]);
+            }
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            s[n][2 * i][c] = acc[n][c] * qs[n][c];
+            s[n][2 * i + 1][c] = acc[n][2 + c] * qs[n][c];
+          }
+      }
+      float ve[4];  // log2 of the value scales
+      if (FP8) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const uint32_t x = __shfl_sync(0xffffffffu, sc, g + 8 * r);
+          const float ks = __uint_as_float((x & 0xffu) << 23);
+          ve[r] = (float)(int)((x >> 8) & 0xffu) - 127.f;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            s[n][r][0] *= ks;
+            s[n][r][1] *= ks;
+          }
+        }
+      }
+      if (mask != 0xffffffffu) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (!((mask >> (g + 8 * r)) & 1)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) s[n][r][0] = s[n][r][1] = -INFINITY;
+          }
+      }
+      uint32_t mask_next = 0;
+      if (tile + 1 < tb) {
+        mask_next = mask_of(tile + 1, page_next);
+        load_k(tile + 1, page_next, mask_next);
+      }
+
+      // running maximum over the tile's 32 keys, weights, sums
+      uint32_t pb[NT][2][2];  // weights of keys (16 jj + g, + 8) for heads 2 t4, 2 t4 + 1
+      uint32_t pl[NT][2][2];  // bf16: the low parts
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float mn[2], al[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float mx = fmaxf(fmaxf(s[n][0][c], s[n][1][c]), fmaxf(s[n][2][c], s[n][3][c]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          mx = fmaxf(mx, m[n][c]);
+          mn[c] = mx == -INFINITY ? 0.f : mx;  // no key yet: weights 2^(-inf) = 0
+          al[c] = ex2(m[n][c] - mn[c]);
+          m[n][c] = mx;
+        }
+        float p[4][2];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) p[r][c] = ex2(s[n][r][c] - mn[c]);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) l[n][c] = l[n][c] * al[c] + ((p[0][c] + p[1][c]) + (p[2][c] + p[3][c]));
+        if (FP8) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float mx = fmaxf(fmaxf(s[n][0][c] + ve[0], s[n][1][c] + ve[1]),
+                             fmaxf(s[n][2][c] + ve[2], s[n][3][c] + ve[3]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            mx = fmaxf(mx, mv[n][c]);
+            mn[c] = mx == -INFINITY ? 0.f : mx;
+            al[c] = ex2(mv[n][c] - mn[c]);
+            mv[n][c] = mx;
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) p[r][c] = ex2(s[n][r][c] + ve[r] - mn[c]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          o[n][i][0] *= al[0];
+          o[n][i][1] *= al[1];
+          o[n][i][2] *= al[0];
+          o[n][i][3] *= al[1];
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (FP8) {
+            pb[n][r >> 1][r & 1] = transpose8x8(pack_f16(p[r][0], p[r][1]));
+          } else {
+            const uint32_t hi = pack_bf16(p[r][0], p[r][1]);
+            const float2 back = bf2f(hi);
+            pb[n][r >> 1][r & 1] = transpose8x8(hi);
+            pl[n][r >> 1][r & 1] = transpose8x8(pack_bf16(p[r][0] - back.x, p[r][1] - back.y));
+          }
+        }
+      }
+
+      // O^T += V^T P^T: row pair i of the accumulators is dims 8 g + 2 i, 8 g + 2 i + 1
+#pragma unroll
+      for (int jj = 0; jj < 2; ++jj) {
+        uint32_t w4[4][4];  // [key][dim pair]
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          if constexpr (FP8) {
+            const uint2 u = vr[jj][x];
+            w4[x][0] = e4m3x2_h(u.x);
+            w4[x][1] = e4m3x2_h(u.x >> 16);
+            w4[x][2] = e4m3x2_h(u.y);
+            w4[x][3] = e4m3x2_h(u.y >> 16);
+          } else {
+            const uint4 u = vr[jj][x];
+            w4[x][0] = u.x;
+            w4[x][1] = u.y;
+            w4[x][2] = u.z;
+            w4[x][3] = u.w;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t af[4] = {__byte_perm(w4[0][i], w4[1][i], 0x5410), __byte_perm(w4[0][i], w4[1][i], 0x7632),
+                                  __byte_perm(w4[2][i], w4[3][i], 0x5410), __byte_perm(w4[2][i], w4[3][i], 0x7632)};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            if (FP8) {
+              mma_f16_16816(o[n][i], af, pb[n][jj][0], pb[n][jj][1]);
+            } else {
+              mma_bf16_16816(o[n][i], af, pb[n][jj][0], pb[n][jj][1]);
+              mma_bf16_16816(o[n][i], af, pl[n][jj][0], pl[n][jj][1]);
+            }
+          }
+        }
+      }
+      if (tile + 1 < tb) {
+        load_v(tile + 1, page_next, mask_next);
+        mask = mask_next;
+        page_next = page_at(tile + 2);
+      }
+    }
+
+    // this warp's share of the item
+    const bool whole = ta == 0 && tb == tiles;
+    const int slot = 2 * (int)w + (ta == 0 ? 1 : 0);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float sum = l[n][c];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        const int hq = n * 8 + 2 * t4 + c;
+        if (hq >= a.group) continue;
+        const float ov[8] = {o[n][0][c], o[n][0][2 + c], o[n][1][c], o[n][1][2 + c],
+                             o[n][2][c], o[n][2][2 + c], o[n][3][c], o[n][3][2 + c]};
+        if (whole) {
+          float inv = sum == 0.f ? 0.f : 1.f / sum;
+          if (FP8) inv *= m[n][c] == -INFINITY ? 1.f : ex2(mv[n][c] - m[n][c]);
+          store_out8(a, b, kvh * a.group + hq, 8 * g, ov, inv);
+        } else {
+          const long long at = (long long)slot * a.group + hq;
+          float4* dst = reinterpret_cast<float4*>(a.part + at * kHD + 8 * g);
+          dst[0] = make_float4(ov[0], ov[1], ov[2], ov[3]);
+          dst[1] = make_float4(ov[4], ov[5], ov[6], ov[7]);
+          if (g == 0) a.stat[at] = make_float4(m[n][c], sum, FP8 ? mv[n][c] : m[n][c], 0.f);
+        }
+      }
+    f = item + tb;
+  }
+}
+
+// Adds up the partial results of the items that several warps shared, in the
+// order of those warps.  One block per (sequence, query head); warp i takes
+// every fourth partial result, lane l dims 2l and 2l + 1.
+__global__ void __launch_bounds__(128) paged_attn_join_kernel(const AttnArgs a, long long n_warps) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int heads = a.pg.kv_heads * a.group;
+  const int b = blockIdx.x / heads, h = blockIdx.x - b * heads;
+  const int kvh = h / a.group, hq = h - kvh * a.group;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int before = a.prefix[b], tiles = a.prefix[b + 1] - before;
+  if (tiles == 0) return;
+  const long long total = (long long)a.prefix[a.B] * a.pg.kv_heads;
+  const long long chunk = (total + n_warps - 1) / n_warps;
+  const long long first = (long long)before * a.pg.kv_heads + (long long)kvh * tiles;
+  const long long w0 = first / chunk, w1 = (first + tiles - 1) / chunk;
+  if (w0 == w1) return;  // written by that warp
+  float m = -INFINITY, mv = -INFINITY, l = 0.f, x = 0.f, y = 0.f;
+  auto add = [&](float pm, float plen, float pmv, float px, float py) {
+    const float nm = fmaxf(m, pm), nv = fmaxf(mv, pmv);
+    const float sm = nm == -INFINITY ? 0.f : nm, sv = nv == -INFINITY ? 0.f : nv;
+    l = l * ex2(m - sm) + plen * ex2(pm - sm);
+    const float f0 = ex2(mv - sv), f1 = ex2(pmv - sv);
+    x = x * f0 + px * f1;
+    y = y * f0 + py * f1;
+    m = nm;
+    mv = nv;
+  };
+  for (long long w = w0 + warp; w <= w1; w += 4) {
+    const long long at = (2 * w + (w == w0 ? 1 : 0)) * a.group + hq;
+    const float4 st = a.stat[at];
+    const float2 v = *reinterpret_cast<const float2*>(a.part + at * kHD + 2 * lane);
+    add(st.x, st.y, st.z, v.x, v.y);
+  }
+  __shared__ float4 st_s[4];
+  __shared__ float2 v_s[4][32];
+  if (lane == 0) st_s[warp] = make_float4(m, l, mv, 0.f);
+  v_s[warp][lane] = make_float2(x, y);
   __syncthreads();
   if (warp) return;
-  const float M = fmaxf(fmaxf(sm[0][64], sm[1][64]), fmaxf(sm[2][64], sm[3][64]));
-  float L = 0.f, x = 0.f, y = 0.f;
-  for (int w = 0; w < 4; ++w) {
-    const float f = sm[w][64] == -INFINITY ? 0.f : __expf(sm[w][64] - M);
-    L += sm[w][65] * f;
-    x += sm[w][2 * lane] * f;
-    y += sm[w][2 * lane + 1] * f;
+  for (int i = 1; i < 4; ++i) {
+    const float4 st = st_s[i];
+    add(st.x, st.y, st.z, v_s[i][lane].x, v_s[i][lane].y);
   }
-  const float inv = len > 0 && M != -INFINITY ? 1.f / L : 0.f;
-  *reinterpret_cast<uint32_t*>(out + b * ldo + h * kHD + 2 * lane) = pack_bf16(x * inv, y * inv);
+  const float inv = l == 0.f ? 0.f : (m == -INFINITY ? 1.f : ex2(mv - m)) / l;
+  *reinterpret_cast<uint32_t*>(a.out + (long long)b * a.ldo + h * kHD + 2 * lane) = pack_bf16(x * inv, y * inv);
 }
 
 // ---------------------------------------------------------------------------
@@ -364,29 +859,78 @@ extern "C" int cdk_paged_gather(const CdkPagedCache* cache, int64_t B, const int
   return launched();
 }
 
+namespace {
+inline int64_t prefix_bytes(int64_t B) { return ((B + 1) * 4 + 15) / 16 * 16; }
+
+template <bool FP8, int NT>
+cudaError_t launch_attn(const AttnArgs& a, unsigned grid, int smem, cudaStream_t st) {
+  static bool done[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!done[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(paged_attn_kernel<FP8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)prefix_bytes(kMaxSeqs));
+    if (e != cudaSuccess) return e;
+    done[dev] = true;
+  }
+  paged_attn_kernel<FP8, NT><<<grid, kAttnThreads, smem, st>>>(a);
+  return cudaGetLastError();
+}
+}  // namespace
+
 extern "C" int64_t cdk_paged_attn_workspace(int64_t B, int64_t H, int64_t kv_heads) {
-  if (B < 0 || B > kMaxSeqs || H <= 0 || kv_heads <= 0 || H % kv_heads || H / kv_heads > kMaxGroup) return -1;
-  return 16;
+  if (B < 0 || B > kMaxSeqs || H <= 0 || H > 65536 || kv_heads <= 0 || H % kv_heads || H / kv_heads > kMaxGroup)
+    return -1;
+  return prefix_bytes(B) + (int64_t)kSlots * (H / kv_heads) * (16 + kHD * 4);
 }
 
 extern "C" int cdk_paged_attn(const void* q, int64_t ldq, const CdkPagedCache* cache, int64_t B, int64_t H,
                               const int32_t* lens, void* out, int64_t ldo, float scale, void* workspace,
                               int64_t workspace_bytes, void* stream) {
   if (B == 0) return 0;
-  Pages pg;
-  if (const int rc = take_pages(cache, &pg)) return rc;
+  AttnArgs a;
+  if (const int rc = take_pages(cache, &a.pg)) return rc;
   if (!q || !lens || !out || B < 0 || H <= 0) return -10;
-  const int64_t need = cdk_paged_attn_workspace(B, H, pg.kv_heads);
+  const int64_t need = cdk_paged_attn_workspace(B, H, a.pg.kv_heads);
   if (need < 0) return -11;
   if (!workspace || workspace_bytes < need || !al16(workspace)) return -12;
   if (ldq < H * kHD || ldq % 8 || ldo < H * kHD || ldo % 8 || !al16(q) || !al16(out)) return -13;
   if (!(scale == scale)) return -14;
-  const dim3 grid((unsigned)H, (unsigned)B);
-  auto* st = reinterpret_cast<cudaStream_t>(stream);
-  auto* qq = reinterpret_cast<const __nv_bfloat16*>(q);
-  auto* oo = reinterpret_cast<__nv_bfloat16*>(out);
-  const int group = (int)(H / pg.kv_heads);
-  if (cache->dtype == 1) paged_attn_kernel<true><<<grid, 128, 0, st>>>(qq, ldq, pg, group, lens, oo, ldo, scale);
-  else paged_attn_kernel<false><<<grid, 128, 0, st>>>(qq, ldq, pg, group, lens, oo, ldo, scale);
-  return launched();
+  const int64_t tiles = ((a.pg.width << a.pg.log_page) + kTK - 1) / kTK;  // per item, at most
+  if (tiles >= (1ll << 31) / kTK || tiles > ((1ll << 31) - 1) / B) return -15;
+  a.q = reinterpret_cast<const __nv_bfloat16*>(q);
+  a.ldq = ldq;
+  a.B = (int)B;
+  a.group = (int)(H / a.pg.kv_heads);
+  a.lens = lens;
+  a.out = reinterpret_cast<__nv_bfloat16*>(out);
+  a.ldo = ldo;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  char* ws = static_cast<char*>(workspace);
+  a.prefix = reinterpret_cast<int32_t*>(ws);
+  a.stat = reinterpret_cast<float4*>(ws + prefix_bytes(B));
+  a.part = reinterpret_cast<float*>(ws + prefix_bytes(B) + (int64_t)kSlots * a.group * 16);
+  auto st = reinterpret_cast<cudaStream_t>(stream);
+  // no more warps than tiles that the tables can hold; one tile per warp is then the smallest share
+  const int64_t bound = tiles * B * a.pg.kv_heads, wpb = kAttnThreads / 32;
+  const unsigned grid = (unsigned)(bound >= kAttnWarps ? kAttnBlocks : (bound + wpb - 1) / wpb + (bound == 0));
+  const int smem = (int)prefix_bytes(B);
+  cudaError_t e;
+  if (cache->dtype == 1) e = a.group <= 8 ? launch_attn<true, 1>(a, grid, smem, st) : launch_attn<true, 2>(a, grid, smem, st);
+  else e = a.group <= 8 ? launch_attn<false, 1>(a, grid, smem, st) : launch_attn<false, 2>(a, grid, smem, st);
+  if (e != cudaSuccess) return (int)e;
+  if (tiles <= 1) return 0;  // an item of one tile is never shared
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(B * H));
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];  // set up while the first kernel drains; it waits for it before its first load
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const long long n_warps = (long long)grid * wpb;
+  e = cudaLaunchKernelEx(&cfg, paged_attn_join_kernel, (const AttnArgs)a, n_warps);
+  return e == cudaSuccess ? 0 : (int)e;
 }
