@@ -159,6 +159,23 @@ def test_order_of_equal_values(V):
 
 
 @pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("V,threads", [(1924, 32), (131071, 256), (70003, 256)])
+def test_best_logits_crowded_into_few_columns(V, threads, bf16):
+    """The best classes all lie in a few strided groups of columns (16-byte pieces, every
+    32nd or 256th of them), hundreds to thousands of them: more than a selection by
+    per-thread maxima keeps."""
+    n = 8 if bf16 else 4
+    x = torch.rand(3, V, generator=torch.Generator().manual_seed(V))
+    crowd = (torch.arange(V) // n) % threads < 20
+    x[:, crowd] += 5
+    x[2, crowd] = 7.0
+    x = (x.to(torch.bfloat16) if bf16 else x).to(DEV)
+    t = torch.zeros(3, dtype=torch.int32, device=DEV)
+    for k in (5, 21, 32):
+        run(x, t, k)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("V", [33, 1924, 40001])
 def test_masked_rows(V, bf16):
     """Almost everything -inf, the type's lowest value, one legal class, none, infinities and NaN."""
