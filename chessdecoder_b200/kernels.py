@@ -8,6 +8,7 @@ PyTorch kernels.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -642,74 +643,122 @@ def mish_bf16(z, a):
 
 # ---------------------------------------------------------------------------
 # Paged KV cache (csrc/paged.cu)
+#
+# A decode step calls these for microseconds of GPU work, so the argument checks
+# are functions of the tensors' layouts (dtype, shape, strides) alone and their
+# results are memoised: a call costs one lookup and the pointers.
 # ---------------------------------------------------------------------------
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+
+
 def _refuse(op, why):
     raise RuntimeError(f"cdk op {op}: {why}")
 
 
+def _lay(t):
+    return None if t is None else (t.dtype, t.shape, t.stride())
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
 def _call(op, fn, dev, *args):
-    """fn(*args, stream) on `dev`'s current stream, with `dev` the current
-    device for the launch (a caller's tensors may live on another one)."""
-    if dev.index == torch.cuda.current_device():
-        rc = fn(*args, C.c_void_p(torch.cuda.current_stream(dev).cuda_stream))
+    """fn(*args, stream) on the current stream of CUDA device `dev`, with that
+    device the current one for the launch (a caller's tensors may live on
+    another one)."""
+    if dev == _current_device():
+        rc = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, C.c_void_p(torch.cuda.current_stream(dev).cuda_stream))
+            rc = fn(*args, _raw_stream(dev))
     if rc:
         _check(rc, op)
 
 
-def _on(op, dev, *ts):
-    """Every tensor on CUDA device `dev`."""
+def _on(op, *ts):
+    """The CUDA device that every tensor given is on."""
+    dev = ts[0].get_device()
     for t in ts:
-        if t is not None and t.device != dev:
-            _refuse(op, f"tensors on {dev} and {t.device}")
-    if dev.type != "cuda":
+        if t is not None and t.get_device() != dev:
+            _refuse(op, f"tensors on {ts[0].device} and {t.device}")
+    if dev < 0:
         raise RuntimeError("chessdecoder_b200 ops need CUDA tensors (no CPU implementation exists)")
+    return dev
 
 
-def _vec(op, name, t, dtype, n):
-    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+def _vec(op, name, lay, dtype, n):
+    if lay is not None and (lay[0] != dtype or lay[1] != (n,) or (n > 1 and lay[2][0] != 1)):
         _refuse(op, f"{name} must be a contiguous {dtype} [{n}]")
 
 
-def _rows16(op, name, t, dtypes, rows, cols):
-    """2-D rows with unit inner stride (the row pitch is free)."""
-    if t.dtype not in dtypes or t.dim() != 2 or t.shape[0] != rows or t.shape[1] < cols or t.stride(1) != 1:
+def _rows2d(op, name, lay, dtypes, rows, cols):
+    """2-D rows with unit inner stride that do not overlap; returns the pitch."""
+    dtype, shape, stride = lay
+    if dtype not in dtypes or len(shape) != 2 or shape[0] != rows or shape[1] < cols or stride[1] != 1:
         _refuse(op, f"{name} must be {' or '.join(map(str, dtypes))} [{rows}, >= {cols}] with unit inner stride")
+    if rows > 1 and stride[0] < cols:
+        _refuse(op, f"the rows of {name} overlap")
+    return stride[0] if rows > 1 else shape[1]
 
 
-def _pages(op, k, v, table, k_scale, v_scale, B):
-    """CdkPagedCache of one layer's pools (see include/cdk.h)."""
-    if k.dim() != 4 or k.shape[3] != 64 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride():
+def _pages_plan(op, k, v, table, k_scale, v_scale, B):
+    """(page_size, kv_heads, and the layout fields of CdkPagedCache) of one
+    layer's pools."""
+    dtype, shape, stride = k
+    if len(shape) != 4 or shape[3] != 64 or v != k:
         _refuse(op, "k_pages and v_pages must be alike, [num_pages, kv_heads, page_size, 64]")
-    n, h, p, _ = k.shape
-    if k.stride(3) != 1 or (p > 1 and k.stride(2) != 64) or (h > 1 and k.stride(1) != 64 * p):
+    n, h, p, _ = shape
+    if stride[3] != 1 or (p > 1 and stride[2] != 64) or (h > 1 and stride[1] != 64 * p):
         _refuse(op, "the rows of a page must be contiguous")
-    c = _lib.CdkPagedCache()
-    if k.dtype == torch.float8_e4m3fn:
+    ld_scale = 0
+    if dtype == torch.float8_e4m3fn:
         if k_scale is None or v_scale is None:
             _refuse(op, "e4m3 pages need k_scale and v_scale")
         for s in (k_scale, v_scale):
-            if s.dtype not in (torch.float8_e8m0fnu, torch.uint8) or s.shape != (n, h, p) \
-                    or s.stride() != k_scale.stride() or (p > 1 and s.stride(2) != 1) or (h > 1 and s.stride(1) != p):
+            if s[0] not in (torch.float8_e8m0fnu, torch.uint8) or s[1] != (n, h, p) or s[2] != k_scale[2] \
+                    or (p > 1 and s[2][2] != 1) or (h > 1 and s[2][1] != p):
                 _refuse(op, f"scales must be float8_e8m0fnu (or uint8) [{n}, {h}, {p}], contiguous in a page")
-        c.k_scale, c.v_scale, c.dtype = k_scale.data_ptr(), v_scale.data_ptr(), 1
-        c.ld_scale = k_scale.stride(0) if n > 1 else h * p
-    elif k.dtype == torch.bfloat16:
+        ld_scale = k_scale[2][0] if n > 1 else h * p
+    elif dtype == torch.bfloat16:
         if k_scale is not None or v_scale is not None:
             _refuse(op, "bf16 pages have no scales")
     else:
         _refuse(op, "pages must be bfloat16 or float8_e4m3fn")
-    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != B or (table.shape[1] > 1
-                                                                                 and table.stride(1) != 1):
+    tdtype, tshape, tstride = table
+    if tdtype != torch.int32 or len(tshape) != 2 or tshape[0] != B or (tshape[1] > 1 and tstride[1] != 1):
         _refuse(op, f"table must be int32 [{B}, pages per sequence] with unit inner stride")
-    c.k, c.v, c.table = k.data_ptr(), v.data_ptr(), table.data_ptr()
-    c.width = table.shape[1]
-    c.ldt = table.stride(0) if B > 1 else table.shape[1]
-    c.num_pages, c.kv_heads, c.page_size = n, h, p
-    c.ld_page = k.stride(0) if n > 1 else h * p * 64
-    return c
+    ldt = tstride[0] if B > 1 else tshape[1]
+    if ldt < tshape[1]:
+        _refuse(op, "the rows of table overlap")
+    return p, h, (ldt, tshape[1], n, stride[0] if n > 1 else h * p * 64, ld_scale, h, p,
+                  int(dtype == torch.float8_e4m3fn), 0)
+
+
+def _cache_arg(k, v, k_scale, v_scale, table, fields):
+    return C.byref(_lib.CdkPagedCache(k.data_ptr(), v.data_ptr(), _ptr(k_scale), _ptr(v_scale), table.data_ptr(),
+                                      *fields))
+
+
+@functools.lru_cache(maxsize=1024)
+def _append_plan(B, S_new, H, k, v, table, ks, vs, qkv, start, num_new, pos, rope, q_out):
+    op = "paged_append"
+    _, Hkv, fields = _pages_plan(op, k, v, table, ks, vs, B)
+    if B < 0 or S_new < 0 or H < 0:
+        _refuse(op, f"B={B}, S_new={S_new}, H={H}")
+    T = B * S_new
+    ldq = _rows2d(op, "qkv", qkv, (torch.float32, torch.bfloat16), T, (H + 2 * Hkv) * 64)
+    _vec(op, "start", start, torch.int32, B)
+    _vec(op, "num_new", num_new, torch.int32, B)
+    if (rope is None) != (pos is None):
+        _refuse(op, "pos and rope go together")
+    if rope is not None:
+        _vec(op, "pos", pos, torch.int32, T)
+        if rope[0] != torch.float32 or len(rope[1]) != 3 or rope[1][1:] != (32, 2) or rope[2] != (64, 2, 1):
+            _refuse(op, "rope must be contiguous fp32 [positions, 32, 2]")
+    ldo = 0 if q_out is None else _rows2d(op, "q_out", q_out, (torch.bfloat16,), T, H * 64)
+    return fields, T, ldq, int(qkv[0] == torch.float32), 0 if rope is None else rope[1][0], ldo
 
 
 @_timed("paged_append")
@@ -722,29 +771,35 @@ def paged_append(qkv, B, S_new, H, k_pages, v_pages, table, start, *, num_new=No
     power-of-two scale a row in k_scale / v_scale.  num_new (int32 [B]): only the
     first num_new[b] tokens of a sequence are real; nothing is written for the
     others.  The rows of one call must be distinct."""
-    op = "paged_append"
-    c = _pages(op, k_pages, v_pages, table, k_scale, v_scale, B)
-    T, Hkv = B * S_new, k_pages.shape[1]
-    _rows16(op, "qkv", qkv, (torch.float32, torch.bfloat16), T, (H + 2 * Hkv) * 64)
-    _vec(op, "start", start, torch.int32, B)
-    if num_new is not None:
-        _vec(op, "num_new", num_new, torch.int32, B)
-    if (rope is None) != (pos is None):
-        _refuse(op, "pos and rope go together")
-    if rope is not None:
-        _vec(op, "pos", pos, torch.int32, T)
-        if rope.dtype != torch.float32 or rope.dim() != 3 or rope.shape[1:] != (32, 2) or not rope.is_contiguous():
-            _refuse(op, "rope must be contiguous fp32 [positions, 32, 2]")
-    if q_out is not None:
-        _rows16(op, "q_out", q_out, (torch.bfloat16,), T, H * 64)
-    _on(op, k_pages.device, v_pages, table, k_scale, v_scale, qkv, start, num_new, pos, rope, q_out)
+    fields, T, ldq, f32, n_rope, ldo = _append_plan(
+        B, S_new, H, _lay(k_pages), _lay(v_pages), _lay(table), _lay(k_scale), _lay(v_scale), _lay(qkv), _lay(start),
+        _lay(num_new), _lay(pos), _lay(rope), _lay(q_out))
+    dev = _on("paged_append", k_pages, v_pages, table, k_scale, v_scale, qkv, start, num_new, pos, rope, q_out)
     if T == 0:
         return
-    _call(op, lib().cdk_paged_append, k_pages.device, qkv.data_ptr(), qkv.stride(0) if T > 1 else qkv.shape[1],
-          int(qkv.dtype == torch.float32), _p(pos), _p(rope), 0 if rope is None else rope.shape[0], B, S_new, H,
-          C.byref(c), start.data_ptr(), _p(num_new), _p(q_out),
-          0 if q_out is None else (q_out.stride(0) if T > 1 else q_out.shape[1]))
+    _call("paged_append", lib().cdk_paged_append, dev, qkv.data_ptr(), ldq, f32, _ptr(pos), _ptr(rope), n_rope, B,
+          S_new, H, _cache_arg(k_pages, v_pages, k_scale, v_scale, table, fields), start.data_ptr(), _ptr(num_new),
+          _ptr(q_out), ldo)
     _count(1)
+
+
+@functools.lru_cache(maxsize=1024)
+def _gather_plan(k, v, table, ks, vs, lens, k_out, v_out):
+    op = "paged_gather"
+    B = table[1][0] if len(table[1]) else -1
+    _, Hkv, fields = _pages_plan(op, k, v, table, ks, vs, B)
+    _vec(op, "lens", lens, torch.int32, B)
+    dtype, shape, stride = k_out
+    if v_out != k_out or dtype != torch.bfloat16 or len(shape) != 4 or shape[0] != B or shape[1] != Hkv \
+            or shape[3] != 64 or stride[3] != 1:
+        _refuse(op, f"k_out and v_out must be alike, bf16 [{B}, {Hkv}, rows, 64] with unit inner stride")
+    strides = tuple(s if n > 1 else 0 for s, n in zip(stride[:3], shape))
+    span = 64
+    for s, n in sorted((s, n) for s, n in zip(strides, shape) if n > 1):
+        if s < span:
+            _refuse(op, "the rows of k_out and v_out must not overlap")
+        span = s * n
+    return fields, B, strides, shape[2]
 
 
 @_timed("paged_gather")
@@ -752,25 +807,13 @@ def paged_gather(k_pages, v_pages, table, lens, k_out, v_out, *, k_scale=None, v
     """Rows [0, lens[b]) of every sequence's paged keys and values as bf16 into
     k_out / v_out [B, kv_heads, S, 64] (any strides but the last); the rows
     behind a sequence's length are left as they were."""
-    op = "paged_gather"
-    B = table.shape[0] if table.dim() == 2 else -1
-    c = _pages(op, k_pages, v_pages, table, k_scale, v_scale, B)
-    _vec(op, "lens", lens, torch.int32, B)
-    for o in (k_out, v_out):
-        if o.dtype != torch.bfloat16 or o.dim() != 4 or o.shape != k_out.shape or o.stride() != k_out.stride() \
-                or o.shape[0] != B or o.shape[1] != k_pages.shape[1] or o.shape[3] != 64 or o.stride(3) != 1:
-            _refuse(op, f"k_out and v_out must be alike, bf16 [{B}, {k_pages.shape[1]}, rows, 64] with unit inner stride")
-    sb, sh, ss, _ = (s if n > 1 else 0 for s, n in zip(k_out.stride(), k_out.shape))
-    span = 64
-    for s, n in sorted((s, n) for s, n in zip((sb, sh, ss), k_out.shape) if n > 1):
-        if s < span:
-            _refuse(op, "the rows of k_out and v_out must not overlap")
-        span = s * n
-    _on(op, k_pages.device, v_pages, table, k_scale, v_scale, lens, k_out, v_out)
-    if k_out.numel() == 0:
+    fields, B, strides, S = _gather_plan(_lay(k_pages), _lay(v_pages), _lay(table), _lay(k_scale), _lay(v_scale),
+                                         _lay(lens), _lay(k_out), _lay(v_out))
+    dev = _on("paged_gather", k_pages, v_pages, table, k_scale, v_scale, lens, k_out, v_out)
+    if B == 0 or S == 0:
         return
-    _call(op, lib().cdk_paged_gather, k_pages.device, C.byref(c), B, lens.data_ptr(), k_out.data_ptr(),
-          v_out.data_ptr(), sb, sh, ss, k_out.shape[2])
+    _call("paged_gather", lib().cdk_paged_gather, dev, _cache_arg(k_pages, v_pages, k_scale, v_scale, table, fields), B,
+          lens.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), *strides, S)
     _count(1)
 
 
@@ -783,6 +826,26 @@ def paged_attn_workspace(B, H, kv_heads):
     return n
 
 
+@functools.lru_cache(maxsize=1024)
+def _attn_plan(k, v, table, ks, vs, q, lens, out, workspace):
+    op = "paged_attn"
+    B = table[1][0] if len(table[1]) else -1
+    _, Hkv, fields = _pages_plan(op, k, v, table, ks, vs, B)
+    cols = out[1][1] if len(out[1]) == 2 else 0
+    if cols % 64 or cols == 0:
+        _refuse(op, "out must be [B, H * 64]")
+    ldo = _rows2d(op, "out", out, (torch.bfloat16,), B, cols)
+    ldq = _rows2d(op, "q", q, (torch.bfloat16,), B, cols)
+    if q[1][1] != cols:
+        _refuse(op, "q and out must have the same heads")
+    _vec(op, "lens", lens, torch.int32, B)
+    need = paged_attn_workspace(B, cols // 64, Hkv)
+    if workspace is not None and (workspace[0] != torch.uint8 or len(workspace[1]) != 1 or workspace[2] != (1,)
+                                  or workspace[1][0] < need):
+        _refuse(op, f"workspace must be contiguous uint8 of at least {need} bytes")
+    return fields, B, cols // 64, ldq, ldo, need, 2 if table[1][1] * k[1][2] > 32 else 1  # an item of one tile needs no join
+
+
 @_timed("paged_attn")
 def paged_attn(q, k_pages, v_pages, table, lens, out, *, k_scale=None, v_scale=None, scale=0.125, workspace=None):
     """Attention of one new token per sequence over its first lens[b] cached
@@ -790,29 +853,18 @@ def paged_attn(q, k_pages, v_pages, table, lens, out, *, k_scale=None, v_scale=N
     (grouped queries).  A sequence of length 0 gets zeros.  workspace (uint8,
     paged_attn_workspace bytes): allocated here when not given; a given one must
     not be shared by calls that can overlap."""
-    op = "paged_attn"
-    B = table.shape[0] if table.dim() == 2 else -1
-    c = _pages(op, k_pages, v_pages, table, k_scale, v_scale, B)
-    if out.dim() != 2 or out.shape[1] % 64 or out.shape[1] == 0:
-        _refuse(op, "out must be [B, H * 64]")
-    H = out.shape[1] // 64
-    _rows16(op, "out", out, (torch.bfloat16,), B, H * 64)
-    _rows16(op, "q", q, (torch.bfloat16,), B, H * 64)
-    if q.shape[1] != H * 64:
-        _refuse(op, "q and out must have the same heads")
-    _vec(op, "lens", lens, torch.int32, B)
-    need = paged_attn_workspace(B, H, k_pages.shape[1])
-    if workspace is not None and (workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need):
-        _refuse(op, f"workspace must be contiguous uint8 of at least {need} bytes")
-    _on(op, k_pages.device, v_pages, table, k_scale, v_scale, q, lens, out, workspace)
+    fields, B, H, ldq, ldo, need, launches = _attn_plan(
+        _lay(k_pages), _lay(v_pages), _lay(table), _lay(k_scale), _lay(v_scale), _lay(q), _lay(lens), _lay(out),
+        _lay(workspace))
+    dev = _on("paged_attn", k_pages, v_pages, table, k_scale, v_scale, q, lens, out, workspace)
     if B == 0:
         return
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=k_pages.device)
-    _call(op, lib().cdk_paged_attn, k_pages.device, q.data_ptr(), q.stride(0) if B > 1 else H * 64, C.byref(c), B, H,
-          lens.data_ptr(), out.data_ptr(), out.stride(0) if B > 1 else H * 64, float(scale), workspace.data_ptr(),
-          workspace.numel())
-    _count(1)
+    _call("paged_attn", lib().cdk_paged_attn, dev, q.data_ptr(), ldq,
+          _cache_arg(k_pages, v_pages, k_scale, v_scale, table, fields), B, H, lens.data_ptr(), out.data_ptr(), ldo,
+          scale, workspace.data_ptr(), need)
+    _count(launches)
 
 
 # ---------------------------------------------------------------------------
@@ -821,18 +873,35 @@ def paged_attn(q, k_pages, v_pages, table, lens, out, *, k_scale=None, v_scale=N
 MAX_TOP = 32
 
 
-def _logits(op, logits, target32, ncls):
-    if logits.dtype not in (torch.float32, torch.bfloat16) or logits.dim() != 2 or (logits.shape[1] > 1
-                                                                                    and logits.stride(1) != 1):
-        _refuse(op, "logits must be fp32 or bf16 [rows, classes] with unit inner stride")
-    rows, cols = logits.shape
-    ncls = cols if ncls is None else ncls
-    if not 0 < ncls <= cols:
-        _refuse(op, f"ncls {ncls} of {cols} columns")
-    if rows > 1 and logits.stride(0) < ncls:
-        _refuse(op, "the rows of logits overlap")
-    _vec(op, "target32", target32, torch.int32, rows)
-    return rows, ncls
+def _logits_plan(op, logits, target32, ncls):
+    shape = logits[1]
+    if ncls is None and len(shape) == 2:
+        ncls = shape[1]
+    if len(shape) != 2 or not 0 < ncls <= shape[1]:
+        _refuse(op, f"logits must be [rows, classes] with 0 < ncls <= classes, got {tuple(shape)} and {ncls}")
+    ldl = _rows2d(op, "logits", logits, (torch.float32, torch.bfloat16), shape[0], ncls)
+    _vec(op, "target32", target32, torch.int32, shape[0])
+    return shape[0], ncls, ldl, int(logits[0] == torch.bfloat16)
+
+
+@functools.lru_cache(maxsize=1024)
+def _stats_plan(logits, target32, lp, entropy, lse, top_ids, top_lp, ncls):
+    op = "token_logprobs"
+    rows, ncls, ldl, dt = _logits_plan(op, logits, target32, ncls)
+    for name, lay in (("lp", lp), ("entropy", entropy), ("lse", lse)):
+        _vec(op, name, lay, torch.float32, rows)
+    if (top_ids is None) != (top_lp is None):
+        _refuse(op, "top_ids and top_lp go together")
+    k = 0
+    if top_ids is not None:
+        k = top_ids[1][1] if len(top_ids[1]) == 2 else -1
+        if not 0 <= k <= min(MAX_TOP, ncls) or top_ids[:2] != (torch.int32, (rows, k)) \
+                or top_lp[:2] != (torch.float32, (rows, k)) \
+                or any(s[2] != (k, 1) for s in (top_ids, top_lp) if rows > 1 and k > 1):
+            _refuse(op, f"top_ids / top_lp must be contiguous int32 / fp32 [{rows}, k], k <= min({MAX_TOP}, classes)")
+        if k == 1 and rows > 1 and (top_ids[2][0] != 1 or top_lp[2][0] != 1):
+            _refuse(op, "top_ids / top_lp must be contiguous")
+    return rows, ncls, ldl, dt, k
 
 
 @_timed("token_logprobs")
@@ -841,27 +910,26 @@ def token_logprobs(logits, target32, lp, *, entropy=None, lse=None, top_ids=None
     [0, ncls)), and where given the entropy, the log-sum-exp and the k best
     classes (top_ids int32 [rows, k], top_lp fp32 [rows, k], k <= 32; equal
     logits in order of their index).  fp32 outputs."""
-    op = "token_logprobs"
-    rows, ncls = _logits(op, logits, target32, ncls)
-    for name, t in (("lp", lp), ("entropy", entropy), ("lse", lse)):
-        if t is not None:
-            _vec(op, name, t, torch.float32, rows)
-    if (top_ids is None) != (top_lp is None):
-        _refuse(op, "top_ids and top_lp go together")
-    k = 0
-    if top_ids is not None:
-        k = top_ids.shape[1] if top_ids.dim() == 2 else -1
-        if not 0 <= k <= min(MAX_TOP, ncls) or top_ids.shape != (rows, k) or top_lp.shape != (rows, k) \
-                or top_ids.dtype != torch.int32 or top_lp.dtype != torch.float32 \
-                or not (top_ids.is_contiguous() and top_lp.is_contiguous()):
-            _refuse(op, f"top_ids / top_lp must be contiguous int32 / fp32 [{rows}, k], k <= min({MAX_TOP}, classes)")
-    _on(op, logits.device, target32, lp, entropy, lse, top_ids, top_lp)
+    rows, ncls, ldl, dt, k = _stats_plan(_lay(logits), _lay(target32), _lay(lp), _lay(entropy), _lay(lse),
+                                         _lay(top_ids), _lay(top_lp), ncls)
+    dev = _on("token_logprobs", logits, target32, lp, entropy, lse, top_ids, top_lp)
     if rows == 0:
         return
-    _call(op, lib().cdk_token_logprobs, logits.device, logits.data_ptr(), int(logits.dtype == torch.bfloat16),
-          logits.stride(0) if rows > 1 else logits.shape[1], rows, ncls, target32.data_ptr(), lp.data_ptr(),
-          _p(entropy), _p(lse), _p(top_ids) if k else None, _p(top_lp) if k else None, k)
+    _call("token_logprobs", lib().cdk_token_logprobs, dev, logits.data_ptr(), dt, ldl, rows, ncls,
+          target32.data_ptr(), lp.data_ptr(), _ptr(entropy), _ptr(lse), _ptr(top_ids) if k else None,
+          _ptr(top_lp) if k else None, k)
     _count(1)
+
+
+@functools.lru_cache(maxsize=1024)
+def _stats_bwd_plan(logits, target32, lse, entropy, dlp, dentropy, dlogits, ncls):
+    op = "token_logprobs_bwd"
+    rows, ncls, ldl, dt = _logits_plan(op, logits, target32, ncls)
+    if dentropy is not None and entropy is None:
+        _refuse(op, "dentropy needs the forward's entropy")
+    for name, lay in (("lse", lse), ("entropy", entropy), ("dlp", dlp), ("dentropy", dentropy)):
+        _vec(op, name, lay, torch.float32, rows)
+    return rows, ncls, ldl, dt, _rows2d(op, "dlogits", dlogits, (logits[0],), rows, ncls)
 
 
 @_timed("token_logprobs_bwd")
@@ -870,20 +938,11 @@ def token_logprobs_bwd(logits, target32, lse, entropy, dlp, dentropy, dlogits, *
     from the forward's lse and entropy; dlp / dentropy fp32 [rows], either may be
     None (zero; entropy is then not needed for dentropy None).  dlogits has the
     logits' type and may be the same tensor."""
-    op = "token_logprobs_bwd"
-    rows, ncls = _logits(op, logits, target32, ncls)
-    if dentropy is not None and entropy is None:
-        _refuse(op, "dentropy needs the forward's entropy")
-    for name, t in (("lse", lse), ("entropy", entropy), ("dlp", dlp), ("dentropy", dentropy)):
-        if t is not None:
-            _vec(op, name, t, torch.float32, rows)
-    _rows16(op, "dlogits", dlogits, (logits.dtype,), rows, ncls)
-    if rows > 1 and dlogits.stride(0) < ncls:
-        _refuse(op, "the rows of dlogits overlap")
-    _on(op, logits.device, target32, lse, entropy, dlp, dentropy, dlogits)
+    rows, ncls, ldl, dt, ldd = _stats_bwd_plan(_lay(logits), _lay(target32), _lay(lse), _lay(entropy), _lay(dlp),
+                                               _lay(dentropy), _lay(dlogits), ncls)
+    dev = _on("token_logprobs_bwd", logits, target32, lse, entropy, dlp, dentropy, dlogits)
     if rows == 0:
         return
-    _call(op, lib().cdk_token_logprobs_bwd, logits.device, logits.data_ptr(), int(logits.dtype == torch.bfloat16),
-          logits.stride(0) if rows > 1 else logits.shape[1], rows, ncls, target32.data_ptr(), lse.data_ptr(),
-          _p(entropy), _p(dlp), _p(dentropy), dlogits.data_ptr(), dlogits.stride(0) if rows > 1 else dlogits.shape[1])
+    _call("token_logprobs_bwd", lib().cdk_token_logprobs_bwd, dev, logits.data_ptr(), dt, ldl, rows, ncls,
+          target32.data_ptr(), lse.data_ptr(), _ptr(entropy), _ptr(dlp), _ptr(dentropy), dlogits.data_ptr(), ldd)
     _count(1)
