@@ -216,17 +216,22 @@ __global__ void __launch_bounds__(256)
 // ---------------------------------------------------------------------------
 // One new token per sequence.
 //
-// o = sum_j p_j v_j / sum_j p_j with p_j = 2^(s_j - m), s = scale log2(e) q . k,
-// m the running maximum: one pass over the cached rows, which is what bounds it
-// (HBM; the products are a few percent of the tensor pipe even for one query).
+// o = sum_j w_j v_j / sum_j w_j with w_j = 2^(s_j - m), s = scale log2(e) q . k:
+// one pass over the cached rows, which is what bounds it (HBM; the products are a
+// few percent of the tensor pipe even for one query).  m is any common reference:
+// it follows the maximum, but only when a score passes it by 8 (weights stay
+// below 2^8), so that most tiles need no exchange between lanes and no rescaling.
 //
-// Work.  The keys of one (sequence, kv head) item are cut into tiles of 32; the
-// tiles of all items, in the order (sequence, head, tile), are dealt to the
-// grid's warps in equal contiguous runs, whatever the lengths.  A warp that
-// holds a whole item writes its output; the others leave partial results (m, l,
-// O) in the workspace, two per warp at most (the item it ends, the item it
-// begins), which paged_attn_join_kernel adds up in a fixed order.  Warps never
-// wait for one another.
+// Work.  The keys of one (sequence, kv head) item are cut into tiles of 32 (bf16)
+// or 64 (e4m3).  Where the tables hold few tiles per item, a block takes an item,
+// its four warps a quarter of the tiles each.  Otherwise the tiles of all items,
+// in the order (sequence, head, tile), are dealt to the grid's warps in equal
+// contiguous runs, whatever the lengths; an item counts kSetup tiles more than it
+// has, for what it costs a warp to begin one.  A warp that holds a whole item writes
+// its output; a block inside one item adds up its warps in shared memory; what is
+// shared beyond that is left as partial results (m, l, O) in the workspace and
+// added up in a fixed order by paged_attn_join_kernel.  Warps never wait for other
+// blocks.
 //
 // Tile.  Scores are taken transposed, S^T = K Q^T, with mma.sync m16n8k16: 16
 // keys by 8 queries, so a group of up to 8 query heads costs what one costs.
@@ -238,18 +243,31 @@ __global__ void __launch_bounds__(256)
 // shared memory, no barrier in the loop: the loads of the next tile's keys are
 // issued before this tile's softmax, those of its values after its products.
 //
-// bf16 pages: the weights are split into two bf16 (p = hi + lo, 2^-17 of p) so
+// bf16 pages: the weights are split into two bf16 (w = hi + lo, 2^-17 of w) so
 // that they add no error beside the output's rounding.  e4m3 pages: codes are
-// exact in fp16; q is scaled to fp16 by a power of two per head; the value scales
-// 2^e_j enter the exponent of the weights, w_j = 2^(s_j + e_j - m'), with their
-// own maximum m', so that a weight is at most 1 whatever the scales are; they are
-// rounded to fp16 (2^-11).
+// exact in fp16; q is scaled to fp16 by a power of two per head.  The products
+// with the values take w_j 2^e_j, e_j the value row's scale, so that m has to
+// follow s_j + e_j: weights then fit fp16 (2^-11) whatever the scales are.  The
+// sum of the w_j alone reaches 2^(8 - e_j); e_j below -96 counts as -96 for m (a
+// row of zeros has the smallest scale), which only values below 448 * 2^-96 feel.
 // ---------------------------------------------------------------------------
-constexpr int kTK = 32;             // keys per tile
 constexpr int kAttnThreads = 128;   // 4 warps; 128 registers: 4 blocks per SM
+constexpr int kWarps = kAttnThreads / 32;
 constexpr int kAttnBlocks = 148 * 4;
-constexpr int kAttnWarps = kAttnBlocks * kAttnThreads / 32;
+constexpr int kAttnWarps = kAttnBlocks * kWarps;
 constexpr int kSlots = 2 * kAttnWarps;
+constexpr float kNoScore = -3.0e38f;  // m before the first key
+constexpr float kSlack = 8.f;
+// Tiles per item up to which a block takes an item: the second kernel's launch
+// and the deal's search cost more than a warp's few tiles in a row.
+constexpr int kItemTiles = 16;
+
+// What beginning an item costs a warp, in tiles of the deal: its table, queries and
+// first rows come one after the other.
+constexpr int kSetup = 2;
+
+template <bool FP8>
+__host__ __device__ constexpr int tile_keys() { return FP8 ? 32 : 32; }
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -306,60 +324,493 @@ struct AttnArgs {
   __nv_bfloat16* out;
   long long ldo;
   float scale_log2;
-  int32_t* prefix;  // workspace: [B + 1] tiles before each sequence, per kv head
-  float4* stat;     // workspace: [kSlots][group] (m, l, m', -)
+  int tile;         // keys per tile
+  int32_t* prefix;  // workspace: [B + 1] shares of the deal before each sequence, per kv head
+  float2* stat;     // workspace: [kSlots][group] (m, l)
   float* part;      // workspace: [kSlots][group][64]
 };
 
-__device__ __forceinline__ int tiles_of(const AttnArgs& a, int b, int* len_out, bool report) {
+__device__ __forceinline__ int length_of(const AttnArgs& a, int b, bool report) {
   long long len = max(a.lens[b], 0);
   const long long cap = a.pg.width << a.pg.log_page;
   if (len > cap) {
     if (report) report_error(kErrIndex);
     len = cap;
   }
-  if (len_out) *len_out = (int)len;
-  return (int)((len + kTK - 1) / kTK);
+  return (int)len;
 }
 
-// Writes `out` of one (sequence, head): 8 dims per lane.
+// Shares of the deal of one item: its tiles and kSetup, nothing for an empty one.
+template <int KT>
+__device__ __forceinline__ int shares_of(int len) {
+  return len > 0 ? (len + KT - 1) / KT + kSetup : 0;
+}
+
+// Writes 8 dims of the output of one (sequence, head).
 __device__ __forceinline__ void store_out8(const AttnArgs& a, int b, int h, int d, const float (&o)[8], float f) {
   *reinterpret_cast<uint4*>(a.out + (long long)b * a.ldo + h * kHD + d) =
       make_uint4(pack_bf16(o[0] * f, o[1] * f), pack_bf16(o[2] * f, o[3] * f), pack_bf16(o[4] * f, o[5] * f),
                  pack_bf16(o[6] * f, o[7] * f));
 }
 
+// State of one warp and item.  Lane (g, t4) = (lane / 4, lane % 4) holds, for
+// heads 8 n + 2 t4 + c of the group, dims 8 g ... 8 g + 7 of O.
+template <int NT>
+struct Acc {
+  float o[NT][4][4];  // [dim pair i][c, 2 + c]: dims 8 g + 2 i and 8 g + 2 i + 1
+  float m[NT][2], l[NT][2];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+      m[n][0] = m[n][1] = kNoScore;
+      l[n][0] = l[n][1] = 0.f;
+    }
+  }
+  __device__ __forceinline__ void sum_lanes() {  // l over the lanes of a column
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], x);
+  }
+  __device__ __forceinline__ void dims(int n, int c, float (&v)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = o[n][i][c];
+      v[2 * i + 1] = o[n][i][2 + c];
+    }
+  }
+};
+
+// Tiles [ta, tb) of one item: acc over its keys below len.
 template <bool FP8, int NT>
-__global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 3) paged_attn_kernel(const AttnArgs a) {
-  extern __shared__ int32_t prefix[];  // [B + 1]
-  __shared__ int warp_sum_[kAttnThreads / 32];
+__device__ __forceinline__ void attend(const AttnArgs& a, int b, int kvh, int ta, int tb, int len, int lane,
+                                       Acc<NT>& acc) {
   constexpr int kRow = FP8 ? kHD : 2 * kHD;  // bytes of a cached row
   constexpr int kKC = FP8 ? 1 : 2;           // 16-byte chunks of a key row per lane
+  constexpr int KT = tile_keys<FP8>(), HV = KT / 32, R = KT / 8, J = KT / 16;
   using VT = typename std::conditional<FP8, uint2, uint4>::type;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int g = lane >> 2, t4 = lane & 3;
   const Pages& pg = a.pg;
+  const int g = lane >> 2, t4 = lane & 3;
+  const int32_t* trow = pg.table + (long long)b * pg.ldt;
+  const int head_row = kvh << pg.log_page;
+  const int pmask = (1 << pg.log_page) - 1;
+
+  // pages of this lane's keys (tile * KT + 32 x + lane); what is not there is masked
+  auto pages_at = [&](int tile, int (&page)[HV]) {
+#pragma unroll
+    for (int x = 0; x < HV; ++x) {
+      const int key = tile * KT + 32 * x + lane;
+      page[x] = tile < tb && key < len ? __ldg(trow + (key >> pg.log_page)) : -1;
+    }
+  };
+  auto masks_of = [&](int tile, const int (&page)[HV], uint32_t (&mask)[HV]) {
+#pragma unroll
+    for (int x = 0; x < HV; ++x) {
+      const bool ok = (unsigned)page[x] < (unsigned)pg.num_pages;
+      mask[x] = __ballot_sync(0xffffffffu, ok);
+      if (mask[x] != 0xffffffffu && !ok && tile * KT + 32 * x + lane < len) report_error(kErrIndex);
+    }
+  };
+  auto all_of = [&](const uint32_t (&mask)[HV]) {
+    bool f = true;
+#pragma unroll
+    for (int x = 0; x < HV; ++x) f = f && mask[x] == 0xffffffffu;
+    return f;
+  };
+
+  uint4 kr[R][kKC];
+  VT vr[J][4];
+  uint32_t sc[HV];  // e4m3: scale bytes of this lane's keys, key | value << 8
+  auto load_k = [&](int tile, const int (&page)[HV], const uint32_t (&mask)[HV], bool full) {
+    const int t0 = tile * KT;
+    if (FP8) {
+#pragma unroll
+      for (int x = 0; x < HV; ++x) {
+        sc[x] = 0;
+        if ((mask[x] >> lane) & 1) {
+          const long long r = (long long)page[x] * pg.ld_scale + head_row + ((t0 + 32 * x + lane) & pmask);
+          sc[x] = (uint32_t)__ldg(pg.ks + r) | ((uint32_t)__ldg(pg.vs + r) << 8);
+        }
+      }
+    }
+    if (pg.log_page >= 5 && full) {  // 32 rows in a row in one page
+#pragma unroll
+      for (int x = 0; x < HV; ++x) {
+        const long long p0 = __shfl_sync(0xffffffffu, page[x], 0);
+        const char* base = pg.k + p0 * pg.ld_page + (long long)(head_row + ((t0 + 32 * x) & pmask) + g) * kRow + t4 * 16;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int c = 0; c < kKC; ++c) kr[4 * x + r][c] = ld_once<uint4>(base + r * 8 * kRow + c * 64);
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int y = g + 8 * (r & 3);  // row within the half r / 4
+        const long long p = __shfl_sync(0xffffffffu, page[r >> 2], y);
+        const char* base = pg.k + p * pg.ld_page + (long long)(head_row + ((t0 + 32 * (r >> 2) + y) & pmask)) * kRow + t4 * 16;
+#pragma unroll
+        for (int c = 0; c < kKC; ++c)
+          kr[r][c] = (mask[r >> 2] >> y) & 1 ? ld_once<uint4>(base + c * 64) : make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+  };
+  auto load_v = [&](int tile, const int (&page)[HV], const uint32_t (&mask)[HV], bool full) {
+    const int t0 = tile * KT;
+    if (pg.log_page >= 5 && full) {
+#pragma unroll
+      for (int x = 0; x < HV; ++x) {
+        const long long p0 = __shfl_sync(0xffffffffu, page[x], 0);
+        const char* base =
+            pg.v + p0 * pg.ld_page + (long long)(head_row + ((t0 + 32 * x) & pmask) + 2 * t4) * kRow + g * (kRow / 8);
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) vr[2 * x + jj][i] = ld_once<VT>(base + (16 * jj + (i & 1) + (i >> 1) * 8) * kRow);
+      }
+    } else {
+#pragma unroll
+      for (int jj = 0; jj < J; ++jj)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int y = 16 * (jj & 1) + 2 * t4 + (i & 1) + (i >> 1) * 8;
+          const long long p = __shfl_sync(0xffffffffu, page[jj >> 1], y);
+          const char* base =
+              pg.v + p * pg.ld_page + (long long)(head_row + ((t0 + 32 * (jj >> 1) + y) & pmask)) * kRow + g * (kRow / 8);
+          vr[jj][i] = (mask[jj >> 1] >> y) & 1 ? ld_once<VT>(base) : VT{};
+        }
+    }
+  };
+
+  int page[HV];
+  uint32_t mask[HV];
+  pages_at(ta, page);
+  masks_of(ta, page, mask);
+  bool full = all_of(mask);
+  load_k(ta, page, mask, full);
+  load_v(ta, page, mask, full);
+  pages_at(ta + 1, page);
+
+  // queries of the group as the B operand: head 8 n + g, 8 (bf16) or 16 (e4m3) dims per chunk and lane
+  uint32_t qf[NT][8];
+  float qs[NT][2];  // factor of the scores of heads 8 n + 2 t4, + 1
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int hq = n * 8 + g;
+    const __nv_bfloat16* qrow = a.q + (long long)b * a.ldq + (kvh * a.group + hq) * kHD;
+    uint4 x = make_uint4(0u, 0u, 0u, 0u), y = x;
+    if (hq < a.group) {
+      x = *reinterpret_cast<const uint4*>(qrow + (FP8 ? 16 : 8) * t4);
+      y = *reinterpret_cast<const uint4*>(qrow + (FP8 ? 16 * t4 + 8 : 32 + 8 * t4));
+    }
+    const uint32_t raw[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    if (!FP8) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) qf[n][i] = raw[i];
+      qs[n][0] = qs[n][1] = a.scale_log2;
+    } else {
+      uint32_t top = 0;  // the row's largest magnitude, as bf16 bits
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = max(top, max(raw[i] & 0x7fffu, (raw[i] >> 16) & 0x7fffu));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // largest in [2^14, 2^15): fp16 then holds all 8 bits of whatever is above 2^-31 of it
+      const int e = min(max((int)(top >> 7), 15), 250);  // exponent field; the factor 2^(141 - e) is a normal number
+      const float up = __uint_as_float((uint32_t)(127 + 141 - e) << 23);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 v = bf2f(raw[i]);
+        qf[n][i] = pack_f16(v.x * up, v.y * up);
+      }
+      // lanes (g, *) hold head g's factor; this lane's score columns are heads 2 t4, 2 t4 + 1
+      qs[n][0] = a.scale_log2 / __shfl_sync(0xffffffffu, up, 8 * t4);
+      qs[n][1] = a.scale_log2 / __shfl_sync(0xffffffffu, up, 8 * t4 + 4);
+    }
+  }
+
+#pragma unroll 1
+  for (int tile = ta; tile < tb; ++tile) {
+    int page2[HV];  // the table two tiles ahead: there when the next tile's scores are done
+    pages_at(tile + 2, page2);
+    // S^T: keys g + 8 r by heads 2 t4 + c -> s[n][r][c]
+    float s[NT][R][2];
+#pragma unroll
+    for (int i = 0; i < R / 2; ++i) {
+      float d[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.f;
+      if (FP8) {
+        const uint4 u = kr[2 * i][0], w4 = kr[2 * i + 1][0];
+        const uint32_t lo[4] = {u.x, u.y, u.z, u.w}, hi[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t af[4] = {e4m3x2_h(lo[j]), e4m3x2_h(hi[j]), e4m3x2_h(lo[j] >> 16), e4m3x2_h(hi[j] >> 16)};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_f16_16816(d[n], af, qf[n][2 * j], qf[n][2 * j + 1]);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < kKC; ++c) {
+          const uint4 u = kr[2 * i][c], w4 = kr[2 * i + 1][c];
+          const uint32_t a0[4] = {u.x, w4.x, u.y, w4.y}, a1[4] = {u.z, w4.z, u.w, w4.w};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma_bf16_16816(d[n], a0, qf[n][4 * c], qf[n][4 * c + 1]);
+            mma_bf16_16816(d[n], a1, qf[n][4 * c + 2], qf[n][4 * c + 3]);
+          }
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          s[n][2 * i][c] = d[n][c] * qs[n][c];
+          s[n][2 * i + 1][c] = d[n][2 + c] * qs[n][c];
+        }
+    }
+    float vs[R];  // value scales
+    if (FP8) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const uint32_t x = __shfl_sync(0xffffffffu, sc[r >> 2], g + 8 * (r & 3));
+        const float ks = __uint_as_float((x & 0xffu) << 23);
+        vs[r] = __uint_as_float((x & 0xff00u) << 15);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          s[n][r][0] *= ks;
+          s[n][r][1] *= ks;
+        }
+      }
+    }
+    if (!full) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (!((mask[r >> 2] >> (g + 8 * (r & 3))) & 1)) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) s[n][r][0] = s[n][r][1] = -INFINITY;
+        }
+    }
+    if (tile + 1 < tb) {
+      masks_of(tile + 1, page, mask);
+      full = all_of(mask);
+      load_k(tile + 1, page, mask, full);
+    }
+
+    // does a score pass the reference?
+    float mx[NT][2];
+    bool pass = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float x = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          x = fmaxf(x, FP8 ? s[n][r][c] + fmaxf((float)(int)(__float_as_uint(vs[r]) >> 23) - 127.f, -96.f) : s[n][r][c]);
+        mx[n][c] = x;
+        pass |= x > acc.m[n][c] + kSlack;
+      }
+    if (__any_sync(0xffffffffu, pass)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float x = mx[n][c];
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+          x = fmaxf(x, acc.m[n][c]);
+          const float al = ex2(acc.m[n][c] - x);
+          acc.m[n][c] = x;
+          acc.l[n][c] *= al;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            acc.o[n][i][c] *= al;
+            acc.o[n][i][2 + c] *= al;
+          }
+        }
+    }
+
+    // weights of keys (16 jj + g, + 8) for heads 2 t4, 2 t4 + 1, as the B operand
+    uint32_t pb[NT][J][2], pl[NT][J][2];  // pl: bf16's low parts
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float p0 = ex2(s[n][r][0] - acc.m[n][0]), p1 = ex2(s[n][r][1] - acc.m[n][1]);
+        sum[0] += p0;
+        sum[1] += p1;
+        if (FP8) {
+          pb[n][r >> 1][r & 1] = transpose8x8(pack_f16(p0 * vs[r], p1 * vs[r]));
+        } else {
+          const uint32_t hi = pack_bf16(p0, p1);
+          const float2 back = bf2f(hi);
+          pb[n][r >> 1][r & 1] = transpose8x8(hi);
+          pl[n][r >> 1][r & 1] = transpose8x8(pack_bf16(p0 - back.x, p1 - back.y));
+        }
+      }
+      acc.l[n][0] += sum[0];
+      acc.l[n][1] += sum[1];
+    }
+
+    // O^T += V^T P^T: the A operand's rows g and g + 8 of product i are dims 8 g + 2 i and 8 g + 2 i + 1
+#pragma unroll
+    for (int jj = 0; jj < J; ++jj) {
+      if constexpr (FP8) {
+        // bytes of two keys interleaved first: one permute gives two dims of both
+        uint32_t lo[4], hi[4];  // keys 2 t4, + 1 and 2 t4 + 8, + 9: [dim pair] = (d of both, d + 1 of both)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t k0 = i < 2 ? vr[jj][0].x : vr[jj][0].y, k1 = i < 2 ? vr[jj][1].x : vr[jj][1].y;
+          const uint32_t k2 = i < 2 ? vr[jj][2].x : vr[jj][2].y, k3 = i < 2 ? vr[jj][3].x : vr[jj][3].y;
+          const uint32_t sel = (i & 1) ? 0x7362u : 0x5140u;
+          lo[i] = __byte_perm(k0, k1, sel);
+          hi[i] = __byte_perm(k2, k3, sel);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t af[4] = {e4m3x2_h(lo[i]), e4m3x2_h(lo[i] >> 16), e4m3x2_h(hi[i]), e4m3x2_h(hi[i] >> 16)};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_f16_16816(acc.o[n][i], af, pb[n][jj][0], pb[n][jj][1]);
+        }
+      } else {
+        const uint32_t w4[4][4] = {{vr[jj][0].x, vr[jj][0].y, vr[jj][0].z, vr[jj][0].w},
+                                   {vr[jj][1].x, vr[jj][1].y, vr[jj][1].z, vr[jj][1].w},
+                                   {vr[jj][2].x, vr[jj][2].y, vr[jj][2].z, vr[jj][2].w},
+                                   {vr[jj][3].x, vr[jj][3].y, vr[jj][3].z, vr[jj][3].w}};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t af[4] = {__byte_perm(w4[0][i], w4[1][i], 0x5410), __byte_perm(w4[0][i], w4[1][i], 0x7632),
+                                  __byte_perm(w4[2][i], w4[3][i], 0x5410), __byte_perm(w4[2][i], w4[3][i], 0x7632)};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma_bf16_16816(acc.o[n][i], af, pb[n][jj][0], pb[n][jj][1]);
+            mma_bf16_16816(acc.o[n][i], af, pl[n][jj][0], pl[n][jj][1]);
+          }
+        }
+      }
+    }
+    if (tile + 1 < tb) {
+      load_v(tile + 1, page, mask, full);
+#pragma unroll
+      for (int x = 0; x < HV; ++x) page[x] = page2[x];
+    }
+  }
+}
+
+// Shared memory of a block, sized by the group: what a block does not take stays
+// L1, where the loads in flight land.
+struct AttnShared {
+  float* o;      // [kWarps][group][64]
+  float2* stat;  // [kWarps][group]
+  int* prefix;   // [B + 1]
+  __device__ __forceinline__ AttnShared(char* p, int group) {
+    o = reinterpret_cast<float*>(p);
+    stat = reinterpret_cast<float2*>(o + kWarps * group * kHD);
+    prefix = reinterpret_cast<int*>(stat + kWarps * group);
+  }
+};
+__host__ __device__ constexpr int shared_bytes(int group) { return kWarps * group * (kHD * 4 + 8); }
+
+// A block whose warps all worked on one item (a warp without tiles has an empty
+// state): their sum goes to the output, or to workspace slot `slot` when other
+// blocks share the item.
+template <int NT>
+__device__ __forceinline__ void merge_block(const AttnArgs& a, const AttnShared& sh, const Acc<NT>& acc, int b, int kvh,
+                                            bool whole, long long slot) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int hq = n * 8 + 2 * t4 + c;
+      if (hq >= a.group) continue;
+      float v[8];
+      acc.dims(n, c, v);
+      float4* dst = reinterpret_cast<float4*>(sh.o + (warp * a.group + hq) * kHD + 8 * g);
+      dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+      dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+      if (g == 0) sh.stat[warp * a.group + hq] = make_float2(acc.m[n][c], acc.l[n][c]);
+    }
+  __syncthreads();
+  for (int i = tid; i < a.group * (kHD / 8); i += kAttnThreads) {
+    const int hq = i / (kHD / 8), d = (i % (kHD / 8)) * 8;
+    float m = kNoScore, l = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sh.stat[w * a.group + hq].x);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = ex2(sh.stat[w * a.group + hq].x - m);
+      l += sh.stat[w * a.group + hq].y * f;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) v[x] += sh.o[(w * a.group + hq) * kHD + d + x] * f;
+    }
+    if (whole) {
+      store_out8(a, b, kvh * a.group + hq, d, v, l == 0.f ? 0.f : 1.f / l);
+    } else {
+      const long long at = slot * a.group + hq;
+      float4* dst = reinterpret_cast<float4*>(a.part + at * kHD + d);
+      dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+      dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+      if (d == 0) a.stat[at] = make_float2(m, l);
+    }
+  }
+}
+
+// A block per (sequence, kv head).
+template <bool FP8, int NT>
+__global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 3) paged_attn_item_kernel(const AttnArgs a) {
+  extern __shared__ __align__(16) char smem[];
+  const AttnShared sh(smem, a.group);
+  constexpr int KT = tile_keys<FP8>();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int b = blockIdx.x / a.pg.kv_heads, kvh = blockIdx.x - b * a.pg.kv_heads;
+  const int len = length_of(a, b, kvh == 0 && threadIdx.x == 0);
+  const int tiles = (len + KT - 1) / KT, per = (tiles + kWarps - 1) / kWarps;
+  const int ta = min(warp * per, tiles), tb = min(ta + per, tiles);
+  Acc<NT> acc;
+  acc.clear();
+  if (ta < tb) attend<FP8, NT>(a, b, kvh, ta, tb, len, lane, acc);
+  acc.sum_lanes();
+  merge_block<NT>(a, sh, acc, b, kvh, true, 0);  // len 0: l = 0, zeros
+}
+
+// Shares [f, f + chunk) of the deal for warp w = f / chunk; see the join for the slots.
+template <bool FP8, int NT>
+__global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 3) paged_attn_kernel(const AttnArgs a) {
+  extern __shared__ __align__(16) char smem[];
+  __shared__ int warp_tiles[kWarps];
+  const AttnShared sh(smem, a.group);
+  int* prefix = sh.prefix;
+  constexpr int KT = tile_keys<FP8>();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int kvn = a.pg.kv_heads;
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may be set up; it waits for this grid
-  {  // tiles before each sequence: thread i takes a contiguous run of sequences
+  {  // shares before each sequence: thread i takes a contiguous run of sequences
     const int per = (a.B + kAttnThreads - 1) / kAttnThreads;
     const int b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
     int sum = 0;
-    for (int b = b0; b < b1; ++b) sum += tiles_of(a, b, nullptr, blockIdx.x == 0);
+    for (int b = b0; b < b1; ++b) sum += shares_of<KT>(length_of(a, b, blockIdx.x == 0));
     int scan = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int v = __shfl_up_sync(0xffffffffu, scan, o);
       if (lane >= o) scan += v;
     }
-    if (lane == 31) warp_sum_[warp] = scan;
+    if (lane == 31) warp_tiles[warp] = scan;
     __syncthreads();
     int at = scan - sum;
-    for (int w = 0; w < warp; ++w) at += warp_sum_[w];
+    for (int w = 0; w < warp; ++w) at += warp_tiles[w];
     for (int b = b0; b < b1; ++b) {
       prefix[b] = at;
       if (blockIdx.x == 0) a.prefix[b] = at;
-      at += tiles_of(a, b, nullptr, false);
+      at += b1 - b0 == 1 ? sum : shares_of<KT>(length_of(a, b, false));
     }
     if (tid == kAttnThreads - 1) {
       prefix[a.B] = at;
@@ -369,404 +820,145 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 3) paged_attn_kern
   }
   for (int b = blockIdx.x; b < a.B; b += gridDim.x)  // sequences without keys
     if (prefix[b] == prefix[b + 1])
-      for (int i = tid; i < pg.kv_heads * a.group * (kHD / 8); i += kAttnThreads)
+      for (int i = tid; i < kvn * a.group * (kHD / 8); i += kAttnThreads)
         *reinterpret_cast<uint4*>(a.out + (long long)b * a.ldo + i * 8) = make_uint4(0u, 0u, 0u, 0u);
 
-  const long long total = (long long)prefix[a.B] * pg.kv_heads;
-  const long long n_warps = (long long)gridDim.x * (kAttnThreads / 32);
+  const long long total = (long long)prefix[a.B] * kvn;
+  const long long n_warps = (long long)gridDim.x * kWarps;
   const long long chunk = (total + n_warps - 1) / n_warps;
-  const long long w = (long long)blockIdx.x * (kAttnThreads / 32) + warp;
+  const long long w0 = (long long)blockIdx.x * kWarps, w = w0 + warp;
+  const long long block_f = w0 * chunk, block_end = min(block_f + kWarps * chunk, total);
+  if (block_f >= block_end) return;
   long long f = w * chunk;
   const long long f_end = min(f + chunk, total);
-  if (f >= f_end) return;
 
-  int b;  // the sequence of flat tile f: last b with prefix[b] * kv_heads <= f
-  {
-    int lo = 0, hi = a.B;
+  struct Item {
+    int b, kvh, n;    // n: its shares
+    long long first;  // the first of them
+  };
+  auto item_of = [&](long long x) {  // of share x < total
+    int lo = 0, hi = a.B;            // last b with prefix[b] * kv_heads <= x
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if ((long long)prefix[mid] * pg.kv_heads <= f) lo = mid;
+      if ((long long)prefix[mid] * kvn <= x) lo = mid;
       else hi = mid;
     }
-    b = lo;
+    Item it;
+    it.b = lo;
+    it.n = prefix[lo + 1] - prefix[lo];
+    const long long first = (long long)prefix[lo] * kvn;
+    it.kvh = (int)((unsigned)(x - first) / (unsigned)it.n);  // below n * kv_heads < 2^31
+    it.first = first + (long long)it.kvh * it.n;
+    return it;
+  };
+  const Item bi = item_of(block_f);
+  if (block_end <= bi.first + bi.n) {  // the block is inside one item
+    const int ta = (int)max(f - bi.first - kSetup, 0ll), tb = (int)(f_end - bi.first) - kSetup;
+    Acc<NT> acc;
+    acc.clear();
+    if (f < f_end && ta < tb) attend<FP8, NT>(a, bi.b, bi.kvh, ta, tb, length_of(a, bi.b, false), lane, acc);
+    acc.sum_lanes();
+    merge_block<NT>(a, sh, acc, bi.b, bi.kvh, block_f == bi.first && block_end == bi.first + bi.n, 2 * w0);
+    return;
   }
   while (f < f_end) {
-    while ((long long)prefix[b + 1] * pg.kv_heads <= f) ++b;
-    const int tiles = prefix[b + 1] - prefix[b];
-    const long long first = (long long)prefix[b] * pg.kv_heads;
-    const int kvh = (int)((f - first) / tiles);
-    const long long item = first + (long long)kvh * tiles;  // flat tile where the item begins
-    const int ta = (int)(f - item);
-    const int tb = (int)min((long long)tiles, f_end - item);
-    int len;
-    tiles_of(a, b, &len, false);
-    const int32_t* trow = pg.table + (long long)b * pg.ldt;
-
-    // page of this lane's key (tile * 32 + lane), -1 where there is none
-    auto page_at = [&](int tile) -> int {
-      const int key = tile * kTK + lane;
-      return tile < tb && key < len ? __ldg(trow + (key >> pg.log_page)) : -1;
-    };
-    auto mask_of = [&](int tile, int page) -> uint32_t {
-      const bool in = tile * kTK + lane < len;
-      const bool ok = in && page >= 0 && page < pg.num_pages;
-      if (in && !ok) report_error(kErrIndex);
-      return __ballot_sync(0xffffffffu, ok);
-    };
-    const long long head_row = (long long)kvh << pg.log_page;
-    const int pmask = (1 << pg.log_page) - 1;
-    uint4 kr[4][kKC];
-    VT vr[2][4];
-    uint32_t sc = 0;  // e4m3: this lane's key's scale bytes, key | value << 8
-
-    // rows of a tile: row x of the tile is in page shfl(page, x)
-    auto load_k = [&](int tile, int page, uint32_t mask) {
-      const int t0 = tile * kTK;
-      if (FP8) {
-        sc = 0;
-        if ((mask >> lane) & 1) {
-          const long long r = (long long)page * pg.ld_scale + head_row + ((t0 + lane) & pmask);
-          sc = (uint32_t)__ldg(pg.ks + r) | ((uint32_t)__ldg(pg.vs + r) << 8);
-        }
-      }
-      if (pg.log_page >= 5 && mask == 0xffffffffu) {
-        const long long p0 = __shfl_sync(0xffffffffu, page, 0);
-        const char* base = pg.k + p0 * pg.ld_page + (head_row + (t0 & pmask) + g) * kRow + t4 * 16;
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int c = 0; c < kKC; ++c) kr[r][c] = ld_once<uint4>(base + r * 8 * kRow + c * 64);
-      } else {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int x = g + 8 * r;
-          const long long p = __shfl_sync(0xffffffffu, page, x);
-          const char* base = pg.k + p * pg.ld_page + (head_row + ((t0 + x) & pmask)) * kRow + t4 * 16;
-#pragma unroll
-          for (int c = 0; c < kKC; ++c)
-            kr[r][c] = (mask >> x) & 1 ? ld_once<uint4>(base + c * 64) : make_uint4(0u, 0u, 0u, 0u);
-        }
-      }
-    };
-    auto load_v = [&](int tile, int page, uint32_t mask) {
-      const int t0 = tile * kTK;
-      if (pg.log_page >= 5 && mask == 0xffffffffu) {
-        const long long p0 = __shfl_sync(0xffffffffu, page, 0);
-        const char* base = pg.v + p0 * pg.ld_page + (head_row + (t0 & pmask) + 2 * t4) * kRow + g * (kRow / 8);
-#pragma unroll
-        for (int jj = 0; jj < 2; ++jj)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) vr[jj][i] = ld_once<VT>(base + (16 * jj + (i & 1) + (i >> 1) * 8) * kRow);
-      } else {
-#pragma unroll
-        for (int jj = 0; jj < 2; ++jj)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int x = 16 * jj + 2 * t4 + (i & 1) + (i >> 1) * 8;
-            const long long p = __shfl_sync(0xffffffffu, page, x);
-            const char* base = pg.v + p * pg.ld_page + (head_row + ((t0 + x) & pmask)) * kRow + g * (kRow / 8);
-            vr[jj][i] = (mask >> x) & 1 ? ld_once<VT>(base) : VT{};
-          }
-      }
-    };
-
-    int page = page_at(ta);
-    int page_next = page_at(ta + 1);
-    uint32_t mask = mask_of(ta, page);
-    load_k(ta, page, mask);
-    load_v(ta, page, mask);
-
-    // queries of the group as the B operand: head n * 8 + g, 8 (bf16) or 16 (e4m3) dims per chunk and lane
-    uint32_t qf[NT][8];
-    float qs[NT][2];  // factor of the scores of heads n * 8 + 2 t4, + 1
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int hq = n * 8 + g;
-      const __nv_bfloat16* qrow = a.q + (long long)b * a.ldq + (kvh * a.group + hq) * kHD;
-      uint4 x = make_uint4(0u, 0u, 0u, 0u), y = x;
-      if (hq < a.group) {
-        x = *reinterpret_cast<const uint4*>(qrow + (FP8 ? 16 : 8) * t4);
-        y = *reinterpret_cast<const uint4*>(qrow + (FP8 ? 16 * t4 + 8 : 32 + 8 * t4));
-      }
-      const uint32_t raw[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-      if (!FP8) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) qf[n][i] = raw[i];
-        qs[n][0] = qs[n][1] = a.scale_log2;
-      } else {
-        uint32_t top = 0;  // the row's largest magnitude, as bf16 bits
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, max(raw[i] & 0x7fffu, (raw[i] >> 16) & 0x7fffu));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // largest in [2^14, 2^15): fp16 then holds all 8 bits of whatever is above 2^-38 of it
-        const int e = min(max((int)(top >> 7), 15), 250);  // exponent field; the factor 2^(141 - e) is a normal number
-        const float up = __uint_as_float((uint32_t)(127 + 141 - e) << 23);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float2 v = bf2f(raw[i]);
-          qf[n][i] = pack_f16(v.x * up, v.y * up);
-        }
-        // lanes (g, *) hold head g's factor; this lane's score columns are heads 2 t4, 2 t4 + 1
-        qs[n][0] = a.scale_log2 / __shfl_sync(0xffffffffu, up, 8 * t4);
-        qs[n][1] = a.scale_log2 / __shfl_sync(0xffffffffu, up, 8 * t4 + 4);
-      }
-    }
-
-    float o[NT][4][4];
-    float m[NT][2], l[NT][2], mv[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
-      m[n][0] = m[n][1] = mv[n][0] = mv[n][1] = -INFINITY;
-      l[n][0] = l[n][1] = 0.f;
-    }
-
-    for (int tile = ta; tile < tb; ++tile) {
-      // S^T: keys g + 8 r by heads 2 t4 + c -> s[n][r][c]
-      float s[NT][4][2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float acc[NT][4];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-        if (FP8) {
-          const uint4 u = kr[2 * i][0], w4 = kr[2 * i + 1][0];
-          const uint32_t lo[4] = {u.x, u.y, u.z, u.w}, hi[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t af[4] = {e4m3x2_h(lo[j]), e4m3x2_h(hi[j]), e4m3x2_h(lo[j] >> 16), e4m3x2_h(hi[j] >> 16)};
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma_f16_16816(acc[n], af, qf[n][2 * j], qf[n][2 * j + 1]);
-          }
-        } else {
-#pragma unroll
-          for (int c = 0; c < kKC; ++c) {
-            const uint4 u = kr[2 * i][c], w4 = kr[2 * i + 1][c];
-            const uint32_t a0[4] = {u.x, w4.x, u.y, w4.y}, a1[4] = {u.z, w4.z, u.w, w4.w};
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              mma_bf16_16816(acc[n], a0, qf[n][4 * c], qf[n][4 * c + 1]);
-              mma_bf16_16816(acc[n], a1, qf[n][4 * c + 2], qf[n][4 * c + 3]);
-            }
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            s[n][2 * i][c] = acc[n][c] * qs[n][c];
-            s[n][2 * i + 1][c] = acc[n][2 + c] * qs[n][c];
-          }
-      }
-      float ve[4];  // log2 of the value scales
-      if (FP8) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const uint32_t x = __shfl_sync(0xffffffffu, sc, g + 8 * r);
-          const float ks = __uint_as_float((x & 0xffu) << 23);
-          ve[r] = (float)(int)((x >> 8) & 0xffu) - 127.f;
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            s[n][r][0] *= ks;
-            s[n][r][1] *= ks;
-          }
-        }
-      }
-      if (mask != 0xffffffffu) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (!((mask >> (g + 8 * r)) & 1)) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n) s[n][r][0] = s[n][r][1] = -INFINITY;
-          }
-      }
-      uint32_t mask_next = 0;
-      if (tile + 1 < tb) {
-        mask_next = mask_of(tile + 1, page_next);
-        load_k(tile + 1, page_next, mask_next);
-      }
-
-      // running maximum over the tile's 32 keys, weights, sums
-      uint32_t pb[NT][2][2];  // weights of keys (16 jj + g, + 8) for heads 2 t4, 2 t4 + 1
-      uint32_t pl[NT][2][2];  // bf16: the low parts
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float mn[2], al[2];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float mx = fmaxf(fmaxf(s[n][0][c], s[n][1][c]), fmaxf(s[n][2][c], s[n][3][c]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          mx = fmaxf(mx, m[n][c]);
-          mn[c] = mx == -INFINITY ? 0.f : mx;  // no key yet: weights 2^(-inf) = 0
-          al[c] = ex2(m[n][c] - mn[c]);
-          m[n][c] = mx;
-        }
-        float p[4][2];
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) p[r][c] = ex2(s[n][r][c] - mn[c]);
-#pragma unroll
-        for (int c = 0; c < 2; ++c) l[n][c] = l[n][c] * al[c] + ((p[0][c] + p[1][c]) + (p[2][c] + p[3][c]));
-        if (FP8) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float mx = fmaxf(fmaxf(s[n][0][c] + ve[0], s[n][1][c] + ve[1]),
-                             fmaxf(s[n][2][c] + ve[2], s[n][3][c] + ve[3]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            mx = fmaxf(mx, mv[n][c]);
-            mn[c] = mx == -INFINITY ? 0.f : mx;
-            al[c] = ex2(mv[n][c] - mn[c]);
-            mv[n][c] = mx;
-          }
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) p[r][c] = ex2(s[n][r][c] + ve[r] - mn[c]);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          o[n][i][0] *= al[0];
-          o[n][i][1] *= al[1];
-          o[n][i][2] *= al[0];
-          o[n][i][3] *= al[1];
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (FP8) {
-            pb[n][r >> 1][r & 1] = transpose8x8(pack_f16(p[r][0], p[r][1]));
-          } else {
-            const uint32_t hi = pack_bf16(p[r][0], p[r][1]);
-            const float2 back = bf2f(hi);
-            pb[n][r >> 1][r & 1] = transpose8x8(hi);
-            pl[n][r >> 1][r & 1] = transpose8x8(pack_bf16(p[r][0] - back.x, p[r][1] - back.y));
-          }
-        }
-      }
-
-      // O^T += V^T P^T: row pair i of the accumulators is dims 8 g + 2 i, 8 g + 2 i + 1
-#pragma unroll
-      for (int jj = 0; jj < 2; ++jj) {
-        uint32_t w4[4][4];  // [key][dim pair]
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          if constexpr (FP8) {
-            const uint2 u = vr[jj][x];
-            w4[x][0] = e4m3x2_h(u.x);
-            w4[x][1] = e4m3x2_h(u.x >> 16);
-            w4[x][2] = e4m3x2_h(u.y);
-            w4[x][3] = e4m3x2_h(u.y >> 16);
-          } else {
-            const uint4 u = vr[jj][x];
-            w4[x][0] = u.x;
-            w4[x][1] = u.y;
-            w4[x][2] = u.z;
-            w4[x][3] = u.w;
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t af[4] = {__byte_perm(w4[0][i], w4[1][i], 0x5410), __byte_perm(w4[0][i], w4[1][i], 0x7632),
-                                  __byte_perm(w4[2][i], w4[3][i], 0x5410), __byte_perm(w4[2][i], w4[3][i], 0x7632)};
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            if (FP8) {
-              mma_f16_16816(o[n][i], af, pb[n][jj][0], pb[n][jj][1]);
-            } else {
-              mma_bf16_16816(o[n][i], af, pb[n][jj][0], pb[n][jj][1]);
-              mma_bf16_16816(o[n][i], af, pl[n][jj][0], pl[n][jj][1]);
-            }
-          }
-        }
-      }
-      if (tile + 1 < tb) {
-        load_v(tile + 1, page_next, mask_next);
-        mask = mask_next;
-        page_next = page_at(tile + 2);
-      }
-    }
-
-    // this warp's share of the item
-    const bool whole = ta == 0 && tb == tiles;
-    const int slot = 2 * (int)w + (ta == 0 ? 1 : 0);
+    const Item it = item_of(f);
+    const long long last = min(it.first + it.n, f_end);
+    const int ta = (int)max(f - it.first - kSetup, 0ll), tb = (int)(last - it.first) - kSetup;
+    f = last;
+    if (ta >= tb) continue;  // nothing but the item's setup
+    Acc<NT> acc;
+    acc.clear();
+    attend<FP8, NT>(a, it.b, it.kvh, ta, tb, length_of(a, it.b, false), lane, acc);
+    acc.sum_lanes();
+    const bool whole = ta == 0 && tb == it.n - kSetup;
+    const long long slot = 2 * w + (ta == 0 ? 1 : 0);
+    const int g = lane >> 2, t4 = lane & 3;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float sum = l[n][c];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
         const int hq = n * 8 + 2 * t4 + c;
         if (hq >= a.group) continue;
-        const float ov[8] = {o[n][0][c], o[n][0][2 + c], o[n][1][c], o[n][1][2 + c],
-                             o[n][2][c], o[n][2][2 + c], o[n][3][c], o[n][3][2 + c]};
+        float v[8];
+        acc.dims(n, c, v);
         if (whole) {
-          float inv = sum == 0.f ? 0.f : 1.f / sum;
-          if (FP8) inv *= m[n][c] == -INFINITY ? 1.f : ex2(mv[n][c] - m[n][c]);
-          store_out8(a, b, kvh * a.group + hq, 8 * g, ov, inv);
+          store_out8(a, it.b, it.kvh * a.group + hq, 8 * g, v, acc.l[n][c] == 0.f ? 0.f : 1.f / acc.l[n][c]);
         } else {
-          const long long at = (long long)slot * a.group + hq;
+          const long long at = slot * a.group + hq;
           float4* dst = reinterpret_cast<float4*>(a.part + at * kHD + 8 * g);
-          dst[0] = make_float4(ov[0], ov[1], ov[2], ov[3]);
-          dst[1] = make_float4(ov[4], ov[5], ov[6], ov[7]);
-          if (g == 0) a.stat[at] = make_float4(m[n][c], sum, FP8 ? mv[n][c] : m[n][c], 0.f);
+          dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+          dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+          if (g == 0) a.stat[at] = make_float2(acc.m[n][c], acc.l[n][c]);
         }
       }
-    f = item + tb;
   }
 }
 
 // Adds up the partial results of the items that several warps shared, in the
-// order of those warps.  One block per (sequence, query head); warp i takes
-// every fourth partial result, lane l dims 2l and 2l + 1.
+// order of the deal.  A block inside an item left one result, in its first warp's
+// slot 0; other warps left the item they end in slot 0, the one they begin in
+// slot 1.  One block per (sequence, query head); warp i takes every fourth result,
+// lane l dims 2l and 2l + 1.
 __global__ void __launch_bounds__(128) paged_attn_join_kernel(const AttnArgs a, long long n_warps) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int heads = a.pg.kv_heads * a.group;
   const int b = blockIdx.x / heads, h = blockIdx.x - b * heads;
   const int kvh = h / a.group, hq = h - kvh * a.group;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int before = a.prefix[b], tiles = a.prefix[b + 1] - before;
-  if (tiles == 0) return;
+  const int before = a.prefix[b], shares = a.prefix[b + 1] - before;
+  if (shares == 0) return;
   const long long total = (long long)a.prefix[a.B] * a.pg.kv_heads;
-  const long long chunk = (total + n_warps - 1) / n_warps;
-  const long long first = (long long)before * a.pg.kv_heads + (long long)kvh * tiles;
-  const long long w0 = first / chunk, w1 = (first + tiles - 1) / chunk;
-  if (w0 == w1) return;  // written by that warp
-  float m = -INFINITY, mv = -INFINITY, l = 0.f, x = 0.f, y = 0.f;
-  auto add = [&](float pm, float plen, float pmv, float px, float py) {
-    const float nm = fmaxf(m, pm), nv = fmaxf(mv, pmv);
-    const float sm = nm == -INFINITY ? 0.f : nm, sv = nv == -INFINITY ? 0.f : nv;
-    l = l * ex2(m - sm) + plen * ex2(pm - sm);
-    const float f0 = ex2(mv - sv), f1 = ex2(pmv - sv);
-    x = x * f0 + px * f1;
-    y = y * f0 + py * f1;
+  const long long chunk = (total + n_warps - 1) / n_warps, span = chunk * kWarps;
+  const long long first = (long long)before * a.pg.kv_heads + (long long)kvh * shares, end = first + shares;
+  // warps with tiles of the item
+  const long long w0 = (first + kSetup) / chunk, w1 = (end - 1) / chunk;
+  // blocks inside the item: [c0, c1); each has tiles of it, having more shares than kSetup
+  static_assert(kWarps > kSetup, "a block inside an item is more than its setup");
+  const long long c0 = (first + span - 1) / span, c1 = end == total ? (end + span - 1) / span : end / span;
+  const long long inside = max(c1 - c0, 0ll), cw = w0 / kWarps;
+  if (w0 == w1 && !(cw >= c0 && cw < c1)) return;                                      // written by that warp
+  if (inside == 1 && c0 * span == first && min((c0 + 1) * span, total) == end) return;  // written by that block
+  const long long head = inside ? max(c0 * kWarps - w0, 0ll) : w1 - w0 + 1;  // warps before them (all, without them)
+  const long long tail = inside ? max(w1 + 1 - c1 * kWarps, 0ll) : 0;        // and after them
+  const long long n = head + inside + tail;
+  float m = kNoScore, l = 0.f, x = 0.f, y = 0.f;
+  auto add = [&](float2 st, float2 v) {
+    const float nm = fmaxf(m, st.x);
+    const float f0 = ex2(m - nm), f1 = ex2(st.x - nm);
+    l = l * f0 + st.y * f1;
+    x = x * f0 + v.x * f1;
+    y = y * f0 + v.y * f1;
     m = nm;
-    mv = nv;
   };
-  for (long long w = w0 + warp; w <= w1; w += 4) {
-    const long long at = (2 * w + (w == w0 ? 1 : 0)) * a.group + hq;
-    const float4 st = a.stat[at];
-    const float2 v = *reinterpret_cast<const float2*>(a.part + at * kHD + 2 * lane);
-    add(st.x, st.y, st.z, v.x, v.y);
+  auto at_of = [&](long long i) {
+    const long long w = i < head ? w0 + i : i < head + inside ? (c0 + i - head) * kWarps : c1 * kWarps + (i - head - inside);
+    const bool begins = (i < head && i == 0);
+    return (2 * w + (begins ? 1 : 0)) * a.group + hq;
+  };
+  for (long long i = warp; i < n; i += 4 * kWarps) {  // four results in flight
+    float2 st[4], v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const long long k = i + u * kWarps;
+      st[u] = make_float2(kNoScore, 0.f);
+      v[u] = make_float2(0.f, 0.f);
+      if (k < n) {
+        const long long at = at_of(k);
+        st[u] = a.stat[at];
+        v[u] = *reinterpret_cast<const float2*>(a.part + at * kHD + 2 * lane);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) add(st[u], v[u]);
   }
-  __shared__ float4 st_s[4];
-  __shared__ float2 v_s[4][32];
-  if (lane == 0) st_s[warp] = make_float4(m, l, mv, 0.f);
+  __shared__ float2 st_s[kWarps], v_s[kWarps][32];
+  if (lane == 0) st_s[warp] = make_float2(m, l);
   v_s[warp][lane] = make_float2(x, y);
   __syncthreads();
   if (warp) return;
-  for (int i = 1; i < 4; ++i) {
-    const float4 st = st_s[i];
-    add(st.x, st.y, st.z, v_s[i][lane].x, v_s[i][lane].y);
-  }
-  const float inv = l == 0.f ? 0.f : (m == -INFINITY ? 1.f : ex2(mv - m)) / l;
+  for (int i = 1; i < kWarps; ++i) add(st_s[i], v_s[i][lane]);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
   *reinterpret_cast<uint32_t*>(a.out + (long long)b * a.ldo + h * kHD + 2 * lane) = pack_bf16(x * inv, y * inv);
 }
 
@@ -779,7 +971,9 @@ int take_pages(const CdkPagedCache* c, Pages* p) {
   if (!c || !c->k || !c->v || (!c->table && c->width != 0)) return -1;
   if (c->dtype != 0 && c->dtype != 1) return -2;
   if (c->dtype == 1 && (!c->k_scale || !c->v_scale)) return -3;
-  if (c->kv_heads <= 0 || c->page_size <= 0 || (c->page_size & (c->page_size - 1)) || c->page_size > 65536) return -4;
+  if (c->kv_heads <= 0 || c->page_size <= 0 || (c->page_size & (c->page_size - 1)) || c->page_size > 65536 ||
+      (int64_t)c->kv_heads * c->page_size > (1 << 24))
+    return -4;
   if (c->num_pages <= 0 || c->num_pages > 0x7fffffff || c->width < 0 || c->width > 0x7fffffff || c->ldt < c->width)
     return -5;
   const int64_t rows = (int64_t)c->kv_heads * c->page_size;
@@ -863,19 +1057,38 @@ namespace {
 inline int64_t prefix_bytes(int64_t B) { return ((B + 1) * 4 + 15) / 16 * 16; }
 
 template <bool FP8, int NT>
-cudaError_t launch_attn(const AttnArgs& a, unsigned grid, int smem, cudaStream_t st) {
+cudaError_t launch_attn(const AttnArgs& a, long long max_tiles, cudaStream_t st) {
+  const long long items = (long long)a.B * a.pg.kv_heads;
+  if (max_tiles <= kItemTiles) {
+    paged_attn_item_kernel<FP8, NT><<<(unsigned)items, kAttnThreads, shared_bytes(a.group), st>>>(a);
+    return cudaGetLastError();
+  }
   static bool done[64] = {false};
   int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || dev < 0 || dev >= 64) return e != cudaSuccess ? e : cudaErrorInvalidDevice;
   if (!done[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(paged_attn_kernel<FP8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)prefix_bytes(kMaxSeqs));
+    e = cudaFuncSetAttribute(paged_attn_kernel<FP8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)prefix_bytes(kMaxSeqs) + shared_bytes(kMaxGroup));
     if (e != cudaSuccess) return e;
     done[dev] = true;
   }
-  paged_attn_kernel<FP8, NT><<<grid, kAttnThreads, smem, st>>>(a);
-  return cudaGetLastError();
+  // no more warps than tiles that the tables can hold: one tile is the smallest share
+  const long long bound = max_tiles * items;
+  const unsigned grid = (unsigned)(bound >= kAttnWarps ? kAttnBlocks : (bound + kWarps - 1) / kWarps);
+  paged_attn_kernel<FP8, NT><<<grid, kAttnThreads, (int)prefix_bytes(a.B) + shared_bytes(a.group), st>>>(a);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(items * a.group));
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];  // set up while the first kernel drains; it waits for it before its first load
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_attn_join_kernel, (const AttnArgs)a, (long long)grid * kWarps);
 }
 }  // namespace
 
@@ -897,8 +1110,10 @@ extern "C" int cdk_paged_attn(const void* q, int64_t ldq, const CdkPagedCache* c
   if (!workspace || workspace_bytes < need || !al16(workspace)) return -12;
   if (ldq < H * kHD || ldq % 8 || ldo < H * kHD || ldo % 8 || !al16(q) || !al16(out)) return -13;
   if (!(scale == scale)) return -14;
-  const int64_t tiles = ((a.pg.width << a.pg.log_page) + kTK - 1) / kTK;  // per item, at most
-  if (tiles >= (1ll << 31) / kTK || tiles > ((1ll << 31) - 1) / B) return -15;
+  a.tile = cache->dtype == 1 ? tile_keys<true>() : tile_keys<false>();
+  const int64_t keys = a.pg.width << a.pg.log_page, tiles = (keys + a.tile - 1) / a.tile;  // per item, at most
+  if (keys >= (1ll << 31) - 64 || (tiles + kSetup) * a.pg.kv_heads > ((1ll << 31) - 1) / B)
+    return -15;
   a.q = reinterpret_cast<const __nv_bfloat16*>(q);
   a.ldq = ldq;
   a.B = (int)B;
@@ -909,28 +1124,10 @@ extern "C" int cdk_paged_attn(const void* q, int64_t ldq, const CdkPagedCache* c
   a.scale_log2 = scale * 1.4426950408889634f;
   char* ws = static_cast<char*>(workspace);
   a.prefix = reinterpret_cast<int32_t*>(ws);
-  a.stat = reinterpret_cast<float4*>(ws + prefix_bytes(B));
+  a.stat = reinterpret_cast<float2*>(ws + prefix_bytes(B));
   a.part = reinterpret_cast<float*>(ws + prefix_bytes(B) + (int64_t)kSlots * a.group * 16);
   auto st = reinterpret_cast<cudaStream_t>(stream);
-  // no more warps than tiles that the tables can hold; one tile per warp is then the smallest share
-  const int64_t bound = tiles * B * a.pg.kv_heads, wpb = kAttnThreads / 32;
-  const unsigned grid = (unsigned)(bound >= kAttnWarps ? kAttnBlocks : (bound + wpb - 1) / wpb + (bound == 0));
-  const int smem = (int)prefix_bytes(B);
-  cudaError_t e;
-  if (cache->dtype == 1) e = a.group <= 8 ? launch_attn<true, 1>(a, grid, smem, st) : launch_attn<true, 2>(a, grid, smem, st);
-  else e = a.group <= 8 ? launch_attn<false, 1>(a, grid, smem, st) : launch_attn<false, 2>(a, grid, smem, st);
-  if (e != cudaSuccess) return (int)e;
-  if (tiles <= 1) return 0;  // an item of one tile is never shared
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(B * H));
-  cfg.blockDim = dim3(128);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];  // set up while the first kernel drains; it waits for it before its first load
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const long long n_warps = (long long)grid * wpb;
-  e = cudaLaunchKernelEx(&cfg, paged_attn_join_kernel, (const AttnArgs)a, n_warps);
-  return e == cudaSuccess ? 0 : (int)e;
+  if (cache->dtype == 1)
+    return (int)(a.group <= 8 ? launch_attn<true, 1>(a, tiles, st) : launch_attn<true, 2>(a, tiles, st));
+  return (int)(a.group <= 8 ? launch_attn<false, 1>(a, tiles, st) : launch_attn<false, 2>(a, tiles, st));
 }
