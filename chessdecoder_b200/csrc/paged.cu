@@ -222,8 +222,8 @@ __global__ void __launch_bounds__(256)
 // it follows the maximum, but only when a score passes it by 8 (weights stay
 // below 2^8), so that most tiles need no exchange between lanes and no rescaling.
 //
-// Work.  The keys of one (sequence, kv head) item are cut into tiles of 32 (bf16)
-// or 64 (e4m3).  Where the tables hold few tiles per item, a block takes an item,
+// Work.  The keys of one (sequence, kv head) item are cut into tiles of 32.
+// Where the tables hold few tiles per item, a block takes an item,
 // its four warps a quarter of the tiles each.  Otherwise the tiles of all items,
 // in the order (sequence, head, tile), are dealt to the grid's warps in equal
 // contiguous runs, whatever the lengths; an item counts kSetup tiles more than it
@@ -251,6 +251,7 @@ __global__ void __launch_bounds__(256)
 // sum of the w_j alone reaches 2^(8 - e_j); e_j below -96 counts as -96 for m (a
 // row of zeros has the smallest scale), which only values below 448 * 2^-96 feel.
 // ---------------------------------------------------------------------------
+constexpr int kTK = 32;             // keys per tile
 constexpr int kAttnThreads = 128;   // 4 warps; 128 registers: 4 blocks per SM
 constexpr int kWarps = kAttnThreads / 32;
 constexpr int kAttnBlocks = 148 * 4;
@@ -266,29 +267,17 @@ constexpr int kItemTiles = 16;
 // first rows come one after the other.
 constexpr int kSetup = 2;
 
-template <bool FP8>
-__host__ __device__ constexpr int tile_keys() { return FP8 ? 32 : 32; }
-
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
-template <typename T>
-__device__ __forceinline__ T ld_once(const char* p);  // read once: no place in L1
-template <>
-__device__ __forceinline__ uint4 ld_once<uint4>(const char* p) {
+__device__ __forceinline__ uint4 ld_once(const char* p) {  // read once: no place in L1
   uint4 v;
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "l"(p));
-  return v;
-}
-template <>
-__device__ __forceinline__ uint2 ld_once<uint2>(const char* p) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
   return v;
 }
 
@@ -305,9 +294,10 @@ __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint32_t e4m3x2_h(uint32_t w) {  // low 16 bits: two codes -> two fp16 (exact)
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
-  return (uint32_t)h.x | ((uint32_t)h.y << 16);
+__device__ __forceinline__ void e4m3x4_h(uint32_t w, uint32_t& lo, uint32_t& hi) {  // four codes -> fp16 (exact)
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
 }
 
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
@@ -324,7 +314,6 @@ struct AttnArgs {
   __nv_bfloat16* out;
   long long ldo;
   float scale_log2;
-  int tile;         // keys per tile
   int32_t* prefix;  // workspace: [B + 1] shares of the deal before each sequence, per kv head
   float2* stat;     // workspace: [kSlots][group] (m, l)
   float* part;      // workspace: [kSlots][group][64]
@@ -341,9 +330,8 @@ __device__ __forceinline__ int length_of(const AttnArgs& a, int b, bool report) 
 }
 
 // Shares of the deal of one item: its tiles and kSetup, nothing for an empty one.
-template <int KT>
 __device__ __forceinline__ int shares_of(int len) {
-  return len > 0 ? (len + KT - 1) / KT + kSetup : 0;
+  return len > 0 ? (len + kTK - 1) / kTK + kSetup : 0;
 }
 
 // Writes 8 dims of the output of one (sequence, head).
@@ -385,337 +373,450 @@ struct Acc {
   }
 };
 
-// Tiles [ta, tb) of one item: acc over its keys below len.
-template <bool FP8, int NT>
-__device__ __forceinline__ void attend(const AttnArgs& a, int b, int kvh, int ta, int tb, int len, int lane,
-                                       Acc<NT>& acc) {
-  constexpr int kRow = FP8 ? kHD : 2 * kHD;  // bytes of a cached row
-  constexpr int kKC = FP8 ? 1 : 2;           // 16-byte chunks of a key row per lane
-  constexpr int KT = tile_keys<FP8>(), HV = KT / 32, R = KT / 8, J = KT / 16;
-  using VT = typename std::conditional<FP8, uint2, uint4>::type;
+// Pages of this lane's key of a tile (key tile * 32 + lane); -1 past the end.
+__device__ __forceinline__ int page_of_key(const AttnArgs& a, const int32_t* trow, int tile, int tb, int len,
+                                           int lane) {
+  const int key = tile * kTK + lane;
+  return tile < tb && key < len ? __ldg(trow + (key >> a.pg.log_page)) : -1;
+}
+// Which of a tile's keys count: inside the length, on a page that there is.
+__device__ __forceinline__ uint32_t mask_of_tile(const AttnArgs& a, int tile, int page, int len, int lane) {
+  const bool ok = (unsigned)page < (unsigned)a.pg.num_pages;
+  const uint32_t mask = __ballot_sync(0xffffffffu, ok);
+  if (mask != 0xffffffffu && !ok && tile * kTK + lane < len) report_error(kErrIndex);
+  return mask;
+}
+
+// The reference follows the scores of a tile where one passes it; mx: this lane's
+// largest per column.
+template <int NT>
+__device__ __forceinline__ void follow(Acc<NT>& acc, const float (&mx)[NT][2]) {
+  bool pass = false;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) pass |= mx[n][0] > acc.m[n][0] + kSlack || mx[n][1] > acc.m[n][1] + kSlack;
+  if (!__any_sync(0xffffffffu, pass)) return;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float x = mx[n][c];
+      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+      x = fmaxf(x, acc.m[n][c]);
+      const float al = ex2(acc.m[n][c] - x);
+      acc.m[n][c] = x;
+      acc.l[n][c] *= al;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        acc.o[n][i][c] *= al;
+        acc.o[n][i][2 + c] *= al;
+      }
+    }
+}
+
+// Tiles [ta, tb) of one item on bf16 pages: acc over its keys below len.
+template <int NT>
+__device__ __forceinline__ void attend_bf16(const AttnArgs& a, int b, int kvh, int ta, int tb, int len, int lane,
+                                            Acc<NT>& acc) {
+  constexpr int kRow = 2 * kHD;  // bytes of a cached row
   const Pages& pg = a.pg;
   const int g = lane >> 2, t4 = lane & 3;
   const int32_t* trow = pg.table + (long long)b * pg.ldt;
   const int head_row = kvh << pg.log_page;
   const int pmask = (1 << pg.log_page) - 1;
 
-  // pages of this lane's keys (tile * KT + 32 x + lane); what is not there is masked
-  auto pages_at = [&](int tile, int (&page)[HV]) {
+  uint4 kr[4][2];  // rows g + 8 r, chunks t4 and 4 + t4
+  uint4 vr[2][4];  // rows 16 jj + 2 t4 + {0, 1, 8, 9}, chunk g
+  auto load_k = [&](int tile, int page, uint32_t mask) {
+    const int t0 = tile * kTK;
+    if (pg.log_page >= 5 && mask == 0xffffffffu) {  // 32 rows in a row in one page
+      const long long p0 = __shfl_sync(0xffffffffu, page, 0);
+      const char* base = pg.k + p0 * pg.ld_page + (long long)(head_row + (t0 & pmask) + g) * kRow + t4 * 16;
 #pragma unroll
-    for (int x = 0; x < HV; ++x) {
-      const int key = tile * KT + 32 * x + lane;
-      page[x] = tile < tb && key < len ? __ldg(trow + (key >> pg.log_page)) : -1;
-    }
-  };
-  auto masks_of = [&](int tile, const int (&page)[HV], uint32_t (&mask)[HV]) {
+      for (int r = 0; r < 4; ++r)
 #pragma unroll
-    for (int x = 0; x < HV; ++x) {
-      const bool ok = (unsigned)page[x] < (unsigned)pg.num_pages;
-      mask[x] = __ballot_sync(0xffffffffu, ok);
-      if (mask[x] != 0xffffffffu && !ok && tile * KT + 32 * x + lane < len) report_error(kErrIndex);
-    }
-  };
-  auto all_of = [&](const uint32_t (&mask)[HV]) {
-    bool f = true;
-#pragma unroll
-    for (int x = 0; x < HV; ++x) f = f && mask[x] == 0xffffffffu;
-    return f;
-  };
-
-  uint4 kr[R][kKC];
-  VT vr[J][4];
-  uint32_t sc[HV];  // e4m3: scale bytes of this lane's keys, key | value << 8
-  auto load_k = [&](int tile, const int (&page)[HV], const uint32_t (&mask)[HV], bool full) {
-    const int t0 = tile * KT;
-    if (FP8) {
-#pragma unroll
-      for (int x = 0; x < HV; ++x) {
-        sc[x] = 0;
-        if ((mask[x] >> lane) & 1) {
-          const long long r = (long long)page[x] * pg.ld_scale + head_row + ((t0 + 32 * x + lane) & pmask);
-          sc[x] = (uint32_t)__ldg(pg.ks + r) | ((uint32_t)__ldg(pg.vs + r) << 8);
-        }
-      }
-    }
-    if (pg.log_page >= 5 && full) {  // 32 rows in a row in one page
-#pragma unroll
-      for (int x = 0; x < HV; ++x) {
-        const long long p0 = __shfl_sync(0xffffffffu, page[x], 0);
-        const char* base = pg.k + p0 * pg.ld_page + (long long)(head_row + ((t0 + 32 * x) & pmask) + g) * kRow + t4 * 16;
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int c = 0; c < kKC; ++c) kr[4 * x + r][c] = ld_once<uint4>(base + r * 8 * kRow + c * 64);
-      }
+        for (int c = 0; c < 2; ++c) kr[r][c] = ld_once(base + r * 8 * kRow + c * 64);
     } else {
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const int y = g + 8 * (r & 3);  // row within the half r / 4
-        const long long p = __shfl_sync(0xffffffffu, page[r >> 2], y);
-        const char* base = pg.k + p * pg.ld_page + (long long)(head_row + ((t0 + 32 * (r >> 2) + y) & pmask)) * kRow + t4 * 16;
+      for (int r = 0; r < 4; ++r) {
+        const int y = g + 8 * r;
+        const long long p = __shfl_sync(0xffffffffu, page, y);
+        const char* base = pg.k + p * pg.ld_page + (long long)(head_row + ((t0 + y) & pmask)) * kRow + t4 * 16;
 #pragma unroll
-        for (int c = 0; c < kKC; ++c)
-          kr[r][c] = (mask[r >> 2] >> y) & 1 ? ld_once<uint4>(base + c * 64) : make_uint4(0u, 0u, 0u, 0u);
+        for (int c = 0; c < 2; ++c) kr[r][c] = (mask >> y) & 1 ? ld_once(base + c * 64) : make_uint4(0u, 0u, 0u, 0u);
       }
     }
   };
-  auto load_v = [&](int tile, const int (&page)[HV], const uint32_t (&mask)[HV], bool full) {
-    const int t0 = tile * KT;
-    if (pg.log_page >= 5 && full) {
+  auto load_v = [&](int tile, int page, uint32_t mask) {
+    const int t0 = tile * kTK;
+    if (pg.log_page >= 5 && mask == 0xffffffffu) {
+      const long long p0 = __shfl_sync(0xffffffffu, page, 0);
+      const char* base = pg.v + p0 * pg.ld_page + (long long)(head_row + (t0 & pmask) + 2 * t4) * kRow + g * 16;
 #pragma unroll
-      for (int x = 0; x < HV; ++x) {
-        const long long p0 = __shfl_sync(0xffffffffu, page[x], 0);
-        const char* base =
-            pg.v + p0 * pg.ld_page + (long long)(head_row + ((t0 + 32 * x) & pmask) + 2 * t4) * kRow + g * (kRow / 8);
+      for (int jj = 0; jj < 2; ++jj)
 #pragma unroll
-        for (int jj = 0; jj < 2; ++jj)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) vr[2 * x + jj][i] = ld_once<VT>(base + (16 * jj + (i & 1) + (i >> 1) * 8) * kRow);
-      }
+        for (int i = 0; i < 4; ++i) vr[jj][i] = ld_once(base + (16 * jj + (i & 1) + (i >> 1) * 8) * kRow);
     } else {
 #pragma unroll
-      for (int jj = 0; jj < J; ++jj)
+      for (int jj = 0; jj < 2; ++jj)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int y = 16 * (jj & 1) + 2 * t4 + (i & 1) + (i >> 1) * 8;
-          const long long p = __shfl_sync(0xffffffffu, page[jj >> 1], y);
-          const char* base =
-              pg.v + p * pg.ld_page + (long long)(head_row + ((t0 + 32 * (jj >> 1) + y) & pmask)) * kRow + g * (kRow / 8);
-          vr[jj][i] = (mask[jj >> 1] >> y) & 1 ? ld_once<VT>(base) : VT{};
+          const int y = 16 * jj + 2 * t4 + (i & 1) + (i >> 1) * 8;
+          const long long p = __shfl_sync(0xffffffffu, page, y);
+          const char* base = pg.v + p * pg.ld_page + (long long)(head_row + ((t0 + y) & pmask)) * kRow + g * 16;
+          vr[jj][i] = (mask >> y) & 1 ? ld_once(base) : make_uint4(0u, 0u, 0u, 0u);
         }
     }
   };
 
-  int page[HV];
-  uint32_t mask[HV];
-  pages_at(ta, page);
-  masks_of(ta, page, mask);
-  bool full = all_of(mask);
-  load_k(ta, page, mask, full);
-  load_v(ta, page, mask, full);
-  pages_at(ta + 1, page);
+  int page = page_of_key(a, trow, ta, tb, len, lane);
+  uint32_t mask = mask_of_tile(a, ta, page, len, lane);
+  load_k(ta, page, mask);
+  load_v(ta, page, mask);
+  page = page_of_key(a, trow, ta + 1, tb, len, lane);
 
-  // queries of the group as the B operand: head 8 n + g, 8 (bf16) or 16 (e4m3) dims per chunk and lane
+  // queries of the group as the B operand: head 8 n + g, its chunks t4 and 4 + t4
   uint32_t qf[NT][8];
-  float qs[NT][2];  // factor of the scores of heads 8 n + 2 t4, + 1
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int hq = n * 8 + g;
     const __nv_bfloat16* qrow = a.q + (long long)b * a.ldq + (kvh * a.group + hq) * kHD;
     uint4 x = make_uint4(0u, 0u, 0u, 0u), y = x;
     if (hq < a.group) {
-      x = *reinterpret_cast<const uint4*>(qrow + (FP8 ? 16 : 8) * t4);
-      y = *reinterpret_cast<const uint4*>(qrow + (FP8 ? 16 * t4 + 8 : 32 + 8 * t4));
+      x = *reinterpret_cast<const uint4*>(qrow + 8 * t4);
+      y = *reinterpret_cast<const uint4*>(qrow + 32 + 8 * t4);
     }
-    const uint32_t raw[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-    if (!FP8) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) qf[n][i] = raw[i];
-      qs[n][0] = qs[n][1] = a.scale_log2;
-    } else {
-      uint32_t top = 0;  // the row's largest magnitude, as bf16 bits
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, max(raw[i] & 0x7fffu, (raw[i] >> 16) & 0x7fffu));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // largest in [2^14, 2^15): fp16 then holds all 8 bits of whatever is above 2^-31 of it
-      const int e = min(max((int)(top >> 7), 15), 250);  // exponent field; the factor 2^(141 - e) is a normal number
-      const float up = __uint_as_float((uint32_t)(127 + 141 - e) << 23);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float2 v = bf2f(raw[i]);
-        qf[n][i] = pack_f16(v.x * up, v.y * up);
-      }
-      // lanes (g, *) hold head g's factor; this lane's score columns are heads 2 t4, 2 t4 + 1
-      qs[n][0] = a.scale_log2 / __shfl_sync(0xffffffffu, up, 8 * t4);
-      qs[n][1] = a.scale_log2 / __shfl_sync(0xffffffffu, up, 8 * t4 + 4);
-    }
+    qf[n][0] = x.x, qf[n][1] = x.y, qf[n][2] = x.z, qf[n][3] = x.w;
+    qf[n][4] = y.x, qf[n][5] = y.y, qf[n][6] = y.z, qf[n][7] = y.w;
   }
 
 #pragma unroll 1
   for (int tile = ta; tile < tb; ++tile) {
-    int page2[HV];  // the table two tiles ahead: there when the next tile's scores are done
-    pages_at(tile + 2, page2);
+    // the table two tiles ahead: there when the next tile's scores are done
+    const int page2 = page_of_key(a, trow, tile + 2, tb, len, lane);
     // S^T: keys g + 8 r by heads 2 t4 + c -> s[n][r][c]
-    float s[NT][R][2];
+    float s[NT][4][2];
 #pragma unroll
-    for (int i = 0; i < R / 2; ++i) {
+    for (int i = 0; i < 2; ++i) {
       float d[NT][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n) d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.f;
-      if (FP8) {
-        const uint4 u = kr[2 * i][0], w4 = kr[2 * i + 1][0];
-        const uint32_t lo[4] = {u.x, u.y, u.z, u.w}, hi[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t af[4] = {e4m3x2_h(lo[j]), e4m3x2_h(hi[j]), e4m3x2_h(lo[j] >> 16), e4m3x2_h(hi[j] >> 16)};
+      for (int c = 0; c < 2; ++c) {
+        const uint4 u = kr[2 * i][c], w4 = kr[2 * i + 1][c];
+        const uint32_t a0[4] = {u.x, w4.x, u.y, w4.y}, a1[4] = {u.z, w4.z, u.w, w4.w};
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_f16_16816(d[n], af, qf[n][2 * j], qf[n][2 * j + 1]);
-        }
-      } else {
-#pragma unroll
-        for (int c = 0; c < kKC; ++c) {
-          const uint4 u = kr[2 * i][c], w4 = kr[2 * i + 1][c];
-          const uint32_t a0[4] = {u.x, w4.x, u.y, w4.y}, a1[4] = {u.z, w4.z, u.w, w4.w};
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            mma_bf16_16816(d[n], a0, qf[n][4 * c], qf[n][4 * c + 1]);
-            mma_bf16_16816(d[n], a1, qf[n][4 * c + 2], qf[n][4 * c + 3]);
-          }
+        for (int n = 0; n < NT; ++n) {
+          mma_bf16_16816(d[n], a0, qf[n][4 * c], qf[n][4 * c + 1]);
+          mma_bf16_16816(d[n], a1, qf[n][4 * c + 2], qf[n][4 * c + 3]);
         }
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          s[n][2 * i][c] = d[n][c] * qs[n][c];
-          s[n][2 * i + 1][c] = d[n][2 + c] * qs[n][c];
+          s[n][2 * i][c] = d[n][c] * a.scale_log2;
+          s[n][2 * i + 1][c] = d[n][2 + c] * a.scale_log2;
         }
     }
-    float vs[R];  // value scales
-    if (FP8) {
+    if (mask != 0xffffffffu) {
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const uint32_t x = __shfl_sync(0xffffffffu, sc[r >> 2], g + 8 * (r & 3));
-        const float ks = __uint_as_float((x & 0xffu) << 23);
-        vs[r] = __uint_as_float((x & 0xff00u) << 15);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          s[n][r][0] *= ks;
-          s[n][r][1] *= ks;
-        }
-      }
-    }
-    if (!full) {
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-        if (!((mask[r >> 2] >> (g + 8 * (r & 3))) & 1)) {
+      for (int r = 0; r < 4; ++r)
+        if (!((mask >> (g + 8 * r)) & 1)) {
 #pragma unroll
           for (int n = 0; n < NT; ++n) s[n][r][0] = s[n][r][1] = -INFINITY;
         }
     }
     if (tile + 1 < tb) {
-      masks_of(tile + 1, page, mask);
-      full = all_of(mask);
-      load_k(tile + 1, page, mask, full);
+      mask = mask_of_tile(a, tile + 1, page, len, lane);
+      load_k(tile + 1, page, mask);
     }
-
-    // does a score pass the reference?
     float mx[NT][2];
-    bool pass = false;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float x = -INFINITY;
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-          x = fmaxf(x, FP8 ? s[n][r][c] + fmaxf((float)(int)(__float_as_uint(vs[r]) >> 23) - 127.f, -96.f) : s[n][r][c]);
-        mx[n][c] = x;
-        pass |= x > acc.m[n][c] + kSlack;
-      }
-    if (__any_sync(0xffffffffu, pass)) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float x = mx[n][c];
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          x = fmaxf(x, acc.m[n][c]);
-          const float al = ex2(acc.m[n][c] - x);
-          acc.m[n][c] = x;
-          acc.l[n][c] *= al;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            acc.o[n][i][c] *= al;
-            acc.o[n][i][2 + c] *= al;
-          }
-        }
-    }
+      for (int c = 0; c < 2; ++c) mx[n][c] = fmaxf(fmaxf(s[n][0][c], s[n][1][c]), fmaxf(s[n][2][c], s[n][3][c]));
+    follow<NT>(acc, mx);
 
-    // weights of keys (16 jj + g, + 8) for heads 2 t4, 2 t4 + 1, as the B operand
-    uint32_t pb[NT][J][2], pl[NT][J][2];  // pl: bf16's low parts
+    // weights of keys (16 jj + g, + 8) for heads 2 t4, 2 t4 + 1, as the B operand: high and low parts
+    uint32_t ph[NT][2][2], pl[NT][2][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float sum[2] = {0.f, 0.f};
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        float p0 = ex2(s[n][r][0] - acc.m[n][0]), p1 = ex2(s[n][r][1] - acc.m[n][1]);
-        sum[0] += p0;
-        sum[1] += p1;
-        if (FP8) {
-          pb[n][r >> 1][r & 1] = transpose8x8(pack_f16(p0 * vs[r], p1 * vs[r]));
-        } else {
-          const uint32_t hi = pack_bf16(p0, p1);
-          const float2 back = bf2f(hi);
-          pb[n][r >> 1][r & 1] = transpose8x8(hi);
-          pl[n][r >> 1][r & 1] = transpose8x8(pack_bf16(p0 - back.x, p1 - back.y));
-        }
+      for (int r = 0; r < 4; ++r) {
+        const float p0 = ex2(s[n][r][0] - acc.m[n][0]), p1 = ex2(s[n][r][1] - acc.m[n][1]);
+        acc.l[n][0] += p0;
+        acc.l[n][1] += p1;
+        const uint32_t hi = pack_bf16(p0, p1);
+        const float2 back = bf2f(hi);
+        ph[n][r >> 1][r & 1] = transpose8x8(hi);
+        pl[n][r >> 1][r & 1] = transpose8x8(pack_bf16(p0 - back.x, p1 - back.y));
       }
-      acc.l[n][0] += sum[0];
-      acc.l[n][1] += sum[1];
-    }
 
     // O^T += V^T P^T: the A operand's rows g and g + 8 of product i are dims 8 g + 2 i and 8 g + 2 i + 1
 #pragma unroll
-    for (int jj = 0; jj < J; ++jj) {
-      if constexpr (FP8) {
-        // bytes of two keys interleaved first: one permute gives two dims of both
-        uint32_t lo[4], hi[4];  // keys 2 t4, + 1 and 2 t4 + 8, + 9: [dim pair] = (d of both, d + 1 of both)
+    for (int jj = 0; jj < 2; ++jj) {
+      const uint32_t w4[4][4] = {{vr[jj][0].x, vr[jj][0].y, vr[jj][0].z, vr[jj][0].w},
+                                 {vr[jj][1].x, vr[jj][1].y, vr[jj][1].z, vr[jj][1].w},
+                                 {vr[jj][2].x, vr[jj][2].y, vr[jj][2].z, vr[jj][2].w},
+                                 {vr[jj][3].x, vr[jj][3].y, vr[jj][3].z, vr[jj][3].w}};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t k0 = i < 2 ? vr[jj][0].x : vr[jj][0].y, k1 = i < 2 ? vr[jj][1].x : vr[jj][1].y;
-          const uint32_t k2 = i < 2 ? vr[jj][2].x : vr[jj][2].y, k3 = i < 2 ? vr[jj][3].x : vr[jj][3].y;
-          const uint32_t sel = (i & 1) ? 0x7362u : 0x5140u;
-          lo[i] = __byte_perm(k0, k1, sel);
-          hi[i] = __byte_perm(k2, k3, sel);
-        }
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t af[4] = {__byte_perm(w4[0][i], w4[1][i], 0x5410), __byte_perm(w4[0][i], w4[1][i], 0x7632),
+                                __byte_perm(w4[2][i], w4[3][i], 0x5410), __byte_perm(w4[2][i], w4[3][i], 0x7632)};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t af[4] = {e4m3x2_h(lo[i]), e4m3x2_h(lo[i] >> 16), e4m3x2_h(hi[i]), e4m3x2_h(hi[i] >> 16)};
-#pragma unroll
-          for (int n = 0; n < NT; ++n) mma_f16_16816(acc.o[n][i], af, pb[n][jj][0], pb[n][jj][1]);
-        }
-      } else {
-        const uint32_t w4[4][4] = {{vr[jj][0].x, vr[jj][0].y, vr[jj][0].z, vr[jj][0].w},
-                                   {vr[jj][1].x, vr[jj][1].y, vr[jj][1].z, vr[jj][1].w},
-                                   {vr[jj][2].x, vr[jj][2].y, vr[jj][2].z, vr[jj][2].w},
-                                   {vr[jj][3].x, vr[jj][3].y, vr[jj][3].z, vr[jj][3].w}};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t af[4] = {__byte_perm(w4[0][i], w4[1][i], 0x5410), __byte_perm(w4[0][i], w4[1][i], 0x7632),
-                                  __byte_perm(w4[2][i], w4[3][i], 0x5410), __byte_perm(w4[2][i], w4[3][i], 0x7632)};
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            mma_bf16_16816(acc.o[n][i], af, pb[n][jj][0], pb[n][jj][1]);
-            mma_bf16_16816(acc.o[n][i], af, pl[n][jj][0], pl[n][jj][1]);
-          }
+        for (int n = 0; n < NT; ++n) {
+          mma_bf16_16816(acc.o[n][i], af, ph[n][jj][0], ph[n][jj][1]);
+          mma_bf16_16816(acc.o[n][i], af, pl[n][jj][0], pl[n][jj][1]);
         }
       }
     }
     if (tile + 1 < tb) {
-      load_v(tile + 1, page, mask, full);
-#pragma unroll
-      for (int x = 0; x < HV; ++x) page[x] = page2[x];
+      load_v(tile + 1, page, mask);
+      page = page2;
     }
   }
 }
 
-// Shared memory of a block, sized by the group: what a block does not take stays
-// L1, where the loads in flight land.
-struct AttnShared {
-  float* o;      // [kWarps][group][64]
-  float2* stat;  // [kWarps][group]
-  int* prefix;   // [B + 1]
-  __device__ __forceinline__ AttnShared(char* p, int group) {
-    o = reinterpret_cast<float*>(p);
-    stat = reinterpret_cast<float2*>(o + kWarps * group * kHD);
-    prefix = reinterpret_cast<int*>(stat + kWarps * group);
+// The same on e4m3 pages.  A tile is half the bytes, so its loads have to be twice
+// as far ahead: they go through a ring of kStages tiles per warp in shared memory
+// (cp.async, rows that do not count filled with zeros), two tiles ahead.
+//
+// Stage: 32 key rows, then 32 value rows, of 64 bytes; two rows to a 128-byte
+// line, whose 16-byte chunks are swapped around by twice the line's number, so
+// that both the fragments' reads (8 key rows by one chunk; 4 value rows, every
+// second one, by half a row) and the copies touch every bank once.
+constexpr int kStages = 3;
+constexpr int kStageBytes = 2 * kTK * kHD;
+
+// Offset of chunk c of a row in its stage.  Rows 8 apart are 512 bytes apart.
+__device__ __forceinline__ int chunk_at(int row, int c) {
+  return (row >> 1) * 128 + (((((row & 1) << 2) | c) ^ (((row >> 1) & 3) << 1)) << 4);
+}
+
+template <int NT>
+__device__ __forceinline__ void attend_e4m3(const AttnArgs& a, int b, int kvh, int ta, int tb, int len, int lane,
+                                            char* ring, Acc<NT>& acc) {
+  const Pages& pg = a.pg;
+  const int g = lane >> 2, t4 = lane & 3;
+  const int32_t* trow = pg.table + (long long)b * pg.ldt;
+  const int head_row = kvh << pg.log_page;
+  const int pmask = (1 << pg.log_page) - 1;
+  const int k_at = chunk_at(g, t4);  // this lane's chunk of key row g (rows g + 8 i: 512 i further)
+  // its half chunk of value row 2 t4; row 2 t4 + 1 is in the same line, four chunks on or back
+  const int v_at = kTK * kHD + chunk_at(2 * t4, g >> 1) + (g & 1) * 8;
+  const uint32_t dst0 = smem_u32(ring) + k_at;
+
+  // Starts the copies of a tile and loads its keys' scale bytes.
+  auto fetch = [&](int tile, int page, int stage, uint32_t& mask, uint32_t& sk, uint32_t& sv) {
+    mask = sk = sv = 0;
+    if (tile < tb) {
+      const int t0 = tile * kTK;
+      mask = mask_of_tile(a, tile, page, len, lane);
+      if ((mask >> lane) & 1) {
+        const long long r = (long long)page * pg.ld_scale + head_row + ((t0 + lane) & pmask);
+        sk = __ldg(pg.ks + r);
+        sv = __ldg(pg.vs + r);
+      }
+      const uint32_t dst = dst0 + stage * kStageBytes;
+      if (pg.log_page >= 5 && mask == 0xffffffffu) {  // 32 rows in a row in one page
+        const long long p0 = __shfl_sync(0xffffffffu, page, 0);
+        const long long at = p0 * pg.ld_page + (long long)(head_row + (t0 & pmask) + g) * kHD + t4 * 16;
+        const char* ks = pg.k + at;
+        const char* vs = pg.v + at;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          cp_async_16(dst + i * 512, ks + i * 8 * kHD);
+          cp_async_16(dst + kTK * kHD + i * 512, vs + i * 8 * kHD);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int y = g + 8 * i;
+          const long long p = __shfl_sync(0xffffffffu, page, y);
+          const bool ok = (mask >> y) & 1;
+          const long long at = ok ? p * pg.ld_page + (long long)(head_row + ((t0 + y) & pmask)) * kHD + t4 * 16 : 0;
+          cp_async_16_zfill(dst + i * 512, pg.k + at, ok);
+          cp_async_16_zfill(dst + kTK * kHD + i * 512, pg.v + at, ok);
+        }
+      }
+    }
+    cp_async_commit();
+  };
+
+  __syncwarp();  // every lane is done with the ring
+  uint32_t mask, mask1, mask2, sk, sv, sk1, sv1, sk2, sv2;
+  {
+    const int p0 = page_of_key(a, trow, ta, tb, len, lane), p1 = page_of_key(a, trow, ta + 1, tb, len, lane);
+    fetch(ta, p0, 0, mask, sk, sv);
+    fetch(ta + 1, p1, 1, mask1, sk1, sv1);
   }
+  int page = page_of_key(a, trow, ta + 2, tb, len, lane);
+  int stage = 0;
+  uint32_t sc = sk | (sv << 8);  // scale bytes of this tile, key | value << 8
+
+  // queries as the B operand: head 8 n + g, 16 dims from 16 t4, scaled to fp16
+  uint32_t qf[NT][8];
+  float qs[NT][2];  // factor of the scores of heads 8 n + 2 t4, + 1
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int hq = n * 8 + g;
+    const __nv_bfloat16* qrow = a.q + (long long)b * a.ldq + (kvh * a.group + hq) * kHD + 16 * t4;
+    uint4 x = make_uint4(0u, 0u, 0u, 0u), y = x;
+    if (hq < a.group) {
+      x = *reinterpret_cast<const uint4*>(qrow);
+      y = *reinterpret_cast<const uint4*>(qrow + 8);
+    }
+    const uint32_t raw[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    uint32_t top = 0;  // the row's largest magnitude, as bf16 bits
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, max(raw[i] & 0x7fffu, (raw[i] >> 16) & 0x7fffu));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // largest in [2^14, 2^15): fp16 then holds all 8 bits of whatever is above 2^-31 of it
+    const int e = min(max((int)(top >> 7), 15), 250);  // exponent field; the factor 2^(141 - e) is a normal number
+    const float up = __uint_as_float((uint32_t)(127 + 141 - e) << 23);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 v = bf2f(raw[i]);
+      qf[n][i] = pack_f16(v.x * up, v.y * up);
+    }
+    // lanes (g, *) hold head g's factor; this lane's score columns are heads 2 t4, 2 t4 + 1
+    qs[n][0] = a.scale_log2 / __shfl_sync(0xffffffffu, up, 8 * t4);
+    qs[n][1] = a.scale_log2 / __shfl_sync(0xffffffffu, up, 8 * t4 + 4);
+  }
+
+#pragma unroll 1
+  for (int tile = ta; tile < tb; ++tile) {
+    cp_async_wait<1>();
+    __syncwarp();  // the tile has landed, for every lane; the stage before it has been read by every lane
+    const int page3 = page_of_key(a, trow, tile + 3, tb, len, lane);
+    fetch(tile + 2, page, stage == 0 ? 2 : stage - 1, mask2, sk2, sv2);
+    page = page3;
+    const char* st = ring + stage * kStageBytes;
+
+    // S^T: keys g + 8 r by heads 2 t4 + c -> s[n][r][c]
+    float s[NT][4][2], vs[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float d[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.f;
+      const uint4 u = *reinterpret_cast<const uint4*>(st + k_at + i * 1024);
+      const uint4 w = *reinterpret_cast<const uint4*>(st + k_at + i * 1024 + 512);
+      const uint32_t lo[4] = {u.x, u.y, u.z, u.w}, hi[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t af[4];
+        e4m3x4_h(lo[j], af[0], af[2]);
+        e4m3x4_h(hi[j], af[1], af[3]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_f16_16816(d[n], af, qf[n][2 * j], qf[n][2 * j + 1]);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = 2 * i + h;
+        const uint32_t x = __shfl_sync(0xffffffffu, sc, g + 8 * r);
+        const float ks = __uint_as_float((x & 0xffu) << 23);
+        vs[r] = __uint_as_float((x & 0xff00u) << 15);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) s[n][r][c] = d[n][2 * h + c] * qs[n][c] * ks;
+      }
+    }
+    if (mask != 0xffffffffu) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (!((mask >> (g + 8 * r)) & 1)) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) s[n][r][0] = s[n][r][1] = -INFINITY;
+        }
+    }
+    float mx[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) mx[n][0] = mx[n][1] = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float e = fmaxf((float)((int)(__float_as_uint(vs[r]) >> 23) - 127), -96.f);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        mx[n][0] = fmaxf(mx[n][0], s[n][r][0] + e);
+        mx[n][1] = fmaxf(mx[n][1], s[n][r][1] + e);
+      }
+    }
+    follow<NT>(acc, mx);
+
+    // weights with the value scales, as the B operand
+    uint32_t pb[NT][2][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float p0 = ex2(s[n][r][0] - acc.m[n][0]), p1 = ex2(s[n][r][1] - acc.m[n][1]);
+        acc.l[n][0] += p0;
+        acc.l[n][1] += p1;
+        pb[n][r >> 1][r & 1] = transpose8x8(pack_f16(p0 * vs[r], p1 * vs[r]));
+      }
+
+    // O^T += V^T P^T; bytes of two keys interleaved first: one permute gives two dims of both
+#pragma unroll
+    for (int jj = 0; jj < 2; ++jj) {
+      uint2 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[i] = *reinterpret_cast<const uint2*>(st + (v_at ^ ((i & 1) << 6)) + jj * 1024 + (i >> 1) * 512);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t sel = (i & 1) ? 0x7362u : 0x5140u;
+        const uint32_t lo = i < 2 ? __byte_perm(v[0].x, v[1].x, sel) : __byte_perm(v[0].y, v[1].y, sel);
+        const uint32_t hi = i < 2 ? __byte_perm(v[2].x, v[3].x, sel) : __byte_perm(v[2].y, v[3].y, sel);
+        uint32_t af[4];
+        e4m3x4_h(lo, af[0], af[1]);
+        e4m3x4_h(hi, af[2], af[3]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_f16_16816(acc.o[n][i], af, pb[n][jj][0], pb[n][jj][1]);
+      }
+    }
+    mask = mask1, mask1 = mask2;
+    sc = sk1 | (sv1 << 8);  // loaded a tile ago
+    sk1 = sk2, sv1 = sv2;
+    stage = stage == kStages - 1 ? 0 : stage + 1;
+  }
+}
+
+template <bool FP8, int NT>
+__device__ __forceinline__ void attend(const AttnArgs& a, int b, int kvh, int ta, int tb, int len, int lane, char* ring,
+                                       Acc<NT>& acc) {
+  if constexpr (FP8) attend_e4m3<NT>(a, b, kvh, ta, tb, len, lane, ring, acc);
+  else attend_bf16<NT>(a, b, kvh, ta, tb, len, lane, acc);
+}
+
+// Shared memory of a block.  e4m3: a warp's results take the place of its ring,
+// which it is done with.  bf16: sized by the group; what a block does not take
+// stays L1, where the loads in flight land.
+struct AttnShared {
+  char* warps;   // a region per warp: o [group][64], stat [group] (m, l), or the ring, on a 128-byte line
+  int region;    // its bytes
+  int group;
+  int* prefix;   // [B + 1]
+  __device__ __forceinline__ AttnShared(char* p, int group_, bool fp8) : region(region_bytes(group_, fp8)), group(group_) {
+    warps = p + ((128 - (smem_u32(p) & 127)) & 127);
+    prefix = reinterpret_cast<int*>(warps + kWarps * region);
+  }
+  __device__ __forceinline__ char* of(int warp) const { return warps + warp * region; }
+  __device__ __forceinline__ float* o(int warp, int hq) const { return reinterpret_cast<float*>(of(warp)) + hq * kHD; }
+  __device__ __forceinline__ float2& stat(int warp, int hq) const {
+    return reinterpret_cast<float2*>(of(warp) + group * kHD * 4)[hq];
+  }
+  static __host__ __device__ constexpr int region_bytes(int group, bool fp8) {
+    const int results = (group * (kHD * 4 + 8) + 15) / 16 * 16;
+    return fp8 && results < kStages * kStageBytes ? kStages * kStageBytes : results;
+  }
+  static __host__ __device__ constexpr int bytes(int group, bool fp8) { return kWarps * region_bytes(group, fp8) + 112; }
 };
-__host__ __device__ constexpr int shared_bytes(int group) { return kWarps * group * (kHD * 4 + 8); }
+static_assert(kMaxGroup * (kHD * 4 + 8) <= kStages * kStageBytes, "a warp's results fit its ring");
 
 // A block whose warps all worked on one item (a warp without tiles has an empty
 // state): their sum goes to the output, or to workspace slot `slot` when other
@@ -724,6 +825,7 @@ template <int NT>
 __device__ __forceinline__ void merge_block(const AttnArgs& a, const AttnShared& sh, const Acc<NT>& acc, int b, int kvh,
                                             bool whole, long long slot) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+  __syncwarp();  // every lane is done with the ring
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -732,23 +834,23 @@ __device__ __forceinline__ void merge_block(const AttnArgs& a, const AttnShared&
       if (hq >= a.group) continue;
       float v[8];
       acc.dims(n, c, v);
-      float4* dst = reinterpret_cast<float4*>(sh.o + (warp * a.group + hq) * kHD + 8 * g);
+      float4* dst = reinterpret_cast<float4*>(sh.o(warp, hq) + 8 * g);
       dst[0] = make_float4(v[0], v[1], v[2], v[3]);
       dst[1] = make_float4(v[4], v[5], v[6], v[7]);
-      if (g == 0) sh.stat[warp * a.group + hq] = make_float2(acc.m[n][c], acc.l[n][c]);
+      if (g == 0) sh.stat(warp, hq) = make_float2(acc.m[n][c], acc.l[n][c]);
     }
   __syncthreads();
   for (int i = tid; i < a.group * (kHD / 8); i += kAttnThreads) {
     const int hq = i / (kHD / 8), d = (i % (kHD / 8)) * 8;
     float m = kNoScore, l = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sh.stat[w * a.group + hq].x);
+    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sh.stat(w, hq).x);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float f = ex2(sh.stat[w * a.group + hq].x - m);
-      l += sh.stat[w * a.group + hq].y * f;
+      const float f = ex2(sh.stat(w, hq).x - m);
+      l += sh.stat(w, hq).y * f;
 #pragma unroll
-      for (int x = 0; x < 8; ++x) v[x] += sh.o[(w * a.group + hq) * kHD + d + x] * f;
+      for (int x = 0; x < 8; ++x) v[x] += sh.o(w, hq)[d + x] * f;
     }
     if (whole) {
       store_out8(a, b, kvh * a.group + hq, d, v, l == 0.f ? 0.f : 1.f / l);
@@ -766,16 +868,16 @@ __device__ __forceinline__ void merge_block(const AttnArgs& a, const AttnShared&
 template <bool FP8, int NT>
 __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 3) paged_attn_item_kernel(const AttnArgs a) {
   extern __shared__ __align__(16) char smem[];
-  const AttnShared sh(smem, a.group);
-  constexpr int KT = tile_keys<FP8>();
+  const AttnShared sh(smem, a.group, FP8);
+  char* ring = sh.of(threadIdx.x >> 5);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int b = blockIdx.x / a.pg.kv_heads, kvh = blockIdx.x - b * a.pg.kv_heads;
   const int len = length_of(a, b, kvh == 0 && threadIdx.x == 0);
-  const int tiles = (len + KT - 1) / KT, per = (tiles + kWarps - 1) / kWarps;
+  const int tiles = (len + kTK - 1) / kTK, per = (tiles + kWarps - 1) / kWarps;
   const int ta = min(warp * per, tiles), tb = min(ta + per, tiles);
   Acc<NT> acc;
   acc.clear();
-  if (ta < tb) attend<FP8, NT>(a, b, kvh, ta, tb, len, lane, acc);
+  if (ta < tb) attend<FP8, NT>(a, b, kvh, ta, tb, len, lane, ring, acc);
   acc.sum_lanes();
   merge_block<NT>(a, sh, acc, b, kvh, true, 0);  // len 0: l = 0, zeros
 }
@@ -785,9 +887,9 @@ template <bool FP8, int NT>
 __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 3) paged_attn_kernel(const AttnArgs a) {
   extern __shared__ __align__(16) char smem[];
   __shared__ int warp_tiles[kWarps];
-  const AttnShared sh(smem, a.group);
+  const AttnShared sh(smem, a.group, FP8);
+  char* ring = sh.of(threadIdx.x >> 5);
   int* prefix = sh.prefix;
-  constexpr int KT = tile_keys<FP8>();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int kvn = a.pg.kv_heads;
 
@@ -796,7 +898,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 3) paged_attn_kern
     const int per = (a.B + kAttnThreads - 1) / kAttnThreads;
     const int b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
     int sum = 0;
-    for (int b = b0; b < b1; ++b) sum += shares_of<KT>(length_of(a, b, blockIdx.x == 0));
+    for (int b = b0; b < b1; ++b) sum += shares_of(length_of(a, b, blockIdx.x == 0));
     int scan = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -810,7 +912,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 3) paged_attn_kern
     for (int b = b0; b < b1; ++b) {
       prefix[b] = at;
       if (blockIdx.x == 0) a.prefix[b] = at;
-      at += b1 - b0 == 1 ? sum : shares_of<KT>(length_of(a, b, false));
+      at += b1 - b0 == 1 ? sum : shares_of(length_of(a, b, false));
     }
     if (tid == kAttnThreads - 1) {
       prefix[a.B] = at;
@@ -856,7 +958,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 3) paged_attn_kern
     const int ta = (int)max(f - bi.first - kSetup, 0ll), tb = (int)(f_end - bi.first) - kSetup;
     Acc<NT> acc;
     acc.clear();
-    if (f < f_end && ta < tb) attend<FP8, NT>(a, bi.b, bi.kvh, ta, tb, length_of(a, bi.b, false), lane, acc);
+    if (f < f_end && ta < tb) attend<FP8, NT>(a, bi.b, bi.kvh, ta, tb, length_of(a, bi.b, false), lane, ring, acc);
     acc.sum_lanes();
     merge_block<NT>(a, sh, acc, bi.b, bi.kvh, block_f == bi.first && block_end == bi.first + bi.n, 2 * w0);
     return;
@@ -869,7 +971,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 3) paged_attn_kern
     if (ta >= tb) continue;  // nothing but the item's setup
     Acc<NT> acc;
     acc.clear();
-    attend<FP8, NT>(a, it.b, it.kvh, ta, tb, length_of(a, it.b, false), lane, acc);
+    attend<FP8, NT>(a, it.b, it.kvh, ta, tb, length_of(a, it.b, false), lane, ring, acc);
     acc.sum_lanes();
     const bool whole = ta == 0 && tb == it.n - kSetup;
     const long long slot = 2 * w + (ta == 0 ? 1 : 0);
@@ -1059,24 +1161,28 @@ inline int64_t prefix_bytes(int64_t B) { return ((B + 1) * 4 + 15) / 16 * 16; }
 template <bool FP8, int NT>
 cudaError_t launch_attn(const AttnArgs& a, long long max_tiles, cudaStream_t st) {
   const long long items = (long long)a.B * a.pg.kv_heads;
-  if (max_tiles <= kItemTiles) {
-    paged_attn_item_kernel<FP8, NT><<<(unsigned)items, kAttnThreads, shared_bytes(a.group), st>>>(a);
-    return cudaGetLastError();
-  }
+  const int smem = AttnShared::bytes(a.group, FP8);
   static bool done[64] = {false};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess || dev < 0 || dev >= 64) return e != cudaSuccess ? e : cudaErrorInvalidDevice;
   if (!done[dev]) {
-    e = cudaFuncSetAttribute(paged_attn_kernel<FP8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)prefix_bytes(kMaxSeqs) + shared_bytes(kMaxGroup));
+    const int most = AttnShared::bytes(kMaxGroup, FP8);
+    e = cudaFuncSetAttribute(paged_attn_item_kernel<FP8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(paged_attn_kernel<FP8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               (int)prefix_bytes(kMaxSeqs) + most);
     if (e != cudaSuccess) return e;
     done[dev] = true;
+  }
+  if (max_tiles <= kItemTiles) {
+    paged_attn_item_kernel<FP8, NT><<<(unsigned)items, kAttnThreads, smem, st>>>(a);
+    return cudaGetLastError();
   }
   // no more warps than tiles that the tables can hold: one tile is the smallest share
   const long long bound = max_tiles * items;
   const unsigned grid = (unsigned)(bound >= kAttnWarps ? kAttnBlocks : (bound + kWarps - 1) / kWarps);
-  paged_attn_kernel<FP8, NT><<<grid, kAttnThreads, (int)prefix_bytes(a.B) + shared_bytes(a.group), st>>>(a);
+  paged_attn_kernel<FP8, NT><<<grid, kAttnThreads, (int)prefix_bytes(a.B) + smem, st>>>(a);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
@@ -1110,8 +1216,7 @@ extern "C" int cdk_paged_attn(const void* q, int64_t ldq, const CdkPagedCache* c
   if (!workspace || workspace_bytes < need || !al16(workspace)) return -12;
   if (ldq < H * kHD || ldq % 8 || ldo < H * kHD || ldo % 8 || !al16(q) || !al16(out)) return -13;
   if (!(scale == scale)) return -14;
-  a.tile = cache->dtype == 1 ? tile_keys<true>() : tile_keys<false>();
-  const int64_t keys = a.pg.width << a.pg.log_page, tiles = (keys + a.tile - 1) / a.tile;  // per item, at most
+  const int64_t keys = a.pg.width << a.pg.log_page, tiles = (keys + kTK - 1) / kTK;  // per item, at most
   if (keys >= (1ll << 31) - 64 || (tiles + kSetup) * a.pg.kv_heads > ((1ll << 31) - 1) / B)
     return -15;
   a.q = reinterpret_cast<const __nv_bfloat16*>(q);
