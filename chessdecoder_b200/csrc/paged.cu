@@ -72,145 +72,191 @@ __device__ __forceinline__ int page_of(const Pages& p, long long b, long long j)
 }
 
 // ---------------------------------------------------------------------------
-// Append.  Eight lanes per (token, head) row of 64, eight values each.  The
+// Append.  A warp takes a token, or every `parts`-th group of four (head) rows of
+// it; eight lanes per row of 64, eight values each.  What belongs to the token --
+// its sequence, place in the cache, position and rotation -- is found once.  The
 // rotation is three separately rounded operations per value (no fused multiply-
 // add), so that a quantised code does not depend on how a compiler contracts
 // them.  Bound by HBM: one read of qkv, one write of each row.
 // ---------------------------------------------------------------------------
+constexpr int kAppendUnroll = 4;
+
 template <bool F32, bool FP8>
 __global__ void __launch_bounds__(256)
     paged_append_kernel(const void* __restrict__ qkv, long long ldq, const int32_t* __restrict__ pos,
-                        const float* __restrict__ rope, long long rope_len, long long S_new, int H, Pages pg,
+                        const float* __restrict__ rope, long long rope_len, unsigned S_new, int H, Pages pg,
                         const int32_t* __restrict__ start, const int32_t* __restrict__ num_new,
-                        __nv_bfloat16* __restrict__ q_out, long long ldo, long long rows) {
-  const long long i = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 3;
-  const int sub = threadIdx.x & 7;
-  const int heads = H + 2 * pg.kv_heads;
-  const bool in = i < rows;
-  const long long t = in ? i / heads : 0;
-  const int h = in ? (int)(i - t * heads) : 0;
-  const long long b = t / S_new;
-  const long long s = t - b * S_new;
-  bool live = in && (num_new == nullptr || s < num_new[b]);
-  const bool is_q = h < H, is_v = h >= H + pg.kv_heads;
-  if (is_q && q_out == nullptr) live = false;
-  float x[8];
-#pragma unroll
-  for (int c = 0; c < 8; ++c) x[c] = 0.f;
-  if (live) {
-    if (F32) {
-      const float4* src = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(qkv) + t * ldq + h * kHD + sub * 8);
-      const float4 a = src[0], c = src[1];
-      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-      x[4] = c.x; x[5] = c.y; x[6] = c.z; x[7] = c.w;
-    } else {
-      const uint4 a = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(qkv) + t * ldq + h * kHD + sub * 8);
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float2 f = bf2f(w[c]);
-        x[2 * c] = f.x;
-        x[2 * c + 1] = f.y;
-      }
-    }
-    if (rope != nullptr && !is_v) {
-      const long long p = pos[t];
-      if (p < 0 || p >= rope_len) {
-        if (sub == 0) report_error(kErrIndex);
-        live = false;
-      } else {
-        const float4* cs = reinterpret_cast<const float4*>(rope + (p * 32 + sub * 4) * 2);
-        const float4 a = cs[0], c = cs[1];
-        const float co[4] = {a.x, a.z, c.x, c.z}, si[4] = {a.y, a.w, c.y, c.w};
-#pragma unroll
-        for (int c4 = 0; c4 < 4; ++c4) {
-          const float u = x[2 * c4], w = x[2 * c4 + 1];
-          x[2 * c4] = __fsub_rn(__fmul_rn(u, co[c4]), __fmul_rn(w, si[c4]));
-          x[2 * c4 + 1] = __fadd_rn(__fmul_rn(w, co[c4]), __fmul_rn(u, si[c4]));
-        }
-      }
-    }
-  }
-  float amax = 0.f;
-  if (FP8) {
-#pragma unroll
-    for (int c = 0; c < 8; ++c) amax = fmaxf(amax, fabsf(x[c]));
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  }
-  if (!live) return;
-  if (is_q) {
-    *reinterpret_cast<uint4*>(q_out + t * ldo + h * kHD + sub * 8) =
-        make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
-    return;
-  }
+                        __nv_bfloat16* __restrict__ q_out, long long ldo, unsigned tokens, unsigned parts) {
+  const int lane = threadIdx.x & 31, sub = lane & 7;
+  const unsigned unit = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const unsigned t = unit / parts, part = unit - t * parts;
+  if (t >= tokens) return;
+  const unsigned b = t / S_new, s = t - b * S_new;
+  if (num_new != nullptr && (int)s >= num_new[b]) return;  // padding
+  const int kvn = pg.kv_heads, heads = H + 2 * kvn;
   const long long slot = (long long)start[b] + s;
   const int page = page_of(pg, b, slot);
-  if (page < 0) return;
-  const int kvh = is_v ? h - H - pg.kv_heads : h - H;
-  const long long r = ((long long)kvh << pg.log_page) + (slot & ((1ll << pg.log_page) - 1));
-  char* dst = (is_v ? pg.v : pg.k) + page * pg.ld_page + r * (kHD * (FP8 ? 1 : 2));
-  if (FP8) {
-    // least e with amax <= 448 * 2^e (448 = 1.75 * 2^8), as an exponent field
-    const uint32_t bits = __float_as_uint(amax);
-    const int byte = max((int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0), 1);
-    const float inv = __uint_as_float((uint32_t)(254 - byte) << 23);
-    uint32_t w[2];
+  const long long place = (long long)page * pg.ld_page + (slot & ((1ll << pg.log_page) - 1)) * (kHD * (FP8 ? 1 : 2));
+  const long long splace = (long long)page * pg.ld_scale + (slot & ((1ll << pg.log_page) - 1));
+  float co[4], si[4];
+  if (rope != nullptr) {
+    const long long p = pos[t];
+    if (p < 0 || p >= rope_len) {
+      if (lane == 0) report_error(kErrIndex);
+      return;
+    }
+    const float4* cs = reinterpret_cast<const float4*>(rope + (p * 32 + sub * 4) * 2);
+    const float4 x = cs[0], y = cs[1];
+    co[0] = x.x, si[0] = x.y, co[1] = x.z, si[1] = x.w;
+    co[2] = y.x, si[2] = y.y, co[3] = y.z, si[3] = y.w;
+  }
+  const char* src = reinterpret_cast<const char*>(qkv) + ((long long)t * ldq + sub * 8) * (F32 ? 4 : 2);
+  const int row0 = (q_out == nullptr ? H : 0) + part * 4 + (lane >> 3), step = parts * 4;
+  // (every lane of the warp runs the same number of rounds: the scale's exchange needs its row's eight lanes)
+  for (int h0 = row0; h0 - (lane >> 3) < heads; h0 += kAppendUnroll * step) {
+    uint4 raw[kAppendUnroll][F32 ? 2 : 1];
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
-      w[c] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[4 * c] * inv, x[4 * c + 1] * inv), __NV_SATFINITE,
-                                                __NV_E4M3) |
-             ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[4 * c + 2] * inv, x[4 * c + 3] * inv), __NV_SATFINITE,
-                                                 __NV_E4M3)
-              << 16);
-    *reinterpret_cast<uint2*>(dst + sub * 8) = make_uint2(w[0], w[1]);
-    if (sub == 0) (is_v ? pg.vs : pg.ks)[page * pg.ld_scale + r] = (uint8_t)byte;
-  } else {
-    *reinterpret_cast<uint4*>(dst + sub * 16) =
-        make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+    for (int u = 0; u < kAppendUnroll; ++u) {
+      const int h = h0 + u * step;
+      if (h < heads) {
+        const uint4* p = reinterpret_cast<const uint4*>(src + (long long)h * (kHD * (F32 ? 4 : 2)));
+        raw[u][0] = p[0];
+        if (F32) raw[u][F32 ? 1 : 0] = p[1];
+      } else {
+        raw[u][0] = make_uint4(0u, 0u, 0u, 0u);
+        if (F32) raw[u][F32 ? 1 : 0] = make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAppendUnroll; ++u) {
+      const int h = h0 + u * step;
+      const bool is_q = h < H, is_v = h >= H + kvn;
+      float x[8];
+      if (F32) {
+        const uint4 a = raw[u][0], c = raw[u][F32 ? 1 : 0];
+        x[0] = __uint_as_float(a.x), x[1] = __uint_as_float(a.y), x[2] = __uint_as_float(a.z), x[3] = __uint_as_float(a.w);
+        x[4] = __uint_as_float(c.x), x[5] = __uint_as_float(c.y), x[6] = __uint_as_float(c.z), x[7] = __uint_as_float(c.w);
+      } else {
+        const uint32_t w[4] = {raw[u][0].x, raw[u][0].y, raw[u][0].z, raw[u][0].w};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float2 f = bf2f(w[c]);
+          x[2 * c] = f.x;
+          x[2 * c + 1] = f.y;
+        }
+      }
+      if (rope != nullptr && !is_v) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float v = x[2 * c], w = x[2 * c + 1];
+          x[2 * c] = __fsub_rn(__fmul_rn(v, co[c]), __fmul_rn(w, si[c]));
+          x[2 * c + 1] = __fadd_rn(__fmul_rn(w, co[c]), __fmul_rn(v, si[c]));
+        }
+      }
+      float amax = 0.f;
+      if (FP8) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) amax = fmaxf(amax, fabsf(x[c]));
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      }
+      if (h >= heads) continue;
+      const uint4 w16 =
+          make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+      if (is_q) {
+        *reinterpret_cast<uint4*>(q_out + (long long)t * ldo + h * kHD + sub * 8) = w16;
+        continue;
+      }
+      if (page < 0) continue;  // reported
+      const long long head = (long long)(is_v ? h - H - kvn : h - H) << pg.log_page;
+      char* dst = (is_v ? pg.v : pg.k) + place + head * (kHD * (FP8 ? 1 : 2));
+      if (FP8) {
+        // least e with amax <= 448 * 2^e (448 = 1.75 * 2^8), as an exponent field
+        const uint32_t bits = __float_as_uint(amax);
+        const int byte = max((int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0), 1);
+        const float inv = __uint_as_float((uint32_t)(254 - byte) << 23);
+        uint32_t w[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          w[c] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[4 * c] * inv, x[4 * c + 1] * inv), __NV_SATFINITE,
+                                                    __NV_E4M3) |
+                 ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[4 * c + 2] * inv, x[4 * c + 3] * inv),
+                                                     __NV_SATFINITE, __NV_E4M3)
+                  << 16);
+        *reinterpret_cast<uint2*>(dst + sub * 8) = make_uint2(w[0], w[1]);
+        if (sub == 0) (is_v ? pg.vs : pg.ks)[splace + head] = (uint8_t)byte;
+      } else {
+        *reinterpret_cast<uint4*>(dst + sub * 16) = w16;
+      }
+    }
   }
 }
 
 // ---------------------------------------------------------------------------
-// Read back.  Grid (row chunks, kv head, sequence); eight lanes per row, key and
-// value of it.
+// Read back.  Grid (chunks of 128 rows, kv head, sequence); a lane takes 16 bytes of
+// a key row and of its value row, of four (bf16) or two (e4m3) rows at a time.
+// Bound by HBM: one read of the pages, one write of the rows.
 // ---------------------------------------------------------------------------
-template <bool FP8>
-__device__ __forceinline__ uint4 load_row8(const char* base, long long row, int sub, const uint8_t* scale,
-                                           long long srow) {
-  if (!FP8) return *reinterpret_cast<const uint4*>(base + row + sub * 16);
-  const uint2 c = *reinterpret_cast<const uint2*>(base + row + sub * 8);
-  const float s = scale_of(scale[srow]);
-  float2 f[4] = {e4m3x2_f(c.x), e4m3x2_f(c.x >> 16), e4m3x2_f(c.y), e4m3x2_f(c.y >> 16)};
-  uint4 o;
-  o.x = pack_bf16(f[0].x * s, f[0].y * s);
-  o.y = pack_bf16(f[1].x * s, f[1].y * s);
-  o.z = pack_bf16(f[2].x * s, f[2].y * s);
-  o.w = pack_bf16(f[3].x * s, f[3].y * s);
-  return o;
-}
+constexpr int kGatherRows = 128;
 
 template <bool FP8>
 __global__ void __launch_bounds__(256)
     paged_gather_kernel(Pages pg, const int32_t* __restrict__ lens, __nv_bfloat16* __restrict__ k_out,
                         __nv_bfloat16* __restrict__ v_out, long long sb, long long sh, long long ss, long long S) {
+  constexpr int kLanes = FP8 ? 4 : 8;        // lanes per row
+  constexpr int kPass = 256 / kLanes;        // rows per block and pass
+  constexpr int kU = kGatherRows / kPass;
   const long long b = blockIdx.z;
-  const int h = blockIdx.y;
-  const long long j = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 3;
-  const int sub = threadIdx.x & 7;
+  const int h = blockIdx.y, sub = threadIdx.x % kLanes;
   long long len = lens[b];
   if (len > S) {
-    if (j == 0 && sub == 0 && h == 0) report_error(kErrIndex);
+    if (blockIdx.x == 0 && threadIdx.x == 0 && h == 0) report_error(kErrIndex);
     len = S;
   }
-  if (j >= len) return;
-  const int page = page_of(pg, b, j);
-  if (page < 0) return;
-  const long long r = ((long long)h << pg.log_page) + (j & ((1ll << pg.log_page) - 1));
-  const long long row = page * pg.ld_page + r * (kHD * (FP8 ? 1 : 2)), srow = page * pg.ld_scale + r;
-  const long long o = b * sb + h * sh + j * ss + sub * 8;
-  *reinterpret_cast<uint4*>(k_out + o) = load_row8<FP8>(pg.k, row, sub, pg.ks, srow);
-  *reinterpret_cast<uint4*>(v_out + o) = load_row8<FP8>(pg.v, row, sub, pg.vs, srow);
+  const long long j0 = (long long)blockIdx.x * kGatherRows + threadIdx.x / kLanes;
+  if ((long long)blockIdx.x * kGatherRows >= len) return;
+  int page[kU];
+#pragma unroll
+  for (int u = 0; u < kU; ++u) page[u] = j0 + u * kPass < len ? page_of(pg, b, j0 + u * kPass) : -1;
+  uint4 kw[kU], vw[kU];
+  uint32_t ke[kU], ve[kU];
+#pragma unroll
+  for (int u = 0; u < kU; ++u) {
+    const long long r = ((long long)h << pg.log_page) + ((j0 + u * kPass) & ((1ll << pg.log_page) - 1));
+    if (page[u] >= 0) {
+      const long long at = page[u] * pg.ld_page + r * (kHD * (FP8 ? 1 : 2)) + sub * 16;
+      kw[u] = *reinterpret_cast<const uint4*>(pg.k + at);
+      vw[u] = *reinterpret_cast<const uint4*>(pg.v + at);
+      if (FP8) {
+        ke[u] = pg.ks[page[u] * pg.ld_scale + r];
+        ve[u] = pg.vs[page[u] * pg.ld_scale + r];
+      }
+    }
+  }
+  auto store = [&](__nv_bfloat16* out, uint4 w, uint32_t e) {
+    if (!FP8) {
+      *reinterpret_cast<uint4*>(out + sub * 8) = w;
+      return;
+    }
+    const float s = scale_of(e);
+    const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+    uint32_t o[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 x = e4m3x2_f(in[i]), y = e4m3x2_f(in[i] >> 16);
+      o[2 * i] = pack_bf16(x.x * s, x.y * s);
+      o[2 * i + 1] = pack_bf16(y.x * s, y.y * s);
+    }
+    reinterpret_cast<uint4*>(out + sub * 16)[0] = make_uint4(o[0], o[1], o[2], o[3]);
+    reinterpret_cast<uint4*>(out + sub * 16)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+  };
+#pragma unroll
+  for (int u = 0; u < kU; ++u)
+    if (page[u] >= 0) {
+      const long long o = b * sb + h * sh + (j0 + u * kPass) * ss;
+      store(k_out + o, kw[u], ke[u]);
+      store(v_out + o, vw[u], ve[u]);
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -1117,15 +1163,19 @@ extern "C" int cdk_paged_append(const void* qkv, int64_t ldq, int qkv_f32, const
   if (ldq < heads * kHD || ldq % (qkv_f32 ? 4 : 8) || !al16(qkv)) return -11;
   if (rope && (!pos || rope_len <= 0 || !al16(rope))) return -12;
   if (q_out && (ldo < H * kHD || ldo % 8 || !al16(q_out))) return -13;
-  if (B > (1ll << 40) / S_new || B * S_new > (1ll << 40) / heads) return -14;
-  const long long rows = B * S_new * heads;
-  const long long blocks = (rows * 8 + 255) / 256;
-  if (blocks > 0x7fffffff) return -14;
+  if (B > 0x7fffffffll / S_new) return -14;
+  // a warp per token; several, down to four rows each, while there are fewer than 16 warps per SM
+  const long long tokens = B * S_new, rows = (q_out ? H : 0) + 2 * (int64_t)pg.kv_heads;
+  long long parts = (148 * 16 + tokens - 1) / tokens;
+  if (parts > (rows + 3) / 4) parts = (rows + 3) / 4;
+  if (tokens * parts > 0xfffffff0ll) parts = 1;
+  const long long blocks = (tokens * parts + 7) / 8;
   auto* st = reinterpret_cast<cudaStream_t>(stream);
   auto* qo = reinterpret_cast<__nv_bfloat16*>(q_out);
 #define CDK_APPEND(F32, FP8)                                                                                     \
-  paged_append_kernel<F32, FP8><<<(unsigned)blocks, 256, 0, st>>>(qkv, ldq, pos, rope, rope_len, S_new, (int)H, pg, \
-                                                                  start, num_new, qo, ldo, rows)
+  paged_append_kernel<F32, FP8><<<(unsigned)blocks, 256, 0, st>>>(qkv, ldq, pos, rope, rope_len, (unsigned)S_new,   \
+                                                                  (int)H, pg, start, num_new, qo, ldo,               \
+                                                                  (unsigned)tokens, (unsigned)parts)
   if (cache->dtype == 1) {
     if (qkv_f32) CDK_APPEND(true, true);
     else CDK_APPEND(false, true);
@@ -1144,7 +1194,7 @@ extern "C" int cdk_paged_gather(const CdkPagedCache* cache, int64_t B, const int
   if (const int rc = take_pages(cache, &pg)) return rc;
   if (!lens || !k_out || !v_out || B < 0 || S < 0) return -10;
   if (sb % 8 || sh % 8 || ss % 8 || !al16(k_out) || !al16(v_out)) return -11;
-  const long long chunks = (S + 31) / 32;
+  const long long chunks = (S + kGatherRows - 1) / kGatherRows;
   if (B > 65535 || pg.kv_heads > 65535 || chunks > 0x7fffffff) return -12;
   const dim3 grid((unsigned)chunks, (unsigned)pg.kv_heads, (unsigned)B);
   auto* st = reinterpret_cast<cudaStream_t>(stream);

@@ -452,14 +452,16 @@ typedef struct CdkPagedCache {
  * power of two is exact, so the only rounding is the code's.  A row holding an
  * infinity keeps it (as code 448 at the largest scale) and loses the others; a
  * NaN stays a NaN.  num_new (int32 [B], NULL = S_new everywhere): tokens
- * s >= num_new[b] are padding: neither q_out nor the cache is touched for them. */
+ * s >= num_new[b] are padding: neither q_out nor the cache is touched for them.
+ * B * S_new < 2^31. */
 int cdk_paged_append(const void* qkv, int64_t ldq, int qkv_f32, const int32_t* pos, const float* rope,
                      int64_t rope_len, int64_t B, int64_t S_new, int64_t H, const CdkPagedCache* cache,
                      const int32_t* start, const int32_t* num_new, void* q_out, int64_t ldo, void* stream);
 /* cdk_paged_gather: rows [0, lens[b]) of every sequence as bf16 into k_out and
  * v_out at element offset b * sb + h * sh + j * ss (+ 0..63; strides multiples
  * of 8, 16-byte aligned bases).  Other rows are left as they were.  lens[b] > S
- * (the rows that the outputs have) sets the index error bit and is cut to S. */
+ * (the rows that the outputs have) sets the index error bit and is cut to S.
+ * B <= 65535. */
 int cdk_paged_gather(const CdkPagedCache* cache, int64_t B, const int32_t* lens, void* k_out, void* v_out, int64_t sb,
                      int64_t sh, int64_t ss, int64_t S, void* stream);
 /* cdk_paged_attn: one new token per sequence, out[b, h] = sum_j p_j v_j with
