@@ -79,14 +79,14 @@ __device__ __forceinline__ int page_of(const Pages& p, long long b, long long j)
 // add), so that a quantised code does not depend on how a compiler contracts
 // them.  Bound by HBM: one read of qkv, one write of each row.
 // ---------------------------------------------------------------------------
-constexpr int kAppendUnroll = 4;
-
 template <bool F32, bool FP8>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 4)
     paged_append_kernel(const void* __restrict__ qkv, long long ldq, const int32_t* __restrict__ pos,
                         const float* __restrict__ rope, long long rope_len, unsigned S_new, int H, Pages pg,
                         const int32_t* __restrict__ start, const int32_t* __restrict__ num_new,
                         __nv_bfloat16* __restrict__ q_out, long long ldo, unsigned tokens, unsigned parts) {
+  constexpr int kU = F32 ? 2 : 4;  // rows in flight per lane: 64 bytes
+  constexpr int kE = FP8 ? 1 : 2;  // bytes per cached value
   const int lane = threadIdx.x & 31, sub = lane & 7;
   const unsigned unit = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const unsigned t = unit / parts, part = unit - t * parts;
@@ -94,10 +94,24 @@ __global__ void __launch_bounds__(256)
   const unsigned b = t / S_new, s = t - b * S_new;
   if (num_new != nullptr && (int)s >= num_new[b]) return;  // padding
   const int kvn = pg.kv_heads, heads = H + 2 * kvn;
-  const long long slot = (long long)start[b] + s;
-  const int page = page_of(pg, b, slot);
-  const long long place = (long long)page * pg.ld_page + (slot & ((1ll << pg.log_page) - 1)) * (kHD * (FP8 ? 1 : 2));
-  const long long splace = (long long)page * pg.ld_scale + (slot & ((1ll << pg.log_page) - 1));
+  const char* src = reinterpret_cast<const char*>(qkv) + ((long long)t * ldq + sub * 8) * (F32 ? 4 : 2);
+  const int step = parts * 4, sub_row = lane >> 3;
+  uint4 raw[kU][F32 ? 2 : 1];
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int h = h0 + u * step;
+      raw[u][0] = make_uint4(0u, 0u, 0u, 0u);
+      if (F32) raw[u][F32 ? 1 : 0] = make_uint4(0u, 0u, 0u, 0u);
+      if (h < heads) {
+        const uint4* p = reinterpret_cast<const uint4*>(src + (long long)h * (kHD * (F32 ? 4 : 2)));
+        raw[u][0] = p[0];
+        if (F32) raw[u][F32 ? 1 : 0] = p[1];
+      }
+    }
+  };
+  int h0 = (q_out == nullptr ? H : 0) + part * 4 + sub_row;
+  load(h0);  // before what follows, whose loads wait for one another
   float co[4], si[4];
   if (rope != nullptr) {
     const long long p = pos[t];
@@ -110,27 +124,17 @@ __global__ void __launch_bounds__(256)
     co[0] = x.x, si[0] = x.y, co[1] = x.z, si[1] = x.w;
     co[2] = y.x, si[2] = y.y, co[3] = y.z, si[3] = y.w;
   }
-  const char* src = reinterpret_cast<const char*>(qkv) + ((long long)t * ldq + sub * 8) * (F32 ? 4 : 2);
-  const int row0 = (q_out == nullptr ? H : 0) + part * 4 + (lane >> 3), step = parts * 4;
+  const long long slot = (long long)start[b] + s;
+  const int page = page_of(pg, b, slot);  // -1: reported, no row is written
+  const int off = (int)(slot & ((1ll << pg.log_page) - 1));
+  const long long place = (long long)page * pg.ld_page + off * (kHD * kE) + sub * (8 * kE);
+  const long long splace = (long long)page * pg.ld_scale + off;
+
   // (every lane of the warp runs the same number of rounds: the scale's exchange needs its row's eight lanes)
-  for (int h0 = row0; h0 - (lane >> 3) < heads; h0 += kAppendUnroll * step) {
-    uint4 raw[kAppendUnroll][F32 ? 2 : 1];
+  while (h0 - sub_row < heads) {
 #pragma unroll
-    for (int u = 0; u < kAppendUnroll; ++u) {
+    for (int u = 0; u < kU; ++u) {
       const int h = h0 + u * step;
-      if (h < heads) {
-        const uint4* p = reinterpret_cast<const uint4*>(src + (long long)h * (kHD * (F32 ? 4 : 2)));
-        raw[u][0] = p[0];
-        if (F32) raw[u][F32 ? 1 : 0] = p[1];
-      } else {
-        raw[u][0] = make_uint4(0u, 0u, 0u, 0u);
-        if (F32) raw[u][F32 ? 1 : 0] = make_uint4(0u, 0u, 0u, 0u);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kAppendUnroll; ++u) {
-      const int h = h0 + u * step;
-      const bool is_q = h < H, is_v = h >= H + kvn;
       float x[8];
       if (F32) {
         const uint4 a = raw[u][0], c = raw[u][F32 ? 1 : 0];
@@ -145,6 +149,7 @@ __global__ void __launch_bounds__(256)
           x[2 * c + 1] = f.y;
         }
       }
+      const bool is_v = h >= H + kvn;
       if (rope != nullptr && !is_v) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -154,26 +159,26 @@ __global__ void __launch_bounds__(256)
         }
       }
       float amax = 0.f;
-      if (FP8) {
+      if (FP8 && h - sub_row + 3 >= H) {  // one of the warp's rows goes to the cache
 #pragma unroll
         for (int c = 0; c < 8; ++c) amax = fmaxf(amax, fabsf(x[c]));
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
       }
       if (h >= heads) continue;
-      const uint4 w16 =
-          make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
-      if (is_q) {
-        *reinterpret_cast<uint4*>(q_out + (long long)t * ldo + h * kHD + sub * 8) = w16;
-        continue;
-      }
-      if (page < 0) continue;  // reported
-      const long long head = (long long)(is_v ? h - H - kvn : h - H) << pg.log_page;
-      char* dst = (is_v ? pg.v : pg.k) + place + head * (kHD * (FP8 ? 1 : 2));
-      if (FP8) {
+      if (!FP8 || h < H) {
+        const uint4 w =
+            make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+        if (h < H) {
+          *reinterpret_cast<uint4*>(q_out + (long long)t * ldo + h * kHD + sub * 8) = w;
+        } else if (page >= 0) {
+          const int head = is_v ? h - H - kvn : h - H;
+          *reinterpret_cast<uint4*>((is_v ? pg.v : pg.k) + place + (((long long)head << pg.log_page) * (kHD * kE))) = w;
+        }
+      } else if (page >= 0) {
         // least e with amax <= 448 * 2^e (448 = 1.75 * 2^8), as an exponent field
         const uint32_t bits = __float_as_uint(amax);
-        const int byte = max((int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0), 1);
+        const int byte = max((int)((bits + 0x1fffffu) >> 23) - 8, 1);  // + 1 where the fraction is above 0x600000
         const float inv = __uint_as_float((uint32_t)(254 - byte) << 23);
         uint32_t w[2];
 #pragma unroll
@@ -183,12 +188,13 @@ __global__ void __launch_bounds__(256)
                  ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[4 * c + 2] * inv, x[4 * c + 3] * inv),
                                                      __NV_SATFINITE, __NV_E4M3)
                   << 16);
-        *reinterpret_cast<uint2*>(dst + sub * 8) = make_uint2(w[0], w[1]);
+        const long long head = (long long)(is_v ? h - H - kvn : h - H) << pg.log_page;
+        *reinterpret_cast<uint2*>((is_v ? pg.v : pg.k) + place + head * kHD) = make_uint2(w[0], w[1]);
         if (sub == 0) (is_v ? pg.vs : pg.ks)[splace + head] = (uint8_t)byte;
-      } else {
-        *reinterpret_cast<uint4*>(dst + sub * 16) = w16;
       }
     }
+    h0 += kU * step;
+    load(h0);
   }
 }
 
