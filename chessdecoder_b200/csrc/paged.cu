@@ -224,15 +224,21 @@ __global__ void __launch_bounds__(256)
   int page[kU];
 #pragma unroll
   for (int u = 0; u < kU; ++u) page[u] = j0 + u * kPass < len ? page_of(pg, b, j0 + u * kPass) : -1;
+  // e4m3: 8 bytes from each half of a row, so that the 16-byte stores of four lanes meet
+  auto load16 = [&](const char* p) {
+    if (!FP8) return *reinterpret_cast<const uint4*>(p);
+    const uint2 x = *reinterpret_cast<const uint2*>(p), y = *reinterpret_cast<const uint2*>(p + 32);
+    return make_uint4(x.x, x.y, y.x, y.y);
+  };
   uint4 kw[kU], vw[kU];
   uint32_t ke[kU], ve[kU];
 #pragma unroll
   for (int u = 0; u < kU; ++u) {
     const long long r = ((long long)h << pg.log_page) + ((j0 + u * kPass) & ((1ll << pg.log_page) - 1));
     if (page[u] >= 0) {
-      const long long at = page[u] * pg.ld_page + r * (kHD * (FP8 ? 1 : 2)) + sub * 16;
-      kw[u] = *reinterpret_cast<const uint4*>(pg.k + at);
-      vw[u] = *reinterpret_cast<const uint4*>(pg.v + at);
+      const long long at = page[u] * pg.ld_page + r * (kHD * (FP8 ? 1 : 2)) + sub * (FP8 ? 8 : 16);
+      kw[u] = load16(pg.k + at);
+      vw[u] = load16(pg.v + at);
       if (FP8) {
         ke[u] = pg.ks[page[u] * pg.ld_scale + r];
         ve[u] = pg.vs[page[u] * pg.ld_scale + r];
@@ -253,8 +259,8 @@ __global__ void __launch_bounds__(256)
       o[2 * i] = pack_bf16(x.x * s, x.y * s);
       o[2 * i + 1] = pack_bf16(y.x * s, y.y * s);
     }
-    reinterpret_cast<uint4*>(out + sub * 16)[0] = make_uint4(o[0], o[1], o[2], o[3]);
-    reinterpret_cast<uint4*>(out + sub * 16)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+    *reinterpret_cast<uint4*>(out + sub * 8) = make_uint4(o[0], o[1], o[2], o[3]);
+    *reinterpret_cast<uint4*>(out + 32 + sub * 8) = make_uint4(o[4], o[5], o[6], o[7]);
   };
 #pragma unroll
   for (int u = 0; u < kU; ++u)
