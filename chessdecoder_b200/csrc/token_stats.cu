@@ -64,45 +64,37 @@ __device__ __forceinline__ float key_value(uint64_t key) {
 
 // ---------------------------------------------------------------------------
 // A row as 16-byte vectors.  Vector v holds elements v * N - mis ... + N - 1, mis
-// the row's distance from a 16-byte boundary, so that whole vectors are aligned
-// whatever the pitch; the first and the last one may be partial.
+// the row's distance from a 16-byte boundary, so that vectors are aligned whatever
+// the pitch.  Those that lie in the row entirely are [begin, end); the elements
+// before and behind them, fewer than N each, are the edges: lane i has edge i.
 // ---------------------------------------------------------------------------
 template <bool BF16>
 struct Row {
   static constexpr int N = BF16 ? 8 : 4;
+  static constexpr int kElt = BF16 ? 2 : 4;
+  static constexpr uint32_t kNone = BF16 ? 0xff80ff80u : 0xff800000u;  // -inf
   const char* base;  // address of element -mis
-  int mis;
-  int ncls;
+  int mis, ncls;
   __device__ __forceinline__ Row(const void* logits, long long ldl, long long r, int n) : ncls(n) {
-    const char* p = reinterpret_cast<const char*>(logits) + r * ldl * (BF16 ? 2 : 4);
-    mis = (int)((reinterpret_cast<uintptr_t>(p) & 15) / (BF16 ? 2 : 4));
-    base = p - mis * (BF16 ? 2 : 4);
+    const char* p = reinterpret_cast<const char*>(logits) + r * ldl * kElt;
+    mis = (int)((reinterpret_cast<uintptr_t>(p) & 15) / kElt);
+    base = p - mis * kElt;
   }
-  __device__ __forceinline__ int vectors() const { return (ncls + mis + N - 1) / N; }
-  __device__ __forceinline__ bool whole(int v) const { return v * N >= mis && v * N - mis + N <= ncls; }
+  __device__ __forceinline__ int begin() const { return mis > 0 ? 1 : 0; }
+  __device__ __forceinline__ int end() const { return max((ncls + mis) / N, begin()); }
   __device__ __forceinline__ float at(int j) const {
     if (BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(base)[j + mis]);
     return reinterpret_cast<const float*>(base)[j + mis];
   }
-  // The N elements of vector v; -inf where it reaches out of the row.
   __device__ __forceinline__ uint4 load(int v) const {
-    if (whole(v)) return *reinterpret_cast<const uint4*>(base + (long long)v * 16);
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (BF16) {
-        const int e0 = v * N - mis + 2 * i;
-        uint32_t lo = 0xff80u, hi = 0xff80u;
-        const uint16_t* p = reinterpret_cast<const uint16_t*>(base);
-        if (e0 >= 0 && e0 < ncls) lo = p[e0 + mis];
-        if (e0 + 1 >= 0 && e0 + 1 < ncls) hi = p[e0 + 1 + mis];
-        w[i] = lo | (hi << 16);
-      } else {
-        const int e0 = v * N - mis + i;
-        w[i] = e0 >= 0 && e0 < ncls ? reinterpret_cast<const uint32_t*>(base)[e0 + mis] : 0xff800000u;
-      }
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
+    return *reinterpret_cast<const uint4*>(base + (long long)v * 16);
+  }
+  // Element of edge i < 32, -1 if there is none: the first ones, then the last ones.
+  __device__ __forceinline__ int edge(int i) const {
+    const int head = mis > 0 ? min(N - mis, ncls) : 0, tail0 = end() * N - mis;
+    if (i < head) return i;
+    const int j = max(tail0, head) + (i - head);
+    return j < ncls && i < 2 * N ? j : -1;
   }
   static __device__ __forceinline__ void values(uint4 u, float (&x)[N]) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -118,90 +110,114 @@ struct Row {
   }
 };
 
+// Largest element of a vector (NaN ignored).
+template <bool BF16>
+__device__ __forceinline__ float vector_max(uint4 u) {
+  if (BF16) {
+    const __nv_bfloat162* w = reinterpret_cast<const __nv_bfloat162*>(&u);
+    const __nv_bfloat162 m = __hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+}
+
 struct Stat {
   float m, s, t;  // m >= the lowest finite number, so x - m is never -inf - -inf
+  __device__ __forceinline__ void rise(float to) {  // a new maximum
+    const float d = fmaxf(m - to, kFar), f = ex2(d * kLog2e);  // (inf - inf stays out: s is a NaN then)
+    t = f * (t + s * d);
+    s *= f;
+    m = to;
+  }
+  __device__ __forceinline__ void add(float x) {
+    if (x > m) rise(x);
+    const float z = x - m, e = ex2(z * kLog2e);
+    s += e;
+    t = fmaf(e, fmaxf(z, kFar), t);
+  }
 };
 
-__device__ __forceinline__ Stat join(const Stat& a, const Stat& b) {
-  Stat c;
-  c.m = fmaxf(a.m, b.m);
-  const float da = fmaxf(a.m - c.m, kFar), db = fmaxf(b.m - c.m, kFar);  // (inf - inf stays out: s is NaN then)
-  const float fa = ex2(da * kLog2e), fb = ex2(db * kLog2e);
-  c.s = a.s * fa + b.s * fb;
-  c.t = fa * (a.t + a.s * da) + fb * (b.t + b.s * db);
-  return c;
+__device__ __forceinline__ Stat join(Stat a, Stat b) {
+  const float m = fmaxf(a.m, b.m);
+  a.rise(m);
+  b.rise(m);
+  return {m, a.s + b.s, a.t + b.t};
 }
 
-__device__ __forceinline__ Stat shfl_xor(const Stat& a, int o) {
-  return {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o),
-          __shfl_xor_sync(0xffffffffu, a.t, o)};
+__device__ __forceinline__ Stat join_warp(Stat a) {
+  a.rise(warp_max(a.m));
+  a.s = warp_sum(a.s);
+  a.t = warp_sum(a.t);
+  return a;
 }
 
-// One thread's share: vectors first, first + step, ... below last.  key: rank of its
-// largest element (want_key), 0 if it has none.
-template <bool BF16>
-__device__ __forceinline__ Stat stream(const Row<BF16>& row, int first, int step, int last, bool want_t, bool want_key,
+// One thread's share of a row: vectors first, first + STEP, ... below last and the
+// edge with index `edge` (or none: -1).  TOP: key = rank of its largest element, 0
+// if it has none.
+template <bool BF16, int STEP, bool TOP>
+__device__ __forceinline__ Stat stream(const Row<BF16>& row, int first, int last, int edge, bool want_t,
                                        uint64_t* key) {
   constexpr int N = Row<BF16>::N;
+  constexpr uint32_t kNone = Row<BF16>::kNone;
   Stat st{kLowest, 0.f, 0.f};
   float best = -INFINITY;  // this thread's largest element, in the chunk that begins at vector where
   int where = first;
-  for (int v0 = first; v0 < last; v0 += kUnroll * step) {
+#pragma unroll 1
+  for (int v0 = first; v0 < last; v0 += kUnroll * STEP) {
     uint4 raw[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int v = v0 + u * step;
-      const uint32_t none = BF16 ? 0xff80ff80u : 0xff800000u;
-      raw[u] = v < last ? row.load(v) : make_uint4(none, none, none, none);
-    }
-    float cm = -INFINITY;
+    for (int u = 0; u < kUnroll; ++u)
+      raw[u] = v0 + u * STEP < last ? row.load(v0 + u * STEP) : make_uint4(kNone, kNone, kNone, kNone);
+    float cm = vector_max<BF16>(raw[0]);
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      float x[N];
-      Row<BF16>::values(raw[u], x);
-#pragma unroll
-      for (int i = 0; i < N; ++i) cm = fmaxf(cm, x[i]);
-    }
-    if (cm > best) {
+    for (int u = 1; u < kUnroll; ++u) cm = fmaxf(cm, vector_max<BF16>(raw[u]));
+    if (TOP && cm > best) {
       best = cm;
       where = v0;
     }
-    if (cm > st.m) {
-      const float d = fmaxf(st.m - cm, kFar), f = ex2(d * kLog2e);
-      st.t = f * (st.t + st.s * d);
-      st.s *= f;
-      st.m = cm;
-    }
-    float s2 = 0.f, t2 = 0.f;
+    if (cm > st.m) st.rise(cm);
+    float s2[2] = {0.f, 0.f}, t2[2] = {0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       float x[N];
       Row<BF16>::values(raw[u], x);
+      if (want_t) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float z = x[i] - st.m, e = ex2(z * kLog2e);
-        s2 += e;
-        if (want_t) t2 = fmaf(e, fmaxf(z, kFar), t2);
+        for (int i = 0; i < N; ++i) {
+          const float z = x[i] - st.m, e = ex2(z * kLog2e);
+          s2[i & 1] += e;
+          t2[i & 1] = fmaf(e, fmaxf(z, kFar), t2[i & 1]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) s2[i & 1] += ex2((x[i] - st.m) * kLog2e);
       }
     }
-    st.s += s2;
-    st.t += t2;
+    st.s += s2[0] + s2[1];
+    st.t += t2[0] + t2[1];
   }
-  if (want_key) {
+  const int e = edge >= 0 ? row.edge(edge) : -1;
+  float xe = -INFINITY;
+  if (e >= 0) {
+    xe = row.at(e);
+    st.add(xe);
+  }
+  if (TOP) {
     // the first element that equals the maximum (a NaN makes s a NaN: ranked elsewhere)
-    uint32_t j = 0xffffffffu;
-    for (int u = kUnroll - 1; u >= 0; --u) {
-      const int v = where + u * step;
-      if (v >= last) continue;
-      float x[N];
-      Row<BF16>::values(row.load(v), x);
+    uint64_t k = 0;
+    if (first < last) {
+      for (int u = kUnroll - 1; u >= 0; --u) {
+        const int v = where + u * STEP;
+        if (v >= last) continue;
+        float x[N];
+        Row<BF16>::values(row.load(v), x);
 #pragma unroll
-      for (int i = N - 1; i >= 0; --i) {
-        const int e = v * N - row.mis + i;
-        if (x[i] == best && e >= 0 && e < row.ncls) j = (uint32_t)e;
+        for (int i = N - 1; i >= 0; --i)
+          if (x[i] == best) k = rank_key(best, (uint32_t)(v * N - row.mis + i));
       }
     }
-    *key = j == 0xffffffffu ? 0 : rank_key(best, j);
+    if (e >= 0) k = max(k, rank_key(xe, (uint32_t)e));
+    *key = k;
   }
   return st;
 }
@@ -232,24 +248,23 @@ __device__ __forceinline__ uint64_t best32(uint64_t a, uint64_t b, int lane) {
   return bitonic_merge(a > r ? a : r, lane);
 }
 
-// Candidates: the elements of thread `owner`'s share (as in stream) whose rank
-// reaches T, taken by threads i = 0 ... n - 1 together.
+// Elements whose rank reaches T join the candidates.
 constexpr int kCandidates = 512;
+__device__ __forceinline__ void take(float x, int e, uint64_t T, uint64_t* cand, int* count) {
+  const uint64_t key = rank_key(x, (uint32_t)e);
+  if (key < T) return;
+  const int at = atomicAdd(count, 1);
+  if (at < kCandidates) cand[at] = key;
+}
 template <bool BF16>
-__device__ __forceinline__ void gather_share(const Row<BF16>& row, int v, uint64_t T, uint64_t* cand, int* count) {
+__device__ __forceinline__ void take_vector(const Row<BF16>& row, int v, uint64_t T, uint64_t* cand, int* count) {
   constexpr int N = Row<BF16>::N;
+  const uint4 raw = row.load(v);
+  if (vector_max<BF16>(raw) < key_value(T)) return;  // (T is the rank of an element, or 0: a NaN, never above)
   float x[N];
-  Row<BF16>::values(row.load(v), x);
+  Row<BF16>::values(raw, x);
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int e = v * N - row.mis + i;
-    if (e < 0 || e >= row.ncls) continue;
-    const uint64_t key = rank_key(x[i], (uint32_t)e);
-    if (key >= T) {
-      const int at = atomicAdd(count, 1);
-      if (at < kCandidates) cand[at] = key;
-    }
-  }
+  for (int i = 0; i < N; ++i) take(x[i], v * N - row.mis + i, T, cand, count);
 }
 
 struct Args {
@@ -284,22 +299,26 @@ __device__ __forceinline__ void finish(const Args& a, const Row<BF16>& row, long
   }
 }
 
-// The k best of vectors [v0, v1) by k passes of one warp: for rows with a NaN, and
-// where more candidates reach T than there is room for (hundreds of the best
-// logits in the share of k threads).
+// The k best of vectors [v0, v1) and the first n_edges edges by k passes of one
+// warp: for rows with a NaN, and where more candidates reach T than there is room
+// for (hundreds of the best logits in the share of k threads).
 template <bool BF16>
-__device__ __noinline__ uint64_t slow_top(const Row<BF16>& row, int v0, int v1, int k, int lane) {
+__device__ __noinline__ uint64_t slow_top(const Row<BF16>& row, int v0, int v1, bool edges, int k, int lane) {
   constexpr int N = Row<BF16>::N;
   uint64_t last = ~0ull, mine = 0;
+  const int e = edges ? row.edge(lane) : -1;
   for (int i = 0; i < k; ++i) {
     uint64_t best = 0;
+    if (e >= 0) {
+      const uint64_t key = rank_key(row.at(e), (uint32_t)e);
+      if (key < last) best = key;
+    }
     for (int v = v0 + lane; v < v1; v += 32) {
       float x[N];
       Row<BF16>::values(row.load(v), x);
 #pragma unroll
       for (int c = 0; c < N; ++c) {
-        const int e = v * N - row.mis + c;
-        const uint64_t key = e >= 0 && e < row.ncls ? rank_key(x[c], (uint32_t)e) : 0;
+        const uint64_t key = rank_key(x[c], (uint32_t)(v * N - row.mis + c));
         if (key < last && key > best) best = key;
       }
     }
@@ -314,138 +333,136 @@ __device__ __noinline__ uint64_t slow_top(const Row<BF16>& row, int v0, int v1, 
   return mine;
 }
 
+// The 32 best of n gathered candidates, descending by lane.
+__device__ __forceinline__ uint64_t best_of(const uint64_t* cand, int n, int lane) {
+  uint64_t top = sort32(lane < n ? cand[lane] : 0, lane);
+#pragma unroll 1
+  for (int i = 32; i < n; i += 32) top = best32(top, sort32(i + lane < n ? cand[i + lane] : 0, lane), lane);
+  return top;
+}
+
 // ---------------------------------------------------------------------------
 // Short rows: a warp per row.
 // ---------------------------------------------------------------------------
 constexpr int kWarpsPerBlock = 8;
 
-template <bool BF16>
-__global__ void __launch_bounds__(kWarpsPerBlock * 32) token_stats_warp_kernel(const Args a) {
-  __shared__ uint64_t cand_s[kWarpsPerBlock][kCandidates];
+template <bool BF16, bool TOP>
+__global__ void __launch_bounds__(kWarpsPerBlock * 32, TOP ? 4 : 6) token_stats_warp_kernel(const Args a) {
+  __shared__ uint64_t cand_s[TOP ? kWarpsPerBlock : 1][TOP ? kCandidates : 1];
   __shared__ int count_s[kWarpsPerBlock];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long r = (long long)blockIdx.x * kWarpsPerBlock + warp;
   if (r >= a.rows) return;
   const Row<BF16> row(a.logits, a.ldl, r, a.ncls);
-  const int nv = row.vectors();
-  uint64_t key = 0;
-  Stat st = stream<BF16>(row, lane, 32, nv, a.entropy != nullptr, a.k > 0, &key);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) st = join(st, shfl_xor(st, o));
-  uint64_t top = 0;
-  if (a.k > 0) {
-    if (st.s != st.s) {
-      top = slow_top<BF16>(row, 0, nv, a.k, lane);
-    } else {
+  const int v0 = row.begin(), v1 = row.end();
+  uint64_t key = 0, top = 0;
+  const Stat st = join_warp(stream<BF16, 32, TOP>(row, v0 + lane, v1, lane, a.entropy != nullptr, &key));
+  if (TOP) {
+    bool slow = st.s != st.s;
+    if (!slow) {
       const uint64_t T = __shfl_sync(0xffffffffu, sort32(key, lane), a.k - 1);
-      uint32_t owners = __ballot_sync(0xffffffffu, key != 0 && key >= T);
+      const bool owner = key != 0 && key >= T;
+      uint32_t owners = __ballot_sync(0xffffffffu, owner);
       if (lane == 0) count_s[warp] = 0;
       __syncwarp();
-      const int per = (nv + 31) / 32;  // vectors of a lane's share
+      const int e = row.edge(lane);
+      if (owner && e >= 0) take(row.at(e), e, T, cand_s[TOP ? warp : 0], &count_s[warp]);
       while (owners) {
         const int c = __ffs(owners) - 1;
         owners &= owners - 1;
-        for (int i = lane; i < per; i += 32)
-          if (c + 32 * i < nv) gather_share<BF16>(row, c + 32 * i, T, cand_s[warp], &count_s[warp]);
+        for (int v = v0 + c + 32 * lane; v < v1; v += 32 * 32)
+          take_vector<BF16>(row, v, T, cand_s[TOP ? warp : 0], &count_s[warp]);
       }
       __syncwarp();
-      const int n = count_s[warp];
-      if (n > kCandidates) {
-        top = slow_top<BF16>(row, 0, nv, a.k, lane);
-      } else {
-        top = sort32(lane < n ? cand_s[warp][lane] : 0, lane);
-        for (int i = 32; i < n; i += 32) top = best32(top, sort32(i + lane < n ? cand_s[warp][i + lane] : 0, lane), lane);
-      }
+      slow = count_s[warp] > kCandidates;
     }
+    top = slow ? slow_top<BF16>(row, v0, v1, true, a.k, lane) : best_of(cand_s[TOP ? warp : 0], count_s[warp], lane);
   }
   finish<BF16>(a, row, r, st, lane, top);
 }
 
 // ---------------------------------------------------------------------------
 // Long rows: a block of 256 threads per row, or a cluster of blocks that share
-// the row's vectors when there are few rows; the blocks' (m, s, t) and best lists
-// are joined by the first of them through distributed shared memory.
+// the row's vectors; the blocks' (m, s, t) and best lists are joined by the first
+// of them through distributed shared memory.
 // ---------------------------------------------------------------------------
 constexpr int kThreads = 256;
 constexpr int kRowWarps = kThreads / 32;
 
+template <bool TOP>
 struct RowShared {
-  uint64_t lists[kRowWarps][32];
-  uint64_t cand[kCandidates];
+  uint64_t lists[TOP ? kRowWarps : 1][32];
+  uint64_t cand[TOP ? kCandidates : 1];
   uint64_t best[32];  // this block's best, descending
-  uint64_t T;
   int owners[32];
   int n_owners, count;
   Stat part[kRowWarps];
   Stat st;            // this block's
 };
 
-__device__ __forceinline__ const RowShared* remote(const RowShared* p, uint32_t rank) {
+template <typename T>
+__device__ __forceinline__ const T* remote(const T* p, uint32_t rank) {
   uint64_t q;
   asm volatile("mapa.u64 %0, %1, %2;" : "=l"(q) : "l"(reinterpret_cast<uint64_t>(p)), "r"(rank));
-  return reinterpret_cast<const RowShared*>(q);
+  return reinterpret_cast<const T*>(q);
 }
 
-template <bool BF16>
-__global__ void __launch_bounds__(kThreads) token_stats_block_kernel(const Args a, int blocks_per_row) {
-  __shared__ RowShared sh;
+template <bool BF16, bool TOP>
+__global__ void __launch_bounds__(kThreads, TOP ? 4 : 6) token_stats_block_kernel(const Args a, int blocks_per_row) {
+  __shared__ RowShared<TOP> sh;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long r = blockIdx.x / blocks_per_row;
   const int rank = (int)(blockIdx.x % blocks_per_row);
   const Row<BF16> row(a.logits, a.ldl, r, a.ncls);
-  const int nv = row.vectors();
-  const int per_block = (nv + blocks_per_row - 1) / blocks_per_row;
-  const int v0 = min(rank * per_block, nv), v1 = min(v0 + per_block, nv);
+  const int begin = row.begin(), end = row.end();
+  const int per_block = (end - begin + blocks_per_row - 1) / blocks_per_row;
+  const int v0 = min(begin + rank * per_block, end), v1 = min(v0 + per_block, end);
+  const int edge = rank == 0 && warp == 0 ? lane : -1;  // the first warp of the first block has the edges
   uint64_t key = 0;
-  Stat st = stream<BF16>(row, v0 + tid, kThreads, v1, a.entropy != nullptr, a.k > 0, &key);
-  const uint64_t mine = key;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) st = join(st, shfl_xor(st, o));
+  Stat st = join_warp(stream<BF16, kThreads, TOP>(row, v0 + tid, v1, edge, a.entropy != nullptr, &key));
   if (lane == 0) sh.part[warp] = st;
-  if (a.k > 0) sh.lists[warp][lane] = sort32(key, lane);
+  if (TOP) sh.lists[TOP ? warp : 0][lane] = sort32(key, lane);
   if (tid == 0) sh.n_owners = sh.count = 0;
   __syncthreads();
   st = sh.part[0];
 #pragma unroll
   for (int w = 1; w < kRowWarps; ++w) st = join(st, sh.part[w]);  // the same order in every thread
-  const bool broken = st.s != st.s;
-  if (a.k > 0 && !broken) {
-    if (warp == 0) {
-      uint64_t l = sh.lists[0][lane];
-#pragma unroll 1
-      for (int w = 1; w < kRowWarps; ++w) l = best32(l, sh.lists[w][lane], lane);
-      if (lane == a.k - 1) sh.T = l;
-    }
-    __syncthreads();
-    const uint64_t T = sh.T;
-    if (mine != 0 && mine >= T) sh.owners[atomicAdd(&sh.n_owners, 1)] = tid;  // at most k of them
-    __syncthreads();
-    const int per = (v1 - v0 + kThreads - 1) / kThreads;
-    for (int i = tid; i < sh.n_owners * per; i += kThreads) {
-      const int v = v0 + sh.owners[i / per] + kThreads * (i % per);
-      if (v < v1) gather_share<BF16>(row, v, T, sh.cand, &sh.count);
-    }
-    __syncthreads();
-  }
   uint64_t top = 0;
-  if (warp == 0 && a.k > 0) {
-    const int n = sh.count;
-    if (broken || n > kCandidates) {
-      top = slow_top<BF16>(row, v0, v1, a.k, lane);
-    } else {
-      top = sort32(lane < n ? sh.cand[lane] : 0, lane);
-      for (int i = 32; i < n; i += 32) top = best32(top, sort32(i + lane < n ? sh.cand[i + lane] : 0, lane), lane);
+  if (TOP) {
+    const bool broken = st.s != st.s;
+    if (!broken) {
+#pragma unroll 1
+      for (int n = kRowWarps / 2; n > 0; n >>= 1) {  // the warps' lists, two and two
+        if (warp < n) sh.lists[TOP ? warp : 0][lane] = best32(sh.lists[TOP ? warp : 0][lane], sh.lists[TOP ? warp + n : 0][lane], lane);
+        __syncthreads();
+      }
+      const uint64_t T = sh.lists[0][a.k - 1];
+      if (key != 0 && key >= T) {
+        sh.owners[atomicAdd(&sh.n_owners, 1)] = tid;  // at most k of them
+        const int e = edge >= 0 ? row.edge(edge) : -1;
+        if (e >= 0) take(row.at(e), e, T, sh.cand, &sh.count);
+      }
+      __syncthreads();
+      const int per = (v1 - v0 + kThreads - 1) / kThreads;
+      for (int i = tid; i < sh.n_owners * per; i += kThreads) {
+        const int v = v0 + sh.owners[i / per] + kThreads * (i % per);
+        if (v < v1) take_vector<BF16>(row, v, T, sh.cand, &sh.count);
+      }
+      __syncthreads();
     }
+    if (warp == 0)
+      top = broken || sh.count > kCandidates ? slow_top<BF16>(row, v0, v1, rank == 0, a.k, lane)
+                                             : best_of(sh.cand, sh.count, lane);
   }
   if (blocks_per_row > 1) {
-    if (warp == 0) sh.best[lane] = top;
+    if (TOP && warp == 0) sh.best[lane] = top;
     if (tid == 0) sh.st = st;
     cluster_sync();
     if (rank == 0 && warp == 0) {
       for (int c = 1; c < blocks_per_row; ++c) {
-        const RowShared* o = remote(&sh, (uint32_t)c);
+        const RowShared<TOP>* o = remote(&sh, (uint32_t)c);
         st = join(st, Stat{o->st.m, o->st.s, o->st.t});
-        if (a.k > 0) top = best32(top, o->best[lane], lane);
+        if (TOP) top = best32(top, o->best[lane], lane);
       }
     }
     cluster_sync();  // the others' shared memory stays until it has been read
@@ -455,57 +472,76 @@ __global__ void __launch_bounds__(kThreads) token_stats_block_kernel(const Args 
 }
 
 // ---------------------------------------------------------------------------
-// Backward: a warp per kUnroll * 32 vectors of a row.  logits and dlogits may be
-// the same: every element is read by the thread that writes it.
+// Backward: a warp per kSlab vectors of a row.  logits and dlogits may be the same:
+// every element is read by the thread that writes it.
 // ---------------------------------------------------------------------------
+constexpr int kSlab = 32 * kUnroll * 4;
+
 template <bool BF16>
 __global__ void __launch_bounds__(256)
-    token_stats_bwd_kernel(const void* logits, long long ldl, long long rows, int ncls,
-                           const int32_t* __restrict__ target, const float* __restrict__ lse,
-                           const float* __restrict__ entropy, const float* __restrict__ dlp,
-                           const float* __restrict__ dentropy, void* dlogits, long long ldd, int slabs) {
-  constexpr int N = Row<BF16>::N;
+    token_stats_bwd_kernel(const void* logits, long long ldl, int ncls, const int32_t* __restrict__ target,
+                           const float* __restrict__ lse, const float* __restrict__ entropy,
+                           const float* __restrict__ dlp, const float* __restrict__ dentropy, void* dlogits,
+                           long long ldd, unsigned units, unsigned slabs) {
+  constexpr int N = Row<BF16>::N, kElt = Row<BF16>::kElt;
   const int lane = threadIdx.x & 31;
-  const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const long long r = unit / slabs;
-  if (r >= rows) return;
-  const int v0 = (int)(unit % slabs) * (32 * kUnroll) + lane;
+  const unsigned unit = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (unit >= units) return;
+  const unsigned r = unit / slabs, slab = unit - r * slabs;
   const Row<BF16> row(logits, ldl, r, ncls);
-  const int nv = row.vectors();
   const int tg = target[r];
   const float g = dlp && tg >= 0 && tg < ncls ? dlp[r] : 0.f;
   const float h = dentropy ? dentropy[r] : 0.f;
   const float L = lse[r], H = dentropy ? entropy[r] : 0.f;
   const bool zero = L == -INFINITY || (g == 0.f && h == 0.f && L == L);  // nothing to read
-  uint4 raw[kUnroll];
-  if (!zero) {
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      if (v0 + 32 * u < nv) raw[u] = row.load(v0 + 32 * u);
+  char* out = reinterpret_cast<char*>(dlogits) + (long long)r * ldd * kElt;
+  // -p (g + h (log p + H)) = p (nc + nh log p)
+  const float nh = -h, nc = -fmaf(h, H, g);
+  auto grad = [&](float x, int e) {
+    if (zero) return 0.f;
+    const float z = x - L, d = ex2(z * kLog2e) * fmaf(nh, fmaxf(z, kFar), nc);
+    return e == tg ? d + g : d;  // (a target outside the classes has g = 0)
+  };
+  auto put = [&](int e, float d) {
+    if (BF16) reinterpret_cast<__nv_bfloat16*>(out)[e] = __float2bfloat16_rn(d);
+    else reinterpret_cast<float*>(out)[e] = d;
+  };
+  const int begin = row.begin(), end = row.end();
+  if ((reinterpret_cast<uintptr_t>(out) & 15) != (uintptr_t)(row.mis * kElt)) {  // vectors do not line up
+    const int e0 = slab * kSlab * N, e1 = slab + 1 == slabs ? ncls : min(e0 + kSlab * N, ncls);
+    for (int e = e0 + lane; e < e1; e += 32) put(e, grad(row.at(e), e));
+    return;
   }
-  char* out = reinterpret_cast<char*>(dlogits) + r * ldd * (BF16 ? 2 : 4);  // element 0
-  const bool same = ((reinterpret_cast<uintptr_t>(out) & 15) / (BF16 ? 2 : 4)) == (uintptr_t)row.mis;
+  char* outv = out - row.mis * kElt;  // vector 0
+  const int v1 = min(begin + (int)(slab + 1) * kSlab, end);
+#pragma unroll 1
+  for (int v0 = begin + (int)slab * kSlab + lane; v0 < v1; v0 += 32 * kUnroll) {
+    uint4 raw[kUnroll];
+    if (!zero) {
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    const int v = v0 + 32 * u;
-    if (v >= nv) break;
-    const int e0 = v * N - row.mis;
-    float d[N];
-    if (zero) {
+      for (int u = 0; u < kUnroll; ++u)
+        if (v0 + 32 * u < v1) raw[u] = row.load(v0 + 32 * u);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      if (v0 + 32 * u >= v1) break;
+      const int e0 = (v0 + 32 * u) * N - row.mis;
+      float d[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) d[i] = 0.f;
-    } else {
-      Row<BF16>::values(raw[u], d);
+      if (!zero) {
+        Row<BF16>::values(raw[u], d);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float z = d[i] - L, p = ex2(z * kLog2e);
-        float y = -p * fmaf(h, z + H, g);
-        if (p == 0.f) y = 0.f;
-        if (e0 + i == tg) y += g;
-        d[i] = y;
+        for (int i = 0; i < N; ++i) {
+          const float z = d[i] - L;
+          d[i] = ex2(z * kLog2e) * fmaf(nh, fmaxf(z, kFar), nc);
+        }
+        if ((unsigned)(tg - e0) < (unsigned)N) {
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+            if (e0 + i == tg) d[i] += g;
+        }
       }
-    }
-    if (same && row.whole(v)) {
       uint4 w;
       if (BF16)
         w = make_uint4(pack_bf16(d[0], d[1]), pack_bf16(d[2 % N], d[3 % N]), pack_bf16(d[4 % N], d[5 % N]),
@@ -513,35 +549,31 @@ __global__ void __launch_bounds__(256)
       else
         w = make_uint4(__float_as_uint(d[0]), __float_as_uint(d[1]), __float_as_uint(d[2 % N]),
                        __float_as_uint(d[3 % N]));
-      *reinterpret_cast<uint4*>(out + (long long)e0 * (BF16 ? 2 : 4)) = w;
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int e = e0 + i;
-        if (e < 0 || e >= ncls) continue;
-        if (BF16) reinterpret_cast<__nv_bfloat16*>(out)[e] = __float2bfloat16_rn(d[i]);
-        else reinterpret_cast<float*>(out)[e] = d[i];
-      }
+      *reinterpret_cast<uint4*>(outv + (long long)(v0 + 32 * u) * 16) = w;
     }
+  }
+  if (slab == 0) {
+    const int e = row.edge(lane);
+    if (e >= 0) put(e, grad(row.at(e), e));
   }
 }
 
 inline bool al(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) % n) == 0; }
 
-template <bool BF16>
+template <bool BF16, bool TOP>
 cudaError_t launch_fwd(const Args& a, cudaStream_t st) {
   const int n = BF16 ? 8 : 4;
-  // A warp per row up to 4096 bytes per lane's four loads twice over; beyond that
-  // (or with fewer rows than would fill the device) a block per row, and a cluster
-  // of blocks per row while there are fewer blocks than two per SM.
+  // A warp per row up to 256 vectors, and up to 1024 where there are rows to fill the
+  // device with warps; beyond that a block per row, or a cluster of up to 8 that share
+  // it while there are fewer than eight blocks per SM and a block has two chunks or more.
   const long long vectors = (a.ncls + n - 1) / n;
   if (vectors <= 8 * 32 || (vectors <= 32 * 32 && a.rows >= 148 * 16)) {
     const long long blocks = (a.rows + kWarpsPerBlock - 1) / kWarpsPerBlock;
-    token_stats_warp_kernel<BF16><<<(unsigned)blocks, kWarpsPerBlock * 32, 0, st>>>(a);
+    token_stats_warp_kernel<BF16, TOP><<<(unsigned)blocks, kWarpsPerBlock * 32, 0, st>>>(a);
     return cudaGetLastError();
   }
   int c = 1;
-  while (c < 8 && a.rows * c < 2 * 148 && vectors >= 2 * c * kThreads * kUnroll) c *= 2;
+  while (c < 8 && a.rows * c < 8 * 148 && vectors >= 2 * (2 * c) * kThreads * kUnroll) c *= 2;
   if (a.rows * c > 0x7fffffffll) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.rows * c));
@@ -553,7 +585,7 @@ cudaError_t launch_fwd(const Args& a, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = c > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, token_stats_block_kernel<BF16>, (const Args)a, c);
+  return cudaLaunchKernelEx(&cfg, token_stats_block_kernel<BF16, TOP>, (const Args)a, c);
 }
 
 }  // namespace
@@ -571,7 +603,8 @@ extern "C" int cdk_token_logprobs(const void* logits, int dtype, int64_t ldl, in
   if (k < 0 || k > kMaxTop || k > ncls) return -6;
   const Args a{logits, ldl, rows, (int)ncls, target, lp, entropy, lse, top_ids, top_lp, (int)k};
   auto* st = reinterpret_cast<cudaStream_t>(stream);
-  return (int)(dtype ? launch_fwd<true>(a, st) : launch_fwd<false>(a, st));
+  if (k) return (int)(dtype ? launch_fwd<true, true>(a, st) : launch_fwd<false, true>(a, st));
+  return (int)(dtype ? launch_fwd<true, false>(a, st) : launch_fwd<false, false>(a, st));
 }
 
 extern "C" int cdk_token_logprobs_bwd(const void* logits, int dtype, int64_t ldl, int64_t rows, int64_t ncls,
@@ -585,15 +618,15 @@ extern "C" int cdk_token_logprobs_bwd(const void* logits, int dtype, int64_t ldl
   if (dentropy && !entropy) return -5;
   if (logits == dlogits && ldl != ldd) return -6;
   const int n = dtype ? 8 : 4;
-  const long long slabs = ((ncls + n - 1) / n + 1 + 32 * kUnroll - 1) / (32 * kUnroll);  // + 1: a row that begins inside a vector
-  const long long blocks = (rows * slabs + 7) / 8;
-  if (blocks > 0x7fffffff) return -7;
+  const long long slabs = ((ncls + n - 1) / n + kSlab - 1) / kSlab;
+  if (rows * slabs > 0xfffffff0ll) return -7;
+  const unsigned units = (unsigned)(rows * slabs), blocks = (units + 7) / 8;
   auto* st = reinterpret_cast<cudaStream_t>(stream);
   if (dtype)
-    token_stats_bwd_kernel<true><<<(unsigned)blocks, 256, 0, st>>>(logits, ldl, rows, (int)ncls, target, lse, entropy,
-                                                                   dlp, dentropy, dlogits, ldd, (int)slabs);
+    token_stats_bwd_kernel<true><<<blocks, 256, 0, st>>>(logits, ldl, (int)ncls, target, lse, entropy, dlp, dentropy,
+                                                         dlogits, ldd, units, (unsigned)slabs);
   else
-    token_stats_bwd_kernel<false><<<(unsigned)blocks, 256, 0, st>>>(logits, ldl, rows, (int)ncls, target, lse, entropy,
-                                                                    dlp, dentropy, dlogits, ldd, (int)slabs);
+    token_stats_bwd_kernel<false><<<blocks, 256, 0, st>>>(logits, ldl, (int)ncls, target, lse, entropy, dlp, dentropy,
+                                                          dlogits, ldd, units, (unsigned)slabs);
   return (int)cudaGetLastError();
 }
