@@ -72,7 +72,6 @@ template <bool BF16>
 struct Row {
   static constexpr int N = BF16 ? 8 : 4;
   static constexpr int kElt = BF16 ? 2 : 4;
-  static constexpr uint32_t kNone = BF16 ? 0xff80ff80u : 0xff800000u;  // -inf
   const char* base;  // address of element -mis
   int mis, ncls;
   __device__ __forceinline__ Row(const void* logits, long long ldl, long long r, int n) : ncls(n) {
@@ -158,41 +157,61 @@ template <bool BF16, int STEP, bool TOP>
 __device__ __forceinline__ Stat stream(const Row<BF16>& row, int first, int last, int edge, bool want_t,
                                        uint64_t* key) {
   constexpr int N = Row<BF16>::N;
-  constexpr uint32_t kNone = Row<BF16>::kNone;
   Stat st{kLowest, 0.f, 0.f};
   float best = -INFINITY;  // this thread's largest element, in the chunk that begins at vector where
   int where = first;
+  auto rise = [&](float cm, int v) {
+    if (TOP && cm > best) {
+      best = cm;
+      where = v;
+    }
+    if (cm > st.m) st.rise(cm);
+  };
+  auto add = [&](uint4 raw, float (&s2)[2], float (&t2)[2]) {
+    float x[N];
+    Row<BF16>::values(raw, x);
+    if (want_t) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float z = x[i] - st.m, e = ex2(z * kLog2e);
+        s2[i & 1] += e;
+        t2[i & 1] = fmaf(e, fmaxf(z, kFar), t2[i & 1]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) s2[i & 1] += ex2((x[i] - st.m) * kLog2e);
+    }
+  };
+  int v = first;
 #pragma unroll 1
-  for (int v0 = first; v0 < last; v0 += kUnroll * STEP) {
+  for (; v + (kUnroll - 1) * STEP < last; v += kUnroll * STEP) {
     uint4 raw[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      raw[u] = v0 + u * STEP < last ? row.load(v0 + u * STEP) : make_uint4(kNone, kNone, kNone, kNone);
+    for (int u = 0; u < kUnroll; ++u) raw[u] = row.load(v + u * STEP);
     float cm = vector_max<BF16>(raw[0]);
 #pragma unroll
     for (int u = 1; u < kUnroll; ++u) cm = fmaxf(cm, vector_max<BF16>(raw[u]));
-    if (TOP && cm > best) {
-      best = cm;
-      where = v0;
-    }
-    if (cm > st.m) st.rise(cm);
+    rise(cm, v);
     float s2[2] = {0.f, 0.f}, t2[2] = {0.f, 0.f};
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      float x[N];
-      Row<BF16>::values(raw[u], x);
-      if (want_t) {
+    for (int u = 0; u < kUnroll; ++u) add(raw[u], s2, t2);
+    st.s += s2[0] + s2[1];
+    st.t += t2[0] + t2[1];
+  }
+  if (v < last) {  // the last chunk, of one to kUnroll - 1 vectors
+    uint4 raw[kUnroll - 1];
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const float z = x[i] - st.m, e = ex2(z * kLog2e);
-          s2[i & 1] += e;
-          t2[i & 1] = fmaf(e, fmaxf(z, kFar), t2[i & 1]);
-        }
-      } else {
+    for (int u = 0; u < kUnroll - 1; ++u)
+      if (v + u * STEP < last) raw[u] = row.load(v + u * STEP);
+    float cm = vector_max<BF16>(raw[0]);
 #pragma unroll
-        for (int i = 0; i < N; ++i) s2[i & 1] += ex2((x[i] - st.m) * kLog2e);
-      }
-    }
+    for (int u = 1; u < kUnroll - 1; ++u)
+      if (v + u * STEP < last) cm = fmaxf(cm, vector_max<BF16>(raw[u]));
+    rise(cm, v);
+    float s2[2] = {0.f, 0.f}, t2[2] = {0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < kUnroll - 1; ++u)
+      if (v + u * STEP < last) add(raw[u], s2, t2);
     st.s += s2[0] + s2[1];
     st.t += t2[0] + t2[1];
   }
@@ -206,15 +225,18 @@ __device__ __forceinline__ Stat stream(const Row<BF16>& row, int first, int last
     // the first element that equals the maximum (a NaN makes s a NaN: ranked elsewhere)
     uint64_t k = 0;
     if (first < last) {
+      int at = 0;
+#pragma unroll
       for (int u = kUnroll - 1; u >= 0; --u) {
-        const int v = where + u * STEP;
-        if (v >= last) continue;
+        const int w = where + u * STEP;
+        if (w >= last) continue;
         float x[N];
-        Row<BF16>::values(row.load(v), x);
+        Row<BF16>::values(row.load(w), x);
 #pragma unroll
         for (int i = N - 1; i >= 0; --i)
-          if (x[i] == best) k = rank_key(best, (uint32_t)(v * N - row.mis + i));
+          if (x[i] == best) at = w * N + i;
       }
+      k = rank_key(best, (uint32_t)(at - row.mis));
     }
     if (e >= 0) k = max(k, rank_key(xe, (uint32_t)e));
     *key = k;
@@ -248,24 +270,40 @@ __device__ __forceinline__ uint64_t best32(uint64_t a, uint64_t b, int lane) {
   return bitonic_merge(a > r ? a : r, lane);
 }
 
-// Elements whose rank reaches T join the candidates.
+// Elements whose rank reaches T join the candidates (room for `most`; count goes on).
 constexpr int kCandidates = 512;
-__device__ __forceinline__ void take(float x, int e, uint64_t T, uint64_t* cand, int* count) {
-  const uint64_t key = rank_key(x, (uint32_t)e);
-  if (key < T) return;
-  const int at = atomicAdd(count, 1);
-  if (at < kCandidates) cand[at] = key;
-}
-template <bool BF16>
-__device__ __forceinline__ void take_vector(const Row<BF16>& row, int v, uint64_t T, uint64_t* cand, int* count) {
-  constexpr int N = Row<BF16>::N;
-  const uint4 raw = row.load(v);
-  if (vector_max<BF16>(raw) < key_value(T)) return;  // (T is the rank of an element, or 0: a NaN, never above)
-  float x[N];
-  Row<BF16>::values(raw, x);
+struct Candidates {
+  uint64_t* list;
+  int* count;
+  int most;
+  uint64_t T;
+  float value;  // T's; T is the rank of an element, or 0: a NaN, below which nothing is
+  __device__ __forceinline__ void take(float x, int e) const {
+    const uint64_t key = rank_key(x, (uint32_t)e);
+    if (key < T) return;
+    const int at = atomicAdd(count, 1);
+    if (at < most) list[at] = key;
+  }
+  template <bool BF16>
+  __device__ __forceinline__ void take_vector(const Row<BF16>& row, int v) const {
+    constexpr int N = Row<BF16>::N;
+    const uint4 raw = row.load(v);
+    if (vector_max<BF16>(raw) < value) return;
+    float x[N];
+    Row<BF16>::values(raw, x);
+    uint32_t left = 0;
 #pragma unroll
-  for (int i = 0; i < N; ++i) take(x[i], v * N - row.mis + i, T, cand, count);
-}
+    for (int i = 0; i < N; ++i) left |= x[i] < value ? 0u : 1u << i;
+    while (left) {  // one of them, mostly
+      const int i = __ffs(left) - 1;
+      left &= left - 1;
+      float y = x[0];
+#pragma unroll
+      for (int c = 1; c < N; ++c) y = i == c ? x[c] : y;
+      take(y, v * N - row.mis + i);
+    }
+  }
+};
 
 struct Args {
   const void* logits;
@@ -345,11 +383,12 @@ __device__ __forceinline__ uint64_t best_of(const uint64_t* cand, int n, int lan
 // Short rows: a warp per row.
 // ---------------------------------------------------------------------------
 constexpr int kWarpsPerBlock = 8;
+constexpr int kWarpCandidates = 160;  // the slow way is short here, and shared memory is warps
 
 template <bool BF16, bool TOP>
 __global__ void __launch_bounds__(kWarpsPerBlock * 32, TOP ? 4 : 6) token_stats_warp_kernel(const Args a) {
-  __shared__ uint64_t cand_s[TOP ? kWarpsPerBlock : 1][TOP ? kCandidates : 1];
-  __shared__ int count_s[kWarpsPerBlock];
+  __shared__ uint64_t cand_s[TOP ? kWarpsPerBlock : 1][TOP ? kWarpCandidates : 1];
+  __shared__ int count_s[kWarpsPerBlock], owners_s[TOP ? kWarpsPerBlock : 1][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long r = (long long)blockIdx.x * kWarpsPerBlock + warp;
   if (r >= a.rows) return;
@@ -362,19 +401,20 @@ __global__ void __launch_bounds__(kWarpsPerBlock * 32, TOP ? 4 : 6) token_stats_
     if (!slow) {
       const uint64_t T = __shfl_sync(0xffffffffu, sort32(key, lane), a.k - 1);
       const bool owner = key != 0 && key >= T;
-      uint32_t owners = __ballot_sync(0xffffffffu, owner);
+      const uint32_t owners = __ballot_sync(0xffffffffu, owner);
+      if (owner) owners_s[TOP ? warp : 0][__popc(owners & ((1u << lane) - 1))] = lane;
       if (lane == 0) count_s[warp] = 0;
       __syncwarp();
+      const Candidates cand{cand_s[TOP ? warp : 0], &count_s[warp], kWarpCandidates, T, key_value(T)};
       const int e = row.edge(lane);
-      if (owner && e >= 0) take(row.at(e), e, T, cand_s[TOP ? warp : 0], &count_s[warp]);
-      while (owners) {
-        const int c = __ffs(owners) - 1;
-        owners &= owners - 1;
-        for (int v = v0 + c + 32 * lane; v < v1; v += 32 * 32)
-          take_vector<BF16>(row, v, T, cand_s[TOP ? warp : 0], &count_s[warp]);
+      if (owner && e >= 0) cand.take(row.at(e), e);
+      const int n = __popc(owners);
+      for (int i = lane; i < n * ((v1 - v0 + 31) >> 5); i += 32) {  // vector i / n of owner i % n
+        const int v = v0 + owners_s[TOP ? warp : 0][i % n] + 32 * (i / n);
+        if (v < v1) cand.take_vector(row, v);
       }
       __syncwarp();
-      slow = count_s[warp] > kCandidates;
+      slow = count_s[warp] > kWarpCandidates;
     }
     top = slow ? slow_top<BF16>(row, v0, v1, true, a.k, lane) : best_of(cand_s[TOP ? warp : 0], count_s[warp], lane);
   }
@@ -437,16 +477,17 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 6) token_stats_block_kerne
         __syncthreads();
       }
       const uint64_t T = sh.lists[0][a.k - 1];
+      const Candidates cand{sh.cand, &sh.count, kCandidates, T, key_value(T)};
       if (key != 0 && key >= T) {
         sh.owners[atomicAdd(&sh.n_owners, 1)] = tid;  // at most k of them
         const int e = edge >= 0 ? row.edge(edge) : -1;
-        if (e >= 0) take(row.at(e), e, T, sh.cand, &sh.count);
+        if (e >= 0) cand.take(row.at(e), e);
       }
       __syncthreads();
-      const int per = (v1 - v0 + kThreads - 1) / kThreads;
-      for (int i = tid; i < sh.n_owners * per; i += kThreads) {
-        const int v = v0 + sh.owners[i / per] + kThreads * (i % per);
-        if (v < v1) take_vector<BF16>(row, v, T, sh.cand, &sh.count);
+      const int n = sh.n_owners, per = (v1 - v0 + kThreads - 1) / kThreads;
+      for (int i = tid; i < n * per; i += kThreads) {  // vector i / n of owner i % n
+        const int v = v0 + sh.owners[i % n] + kThreads * (i / n);
+        if (v < v1) cand.take_vector(row, v);
       }
       __syncthreads();
     }
@@ -565,7 +606,7 @@ cudaError_t launch_fwd(const Args& a, cudaStream_t st) {
   const int n = BF16 ? 8 : 4;
   // A warp per row up to 256 vectors, and up to 1024 where there are rows to fill the
   // device with warps; beyond that a block per row, or a cluster of up to 8 that share
-  // it while there are fewer than eight blocks per SM and a block has two chunks or more.
+  // it while there are fewer than two blocks per SM and a block has two chunks or more.
   const long long vectors = (a.ncls + n - 1) / n;
   if (vectors <= 8 * 32 || (vectors <= 32 * 32 && a.rows >= 148 * 16)) {
     const long long blocks = (a.rows + kWarpsPerBlock - 1) / kWarpsPerBlock;
@@ -573,7 +614,7 @@ cudaError_t launch_fwd(const Args& a, cudaStream_t st) {
     return cudaGetLastError();
   }
   int c = 1;
-  while (c < 8 && a.rows * c < 8 * 148 && vectors >= 2 * (2 * c) * kThreads * kUnroll) c *= 2;
+  while (c < 8 && a.rows * c < 2 * 148 && vectors >= 2 * (2 * c) * kThreads * kUnroll) c *= 2;
   if (a.rows * c > 0x7fffffffll) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.rows * c));
