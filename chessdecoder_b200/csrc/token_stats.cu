@@ -150,16 +150,16 @@ __device__ __forceinline__ Stat join_warp(Stat a) {
   return a;
 }
 
-// One thread's share of a row: vectors first, first + STEP, ... below last and the
-// edge with index `edge` (or none: -1).  TOP: key = rank of its largest element, 0
+// One thread's share of a row: vectors first + tid, first + tid + STEP, ... below
+// last and the edge with index `edge` (or none: -1).  TOP: key = rank of its largest element, 0
 // if it has none.
 template <bool BF16, int STEP, bool TOP>
-__device__ __forceinline__ Stat stream(const Row<BF16>& row, int first, int last, int edge, bool want_t,
-                                       uint64_t* key) {
+__device__ __forceinline__ Stat stream(const Row<BF16>& row, int first, int tid, int last, int edge,
+                                       bool want_t, uint64_t* key) {
   constexpr int N = Row<BF16>::N;
   Stat st{kLowest, 0.f, 0.f};
   float best = -INFINITY;  // this thread's largest element, in the chunk that begins at vector where
-  int where = first;
+  int where = first + tid;
   auto rise = [&](float cm, int v) {
     if (TOP && cm > best) {
       best = cm;
@@ -182,9 +182,9 @@ __device__ __forceinline__ Stat stream(const Row<BF16>& row, int first, int last
       for (int i = 0; i < N; ++i) s2[i & 1] += ex2((x[i] - st.m) * kLog2e);
     }
   };
-  int v = first;
 #pragma unroll 1
-  for (; v + (kUnroll - 1) * STEP < last; v += kUnroll * STEP) {
+  for (; first + kUnroll * STEP <= last; first += kUnroll * STEP) {  // chunks that every thread has whole
+    const int v = first + tid;
     uint4 raw[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) raw[u] = row.load(v + u * STEP);
@@ -198,19 +198,20 @@ __device__ __forceinline__ Stat stream(const Row<BF16>& row, int first, int last
     st.s += s2[0] + s2[1];
     st.t += t2[0] + t2[1];
   }
-  if (v < last) {  // the last chunk, of one to kUnroll - 1 vectors
-    uint4 raw[kUnroll - 1];
+  const int v = first + tid;
+  if (v < last) {  // what is left: a vector at least
+    uint4 raw[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll - 1; ++u)
+    for (int u = 0; u < kUnroll; ++u)
       if (v + u * STEP < last) raw[u] = row.load(v + u * STEP);
     float cm = vector_max<BF16>(raw[0]);
 #pragma unroll
-    for (int u = 1; u < kUnroll - 1; ++u)
+    for (int u = 1; u < kUnroll; ++u)
       if (v + u * STEP < last) cm = fmaxf(cm, vector_max<BF16>(raw[u]));
     rise(cm, v);
     float s2[2] = {0.f, 0.f}, t2[2] = {0.f, 0.f};
 #pragma unroll
-    for (int u = 0; u < kUnroll - 1; ++u)
+    for (int u = 0; u < kUnroll; ++u)
       if (v + u * STEP < last) add(raw[u], s2, t2);
     st.s += s2[0] + s2[1];
     st.t += t2[0] + t2[1];
@@ -224,7 +225,7 @@ __device__ __forceinline__ Stat stream(const Row<BF16>& row, int first, int last
   if (TOP) {
     // the first element that equals the maximum (a NaN makes s a NaN: ranked elsewhere)
     uint64_t k = 0;
-    if (first < last) {
+    if (where < last) {
       int at = 0;
 #pragma unroll
       for (int u = kUnroll - 1; u >= 0; --u) {
@@ -285,9 +286,8 @@ struct Candidates {
     if (at < most) list[at] = key;
   }
   template <bool BF16>
-  __device__ __forceinline__ void take_vector(const Row<BF16>& row, int v) const {
+  __device__ __forceinline__ void take_vector(const Row<BF16>& row, int v, uint4 raw) const {
     constexpr int N = Row<BF16>::N;
-    const uint4 raw = row.load(v);
     if (vector_max<BF16>(raw) < value) return;
     float x[N];
     Row<BF16>::values(raw, x);
@@ -301,6 +301,26 @@ struct Candidates {
 #pragma unroll
       for (int c = 1; c < N; ++c) y = i == c ? x[c] : y;
       take(y, v * N - row.mis + i);
+    }
+  }
+  // Second look at the shares of n threads (vectors v0 + owner, + STEP, ... below v1) by
+  // THREADS threads: 2^lg of them, the least power of two that covers a share, per owner.
+  template <bool BF16, int STEP, int THREADS>
+  __device__ __forceinline__ void take_shares(const Row<BF16>& row, int v0, int v1, const int* owners, int n,
+                                              int tid) const {
+    const int per = (v1 - v0 + STEP - 1) / STEP, lg = per > 1 ? 32 - __clz(per - 1) : 0;
+    for (int i0 = tid; i0 < n << lg; i0 += 4 * THREADS) {
+      uint4 raw[4];
+      int v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * THREADS;
+        v[u] = i < n << lg ? v0 + owners[i >> lg] + STEP * (i & ((1 << lg) - 1)) : v1;
+        if (v[u] < v1) raw[u] = row.load(v[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (v[u] < v1) take_vector(row, v[u], raw[u]);
     }
   }
 };
@@ -395,7 +415,7 @@ __global__ void __launch_bounds__(kWarpsPerBlock * 32, TOP ? 4 : 6) token_stats_
   const Row<BF16> row(a.logits, a.ldl, r, a.ncls);
   const int v0 = row.begin(), v1 = row.end();
   uint64_t key = 0, top = 0;
-  const Stat st = join_warp(stream<BF16, 32, TOP>(row, v0 + lane, v1, lane, a.entropy != nullptr, &key));
+  const Stat st = join_warp(stream<BF16, 32, TOP>(row, v0, lane, v1, lane, a.entropy != nullptr, &key));
   if (TOP) {
     bool slow = st.s != st.s;
     if (!slow) {
@@ -408,11 +428,7 @@ __global__ void __launch_bounds__(kWarpsPerBlock * 32, TOP ? 4 : 6) token_stats_
       const Candidates cand{cand_s[TOP ? warp : 0], &count_s[warp], kWarpCandidates, T, key_value(T)};
       const int e = row.edge(lane);
       if (owner && e >= 0) cand.take(row.at(e), e);
-      const int n = __popc(owners);
-      for (int i = lane; i < n * ((v1 - v0 + 31) >> 5); i += 32) {  // vector i / n of owner i % n
-        const int v = v0 + owners_s[TOP ? warp : 0][i % n] + 32 * (i / n);
-        if (v < v1) cand.take_vector(row, v);
-      }
+      cand.take_shares<BF16, 32, 32>(row, v0, v1, owners_s[TOP ? warp : 0], __popc(owners), lane);
       __syncwarp();
       slow = count_s[warp] > kWarpCandidates;
     }
@@ -459,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 6) token_stats_block_kerne
   const int v0 = min(begin + rank * per_block, end), v1 = min(v0 + per_block, end);
   const int edge = rank == 0 && warp == 0 ? lane : -1;  // the first warp of the first block has the edges
   uint64_t key = 0;
-  Stat st = join_warp(stream<BF16, kThreads, TOP>(row, v0 + tid, v1, edge, a.entropy != nullptr, &key));
+  Stat st = join_warp(stream<BF16, kThreads, TOP>(row, v0, tid, v1, edge, a.entropy != nullptr, &key));
   if (lane == 0) sh.part[warp] = st;
   if (TOP) sh.lists[TOP ? warp : 0][lane] = sort32(key, lane);
   if (tid == 0) sh.n_owners = sh.count = 0;
@@ -484,11 +500,7 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 6) token_stats_block_kerne
         if (e >= 0) cand.take(row.at(e), e);
       }
       __syncthreads();
-      const int n = sh.n_owners, per = (v1 - v0 + kThreads - 1) / kThreads;
-      for (int i = tid; i < n * per; i += kThreads) {  // vector i / n of owner i % n
-        const int v = v0 + sh.owners[i % n] + kThreads * (i / n);
-        if (v < v1) cand.take_vector(row, v);
-      }
+      cand.take_shares<BF16, kThreads, kThreads>(row, v0, v1, sh.owners, sh.n_owners, tid);
       __syncthreads();
     }
     if (warp == 0)
