@@ -75,10 +75,9 @@ def _i64(t, device):
     return None if t is None else t.to(device=device, dtype=torch.int64).contiguous()
 
 
-class BatchedBackbone:
-    """Batched KV-cache backbone (dense ChessDecoder; the exported module has no
-    MoE).  ``max_seq_len``: cache capacity (keys per sequence), default the
-    model's."""
+class _Backbone:
+    """The weights and the layer loop of the KV-cache backbones; a subclass makes
+    the caches and hands ``_layers_forward`` its attention."""
 
     def __init__(self, cfg: Optional[ModelConfig] = None, batch_size: int = 1, max_seq_len: Optional[int] = None,
                  state_dict=None, device="cuda", seed: int = 0, store: Optional[ParamStore] = None,
@@ -98,9 +97,8 @@ class BatchedBackbone:
             store.load_state_dict({k: v.to(self.device) for k, v in sd.items()})
         self.store = store
         self.rope = rope_table(max(cfg.max_seq_len, self.max_len), cfg.head_dim).to(self.device)
-        L, H = cfg.num_layers, cfg.num_heads
-        self.causal = KVCache(L, self.B, H, self.max_len, self.device, "causal")
-        self.prefix = KVCache(L, self.B, H, self.max_len, self.device, "prefix")
+        L = cfg.num_layers
+        self._make_caches()
         # incremental steps replay from CUDA graphs (first call eager, second captures)
         self.use_graphs = bool(use_graphs) and self.device.type == "cuda"
         self._graphs = {}
@@ -119,6 +117,130 @@ class BatchedBackbone:
         self.last_hidden16 = None
         self._sms = (torch.cuda.get_device_properties(self.device).multi_processor_count
                      if self.device.type == "cuda" else 148)
+
+    def _make_caches(self):
+        raise NotImplementedError
+
+    # -- core forward --------------------------------------------------------
+    def _arange32(self, n):
+        t = self._ar.get(n)
+        if t is None:
+            t = self._ar[n] = torch.arange(n, dtype=torch.int32, device=self.device)
+        return t
+
+    def _embed(self, ids, ov, om_u8):
+        """tok_embedding, with the rows under the override mask replaced by the
+        Fourier encoding of their value (backbone_causal.py:100-109: every row
+        is encoded, then blended)."""
+        cfg, st = self.cfg, self.store
+        T, E, nf = ids.numel(), cfg.embed_dim, cfg.num_fourier_freq
+        dev = self.device
+        rows = self._arange32(T)
+        ones = torch.ones(T, dtype=torch.uint8, device=dev)
+        fvals = torch.empty(T, device=dev)
+        feat = torch.empty(T, 2 * nf, device=dev)
+        K.fourier_features(ov, ov, ones, torch.zeros_like(ones), None, None, st.param("fourier_encoder.frequencies"),
+                           rows, fvals, feat)
+        frows = torch.empty(T, E, device=dev)
+        K.gemm_f32(feat, st.param("fourier_encoder.proj.weight"), frows, bias=st.param("fourier_encoder.proj.bias"),
+                   M=T)
+        slot = torch.empty(T, dtype=torch.int32, device=dev)
+        K.decode_slots(om_u8, slot)
+        h0 = torch.empty(T, E, device=dev)
+        K.embed_fwd(ids, st.param("tok_embedding.weight"), slot, frows, h0)
+        return h0
+
+    def _layers_forward(self, x, B, S, attend):
+        """Every layer and the final norm over the rows x [B * S, E]; attend(i,
+        qkv, ao) puts layer i's keys and values (fp32 rows q | k | v, not
+        rotated) into its cache and its attention output into ao (bf16)."""
+        cfg, dev = self.cfg, self.device
+        E, F = cfg.embed_dim, cfg.ff
+        T = B * S
+        n1 = torch.empty(T, E, device=dev, dtype=torch.bfloat16)
+        qkv = torch.empty(T, 3 * E, device=dev)
+        ao = torch.empty(T, E, device=dev, dtype=torch.bfloat16)
+        u = torch.empty(T, F, device=dev, dtype=torch.bfloat16)
+        h1 = torch.empty(T, E, device=dev)
+        # Few rows (incremental steps, small blocks): 128 x 256 output tiles
+        # would leave most SMs idle while the weights stream, so the
+        # projections run split-K, reduce-adding fp32 partial sums into a zeroed
+        # output (or into a copy of the residual); SwiGLU then runs on the sums.
+        small = T <= 512
+        if small:
+            gu32 = torch.empty(T, 2 * F, device=dev)
+        else:
+            gu = torch.empty(T, 2 * F, device=dev, dtype=torch.bfloat16)
+        for i, w in enumerate(self._layers):
+            K.rmsnorm_fwd(x, w["s1"], y16=n1)
+            if small:
+                qkv.zero_()
+                K.gemm(n1, w["wqkv"], kind=K.EPI_ATOMIC_F32, out=qkv, split_k=_splits(T, 3 * E, E, self._sms))
+            else:
+                K.gemm(n1, w["wqkv"], kind=K.EPI_STORE_F32, out=qkv)
+            attend(i, qkv, ao)
+            xn = torch.empty(T, E, device=dev)
+            if small:
+                h1.copy_(x)
+                K.gemm(ao, w["wo"], kind=K.EPI_ATOMIC_F32, out=h1, split_k=_splits(T, E, E, self._sms))
+                K.rmsnorm_fwd(h1, w["s2"], y16=n1)
+                gu32.zero_()
+                K.gemm(n1, w["w13"], kind=K.EPI_ATOMIC_F32, out=gu32, split_k=_splits(T, 2 * F, E, self._sms))
+                K.swiglu_f32(gu32, u)
+                xn.copy_(h1)
+                K.gemm(u, w["w2"], kind=K.EPI_ATOMIC_F32, out=xn, split_k=_splits(T, E, F, self._sms))
+            else:
+                K.gemm(ao, w["wo"], kind=K.EPI_RESID_F32, out=h1, resid=x)
+                K.rmsnorm_fwd(h1, w["s2"], y16=n1)
+                K.gemm(n1, w["w13"], kind=K.EPI_SWIGLU, out=u, out2=gu, half_n=F)
+                K.gemm(u, w["w2"], kind=K.EPI_RESID_F32, out=xn, resid=h1)
+            x = xn
+        h16 = torch.empty(T, E, device=dev, dtype=torch.bfloat16)
+        h32 = torch.empty(T, E, device=dev)
+        K.rmsnorm_fwd(x, self.store.param("norm.scale"), y16=h16, y32=h32)
+        self.last_hidden16 = h16.view(B, S, E)
+        return h32.view(B, S, E)
+
+    # -- value heads (evalWlHead / evalDHead, batched_engine.cpp:151-180) -------
+    def value_head(self, name: str = "wl_head", h16=None, temperature: float = 0.0, seed: int = 0):
+        """WL or D value head on hidden states h16 [B, E] bf16 (default: the
+        last position of the latest call): Linear -> Mish -> Linear to bucket
+        logits, a bucket picked as in cdk_head_select (argmax, or a sample at a
+        temperature), its unscaled log-probability, and its centre value.
+        Returns (bucket [B] int64, value [B] fp32, log_prob [B] fp32, logits)."""
+        if name not in ("wl_head", "d_head"):
+            raise ValueError("value heads are wl_head and d_head")
+        st, cfg, dev = self.store, self.cfg, self.device
+        if h16 is None:
+            h16 = self.last_hidden16[:, -1, :]
+        B = h16.shape[0]
+        hv, nb = cfg.value_hidden_size, cfg.n_buckets
+        z = torch.empty(B, hv, device=dev)
+        K.gemm(h16, st.bf16(f"{name}.mlp.0.weight"), kind=K.EPI_STORE_F32, out=z, bias=st.param(f"{name}.mlp.0.bias"))
+        a16 = torch.empty(B, hv, device=dev, dtype=torch.bfloat16)
+        K.mish_bf16(z, a16)
+        logits = torch.empty(B, nb, device=dev)
+        K.gemm(a16, st.bf16(f"{name}.mlp.2.weight"), kind=K.EPI_STORE_F32, out=logits,
+               bias=st.param(f"{name}.mlp.2.bias"))
+        idx = torch.empty(B, dtype=torch.int64, device=dev)
+        lp = torch.empty(B, device=dev)
+        seed_t = torch.full((1,), int(seed) & 0x7FFFFFFFFFFFFFFF, dtype=torch.int64, device=dev)
+        K.head_select(logits, idx, temperature=temperature, seed=seed_t, lp=lp)
+        if name not in self._centers:
+            self._centers[name] = (make_wl_buckets(cfg.n_buckets, cfg.wl_sigma) if name == "wl_head"
+                                   else make_d_buckets(cfg.n_buckets)).to(dev)
+        return idx, self._centers[name][idx], lp, logits
+
+
+class BatchedBackbone(_Backbone):
+    """Batched KV-cache backbone (dense ChessDecoder; the exported module has no
+    MoE).  ``max_seq_len``: cache capacity (keys per sequence), default the
+    model's."""
+
+    def _make_caches(self):
+        L, H = self.cfg.num_layers, self.cfg.num_heads
+        self.causal = KVCache(L, self.B, H, self.max_len, self.device, "causal")
+        self.prefix = KVCache(L, self.B, H, self.max_len, self.device, "prefix")
 
     # -- lengths ------------------------------------------------------------
     @property
@@ -152,35 +274,6 @@ class BatchedBackbone:
         K.decode_mark(self.prefix.valid, self.B, self.prefix.len_dev, start=int(start), count=int(count),
                       active=_u8(active, self.device))
 
-    # -- core forward --------------------------------------------------------
-    def _arange32(self, n):
-        t = self._ar.get(n)
-        if t is None:
-            t = self._ar[n] = torch.arange(n, dtype=torch.int32, device=self.device)
-        return t
-
-    def _embed(self, ids, ov, om_u8):
-        """tok_embedding, with the rows under the override mask replaced by the
-        Fourier encoding of their value (backbone_causal.py:100-109: every row
-        is encoded, then blended)."""
-        cfg, st = self.cfg, self.store
-        T, E, nf = ids.numel(), cfg.embed_dim, cfg.num_fourier_freq
-        dev = self.device
-        rows = self._arange32(T)
-        ones = torch.ones(T, dtype=torch.uint8, device=dev)
-        fvals = torch.empty(T, device=dev)
-        feat = torch.empty(T, 2 * nf, device=dev)
-        K.fourier_features(ov, ov, ones, torch.zeros_like(ones), None, None, st.param("fourier_encoder.frequencies"),
-                           rows, fvals, feat)
-        frows = torch.empty(T, E, device=dev)
-        K.gemm_f32(feat, st.param("fourier_encoder.proj.weight"), frows, bias=st.param("fourier_encoder.proj.bias"),
-                   M=T)
-        slot = torch.empty(T, dtype=torch.int32, device=dev)
-        K.decode_slots(om_u8, slot)
-        h0 = torch.empty(T, E, device=dev)
-        K.embed_fwd(ids, st.param("tok_embedding.weight"), slot, frows, h0)
-        return h0
-
     def _forward(self, cache: KVCache, ids, pos, ov, om, *, block_mode, active=None, num_real=None, full=None):
         """One pass of S new tokens per sequence over ``cache`` (keys [0, len)
         plus the new block); writes the new k / v rows at [len, len + S) but
@@ -191,7 +284,7 @@ class BatchedBackbone:
             raise ValueError(f"batch {B} != {self.B}")
         if cache.len + S > self.max_len:
             raise ValueError(f"cache full: {cache.len} + {S} > {self.max_len}")
-        E, F, H = cfg.embed_dim, cfg.ff, cfg.num_heads
+        E, H = cfg.embed_dim, cfg.num_heads
         T = B * S
         ids = ids.to(device=dev, dtype=torch.int64).reshape(-1).contiguous()
         pos32 = pos.to(device=dev, dtype=torch.int32).reshape(-1).contiguous()
@@ -207,28 +300,9 @@ class BatchedBackbone:
         if fresh:
             qkv16 = torch.empty(T, 3 * E, device=dev, dtype=torch.bfloat16)
             lse = torch.empty(B * H * S, device=dev)
-        n1 = torch.empty(T, E, device=dev, dtype=torch.bfloat16)
-        qkv = torch.empty(T, 3 * E, device=dev)
         q16 = torch.empty(T, E, device=dev, dtype=torch.bfloat16)
-        ao = torch.empty(T, E, device=dev, dtype=torch.bfloat16)
-        u = torch.empty(T, F, device=dev, dtype=torch.bfloat16)
-        h1 = torch.empty(T, E, device=dev)
-        # Few rows (incremental steps, small blocks): 128 x 256 output tiles
-        # would leave most SMs idle while the weights stream, so the
-        # projections run split-K, reduce-adding fp32 partial sums into a zeroed
-        # output (or into a copy of the residual); SwiGLU then runs on the sums.
-        small = T <= 512
-        if small:
-            gu32 = torch.empty(T, 2 * F, device=dev)
-        else:
-            gu = torch.empty(T, 2 * F, device=dev, dtype=torch.bfloat16)
-        for i, w in enumerate(self._layers):
-            K.rmsnorm_fwd(x, w["s1"], y16=n1)
-            if small:
-                qkv.zero_()
-                K.gemm(n1, w["wqkv"], kind=K.EPI_ATOMIC_F32, out=qkv, split_k=_splits(T, 3 * E, E, self._sms))
-            else:
-                K.gemm(n1, w["wqkv"], kind=K.EPI_STORE_F32, out=qkv)
+
+        def attend(i, qkv, ao):
             if fresh:
                 K.kv_append(qkv, B, S, H, cache.k[i], cache.v[i], cache.len_dev, pos=pos32, rope=self.rope,
                             q_out=qkv16, qkv_out=True)
@@ -238,27 +312,8 @@ class BatchedBackbone:
                             q_out=q16)
                 K.decode_attn(q16, cache.k[i], cache.v[i], cache.len_dev, S, B, H, cache.valid, ao,
                               block_mode=block_mode, active=active, num_real=num_real, full_mask=full)
-            xn = torch.empty(T, E, device=dev)
-            if small:
-                h1.copy_(x)
-                K.gemm(ao, w["wo"], kind=K.EPI_ATOMIC_F32, out=h1, split_k=_splits(T, E, E, self._sms))
-                K.rmsnorm_fwd(h1, w["s2"], y16=n1)
-                gu32.zero_()
-                K.gemm(n1, w["w13"], kind=K.EPI_ATOMIC_F32, out=gu32, split_k=_splits(T, 2 * F, E, self._sms))
-                K.swiglu_f32(gu32, u)
-                xn.copy_(h1)
-                K.gemm(u, w["w2"], kind=K.EPI_ATOMIC_F32, out=xn, split_k=_splits(T, E, F, self._sms))
-            else:
-                K.gemm(ao, w["wo"], kind=K.EPI_RESID_F32, out=h1, resid=x)
-                K.rmsnorm_fwd(h1, w["s2"], y16=n1)
-                K.gemm(n1, w["w13"], kind=K.EPI_SWIGLU, out=u, out2=gu, half_n=F)
-                K.gemm(u, w["w2"], kind=K.EPI_RESID_F32, out=xn, resid=h1)
-            x = xn
-        h16 = torch.empty(T, E, device=dev, dtype=torch.bfloat16)
-        h32 = torch.empty(T, E, device=dev)
-        K.rmsnorm_fwd(x, self.store.param("norm.scale"), y16=h16, y32=h32)
-        self.last_hidden16 = h16.view(B, S, E)
-        return h32.view(B, S, E)
+
+        return self._layers_forward(x, B, S, attend)
 
     # -- causal mode (batched_backbone.cpp:110-177) -------------------------
     def causal_forward(self, ids, pos, ov, om, active, num_real):
@@ -365,36 +420,6 @@ class BatchedBackbone:
                 cache.len += 1
         out = st.hist[:n_steps].clone()
         return (out, st.lp_hist[:n_steps].clone()) if return_log_probs else out
-
-    # -- value heads (evalWlHead / evalDHead, batched_engine.cpp:151-180) -------
-    def value_head(self, name: str = "wl_head", h16=None, temperature: float = 0.0, seed: int = 0):
-        """WL or D value head on hidden states h16 [B, E] bf16 (default: the
-        last position of the latest call): Linear -> Mish -> Linear to bucket
-        logits, a bucket picked as in cdk_head_select (argmax, or a sample at a
-        temperature), its unscaled log-probability, and its centre value.
-        Returns (bucket [B] int64, value [B] fp32, log_prob [B] fp32, logits)."""
-        if name not in ("wl_head", "d_head"):
-            raise ValueError("value heads are wl_head and d_head")
-        st, cfg, dev = self.store, self.cfg, self.device
-        if h16 is None:
-            h16 = self.last_hidden16[:, -1, :]
-        B = h16.shape[0]
-        hv, nb = cfg.value_hidden_size, cfg.n_buckets
-        z = torch.empty(B, hv, device=dev)
-        K.gemm(h16, st.bf16(f"{name}.mlp.0.weight"), kind=K.EPI_STORE_F32, out=z, bias=st.param(f"{name}.mlp.0.bias"))
-        a16 = torch.empty(B, hv, device=dev, dtype=torch.bfloat16)
-        K.mish_bf16(z, a16)
-        logits = torch.empty(B, nb, device=dev)
-        K.gemm(a16, st.bf16(f"{name}.mlp.2.weight"), kind=K.EPI_STORE_F32, out=logits,
-               bias=st.param(f"{name}.mlp.2.bias"))
-        idx = torch.empty(B, dtype=torch.int64, device=dev)
-        lp = torch.empty(B, device=dev)
-        seed_t = torch.full((1,), int(seed) & 0x7FFFFFFFFFFFFFFF, dtype=torch.int64, device=dev)
-        K.head_select(logits, idx, temperature=temperature, seed=seed_t, lp=lp)
-        if name not in self._centers:
-            self._centers[name] = (make_wl_buckets(cfg.n_buckets, cfg.wl_sigma) if name == "wl_head"
-                                   else make_d_buckets(cfg.n_buckets)).to(dev)
-        return idx, self._centers[name][idx], lp, logits
 
     def _gen_body(self, st):
         self._incremental_body(self.causal, st.ids, st.pos, None, None, st.active)

@@ -9,6 +9,10 @@ around nothing: every op has a fake impl) see ordinary operators.
 * ``cdk::soft_bucket_ce(logits, target, centers, valid) -> (loss, dlogits)`` --
   utils/training.py:24-50; the gradient of the logits comes out of the same
   kernel and is the saved tensor of the autograd formula.
+* ``cdk::token_logprobs(logits, target, k) -> (lp, entropy, lse, top_ids,
+  top_lp)`` -- log-probabilities of given tokens with the entropy and the k best
+  alternatives (rl/log_probs.py:58-101 is the first of them); lp and entropy are
+  differentiable.
 * ``cdk::backbone_fwd(...) -> (h, handle)`` and ``cdk::backbone_bwd_(handle,
   dh, grad)`` -- embedding + Fourier injection, every layer and the final
   norm (model.py:143-187).  The forward keeps its activations on the device
@@ -22,7 +26,7 @@ from __future__ import annotations
 
 import itertools
 import weakref
-from typing import List, Optional
+from typing import List, Optional, Tuple
 
 import torch
 from torch import Tensor
@@ -135,6 +139,79 @@ def _sb_bwd(ctx, grads):
 
 
 soft_bucket_ce.register_autograd(_sb_bwd, setup_context=_sb_setup)
+
+# ---------------------------------------------------------------------------
+# Token statistics
+# ---------------------------------------------------------------------------
+
+
+def _stat_rows(logits: Tensor, target: Tensor):
+    """(rows [n, V] with unit inner stride, int32 targets [n]); a target outside
+    the classes, of whatever magnitude, becomes -100."""
+    V = logits.shape[-1]
+    if logits.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("cdk::token_logprobs needs fp32 or bf16 logits")
+    if target.shape != logits.shape[:-1] or target.is_floating_point():
+        raise ValueError(f"cdk::token_logprobs needs integer targets {tuple(logits.shape[:-1])}")
+    x = logits.detach().reshape(-1, V)
+    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < V):
+        x = x.contiguous()
+    t = target.reshape(-1)
+    return x, torch.where((t >= 0) & (t < V), t, -100).to(torch.int32)
+
+
+@torch.library.custom_op("cdk::token_logprobs", mutates_args=())
+def token_logprobs(logits: Tensor, target: Tensor, k: int) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """(lp, entropy, lse [...], top_ids int32, top_lp [..., k]) of logits
+    [..., V] (fp32 or bf16) and targets [...]: lp = log_softmax(logits)[target],
+    0 where the target is outside the classes (padding).  lp and entropy carry
+    gradients; k <= min(32, V), 0: no alternatives."""
+    x, t = _stat_rows(logits, target)
+    n, lead = x.shape[0], logits.shape[:-1]
+    lp, ent, lse = (torch.empty(n, device=x.device) for _ in range(3))
+    ids = torch.empty(n, k, dtype=torch.int32, device=x.device)
+    top = torch.empty(n, k, device=x.device)
+    K.token_logprobs(x, t, lp, entropy=ent, lse=lse, top_ids=ids, top_lp=top)
+    return lp.view(lead), ent.view(lead), lse.view(lead), ids.view(*lead, k), top.view(*lead, k)
+
+
+@token_logprobs.register_fake
+def _(logits, target, k):
+    lead = logits.shape[:-1]
+    f = logits.new_empty(lead, dtype=torch.float32)
+    return (f, torch.empty_like(f), torch.empty_like(f), logits.new_empty(*lead, k, dtype=torch.int32),
+            logits.new_empty(*lead, k, dtype=torch.float32))
+
+
+@torch.library.custom_op("cdk::token_logprobs_backward", mutates_args=())
+def token_logprobs_backward(logits: Tensor, target: Tensor, lse: Tensor, entropy: Tensor, dlp: Optional[Tensor],
+                            dentropy: Optional[Tensor]) -> Tensor:
+    """d(logits), in their shape and type, from the gradients of lp and entropy."""
+    x, t = _stat_rows(logits, target)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    g, h = (None if d is None else d.to(torch.float32).reshape(-1).contiguous() for d in (dlp, dentropy))
+    K.token_logprobs_bwd(x, t, lse.reshape(-1), entropy.reshape(-1), g, h, dx)
+    return dx.view(logits.shape)
+
+
+@token_logprobs_backward.register_fake
+def _(logits, target, lse, entropy, dlp, dentropy):
+    return logits.new_empty(logits.shape)
+
+
+def _stats_setup(ctx, inputs, output):
+    logits, target, _ = inputs
+    _, ent, lse, ids, top = output
+    ctx.save_for_backward(logits, target, lse, ent)
+    ctx.mark_non_differentiable(lse, ids, top)
+
+
+def _stats_bwd(ctx, dlp, dentropy, *_):
+    logits, target, lse, ent = ctx.saved_tensors
+    return torch.ops.cdk.token_logprobs_backward(logits, target, lse, ent, dlp, dentropy), None, None
+
+
+token_logprobs.register_autograd(_stats_bwd, setup_context=_stats_setup)
 
 # ---------------------------------------------------------------------------
 # Backbone

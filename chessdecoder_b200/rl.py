@@ -11,7 +11,8 @@ with a Schulman KL penalty, normalised by the number of action tokens.  Here:
   their targets, and per action row the rollout and reference log-probs and
   the sequence's advantage);
 * ``GRPOStep.log_probs``: the prefix forward and the per-token log-probs
-  (frozen / rollout policy; ``compute_ref_log_probs``);
+  (frozen / rollout policy; ``compute_ref_log_probs``); ``score``: those with
+  the entropy and the best alternatives of every action;
 * ``GRPOStep.forward_backward``: prefix forward, the two move heads on their
   action rows with the fused per-token GRPO kernel (``cdk_grpo_token``: log-
   softmax, ratio, clipping, KL, loss and the logit gradient in one pass), the
@@ -157,6 +158,33 @@ class GRPOStep:
         (compute_ref_log_probs / the rollout policy's log-probs)."""
         hN16, _, _ = self._forward(rb)
         return self._scatter(rb, [self._head(h[0], h[1], h[2], hN16) for h in rb.heads])
+
+    @torch.no_grad()
+    def score(self, rb: RLBatch, top_k: int = 0) -> dict:
+        """What the policy makes of the batch's actions: ``log_probs`` and
+        ``entropy`` [B, S] at the action positions, the action ``mask``, and per
+        head ``heads[name]`` = (flat positions [n], top_ids int32, top_log_probs
+        [n, top_k]): the top_k (<= 32) best moves there, in move-vocabulary
+        indices."""
+        st = self.store
+        hN16, _, _ = self._forward(rb)
+        lps, ents, heads = [], [], {}
+        for name, rows, tgt, flat, _ in rb.heads:
+            n, V_ = rows.numel(), V.move_vocab_size
+            lp, ent = torch.empty(n, device=self.device), torch.empty(n, device=self.device)
+            ids = torch.empty(n, top_k, dtype=torch.int32, device=self.device)
+            top = torch.empty(n, top_k, device=self.device)
+            if n:
+                hp = torch.empty(n, self.cfg.embed_dim, device=self.device, dtype=torch.bfloat16)
+                K.gather_rows_bf16(hN16, rows, hp)
+                logits = torch.empty(n, V_, device=self.device)
+                K.gemm(hp, st.bf16(f"{name}.weight"), kind=K.EPI_STORE_F32, out=logits, bias=st.param(f"{name}.bias"))
+                K.token_logprobs(logits, tgt, lp, entropy=ent, top_ids=ids, top_lp=top)
+            lps.append(lp)
+            ents.append(ent)
+            heads[name] = (flat, ids, top)
+        log_probs, mask = self._scatter(rb, lps)
+        return {"log_probs": log_probs, "entropy": self._scatter(rb, ents)[0], "mask": mask, "heads": heads}
 
     def forward_backward(self, rb: RLBatch):
         """GRPO loss (device [1]) with every gradient in the store (zeroed

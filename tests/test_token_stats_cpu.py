@@ -55,3 +55,18 @@ def test_c_entries_refuse():
         x, dt, ldl, R, V, 64, lse, ent, 64, h, dx, ldd, None)
     assert b(R=0) == 0 and b(lse=None) == -1 and b(dx=None) == -1 and b(dt=3) == -2 and b(ldd=9) == -3
     assert b(dx=130) == -4 and b(ent=None) == -5 and b(dx=64, ldd=12) == -6
+
+
+def test_op_under_fake_tensors():
+    """cdk::token_logprobs has a fake implementation: shapes, types and what carries a gradient."""
+    import chessdecoder_b200.ops  # noqa: F401
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        x = torch.empty(3, 4, 50, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+        t = torch.empty(3, 4, device="cuda", dtype=torch.long)
+        lp, ent, lse, ids, top = torch.ops.cdk.token_logprobs(x, t, 5)
+        assert lp.shape == ent.shape == lse.shape == (3, 4) and ids.shape == top.shape == (3, 4, 5)
+        assert (lp.dtype, ids.dtype, top.dtype) == (F32, I32, F32)
+        assert lp.requires_grad and ent.requires_grad and not (lse.requires_grad or top.requires_grad)
+        dx = torch.ops.cdk.token_logprobs_backward(x, t, lse, ent, lp, None)
+        assert dx.shape == x.shape and dx.dtype == x.dtype
