@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libcdk.so"
@@ -36,23 +37,10 @@ class CdkGemmEpilogue(C.Structure):
     ]
 
 
-class CdkPagedCache(C.Structure):
-    _fields_ = [
-        ("k", _vp),
-        ("v", _vp),
-        ("k_scale", _vp),
-        ("v_scale", _vp),
-        ("table", _vp),
-        ("ldt", _i64),
-        ("width", _i64),
-        ("num_pages", _i64),
-        ("ld_page", _i64),
-        ("ld_scale", _i64),
-        ("kv_heads", _i32),
-        ("page_size", _i32),
-        ("dtype", _i32),
-        ("reserved", _i32),
-    ]
+# CdkPagedCache as packed bytes (native alignment, as the compiler lays it out): k, v,
+# k_scale, v_scale, table; ldt, width, num_pages, ld_page, ld_scale; kv_heads,
+# page_size, dtype, reserved.
+PAGED_CACHE = struct.Struct("@5P5q4i")
 
 
 # name -> (restype, argtypes); mirrors include/cdk.h
@@ -122,11 +110,11 @@ SIGNATURES = {
     "cdk_swiglu_f32": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _vp]),
     "cdk_head_select": (_int, [_vp, _i64, _i64, _i64, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
     "cdk_mish_bf16": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _vp]),
-    "cdk_paged_append": (_int, [_vp, _i64, _int, _vp, _vp, _i64, _i64, _i64, _i64, C.POINTER(CdkPagedCache), _vp, _vp,
+    "cdk_paged_append": (_int, [_vp, _i64, _int, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp,
                                 _vp, _i64, _vp]),
-    "cdk_paged_gather": (_int, [C.POINTER(CdkPagedCache), _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp]),
-    "cdk_paged_attn_workspace": (_i64, [_i64, _i64, _i64]),
-    "cdk_paged_attn": (_int, [_vp, _i64, C.POINTER(CdkPagedCache), _i64, _i64, _vp, _vp, _i64, _f32, _vp, _i64, _vp]),
+    "cdk_paged_gather": (_int, [_vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp]),
+    "cdk_paged_attn_workspace": (_i64, [_i64, _i64, _i64, _i64]),
+    "cdk_paged_attn": (_int, [_vp, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _f32, _vp, _i64, _vp]),
     "cdk_token_logprobs": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
     "cdk_token_logprobs_bwd": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
 }

@@ -1260,9 +1260,11 @@ cudaError_t launch_attn(const AttnArgs& a, long long max_tiles, cudaStream_t st)
 }
 }  // namespace
 
-extern "C" int64_t cdk_paged_attn_workspace(int64_t B, int64_t H, int64_t kv_heads) {
-  if (B < 0 || B > kMaxSeqs || H <= 0 || H > 65536 || kv_heads <= 0 || H % kv_heads || H / kv_heads > kMaxGroup)
+extern "C" int64_t cdk_paged_attn_workspace(int64_t B, int64_t H, int64_t kv_heads, int64_t max_keys) {
+  if (B < 0 || B > kMaxSeqs || H <= 0 || H > 65536 || kv_heads <= 0 || H % kv_heads || H / kv_heads > kMaxGroup ||
+      max_keys < 0)
     return -1;
+  if (max_keys <= (int64_t)kItemTiles * kTK) return 0;
   return prefix_bytes(B) + (int64_t)kSlots * (H / kv_heads) * (16 + kHD * 4);
 }
 
@@ -1273,12 +1275,12 @@ extern "C" int cdk_paged_attn(const void* q, int64_t ldq, const CdkPagedCache* c
   AttnArgs a;
   if (const int rc = take_pages(cache, &a.pg)) return rc;
   if (!q || !lens || !out || B < 0 || H <= 0) return -10;
-  const int64_t need = cdk_paged_attn_workspace(B, H, a.pg.kv_heads);
+  const int64_t keys = a.pg.width << a.pg.log_page, tiles = (keys + kTK - 1) / kTK;  // per item, at most
+  const int64_t need = cdk_paged_attn_workspace(B, H, a.pg.kv_heads, keys);
   if (need < 0) return -11;
-  if (!workspace || workspace_bytes < need || !al16(workspace)) return -12;
+  if (need > 0 && (!workspace || workspace_bytes < need || !al16(workspace))) return -12;
   if (ldq < H * kHD || ldq % 8 || ldo < H * kHD || ldo % 8 || !al16(q) || !al16(out)) return -13;
   if (!(scale == scale)) return -14;
-  const int64_t keys = a.pg.width << a.pg.log_page, tiles = (keys + kTK - 1) / kTK;  // per item, at most
   if (keys >= (1ll << 31) - 64 || (tiles + kSetup) * a.pg.kv_heads > ((1ll << 31) - 1) / B)
     return -15;
   a.q = reinterpret_cast<const __nv_bfloat16*>(q);

@@ -618,7 +618,9 @@ cudaError_t launch_fwd(const Args& a, cudaStream_t st) {
   const int n = BF16 ? 8 : 4;
   // A warp per row up to 256 vectors, and up to 1024 where there are rows to fill the
   // device with warps; beyond that a block per row, or a cluster of up to 8 that share
-  // it while there are fewer than two blocks per SM and a block has two chunks or more.
+  // it (two chunks each at least) while there are few blocks per SM: fewer than four
+  // (300 rows of 131071 fp32: 35 -> 29 us), or two with alternatives, since every block
+  // then selects its own (509 rows of 131071 bf16, 20 of them: 42 us, 49 with two blocks).
   const long long vectors = (a.ncls + n - 1) / n;
   if (vectors <= 8 * 32 || (vectors <= 32 * 32 && a.rows >= 148 * 16)) {
     const long long blocks = (a.rows + kWarpsPerBlock - 1) / kWarpsPerBlock;
@@ -626,7 +628,7 @@ cudaError_t launch_fwd(const Args& a, cudaStream_t st) {
     return cudaGetLastError();
   }
   int c = 1;
-  while (c < 8 && a.rows * c < 2 * 148 && vectors >= 2 * (2 * c) * kThreads * kUnroll) c *= 2;
+  while (c < 8 && a.rows * c < (TOP ? 2 : 4) * 148 && vectors >= 2 * (2 * c) * kThreads * kUnroll) c *= 2;
   if (a.rows * c > 0x7fffffffll) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.rows * c));

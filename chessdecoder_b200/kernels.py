@@ -657,7 +657,7 @@ def _refuse(op, why):
 
 
 def _lay(t):
-    return None if t is None else (t.dtype, t.shape, t.stride())
+    return None if t is None else (t.dtype, t.shape, t.stride(), t.get_device())
 
 
 def _ptr(t):
@@ -677,12 +677,11 @@ def _call(op, fn, dev, *args):
         _check(rc, op)
 
 
-def _on(op, *ts):
-    """The CUDA device that every tensor given is on."""
-    dev = ts[0].get_device()
-    for t in ts:
-        if t is not None and t.get_device() != dev:
-            _refuse(op, f"tensors on {ts[0].device} and {t.device}")
+def _on(op, *lays):
+    """The CUDA device that every tensor of these layouts is on."""
+    dev = lays[0][3]
+    if any(lay is not None and lay[3] != dev for lay in lays):
+        _refuse(op, "tensors on different devices")
     if dev < 0:
         raise RuntimeError("chessdecoder_b200 ops need CUDA tensors (no CPU implementation exists)")
     return dev
@@ -695,7 +694,7 @@ def _vec(op, name, lay, dtype, n):
 
 def _rows2d(op, name, lay, dtypes, rows, cols):
     """2-D rows with unit inner stride that do not overlap; returns the pitch."""
-    dtype, shape, stride = lay
+    dtype, shape, stride, _ = lay
     if dtype not in dtypes or len(shape) != 2 or shape[0] != rows or shape[1] < cols or stride[1] != 1:
         _refuse(op, f"{name} must be {' or '.join(map(str, dtypes))} [{rows}, >= {cols}] with unit inner stride")
     if rows > 1 and stride[0] < cols:
@@ -706,7 +705,7 @@ def _rows2d(op, name, lay, dtypes, rows, cols):
 def _pages_plan(op, k, v, table, k_scale, v_scale, B):
     """(page_size, kv_heads, and the layout fields of CdkPagedCache) of one
     layer's pools."""
-    dtype, shape, stride = k
+    dtype, shape, stride, _ = k
     if len(shape) != 4 or shape[3] != 64 or v != k:
         _refuse(op, "k_pages and v_pages must be alike, [num_pages, kv_heads, page_size, 64]")
     n, h, p, _ = shape
@@ -726,7 +725,7 @@ def _pages_plan(op, k, v, table, k_scale, v_scale, B):
             _refuse(op, "bf16 pages have no scales")
     else:
         _refuse(op, "pages must be bfloat16 or float8_e4m3fn")
-    tdtype, tshape, tstride = table
+    tdtype, tshape, tstride, _ = table
     if tdtype != torch.int32 or len(tshape) != 2 or tshape[0] != B or (tshape[1] > 1 and tstride[1] != 1):
         _refuse(op, f"table must be int32 [{B}, pages per sequence] with unit inner stride")
     ldt = tstride[0] if B > 1 else tshape[1]
@@ -737,8 +736,8 @@ def _pages_plan(op, k, v, table, k_scale, v_scale, B):
 
 
 def _cache_arg(k, v, k_scale, v_scale, table, fields):
-    return C.byref(_lib.CdkPagedCache(k.data_ptr(), v.data_ptr(), _ptr(k_scale), _ptr(v_scale), table.data_ptr(),
-                                      *fields))
+    return _lib.PAGED_CACHE.pack(k.data_ptr(), v.data_ptr(), 0 if k_scale is None else k_scale.data_ptr(),
+                                 0 if v_scale is None else v_scale.data_ptr(), table.data_ptr(), *fields)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -758,7 +757,8 @@ def _append_plan(B, S_new, H, k, v, table, ks, vs, qkv, start, num_new, pos, rop
         if rope[0] != torch.float32 or len(rope[1]) != 3 or rope[1][1:] != (32, 2) or rope[2] != (64, 2, 1):
             _refuse(op, "rope must be contiguous fp32 [positions, 32, 2]")
     ldo = 0 if q_out is None else _rows2d(op, "q_out", q_out, (torch.bfloat16,), T, H * 64)
-    return fields, T, ldq, int(qkv[0] == torch.float32), 0 if rope is None else rope[1][0], ldo
+    dev = _on(op, k, v, table, ks, vs, qkv, start, num_new, pos, rope, q_out)
+    return dev, fields, T, ldq, int(qkv[0] == torch.float32), 0 if rope is None else rope[1][0], ldo
 
 
 @_timed("paged_append")
@@ -771,10 +771,9 @@ def paged_append(qkv, B, S_new, H, k_pages, v_pages, table, start, *, num_new=No
     power-of-two scale a row in k_scale / v_scale.  num_new (int32 [B]): only the
     first num_new[b] tokens of a sequence are real; nothing is written for the
     others.  The rows of one call must be distinct."""
-    fields, T, ldq, f32, n_rope, ldo = _append_plan(
+    dev, fields, T, ldq, f32, n_rope, ldo = _append_plan(
         B, S_new, H, _lay(k_pages), _lay(v_pages), _lay(table), _lay(k_scale), _lay(v_scale), _lay(qkv), _lay(start),
         _lay(num_new), _lay(pos), _lay(rope), _lay(q_out))
-    dev = _on("paged_append", k_pages, v_pages, table, k_scale, v_scale, qkv, start, num_new, pos, rope, q_out)
     if T == 0:
         return
     _call("paged_append", lib().cdk_paged_append, dev, qkv.data_ptr(), ldq, f32, _ptr(pos), _ptr(rope), n_rope, B,
@@ -789,7 +788,7 @@ def _gather_plan(k, v, table, ks, vs, lens, k_out, v_out):
     B = table[1][0] if len(table[1]) else -1
     _, Hkv, fields = _pages_plan(op, k, v, table, ks, vs, B)
     _vec(op, "lens", lens, torch.int32, B)
-    dtype, shape, stride = k_out
+    dtype, shape, stride, _ = k_out
     if v_out != k_out or dtype != torch.bfloat16 or len(shape) != 4 or shape[0] != B or shape[1] != Hkv \
             or shape[3] != 64 or stride[3] != 1:
         _refuse(op, f"k_out and v_out must be alike, bf16 [{B}, {Hkv}, rows, 64] with unit inner stride")
@@ -799,7 +798,7 @@ def _gather_plan(k, v, table, ks, vs, lens, k_out, v_out):
         if s < span:
             _refuse(op, "the rows of k_out and v_out must not overlap")
         span = s * n
-    return fields, B, strides, shape[2]
+    return _on(op, k, v, table, ks, vs, lens, k_out, v_out), fields, B, strides, shape[2]
 
 
 @_timed("paged_gather")
@@ -807,9 +806,8 @@ def paged_gather(k_pages, v_pages, table, lens, k_out, v_out, *, k_scale=None, v
     """Rows [0, lens[b]) of every sequence's paged keys and values as bf16 into
     k_out / v_out [B, kv_heads, S, 64] (any strides but the last); the rows
     behind a sequence's length are left as they were."""
-    fields, B, strides, S = _gather_plan(_lay(k_pages), _lay(v_pages), _lay(table), _lay(k_scale), _lay(v_scale),
-                                         _lay(lens), _lay(k_out), _lay(v_out))
-    dev = _on("paged_gather", k_pages, v_pages, table, k_scale, v_scale, lens, k_out, v_out)
+    dev, fields, B, strides, S = _gather_plan(_lay(k_pages), _lay(v_pages), _lay(table), _lay(k_scale), _lay(v_scale),
+                                              _lay(lens), _lay(k_out), _lay(v_out))
     if B == 0 or S == 0:
         return
     _call("paged_gather", lib().cdk_paged_gather, dev, _cache_arg(k_pages, v_pages, k_scale, v_scale, table, fields), B,
@@ -817,9 +815,10 @@ def paged_gather(k_pages, v_pages, table, lens, k_out, v_out, *, k_scale=None, v
     _count(1)
 
 
-def paged_attn_workspace(B, H, kv_heads):
-    """Bytes of workspace that paged_attn needs."""
-    n = int(lib().cdk_paged_attn_workspace(B, H, kv_heads))
+def paged_attn_workspace(B, H, kv_heads, max_keys=1 << 30):
+    """Bytes of workspace that paged_attn needs for tables of max_keys keys per
+    sequence (the default: whatever the table); short tables need none."""
+    n = int(lib().cdk_paged_attn_workspace(B, H, kv_heads, max_keys))
     if n < 0:
         _refuse("paged_attn", f"B={B}, H={H}, kv_heads={kv_heads}: at most 16384 sequences, H a multiple of kv_heads "
                 "with at most 16 query heads each")
@@ -839,11 +838,11 @@ def _attn_plan(k, v, table, ks, vs, q, lens, out, workspace):
     if q[1][1] != cols:
         _refuse(op, "q and out must have the same heads")
     _vec(op, "lens", lens, torch.int32, B)
-    need = paged_attn_workspace(B, cols // 64, Hkv)
-    if workspace is not None and (workspace[0] != torch.uint8 or len(workspace[1]) != 1 or workspace[2] != (1,)
+    need = paged_attn_workspace(B, cols // 64, Hkv, table[1][1] * k[1][2])
+    if need and workspace is not None and (workspace[0] != torch.uint8 or len(workspace[1]) != 1 or workspace[2] != (1,)
                                   or workspace[1][0] < need):
         _refuse(op, f"workspace must be contiguous uint8 of at least {need} bytes")
-    return fields, B, cols // 64, ldq, ldo, need, 2 if table[1][1] * k[1][2] > 32 else 1  # an item of one tile needs no join
+    return _on(op, k, v, table, ks, vs, q, lens, out, workspace), fields, B, cols // 64, ldq, ldo, need
 
 
 @_timed("paged_attn")
@@ -853,18 +852,17 @@ def paged_attn(q, k_pages, v_pages, table, lens, out, *, k_scale=None, v_scale=N
     (grouped queries).  A sequence of length 0 gets zeros.  workspace (uint8,
     paged_attn_workspace bytes): allocated here when not given; a given one must
     not be shared by calls that can overlap."""
-    fields, B, H, ldq, ldo, need, launches = _attn_plan(
+    dev, fields, B, H, ldq, ldo, need = _attn_plan(
         _lay(k_pages), _lay(v_pages), _lay(table), _lay(k_scale), _lay(v_scale), _lay(q), _lay(lens), _lay(out),
         _lay(workspace))
-    dev = _on("paged_attn", k_pages, v_pages, table, k_scale, v_scale, q, lens, out, workspace)
     if B == 0:
         return
-    if workspace is None:
+    if need and workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=k_pages.device)
     _call("paged_attn", lib().cdk_paged_attn, dev, q.data_ptr(), ldq,
           _cache_arg(k_pages, v_pages, k_scale, v_scale, table, fields), B, H, lens.data_ptr(), out.data_ptr(), ldo,
-          scale, workspace.data_ptr(), need)
-    _count(launches)
+          scale, workspace.data_ptr() if need else None, need)
+    _count(2 if need else 1)  # the item kernel, or the deal and the join
 
 
 # ---------------------------------------------------------------------------
@@ -901,7 +899,7 @@ def _stats_plan(logits, target32, lp, entropy, lse, top_ids, top_lp, ncls):
             _refuse(op, f"top_ids / top_lp must be contiguous int32 / fp32 [{rows}, k], k <= min({MAX_TOP}, classes)")
         if k == 1 and rows > 1 and (top_ids[2][0] != 1 or top_lp[2][0] != 1):
             _refuse(op, "top_ids / top_lp must be contiguous")
-    return rows, ncls, ldl, dt, k
+    return _on(op, logits, target32, lp, entropy, lse, top_ids, top_lp), rows, ncls, ldl, dt, k
 
 
 @_timed("token_logprobs")
@@ -910,9 +908,8 @@ def token_logprobs(logits, target32, lp, *, entropy=None, lse=None, top_ids=None
     [0, ncls)), and where given the entropy, the log-sum-exp and the k best
     classes (top_ids int32 [rows, k], top_lp fp32 [rows, k], k <= 32; equal
     logits in order of their index).  fp32 outputs."""
-    rows, ncls, ldl, dt, k = _stats_plan(_lay(logits), _lay(target32), _lay(lp), _lay(entropy), _lay(lse),
-                                         _lay(top_ids), _lay(top_lp), ncls)
-    dev = _on("token_logprobs", logits, target32, lp, entropy, lse, top_ids, top_lp)
+    dev, rows, ncls, ldl, dt, k = _stats_plan(_lay(logits), _lay(target32), _lay(lp), _lay(entropy), _lay(lse),
+                                              _lay(top_ids), _lay(top_lp), ncls)
     if rows == 0:
         return
     _call("token_logprobs", lib().cdk_token_logprobs, dev, logits.data_ptr(), dt, ldl, rows, ncls,
@@ -929,7 +926,8 @@ def _stats_bwd_plan(logits, target32, lse, entropy, dlp, dentropy, dlogits, ncls
         _refuse(op, "dentropy needs the forward's entropy")
     for name, lay in (("lse", lse), ("entropy", entropy), ("dlp", dlp), ("dentropy", dentropy)):
         _vec(op, name, lay, torch.float32, rows)
-    return rows, ncls, ldl, dt, _rows2d(op, "dlogits", dlogits, (logits[0],), rows, ncls)
+    ldd = _rows2d(op, "dlogits", dlogits, (logits[0],), rows, ncls)
+    return _on(op, logits, target32, lse, entropy, dlp, dentropy, dlogits), rows, ncls, ldl, dt, ldd
 
 
 @_timed("token_logprobs_bwd")
@@ -938,9 +936,8 @@ def token_logprobs_bwd(logits, target32, lse, entropy, dlp, dentropy, dlogits, *
     from the forward's lse and entropy; dlp / dentropy fp32 [rows], either may be
     None (zero; entropy is then not needed for dentropy None).  dlogits has the
     logits' type and may be the same tensor."""
-    rows, ncls, ldl, dt, ldd = _stats_bwd_plan(_lay(logits), _lay(target32), _lay(lse), _lay(entropy), _lay(dlp),
-                                               _lay(dentropy), _lay(dlogits), ncls)
-    dev = _on("token_logprobs_bwd", logits, target32, lse, entropy, dlp, dentropy, dlogits)
+    dev, rows, ncls, ldl, dt, ldd = _stats_bwd_plan(_lay(logits), _lay(target32), _lay(lse), _lay(entropy), _lay(dlp),
+                                                    _lay(dentropy), _lay(dlogits), ncls)
     if rows == 0:
         return
     _call("token_logprobs_bwd", lib().cdk_token_logprobs_bwd, dev, logits.data_ptr(), dt, ldl, rows, ncls,

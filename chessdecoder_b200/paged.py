@@ -255,7 +255,7 @@ class PagedBackbone(_Backbone):
         else:
             if self._step == "warm":
                 self._step = _Captured(self)
-            h = self._step.replay(ids, ov, om)
+            h = self._step.replay(self, ids, ov, om)
         self.cache.advance(flags)
         return h
 
@@ -298,14 +298,15 @@ class PagedBackbone(_Backbone):
 
 
 class _Captured:
-    """PagedBackbone.step as a CUDA graph with static inputs."""
+    """PagedBackbone.step as a CUDA graph with static inputs.  (It does not hold
+    the backbone: a cycle would leave the graph's end to the garbage collector,
+    which may run while another graph is being captured, and that ends a capture.)"""
 
     def __init__(self, bb: PagedBackbone):
         dev, B = bb.device, bb.B
         self.ids = torch.zeros(B, 1, dtype=torch.int64, device=dev)
         self.ov = torch.zeros(B, 1, device=dev)
         self.om = torch.zeros(B, 1, dtype=torch.bool, device=dev)
-        self.bb = bb
         self.graph = torch.cuda.CUDAGraph()
         torch.cuda.synchronize(dev)
         n0 = K.LAUNCHES[0]
@@ -315,7 +316,7 @@ class _Captured:
         K.LAUNCHES[0] = n0
         self.out16 = bb.last_hidden16
 
-    def replay(self, ids, ov, om):
+    def replay(self, bb: PagedBackbone, ids, ov, om):
         self.ids.copy_(ids, non_blocking=True)
         for buf, t in ((self.ov, ov), (self.om, om)):
             if t is None:
@@ -324,7 +325,7 @@ class _Captured:
                 buf.copy_(t.reshape(buf.shape), non_blocking=True)
         self.graph.replay()
         K.LAUNCHES[0] += self.n_launch
-        self.bb.last_hidden16 = self.out16
+        bb.last_hidden16 = self.out16
         return self.out
 
 

@@ -469,9 +469,10 @@ int cdk_paged_gather(const CdkPagedCache* cache, int64_t B, const int32_t* lens,
  * h / (H / kv_heads) (H a multiple of kv_heads, at most 16 query heads each).
  * q, out bf16 [B, H * 64] with pitches ldq, ldo (multiples of 8, 16-byte aligned
  * bases).  lens[b] == 0 gives zeros.  B <= 16384.  workspace:
- * cdk_paged_attn_workspace bytes, 16-byte aligned, not shared by calls that can
- * overlap; nothing in it needs clearing or is kept between calls. */
-int64_t cdk_paged_attn_workspace(int64_t B, int64_t H, int64_t kv_heads);
+ * cdk_paged_attn_workspace bytes for tables that hold max_keys = width * page_size
+ * keys (0 bytes where short tables need none), 16-byte aligned, not shared by
+ * calls that can overlap; nothing in it needs clearing or is kept between calls. */
+int64_t cdk_paged_attn_workspace(int64_t B, int64_t H, int64_t kv_heads, int64_t max_keys);
 int cdk_paged_attn(const void* q, int64_t ldq, const CdkPagedCache* cache, int64_t B, int64_t H, const int32_t* lens,
                    void* out, int64_t ldo, float scale, void* workspace, int64_t workspace_bytes, void* stream);
 

@@ -50,3 +50,14 @@ def test_cache_types_and_refusals():
     for cfg in (ModelConfig(moe_experts=4), ModelConfig(embed_dim=256, num_heads=2)):
         with pytest.raises(ValueError):
             PagedBackbone(cfg, 2, device="cpu")
+
+
+def test_captured_steps_form_no_cycle():
+    """What a backbone keeps of its graphs does not point back at it, so that it
+    (and its graphs) end with its last reference, not in a later collection."""
+    import inspect
+
+    from chessdecoder_b200 import paged
+    for cls in (paged._Captured, paged._GenLoop):
+        source = inspect.getsource(cls)
+        assert "self.bb" not in source and "= bb\n" not in source

@@ -1,8 +1,6 @@
 """Refusals of the paged cache's entry points without a GPU: the Python wrappers'
 argument checks on CPU tensors, and the C entries' host checks (they return
 before any launch)."""
-import ctypes as C
-
 import pytest
 import torch
 
@@ -38,7 +36,8 @@ def _attn(**kw):
     (dict(q=_z(3, 128)), "q must be"), (dict(q=_z(3, 256, dtype=torch.float32)), "q must be"),
     (dict(out=_z(3, 192), q=_z(3, 192)), "multiple of"), (dict(out=_z(3, 100), q=_z(3, 100)), "H \\* 64"),
     (dict(out=_z(3, 64 * 34), q=_z(3, 64 * 34)), "at most 16"),
-    (dict(workspace=_z(1, dtype=torch.uint8)), "workspace"), (dict(), "need CUDA tensors"),
+    (dict(table=_z(3, 99, dtype=I32), workspace=_z(1, dtype=torch.uint8)), "workspace"),
+    (dict(), "need CUDA tensors"),
 ])
 def test_attn_refuses(kw, why):
     with pytest.raises(RuntimeError, match=why):
@@ -70,29 +69,27 @@ def test_gather_refuses(ko, vo, why):
 
 
 def _cache(**kw):
-    c = _lib.CdkPagedCache(k=4096, v=8192, k_scale=None, v_scale=None, table=64, ldt=2, width=2, num_pages=4,
-                           ld_page=2 * 16 * 64, ld_scale=0, kv_heads=2, page_size=16, dtype=0)
-    for k, v in kw.items():
-        setattr(c, k, v)
-    return c
+    c = dict(k=4096, v=8192, k_scale=0, v_scale=0, table=64, ldt=200, width=200, num_pages=4, ld_page=2 * 16 * 64,
+             ld_scale=0, kv_heads=2, page_size=16, dtype=0, reserved=0)
+    return _lib.PAGED_CACHE.pack(*{**c, **kw}.values())
 
 
 #: refused by the C entries before anything is launched (the addresses are never followed)
-BAD_CACHE = [(dict(k=None), -1), (dict(table=None), -1), (dict(dtype=2), -2), (dict(dtype=1), -3),
+BAD_CACHE = [(dict(k=0), -1), (dict(table=0), -1), (dict(dtype=2), -2), (dict(dtype=1), -3),
              (dict(page_size=12), -4), (dict(page_size=0), -4), (dict(kv_heads=0), -4), (dict(num_pages=0), -5),
-             (dict(ldt=1), -5), (dict(ld_page=2000), -6), (dict(ld_page=2 * 16 * 64 + 4), -6), (dict(k=4100), -7)]
+             (dict(ldt=199), -5), (dict(ld_page=2000), -6), (dict(ld_page=2 * 16 * 64 + 4), -6), (dict(k=4100), -7)]
 
 
 @pytest.mark.parametrize("kw,rc", BAD_CACHE)
 def test_c_entries_refuse_a_bad_cache(kw, rc):
-    lib, c = _lib.load(), C.byref(_cache(**kw))
+    lib, c = _lib.load(), _cache(**kw)
     assert lib.cdk_paged_attn(64, 128, c, 3, 2, 64, 64, 128, 0.125, 64, 1 << 30, None) == rc
     assert lib.cdk_paged_append(64, 384, 0, None, None, 0, 3, 1, 2, c, 64, None, None, 0, None) == rc
     assert lib.cdk_paged_gather(c, 3, 64, 64, 64, 64, 64, 64, 5, None) == rc
 
 
 def test_c_entries_refuse_bad_arguments():
-    lib, c = _lib.load(), C.byref(_cache())
+    lib, c = _lib.load(), _cache()
     attn = lambda q=64, ldq=128, B=3, H=2, out=64, ldo=128, scale=0.125, ws=64, n=1 << 40: lib.cdk_paged_attn(  # noqa: E731
         q, ldq, c, B, H, 64, out, ldo, scale, ws, n, None)
     assert attn(q=None) == -10 and attn(H=3) == -11 and attn(H=34) == -11 and attn(B=20000) == -11
@@ -106,7 +103,8 @@ def test_c_entries_refuse_bad_arguments():
     assert app(B=1 << 39, S=4) == -14 and app(S=0) == 0
     gat = lambda B=3, sb=64, S=5, ko=64: lib.cdk_paged_gather(c, B, 64, ko, 64, sb, 64, 64, S, None)  # noqa: E731
     assert gat(ko=None) == -10 and gat(sb=60) == -11 and gat(ko=72) == -11 and gat(B=70000) == -12 and gat(S=0) == 0
-    assert lib.cdk_paged_attn_workspace(3, 5, 2) == -1 and lib.cdk_paged_attn_workspace(3, 4, 2) > 0
+    assert lib.cdk_paged_attn_workspace(3, 5, 2, 9) == -1 and lib.cdk_paged_attn_workspace(3, 4, 2, -1) == -1
+    assert lib.cdk_paged_attn_workspace(3, 4, 2, 5000) > 0 and lib.cdk_paged_attn_workspace(3, 4, 2, 64) == 0
 
 
 def test_the_tests_own_e4m3_is_torchs():
