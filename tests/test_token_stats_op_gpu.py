@@ -77,6 +77,7 @@ def test_op_forward_and_backward_in_a_graph():
             x.grad = torch.autograd.grad(loss_of(lp, ent, c), x)[0]
     torch.cuda.current_stream().wait_stream(s)
     eager = x.grad.clone()
+    del lp, ent  # no eager graph of the leaf lives during the capture
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g):
         lp, ent, *_ = torch.ops.cdk.token_logprobs(x, t, 0)
