@@ -881,7 +881,7 @@ static_assert(kMaxGroup * (kHD * 4 + 8) <= kStages * kStageBytes, "a warp's resu
 // blocks share the item.
 template <int NT>
 __device__ __forceinline__ void merge_block(const AttnArgs& a, const AttnShared& sh, const Acc<NT>& acc, int b, int kvh,
-                                            bool whole, long long slot) {
+                                            bool whole, int slot) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
   __syncwarp();  // every lane is done with the ring
 #pragma unroll
@@ -913,7 +913,7 @@ __device__ __forceinline__ void merge_block(const AttnArgs& a, const AttnShared&
     if (whole) {
       store_out8(a, b, kvh * a.group + hq, d, v, l == 0.f ? 0.f : 1.f / l);
     } else {
-      const long long at = slot * a.group + hq;
+      const int at = slot * a.group + hq;
       float4* dst = reinterpret_cast<float4*>(a.part + at * kHD + d);
       dst[0] = make_float4(v[0], v[1], v[2], v[3]);
       dst[1] = make_float4(v[4], v[5], v[6], v[7]);
@@ -983,48 +983,48 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 3) paged_attn_kern
       for (int i = tid; i < kvn * a.group * (kHD / 8); i += kAttnThreads)
         *reinterpret_cast<uint4*>(a.out + (long long)b * a.ldo + i * 8) = make_uint4(0u, 0u, 0u, 0u);
 
-  const long long total = (long long)prefix[a.B] * kvn;
-  const long long n_warps = (long long)gridDim.x * kWarps;
-  const long long chunk = (total + n_warps - 1) / n_warps;
-  const long long w0 = (long long)blockIdx.x * kWarps, w = w0 + warp;
-  const long long block_f = w0 * chunk, block_end = min(block_f + kWarps * chunk, total);
+  // shares, and w * chunk with them, fit 32 bits: total < 2^31 (checked on the host)
+  const unsigned total = (unsigned)prefix[a.B] * kvn, n_warps = gridDim.x * kWarps;
+  const unsigned chunk = (total + n_warps - 1) / n_warps;
+  const unsigned w0 = blockIdx.x * kWarps, w = w0 + warp;
+  const unsigned block_f = w0 * chunk, block_end = min(block_f + kWarps * chunk, total);
   if (block_f >= block_end) return;
-  long long f = w * chunk;
-  const long long f_end = min(f + chunk, total);
+  unsigned f = w * chunk;
+  const unsigned f_end = min(f + chunk, total);
 
   struct Item {
-    int b, kvh, n;    // n: its shares
-    long long first;  // the first of them
+    int b, kvh, n;   // n: its shares
+    unsigned first;  // the first of them
   };
-  auto item_of = [&](long long x) {  // of share x < total
-    int lo = 0, hi = a.B;            // last b with prefix[b] * kv_heads <= x
+  auto item_of = [&](unsigned x) {  // of share x < total
+    int lo = 0, hi = a.B;           // last b with prefix[b] * kv_heads <= x
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if ((long long)prefix[mid] * kvn <= x) lo = mid;
+      if ((unsigned)prefix[mid] * kvn <= x) lo = mid;
       else hi = mid;
     }
     Item it;
     it.b = lo;
     it.n = prefix[lo + 1] - prefix[lo];
-    const long long first = (long long)prefix[lo] * kvn;
-    it.kvh = (int)((unsigned)(x - first) / (unsigned)it.n);  // below n * kv_heads < 2^31
-    it.first = first + (long long)it.kvh * it.n;
+    const unsigned first = (unsigned)prefix[lo] * kvn;
+    it.kvh = (int)((x - first) / (unsigned)it.n);
+    it.first = first + it.kvh * it.n;
     return it;
   };
   const Item bi = item_of(block_f);
   if (block_end <= bi.first + bi.n) {  // the block is inside one item
-    const int ta = (int)max(f - bi.first - kSetup, 0ll), tb = (int)(f_end - bi.first) - kSetup;
+    const int ta = max((int)(f - bi.first) - kSetup, 0), tb = (int)(f_end - bi.first) - kSetup;
     Acc<NT> acc;
     acc.clear();
     if (f < f_end && ta < tb) attend<FP8, NT>(a, bi.b, bi.kvh, ta, tb, length_of(a, bi.b, false), lane, ring, acc);
     acc.sum_lanes();
-    merge_block<NT>(a, sh, acc, bi.b, bi.kvh, block_f == bi.first && block_end == bi.first + bi.n, 2 * w0);
+    merge_block<NT>(a, sh, acc, bi.b, bi.kvh, block_f == bi.first && block_end == bi.first + bi.n, 2 * (int)w0);
     return;
   }
   while (f < f_end) {
     const Item it = item_of(f);
-    const long long last = min(it.first + it.n, f_end);
-    const int ta = (int)max(f - it.first - kSetup, 0ll), tb = (int)(last - it.first) - kSetup;
+    const unsigned last = min(it.first + it.n, f_end);
+    const int ta = max((int)(f - it.first) - kSetup, 0), tb = (int)(last - it.first) - kSetup;
     f = last;
     if (ta >= tb) continue;  // nothing but the item's setup
     Acc<NT> acc;
@@ -1032,7 +1032,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 3) paged_attn_kern
     attend<FP8, NT>(a, it.b, it.kvh, ta, tb, length_of(a, it.b, false), lane, ring, acc);
     acc.sum_lanes();
     const bool whole = ta == 0 && tb == it.n - kSetup;
-    const long long slot = 2 * w + (ta == 0 ? 1 : 0);
+    const int slot = 2 * (int)w + (ta == 0 ? 1 : 0);
     const int g = lane >> 2, t4 = lane & 3;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -1045,7 +1045,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 3) paged_attn_kern
         if (whole) {
           store_out8(a, it.b, it.kvh * a.group + hq, 8 * g, v, acc.l[n][c] == 0.f ? 0.f : 1.f / acc.l[n][c]);
         } else {
-          const long long at = slot * a.group + hq;
+          const int at = slot * a.group + hq;
           float4* dst = reinterpret_cast<float4*>(a.part + at * kHD + 8 * g);
           dst[0] = make_float4(v[0], v[1], v[2], v[3]);
           dst[1] = make_float4(v[4], v[5], v[6], v[7]);
@@ -1060,7 +1060,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 3) paged_attn_kern
 // slot 0; other warps left the item they end in slot 0, the one they begin in
 // slot 1.  One block per (sequence, query head); warp i takes every fourth result,
 // lane l dims 2l and 2l + 1.
-__global__ void __launch_bounds__(128) paged_attn_join_kernel(const AttnArgs a, long long n_warps) {
+__global__ void __launch_bounds__(128) paged_attn_join_kernel(const AttnArgs a, unsigned n_warps) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int heads = a.pg.kv_heads * a.group;
   const int b = blockIdx.x / heads, h = blockIdx.x - b * heads;
@@ -1068,20 +1068,20 @@ __global__ void __launch_bounds__(128) paged_attn_join_kernel(const AttnArgs a, 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int before = a.prefix[b], shares = a.prefix[b + 1] - before;
   if (shares == 0) return;
-  const long long total = (long long)a.prefix[a.B] * a.pg.kv_heads;
-  const long long chunk = (total + n_warps - 1) / n_warps, span = chunk * kWarps;
-  const long long first = (long long)before * a.pg.kv_heads + (long long)kvh * shares, end = first + shares;
+  const unsigned kvn = a.pg.kv_heads, total = (unsigned)a.prefix[a.B] * kvn;
+  const unsigned chunk = (total + n_warps - 1) / n_warps, span = chunk * kWarps;
+  const unsigned first = before * kvn + kvh * shares, end = first + shares;
   // warps with tiles of the item
-  const long long w0 = (first + kSetup) / chunk, w1 = (end - 1) / chunk;
+  const int w0 = (int)((first + kSetup) / chunk), w1 = (int)((end - 1) / chunk);
   // blocks inside the item: [c0, c1); each has tiles of it, having more shares than kSetup
   static_assert(kWarps > kSetup, "a block inside an item is more than its setup");
-  const long long c0 = (first + span - 1) / span, c1 = end == total ? (end + span - 1) / span : end / span;
-  const long long inside = max(c1 - c0, 0ll), cw = w0 / kWarps;
-  if (w0 == w1 && !(cw >= c0 && cw < c1)) return;                                      // written by that warp
+  const int c0 = (int)((first + span - 1) / span), c1 = (int)((end == total ? end + span - 1 : end) / span);
+  const int inside = max(c1 - c0, 0), cw = w0 / kWarps;
+  if (w0 == w1 && !(cw >= c0 && cw < c1)) return;                                // written by that warp
   if (inside == 1 && c0 * span == first && min((c0 + 1) * span, total) == end) return;  // written by that block
-  const long long head = inside ? max(c0 * kWarps - w0, 0ll) : w1 - w0 + 1;  // warps before them (all, without them)
-  const long long tail = inside ? max(w1 + 1 - c1 * kWarps, 0ll) : 0;        // and after them
-  const long long n = head + inside + tail;
+  const int head = inside ? max(c0 * kWarps - w0, 0) : w1 - w0 + 1;  // warps before them (all, without them)
+  const int tail = inside ? max(w1 + 1 - c1 * kWarps, 0) : 0;        // and after them
+  const int n = head + inside + tail;
   float m = kNoScore, l = 0.f, x = 0.f, y = 0.f;
   auto add = [&](float2 st, float2 v) {
     const float nm = fmaxf(m, st.x);
@@ -1091,20 +1091,20 @@ __global__ void __launch_bounds__(128) paged_attn_join_kernel(const AttnArgs a, 
     y = y * f0 + v.y * f1;
     m = nm;
   };
-  auto at_of = [&](long long i) {
-    const long long w = i < head ? w0 + i : i < head + inside ? (c0 + i - head) * kWarps : c1 * kWarps + (i - head - inside);
+  auto at_of = [&](int i) {
+    const int w = i < head ? w0 + i : i < head + inside ? (c0 + i - head) * kWarps : c1 * kWarps + (i - head - inside);
     const bool begins = (i < head && i == 0);
     return (2 * w + (begins ? 1 : 0)) * a.group + hq;
   };
-  for (long long i = warp; i < n; i += 4 * kWarps) {  // four results in flight
+  for (int i = warp; i < n; i += 4 * kWarps) {  // four results in flight
     float2 st[4], v[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const long long k = i + u * kWarps;
+      const int k = i + u * kWarps;
       st[u] = make_float2(kNoScore, 0.f);
       v[u] = make_float2(0.f, 0.f);
       if (k < n) {
-        const long long at = at_of(k);
+        const int at = at_of(k);
         st[u] = a.stat[at];
         v[u] = *reinterpret_cast<const float2*>(a.part + at * kHD + 2 * lane);
       }
@@ -1256,7 +1256,7 @@ cudaError_t launch_attn(const AttnArgs& a, long long max_tiles, cudaStream_t st)
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_attn_join_kernel, (const AttnArgs)a, (long long)grid * kWarps);
+  return cudaLaunchKernelEx(&cfg, paged_attn_join_kernel, (const AttnArgs)a, grid * (unsigned)kWarps);
 }
 }  // namespace
 
