@@ -182,12 +182,22 @@ __device__ __forceinline__ Stat stream(const Row<BF16>& row, int first, int tid,
       for (int i = 0; i < N; ++i) s2[i & 1] += ex2((x[i] - st.m) * kLog2e);
     }
   };
-#pragma unroll 1
-  for (; first + kUnroll * STEP <= last; first += kUnroll * STEP) {  // chunks that every thread has whole
-    const int v = first + tid;
-    uint4 raw[kUnroll];
+  uint4 raw[kUnroll];
+  bool more = first + kUnroll * STEP <= last;  // a chunk that every thread has whole
+  if (more) {
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) raw[u] = row.load(v + u * STEP);
+    for (int u = 0; u < kUnroll; ++u) raw[u] = row.load(first + tid + u * STEP);
+  }
+#pragma unroll 1
+  while (more) {
+    const int v = first + tid;
+    first += kUnroll * STEP;
+    more = first + kUnroll * STEP <= last;
+    uint4 next[kUnroll];
+    if (more) {  // the next chunk is on its way while this one is added up
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) next[u] = row.load(first + tid + u * STEP);
+    }
     float cm = vector_max<BF16>(raw[0]);
 #pragma unroll
     for (int u = 1; u < kUnroll; ++u) cm = fmaxf(cm, vector_max<BF16>(raw[u]));
@@ -197,10 +207,11 @@ __device__ __forceinline__ Stat stream(const Row<BF16>& row, int first, int tid,
     for (int u = 0; u < kUnroll; ++u) add(raw[u], s2, t2);
     st.s += s2[0] + s2[1];
     st.t += t2[0] + t2[1];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) raw[u] = next[u];
   }
   const int v = first + tid;
   if (v < last) {  // what is left: a vector at least
-    uint4 raw[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
       if (v + u * STEP < last) raw[u] = row.load(v + u * STEP);
@@ -406,7 +417,7 @@ constexpr int kWarpsPerBlock = 8;
 constexpr int kWarpCandidates = 160;  // the slow way is short here, and shared memory is warps
 
 template <bool BF16, bool TOP>
-__global__ void __launch_bounds__(kWarpsPerBlock * 32, TOP ? 4 : 6) token_stats_warp_kernel(const Args a) {
+__global__ void __launch_bounds__(kWarpsPerBlock * 32, TOP ? 4 : 5) token_stats_warp_kernel(const Args a) {
   __shared__ uint64_t cand_s[TOP ? kWarpsPerBlock : 1][TOP ? kWarpCandidates : 1];
   __shared__ int count_s[kWarpsPerBlock], owners_s[TOP ? kWarpsPerBlock : 1][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -464,7 +475,7 @@ __device__ __forceinline__ const T* remote(const T* p, uint32_t rank) {
 }
 
 template <bool BF16, bool TOP>
-__global__ void __launch_bounds__(kThreads, TOP ? 4 : 6) token_stats_block_kernel(const Args a, int blocks_per_row) {
+__global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) token_stats_block_kernel(const Args a, int blocks_per_row) {
   __shared__ RowShared<TOP> sh;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long r = blockIdx.x / blocks_per_row;
