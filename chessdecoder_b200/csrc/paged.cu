@@ -733,7 +733,7 @@ __device__ __forceinline__ void attend_e4m3(const AttnArgs& a, int b, int kvh, i
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
     // largest in [2^14, 2^15): fp16 then holds all 8 bits of whatever is above 2^-31 of it
-    const int e = min(max((int)(top >> 7), 15), 250);  // exponent field; the factor 2^(141 - e) is a normal number
+    const int e = max((int)(top >> 7), 15);  // exponent field, <= 255; the factor 2^(141 - e) is a normal number
     const float up = __uint_as_float((uint32_t)(127 + 141 - e) << 23);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -781,7 +781,7 @@ __device__ __forceinline__ void attend_e4m3(const AttnArgs& a, int b, int kvh, i
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int c = 0; c < 2; ++c) s[n][r][c] = d[n][2 * h + c] * qs[n][c] * ks;
+          for (int c = 0; c < 2; ++c) s[n][r][c] = d[n][2 * h + c] * (qs[n][c] * ks);
       }
     }
     if (mask != 0xffffffffu) {

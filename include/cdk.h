@@ -415,7 +415,7 @@ int cdk_mish_bf16(const float* z, int64_t ldz, int64_t rows, int64_t cols, void*
  *             [num_pages][kv_heads][page_size][64], ld_page elements from page
  *             to page (a multiple of 8 for bf16, 16 for e4m3; 16-byte aligned
  *             base)
- *   k_scale, v_scale   dtype 1: one byte e per row, [num_pages][kv_heads]
+ *   k_scale, v_scale   dtype 1: one byte e, 1 .. 254, per row, [num_pages][kv_heads]
  *             [page_size], ld_scale bytes from page to page; the row stands for
  *             code * 2^(e - 127).  dtype 0: unused.
  *   table     int32 [B][width], row pitch ldt: row j of sequence b is row

@@ -115,3 +115,38 @@ def test_the_tests_own_e4m3_is_torchs():
     unit = torch.pow(torch.tensor(2.0, dtype=torch.float64), e.double())
     assert (top <= 448 * unit).all() and (top > 224 * unit).all()
     assert ((v - x).abs() <= (2.0 ** -4 * x.abs()).double().maximum(2.0 ** -10 * unit[:, None])).all()
+
+
+def test_calls_launch_on_the_tensors_device(monkeypatch):
+    """A call on tensors of another device than the current one makes that device
+    current around the launch and takes its stream."""
+    seen, current = [], [0]
+
+    class Device:
+        def __init__(self, i):
+            self.i = i
+
+        def __enter__(self):
+            self.was, current[0] = current[0], self.i
+
+        def __exit__(self, *a):
+            current[0] = self.was
+
+    monkeypatch.setattr(K, "_current_device", lambda: current[0])
+    monkeypatch.setattr(K, "_raw_stream", lambda dev: 100 + dev)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    fn = lambda *a: seen.append((current[0], a)) or 0  # noqa: E731
+    K._call("op", fn, 0, 7)
+    K._call("op", fn, 3, 8)
+    assert seen == [(0, (7, 100)), (3, (8, 103))] and current[0] == 0
+    with pytest.raises(RuntimeError, match="op failed with status -5"):
+        K._call("op", lambda *a: -5, 0)
+
+
+def test_layouts_of_different_devices_are_refused():
+    lay = lambda dev: (torch.float32, (3,), (1,), dev)  # noqa: E731
+    assert K._on("op", lay(1), None, lay(1)) == 1
+    with pytest.raises(RuntimeError, match="different devices"):
+        K._on("op", lay(1), lay(0))
+    with pytest.raises(RuntimeError, match="need CUDA tensors"):
+        K._on("op", lay(-1), lay(-1))

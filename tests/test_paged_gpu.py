@@ -241,6 +241,31 @@ def test_attn_sharp_and_flat_scores(fp8):
 
 
 @pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("qe,ke,se", [(125, -113, -12), (-120, 100, 20), (0, -126, 126), (60, 60, -120)])
+def test_attn_far_magnitudes(qe, ke, se, fp8):
+    """Queries and keys near the ends of the number range whose scores are ordinary,
+    values of 2^-90 and rows of zeros among them."""
+    lens, H, p = [70, 33], 4, 16
+    table, n = table_of(lens, p, 3)
+    kp, vp, ks, vs = pool(n, 2, p, fp8, 3)
+    if fp8:
+        ks = (ks.view(torch.uint8).int() + ke).clamp(1, 247).to(torch.uint8).view(torch.float8_e8m0fnu)
+        vs = (vs.view(torch.uint8).int() - 90).to(torch.uint8).view(torch.float8_e8m0fnu)
+        vp.view(torch.uint8)[:, :, ::3] = 0
+        vs.view(torch.uint8)[:, :, ::3] = 1
+    else:
+        kp, vp = (kp.float() * 2.0 ** ke).to(torch.bfloat16), (vp.float() * 2.0 ** -90).to(torch.bfloat16)
+        vp[:, :, ::3] = 0
+    g = torch.Generator().manual_seed(2)
+    q = (torch.randn(2, H * D, generator=g).clamp(-3, 3) * 2.0 ** qe).to(torch.bfloat16).to(DEV)
+    out = torch.empty(2, H * D, dtype=torch.bfloat16, device=DEV)
+    scale = 0.125 * 2.0 ** se
+    K.paged_attn(q, kp, vp, table, torch.tensor(lens, dtype=torch.int32, device=DEV), out, k_scale=ks, v_scale=vs,
+                 scale=scale)
+    check_attn(out, q, kp, vp, ks, vs, table, lens, H, scale)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
 def test_attn_strides_and_layer_views(fp8):
     lens, H, Hkv, p = [90, 0, 17], 6, 3, 16
     table, n = table_of(lens, p, 4, width=None)
