@@ -77,7 +77,12 @@ __device__ __forceinline__ int page_of(const Pages& p, long long b, long long j)
 // its sequence, place in the cache, position and rotation -- is found once.  The
 // rotation is three separately rounded operations per value (no fused multiply-
 // add), so that a quantised code does not depend on how a compiler contracts
-// them.  Bound by HBM: one read of qkv, one write of each row.
+// them.  Bound by HBM: one read of qkv, one write of each row.  Measured on one
+// B200 (16 + 16 + 16 heads): 18,200 fp32 tokens rotated into bf16 pages 54 us, 96%
+// of the copy rate, into e4m3 pages 51 us (90%); bf16 rows into e4m3 pages 27 us
+// (64%: a third of the bytes for the same 30 instructions a row; issue slots are
+// 65% busy).  A lane per eight values with all indices its own took 70 us there,
+// a warp per token whose row loads came after the place was looked up 35.
 // ---------------------------------------------------------------------------
 template <bool F32, bool FP8>
 __global__ void __launch_bounds__(256, 4)
@@ -201,7 +206,10 @@ __global__ void __launch_bounds__(256, 4)
 // ---------------------------------------------------------------------------
 // Read back.  Grid (chunks of 128 rows, kv head, sequence); a lane takes 16 bytes of
 // a key row and of its value row, of four (bf16) or two (e4m3) rows at a time.
-// Bound by HBM: one read of the pages, one write of the rows.
+// Bound by HBM: one read of the pages, one write of the rows.  Measured on one B200:
+// 16 sequences of up to 8191 tokens, 16 heads: e4m3 67 us (95% of the copy rate; 81
+// with 16 contiguous bytes of codes a lane, whose two stores each fill half a
+// sector), bf16 86 us (98%).
 // ---------------------------------------------------------------------------
 constexpr int kGatherRows = 128;
 
@@ -308,6 +316,12 @@ __global__ void __launch_bounds__(256)
 // follow s_j + e_j: weights then fit fp16 (2^-11) whatever the scales are.  The
 // sum of the w_j alone reaches 2^(8 - e_j); e_j below -96 counts as -96 for m (a
 // row of zeros has the smallest scale), which only values below 448 * 2^-96 feel.
+//
+// Measured on one B200 (16 heads, device time, both kernels): bf16, 256 sequences of
+// up to 4095 keys 334 us (2.15 GB: the copy rate), 64 of up to 2000 48 us (85%),
+// 64 x 512 (an item per block) 25 us (83%); e4m3, 256 x 2000 176 us (94%), 6 of up to
+// 65536 with groups of 8 heads 28 us (59%: of the 11 us over the floor about 5 pass
+// before the first rows arrive -- launch, lengths, table, rows -- and 3 in the join).
 // ---------------------------------------------------------------------------
 constexpr int kTK = 32;             // keys per tile
 constexpr int kAttnThreads = 128;   // 4 warps; 128 registers: 4 blocks per SM
@@ -318,11 +332,14 @@ constexpr int kSlots = 2 * kAttnWarps;
 constexpr float kNoScore = -3.0e38f;  // m before the first key
 constexpr float kSlack = 8.f;
 // Tiles per item up to which a block takes an item: the second kernel's launch
-// and the deal's search cost more than a warp's few tiles in a row.
+// and the deal's search cost more than a warp's few tiles in a row (64 x 512 keys:
+// 25 us; the deal takes 30 for 64 x 520; one game of 137 keys: 4.1 us and 6.8).
 constexpr int kItemTiles = 16;
 
 // What beginning an item costs a warp, in tiles of the deal: its table, queries and
-// first rows come one after the other.
+// first rows come one after the other.  (64 sequences of 0 .. 2000 keys: 72 us
+// without, 59 with 1, 50 with 2, 51 with 3 -- a warp that is dealt fourteen items of
+// one tile waits for fourteen such chains.)
 constexpr int kSetup = 2;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -639,7 +656,8 @@ __device__ __forceinline__ void attend_bf16(const AttnArgs& a, int b, int kvh, i
 
 // The same on e4m3 pages.  A tile is half the bytes, so its loads have to be twice
 // as far ahead: they go through a ring of kStages tiles per warp in shared memory
-// (cp.async, rows that do not count filled with zeros), two tiles ahead.
+// (cp.async, rows that do not count filled with zeros), two tiles ahead.  (Through
+// registers, one tile ahead: 266 us against 176 for 256 x 2000 keys x 16 heads.)
 //
 // Stage: 32 key rows, then 32 value rows, of 64 bytes; two rows to a 128-byte
 // line, whose 16-byte chunks are swapped around by twice the line's number, so

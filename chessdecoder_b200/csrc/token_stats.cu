@@ -11,16 +11,21 @@
 //
 // Bound by HBM: the forward reads each logit once, the backward reads and writes
 // it once.  The forward spends one ex2 and about eight other instructions per
-// logit, a half (fp32) to all but a fifth (bf16) of what the SM issues in the
-// time that HBM takes.
+// logit, half (fp32) to most (bf16) of what an SM issues in the time that HBM takes.
 //
 // Alternatives.  Each thread's largest logit comes with its running maximum.  T,
 // the k-th largest of these (as a (value, index) rank), is a lower bound of the
 // k-th best of the row, and only the k threads that reach T can hold one of the
-// k best: their logits are read again (k of 32 or 256 threads' share, from L2),
-// those that reach T are gathered in shared memory -- k and a few -- and sorted by
-// a warp.  So the streaming pass has no work for the alternatives but to note
-// in which of its chunks a thread's maximum lay.
+// k best: their logits are read again (k of 32 or 256 threads' share), those that
+// reach T are gathered in shared memory -- k and a few -- and sorted by a warp.  So
+// the streaming pass has no work for the alternatives but to note in which of its
+// chunks a thread's maximum lay.
+//
+// Measured on one B200 (device time, share of the copy rate): 16384 x 1924 fp32
+// forward 23.5 us (83%), with 5 alternatives 37 us (53%), gradient 41 us (95%); 509 x
+// 131071 bf16 forward 32 us (64%), with 20 alternatives 40 us (52%: selecting takes
+// each block about 4 us at its end, when its neighbours do the same), gradient 43 us
+// (96%); 300 x 131071 fp32 forward 28.6 us (85%).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>
