@@ -72,134 +72,187 @@ __device__ __forceinline__ int page_of(const Pages& p, long long b, long long j)
 }
 
 // ---------------------------------------------------------------------------
-// Append.  A warp takes a token, or every `parts`-th group of four (head) rows of
-// it; eight lanes per row of 64, eight values each.  What belongs to the token --
+// Append.  A warp takes a token, or every `parts`-th group of four heads of it;
+// eight lanes per row of 64, eight values each; key and value of a head together,
+// since they go to the same place of two pools.  What belongs to the token --
 // its sequence, place in the cache, position and rotation -- is found once.  The
 // rotation is three separately rounded operations per value (no fused multiply-
 // add), so that a quantised code does not depend on how a compiler contracts
 // them.  Bound by HBM: one read of qkv, one write of each row.  Measured on one
-// B200 (16 + 16 + 16 heads): 18,200 fp32 tokens rotated into bf16 pages 54 us, 96%
-// of the copy rate, into e4m3 pages 51 us (90%); bf16 rows into e4m3 pages 27 us
-// (64%: a third of the bytes for the same 30 instructions a row; issue slots are
-// 65% busy).  A lane per eight values with all indices its own took 70 us there,
-// a warp per token whose row loads came after the place was looked up 35.
+// B200 (16 + 16 + 16 heads): 18,200 fp32 tokens rotated into bf16 pages 54 us, 97%
+// of the copy rate, into e4m3 pages 49 us (94%); bf16 rows into e4m3 pages 24 us
+// (73%: fewer bytes for the same instructions).  A lane per eight values with all
+// indices its own took 70 us there; a warp per token whose row loads came after
+// the place was looked up 35, before it 27; keys and values together 24.
 // ---------------------------------------------------------------------------
+// Eight values of a row as loaded, and as numbers.
+template <bool F32>
+struct Raw8 {
+  uint4 w[F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const char* p) {
+    w[0] = *reinterpret_cast<const uint4*>(p);
+    if (F32) w[F32 ? 1 : 0] = reinterpret_cast<const uint4*>(p)[1];
+  }
+  __device__ __forceinline__ void values(float (&x)[8]) const {
+    const uint32_t a[4] = {w[0].x, w[0].y, w[0].z, w[0].w};
+    if (F32) {
+      const uint4 c = w[F32 ? 1 : 0];
+      const uint32_t d[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] = __uint_as_float(a[i]);
+        x[4 + i] = __uint_as_float(d[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = bf2f(a[i]);
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+      }
+    }
+  }
+};
+
+// cos and sin of a lane's four pairs.
+struct Turn {
+  float c[4], s[4];
+  __device__ __forceinline__ void load(const float* p) {
+    const float4 x = reinterpret_cast<const float4*>(p)[0], y = reinterpret_cast<const float4*>(p)[1];
+    c[0] = x.x, s[0] = x.y, c[1] = x.z, s[1] = x.w;
+    c[2] = y.x, s[2] = y.y, c[3] = y.z, s[3] = y.w;
+  }
+  __device__ __forceinline__ void apply(float (&x)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float v = x[2 * i], w = x[2 * i + 1];
+      x[2 * i] = __fsub_rn(__fmul_rn(v, c[i]), __fmul_rn(w, s[i]));
+      x[2 * i + 1] = __fadd_rn(__fmul_rn(w, c[i]), __fmul_rn(v, s[i]));
+    }
+  }
+};
+
+__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+  return make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+}
+
+// e4m3 codes of this lane's eight of a row's 64 values; the row is on eight lanes in a
+// row of a warp that is here as a whole.  byte: the scale's.
+__device__ __forceinline__ uint2 quantise8(const float (&x)[8], int* byte) {
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  // least e with amax <= 448 * 2^e (448 = 1.75 * 2^8), as an exponent field: + 1 where the fraction is above 0x600000
+  *byte = max((int)((__float_as_uint(amax) + 0x1fffffu) >> 23) - 8, 1);
+  const float inv = __uint_as_float((uint32_t)(254 - *byte) << 23);
+  uint32_t w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    w[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[4 * i] * inv, x[4 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3) |
+           ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[4 * i + 2] * inv, x[4 * i + 3] * inv), __NV_SATFINITE,
+                                               __NV_E4M3)
+            << 16);
+  return make_uint2(w[0], w[1]);
+}
+
 template <bool F32, bool FP8>
 __global__ void __launch_bounds__(256, 4)
     paged_append_kernel(const void* __restrict__ qkv, long long ldq, const int32_t* __restrict__ pos,
                         const float* __restrict__ rope, long long rope_len, unsigned S_new, int H, Pages pg,
                         const int32_t* __restrict__ start, const int32_t* __restrict__ num_new,
                         __nv_bfloat16* __restrict__ q_out, long long ldo, unsigned tokens, unsigned parts) {
-  constexpr int kU = F32 ? 2 : 4;  // rows in flight per lane: 64 bytes
-  constexpr int kE = FP8 ? 1 : 2;  // bytes per cached value
+  constexpr int kU = F32 ? 1 : 2;          // heads in flight per lane: 64 bytes of key and value rows
+  constexpr int kE = FP8 ? 1 : 2;          // bytes per cached value
+  constexpr int kIn = kHD * (F32 ? 4 : 2);  // bytes of a row of qkv
   const int lane = threadIdx.x & 31, sub = lane & 7;
   const unsigned unit = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const unsigned t = unit / parts, part = unit - t * parts;
   if (t >= tokens) return;
   const unsigned b = t / S_new, s = t - b * S_new;
   if (num_new != nullptr && (int)s >= num_new[b]) return;  // padding
-  const int kvn = pg.kv_heads, heads = H + 2 * kvn;
-  const char* src = reinterpret_cast<const char*>(qkv) + ((long long)t * ldq + sub * 8) * (F32 ? 4 : 2);
-  const int step = parts * 4, sub_row = lane >> 3;
-  uint4 raw[kU][F32 ? 2 : 1];
-  auto load = [&](int h0) {
+  const int kvn = pg.kv_heads, step = parts * 4, h0 = part * 4 + (lane >> 3);
+  const char* src = reinterpret_cast<const char*>(qkv) + (long long)t * ldq * (F32 ? 4 : 2) + sub * (kIn / 8);
+  const char* src_k = src + H * kIn;
+  const int v_off = kvn * kIn;
+  Raw8<F32> kr[kU], vr[kU];
+  auto load = [&](int h) {
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int h = h0 + u * step;
-      raw[u][0] = make_uint4(0u, 0u, 0u, 0u);
-      if (F32) raw[u][F32 ? 1 : 0] = make_uint4(0u, 0u, 0u, 0u);
-      if (h < heads) {
-        const uint4* p = reinterpret_cast<const uint4*>(src + (long long)h * (kHD * (F32 ? 4 : 2)));
-        raw[u][0] = p[0];
-        if (F32) raw[u][F32 ? 1 : 0] = p[1];
+    for (int u = 0; u < kU; ++u)
+      if (h + u * step < kvn) {
+        kr[u].load(src_k + (h + u * step) * kIn);
+        vr[u].load(src_k + (h + u * step) * kIn + v_off);
       }
-    }
   };
-  int h0 = (q_out == nullptr ? H : 0) + part * 4 + sub_row;
   load(h0);  // before what follows, whose loads wait for one another
-  float co[4], si[4];
+  Turn turn;
   if (rope != nullptr) {
     const long long p = pos[t];
     if (p < 0 || p >= rope_len) {
       if (lane == 0) report_error(kErrIndex);
       return;
     }
-    const float4* cs = reinterpret_cast<const float4*>(rope + (p * 32 + sub * 4) * 2);
-    const float4 x = cs[0], y = cs[1];
-    co[0] = x.x, si[0] = x.y, co[1] = x.z, si[1] = x.w;
-    co[2] = y.x, si[2] = y.y, co[3] = y.z, si[3] = y.w;
+    turn.load(rope + (p * 32 + sub * 4) * 2);
   }
   const long long slot = (long long)start[b] + s;
   const int page = page_of(pg, b, slot);  // -1: reported, no row is written
-  const int off = (int)(slot & ((1ll << pg.log_page) - 1));
-  const long long place = (long long)page * pg.ld_page + off * (kHD * kE) + sub * (8 * kE);
-  const long long splace = (long long)page * pg.ld_scale + off;
+  const unsigned off = (unsigned)(slot & ((1ll << pg.log_page) - 1));  // row in its page and head
+  char* dst_k = pg.k + (long long)page * pg.ld_page + sub * (8 * kE);
+  char* dst_v = pg.v + (long long)page * pg.ld_page + sub * (8 * kE);
 
   // (every lane of the warp runs the same number of rounds: the scale's exchange needs its row's eight lanes)
-  while (h0 - sub_row < heads) {
+#pragma unroll 1
+  for (int h = h0; h - (lane >> 3) < kvn; h += kU * step) {
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      const int h = h0 + u * step;
+      const int hh = h + u * step;
+      const bool live = hh < kvn && page >= 0;
+      const unsigned row = ((unsigned)hh << pg.log_page) + off;  // below 2^24 where it is live
       float x[8];
-      if (F32) {
-        const uint4 a = raw[u][0], c = raw[u][F32 ? 1 : 0];
-        x[0] = __uint_as_float(a.x), x[1] = __uint_as_float(a.y), x[2] = __uint_as_float(a.z), x[3] = __uint_as_float(a.w);
-        x[4] = __uint_as_float(c.x), x[5] = __uint_as_float(c.y), x[6] = __uint_as_float(c.z), x[7] = __uint_as_float(c.w);
-      } else {
-        const uint32_t w[4] = {raw[u][0].x, raw[u][0].y, raw[u][0].z, raw[u][0].w};
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const float2 f = bf2f(w[c]);
-          x[2 * c] = f.x;
-          x[2 * c + 1] = f.y;
+      kr[u].values(x);
+      if (rope != nullptr) turn.apply(x);
+      int byte;
+      if (FP8) {
+        const uint2 w = quantise8(x, &byte);
+        if (live) {
+          *reinterpret_cast<uint2*>(dst_k + (size_t)row * (kHD * kE)) = w;
+          if (sub == 0) pg.ks[(long long)page * pg.ld_scale + row] = (uint8_t)byte;
         }
+      } else if (live) {
+        *reinterpret_cast<uint4*>(dst_k + (size_t)row * (kHD * kE)) = pack8(x);
       }
-      const bool is_v = h >= H + kvn;
-      if (rope != nullptr && !is_v) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const float v = x[2 * c], w = x[2 * c + 1];
-          x[2 * c] = __fsub_rn(__fmul_rn(v, co[c]), __fmul_rn(w, si[c]));
-          x[2 * c + 1] = __fadd_rn(__fmul_rn(w, co[c]), __fmul_rn(v, si[c]));
+      vr[u].values(x);
+      if (FP8) {
+        const uint2 w = quantise8(x, &byte);
+        if (live) {
+          *reinterpret_cast<uint2*>(dst_v + (size_t)row * (kHD * kE)) = w;
+          if (sub == 0) pg.vs[(long long)page * pg.ld_scale + row] = (uint8_t)byte;
         }
-      }
-      float amax = 0.f;
-      if (FP8 && h - sub_row + 3 >= H) {  // one of the warp's rows goes to the cache
-#pragma unroll
-        for (int c = 0; c < 8; ++c) amax = fmaxf(amax, fabsf(x[c]));
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-      }
-      if (h >= heads) continue;
-      if (!FP8 || h < H) {
-        const uint4 w =
-            make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
-        if (h < H) {
-          *reinterpret_cast<uint4*>(q_out + (long long)t * ldo + h * kHD + sub * 8) = w;
-        } else if (page >= 0) {
-          const int head = is_v ? h - H - kvn : h - H;
-          *reinterpret_cast<uint4*>((is_v ? pg.v : pg.k) + place + (((long long)head << pg.log_page) * (kHD * kE))) = w;
-        }
-      } else if (page >= 0) {
-        // least e with amax <= 448 * 2^e (448 = 1.75 * 2^8), as an exponent field
-        const uint32_t bits = __float_as_uint(amax);
-        const int byte = max((int)((bits + 0x1fffffu) >> 23) - 8, 1);  // + 1 where the fraction is above 0x600000
-        const float inv = __uint_as_float((uint32_t)(254 - byte) << 23);
-        uint32_t w[2];
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-          w[c] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[4 * c] * inv, x[4 * c + 1] * inv), __NV_SATFINITE,
-                                                    __NV_E4M3) |
-                 ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[4 * c + 2] * inv, x[4 * c + 3] * inv),
-                                                     __NV_SATFINITE, __NV_E4M3)
-                  << 16);
-        const long long head = (long long)(is_v ? h - H - kvn : h - H) << pg.log_page;
-        *reinterpret_cast<uint2*>((is_v ? pg.v : pg.k) + place + head * kHD) = make_uint2(w[0], w[1]);
-        if (sub == 0) (is_v ? pg.vs : pg.ks)[splace + head] = (uint8_t)byte;
+      } else if (live) {
+        *reinterpret_cast<uint4*>(dst_v + (size_t)row * (kHD * kE)) = pack8(x);
       }
     }
-    h0 += kU * step;
-    load(h0);
+    load(h + kU * step);
+  }
+
+  if (q_out == nullptr) return;
+  uint4* qo = reinterpret_cast<uint4*>(q_out + (long long)t * ldo) + sub;
+  constexpr int kQ = 2 * kU;
+#pragma unroll 1
+  for (int h = h0; h < H; h += kQ * step) {
+    Raw8<F32> qr[kQ];
+#pragma unroll
+    for (int u = 0; u < kQ; ++u)
+      if (h + u * step < H) qr[u].load(src + (h + u * step) * kIn);
+#pragma unroll
+    for (int u = 0; u < kQ; ++u) {
+      if (h + u * step >= H) break;
+      float x[8];
+      qr[u].values(x);
+      if (rope != nullptr) turn.apply(x);
+      qo[(h + u * step) * 8] = pack8(x);
+    }
   }
 }
 
@@ -1194,10 +1247,10 @@ extern "C" int cdk_paged_append(const void* qkv, int64_t ldq, int qkv_f32, const
   if (rope && (!pos || rope_len <= 0 || !al16(rope))) return -12;
   if (q_out && (ldo < H * kHD || ldo % 8 || !al16(q_out))) return -13;
   if (B > 0x7fffffffll / S_new) return -14;
-  // a warp per token; several, down to four rows each, while there are fewer than 16 warps per SM
-  const long long tokens = B * S_new, rows = (q_out ? H : 0) + 2 * (int64_t)pg.kv_heads;
+  // a warp per token; several, down to four heads each, while there are fewer than 16 warps per SM
+  const long long tokens = B * S_new, most = q_out && H > pg.kv_heads ? H : pg.kv_heads;
   long long parts = (148 * 16 + tokens - 1) / tokens;
-  if (parts > (rows + 3) / 4) parts = (rows + 3) / 4;
+  if (parts > (most + 3) / 4) parts = (most + 3) / 4;
   if (tokens * parts > 0xfffffff0ll) parts = 1;
   const long long blocks = (tokens * parts + 7) / 8;
   auto* st = reinterpret_cast<cudaStream_t>(stream);
