@@ -373,8 +373,9 @@ __global__ void __launch_bounds__(256)
 // Measured on one B200 (16 heads, device time, both kernels): bf16, 256 sequences of
 // up to 4095 keys 334 us (2.15 GB: the copy rate), 64 of up to 2000 48 us (85%),
 // 64 x 512 (an item per block) 25 us (83%); e4m3, 256 x 2000 176 us (94%), 6 of up to
-// 65536 with groups of 8 heads 28 us (59%: of the 11 us over the floor about 5 pass
-// before the first rows arrive -- launch, lengths, table, rows -- and 3 in the join).
+// 65536 with groups of 8 heads 27 us (62%: of the 10 us over the floor about 5 pass
+// before the first rows arrive -- launch, lengths, table, rows -- and 2 in the join).
+// Pages of 16 rows: 256 sequences of up to 4000 keys 338 us bf16 (96%), 188 e4m3 (88%).
 // ---------------------------------------------------------------------------
 constexpr int kTK = 32;             // keys per tile
 constexpr int kAttnThreads = 128;   // 4 warps; 128 registers: 4 blocks per SM
@@ -543,8 +544,9 @@ __device__ __forceinline__ void follow(Acc<NT>& acc, const float (&mx)[NT][2]) {
     }
 }
 
-// Tiles [ta, tb) of one item on bf16 pages: acc over its keys below len.
-template <int NT>
+// Tiles [ta, tb) of one item on bf16 pages: acc over its keys below len.  WIDE: pages
+// hold tiles whole.
+template <int NT, bool WIDE>
 __device__ __forceinline__ void attend_bf16(const AttnArgs& a, int b, int kvh, int ta, int tb, int len, int lane,
                                             Acc<NT>& acc) {
   constexpr int kRow = 2 * kHD;  // bytes of a cached row
@@ -558,13 +560,24 @@ __device__ __forceinline__ void attend_bf16(const AttnArgs& a, int b, int kvh, i
   uint4 vr[2][4];  // rows 16 jj + 2 t4 + {0, 1, 8, 9}, chunk g
   auto load_k = [&](int tile, int page, uint32_t mask) {
     const int t0 = tile * kTK;
-    if (pg.log_page >= 5 && mask == 0xffffffffu) {  // 32 rows in a row in one page
+    if (WIDE && mask == 0xffffffffu) {
       const long long p0 = __shfl_sync(0xffffffffu, page, 0);
       const char* base = pg.k + p0 * pg.ld_page + (long long)(head_row + (t0 & pmask) + g) * kRow + t4 * 16;
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int c = 0; c < 2; ++c) kr[r][c] = ld_once(base + r * 8 * kRow + c * 64);
+    } else if (!WIDE && pg.log_page == 4 && mask == 0xffffffffu) {  // 16 rows in a row in one page
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const long long p = __shfl_sync(0xffffffffu, page, 16 * x);
+        const char* base =
+            pg.k + p * pg.ld_page + (long long)(head_row + ((t0 + 16 * x) & pmask) + g) * kRow + t4 * 16;
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) kr[2 * x + r][c] = ld_once(base + r * 8 * kRow + c * 64);
+      }
     } else {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -578,13 +591,22 @@ __device__ __forceinline__ void attend_bf16(const AttnArgs& a, int b, int kvh, i
   };
   auto load_v = [&](int tile, int page, uint32_t mask) {
     const int t0 = tile * kTK;
-    if (pg.log_page >= 5 && mask == 0xffffffffu) {
+    if (WIDE && mask == 0xffffffffu) {
       const long long p0 = __shfl_sync(0xffffffffu, page, 0);
       const char* base = pg.v + p0 * pg.ld_page + (long long)(head_row + (t0 & pmask) + 2 * t4) * kRow + g * 16;
 #pragma unroll
       for (int jj = 0; jj < 2; ++jj)
 #pragma unroll
         for (int i = 0; i < 4; ++i) vr[jj][i] = ld_once(base + (16 * jj + (i & 1) + (i >> 1) * 8) * kRow);
+    } else if (!WIDE && pg.log_page == 4 && mask == 0xffffffffu) {
+#pragma unroll
+      for (int jj = 0; jj < 2; ++jj) {
+        const long long p = __shfl_sync(0xffffffffu, page, 16 * jj);
+        const char* base =
+            pg.v + p * pg.ld_page + (long long)(head_row + ((t0 + 16 * jj) & pmask) + 2 * t4) * kRow + g * 16;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vr[jj][i] = ld_once(base + ((i & 1) + (i >> 1) * 8) * kRow);
+      }
     } else {
 #pragma unroll
       for (int jj = 0; jj < 2; ++jj)
@@ -724,7 +746,7 @@ __device__ __forceinline__ int chunk_at(int row, int c) {
   return (row >> 1) * 128 + (((((row & 1) << 2) | c) ^ (((row >> 1) & 3) << 1)) << 4);
 }
 
-template <int NT>
+template <int NT, bool WIDE>
 __device__ __forceinline__ void attend_e4m3(const AttnArgs& a, int b, int kvh, int ta, int tb, int len, int lane,
                                             char* ring, Acc<NT>& acc) {
   const Pages& pg = a.pg;
@@ -749,7 +771,7 @@ __device__ __forceinline__ void attend_e4m3(const AttnArgs& a, int b, int kvh, i
         sv = __ldg(pg.vs + r);
       }
       const uint32_t dst = dst0 + stage * kStageBytes;
-      if (pg.log_page >= 5 && mask == 0xffffffffu) {  // 32 rows in a row in one page
+      if (WIDE && mask == 0xffffffffu) {
         const long long p0 = __shfl_sync(0xffffffffu, page, 0);
         const long long at = p0 * pg.ld_page + (long long)(head_row + (t0 & pmask) + g) * kHD + t4 * 16;
         const char* ks = pg.k + at;
@@ -758,6 +780,17 @@ __device__ __forceinline__ void attend_e4m3(const AttnArgs& a, int b, int kvh, i
         for (int i = 0; i < 4; ++i) {
           cp_async_16(dst + i * 512, ks + i * 8 * kHD);
           cp_async_16(dst + kTK * kHD + i * 512, vs + i * 8 * kHD);
+        }
+      } else if (!WIDE && pg.log_page == 4 && mask == 0xffffffffu) {  // 16 rows in a row in one page
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const long long p = __shfl_sync(0xffffffffu, page, 16 * x);
+          const long long at = p * pg.ld_page + (long long)(head_row + ((t0 + 16 * x) & pmask) + g) * kHD + t4 * 16;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            cp_async_16(dst + (2 * x + i) * 512, pg.k + at + i * 8 * kHD);
+            cp_async_16(dst + kTK * kHD + (2 * x + i) * 512, pg.v + at + i * 8 * kHD);
+          }
         }
       } else {
 #pragma unroll
@@ -915,11 +948,11 @@ __device__ __forceinline__ void attend_e4m3(const AttnArgs& a, int b, int kvh, i
   }
 }
 
-template <bool FP8, int NT>
+template <bool FP8, int NT, bool WIDE>
 __device__ __forceinline__ void attend(const AttnArgs& a, int b, int kvh, int ta, int tb, int len, int lane, char* ring,
                                        Acc<NT>& acc) {
-  if constexpr (FP8) attend_e4m3<NT>(a, b, kvh, ta, tb, len, lane, ring, acc);
-  else attend_bf16<NT>(a, b, kvh, ta, tb, len, lane, acc);
+  if constexpr (FP8) attend_e4m3<NT, WIDE>(a, b, kvh, ta, tb, len, lane, ring, acc);
+  else attend_bf16<NT, WIDE>(a, b, kvh, ta, tb, len, lane, acc);
 }
 
 // Shared memory of a block.  e4m3: a warp's results take the place of its ring,
@@ -994,7 +1027,7 @@ __device__ __forceinline__ void merge_block(const AttnArgs& a, const AttnShared&
 }
 
 // A block per (sequence, kv head).
-template <bool FP8, int NT>
+template <bool FP8, int NT, bool WIDE>
 __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 3) paged_attn_item_kernel(const AttnArgs a) {
   extern __shared__ __align__(16) char smem[];
   const AttnShared sh(smem, a.group, FP8);
@@ -1006,13 +1039,13 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 3) paged_attn_item
   const int ta = min(warp * per, tiles), tb = min(ta + per, tiles);
   Acc<NT> acc;
   acc.clear();
-  if (ta < tb) attend<FP8, NT>(a, b, kvh, ta, tb, len, lane, ring, acc);
+  if (ta < tb) attend<FP8, NT, WIDE>(a, b, kvh, ta, tb, len, lane, ring, acc);
   acc.sum_lanes();
   merge_block<NT>(a, sh, acc, b, kvh, true, 0);  // len 0: l = 0, zeros
 }
 
 // Shares [f, f + chunk) of the deal for warp w = f / chunk; see the join for the slots.
-template <bool FP8, int NT>
+template <bool FP8, int NT, bool WIDE>
 __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 3) paged_attn_kernel(const AttnArgs a) {
   extern __shared__ __align__(16) char smem[];
   __shared__ int warp_tiles[kWarps];
@@ -1087,7 +1120,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 3) paged_attn_kern
     const int ta = max((int)(f - bi.first) - kSetup, 0), tb = (int)(f_end - bi.first) - kSetup;
     Acc<NT> acc;
     acc.clear();
-    if (f < f_end && ta < tb) attend<FP8, NT>(a, bi.b, bi.kvh, ta, tb, length_of(a, bi.b, false), lane, ring, acc);
+    if (f < f_end && ta < tb) attend<FP8, NT, WIDE>(a, bi.b, bi.kvh, ta, tb, length_of(a, bi.b, false), lane, ring, acc);
     acc.sum_lanes();
     merge_block<NT>(a, sh, acc, bi.b, bi.kvh, block_f == bi.first && block_end == bi.first + bi.n, 2 * (int)w0);
     return;
@@ -1100,7 +1133,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 3) paged_attn_kern
     if (ta >= tb) continue;  // nothing but the item's setup
     Acc<NT> acc;
     acc.clear();
-    attend<FP8, NT>(a, it.b, it.kvh, ta, tb, length_of(a, it.b, false), lane, ring, acc);
+    attend<FP8, NT, WIDE>(a, it.b, it.kvh, ta, tb, length_of(a, it.b, false), lane, ring, acc);
     acc.sum_lanes();
     const bool whole = ta == 0 && tb == it.n - kSetup;
     const int slot = 2 * (int)w + (ta == 0 ? 1 : 0);
@@ -1129,9 +1162,12 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 3) paged_attn_kern
 // Adds up the partial results of the items that several warps shared, in the
 // order of the deal.  A block inside an item left one result, in its first warp's
 // slot 0; other warps left the item they end in slot 0, the one they begin in
-// slot 1.  One block per (sequence, query head); warp i takes every fourth result,
-// lane l dims 2l and 2l + 1.
-__global__ void __launch_bounds__(128) paged_attn_join_kernel(const AttnArgs a, unsigned n_warps) {
+// slot 1.  One block per (sequence, query head); eight lanes take a result, eight
+// dims each, so a warp has eight results in flight (one sequence of 131072 keys with
+// one kv head, 512 results for each of its 8 heads: 17 us, 32 with a result per warp).
+constexpr int kJoinWarps = 16;  // at most
+
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_attn_join_kernel(const AttnArgs a, unsigned n_warps) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int heads = a.pg.kv_heads * a.group;
   const int b = blockIdx.x / heads, h = blockIdx.x - b * heads;
@@ -1153,13 +1189,13 @@ __global__ void __launch_bounds__(128) paged_attn_join_kernel(const AttnArgs a, 
   const int head = inside ? max(c0 * kWarps - w0, 0) : w1 - w0 + 1;  // warps before them (all, without them)
   const int tail = inside ? max(w1 + 1 - c1 * kWarps, 0) : 0;        // and after them
   const int n = head + inside + tail;
-  float m = kNoScore, l = 0.f, x = 0.f, y = 0.f;
-  auto add = [&](float2 st, float2 v) {
-    const float nm = fmaxf(m, st.x);
-    const float f0 = ex2(m - nm), f1 = ex2(st.x - nm);
-    l = l * f0 + st.y * f1;
-    x = x * f0 + v.x * f1;
-    y = y * f0 + v.y * f1;
+  const int sub = lane >> 3, d = (lane & 7) * 8, warps = blockDim.x >> 5;
+  float m = kNoScore, l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  auto add = [&](float pm, float pl, const float (&po)[8]) {
+    const float nm = fmaxf(m, pm), f0 = ex2(m - nm), f1 = ex2(pm - nm);
+    l = l * f0 + pl * f1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = o[i] * f0 + po[i] * f1;
     m = nm;
   };
   auto at_of = [&](int i) {
@@ -1167,30 +1203,50 @@ __global__ void __launch_bounds__(128) paged_attn_join_kernel(const AttnArgs a, 
     const bool begins = (i < head && i == 0);
     return (2 * w + (begins ? 1 : 0)) * a.group + hq;
   };
-  for (int i = warp; i < n; i += 4 * kWarps) {  // four results in flight
-    float2 st[4], v[4];
+  for (int i = warp * 4 + sub; i - sub < n; i += 8 * warps) {
+    float2 st[2];
+    float v[2][8];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int k = i + u * kWarps;
+    for (int u = 0; u < 2; ++u) {
+      const int k = i + u * 4 * warps;
       st[u] = make_float2(kNoScore, 0.f);
-      v[u] = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) v[u][c] = 0.f;
       if (k < n) {
         const int at = at_of(k);
         st[u] = a.stat[at];
-        v[u] = *reinterpret_cast<const float2*>(a.part + at * kHD + 2 * lane);
+        const float4* p = reinterpret_cast<const float4*>(a.part + at * kHD + d);
+        const float4 x = p[0], y = p[1];
+        v[u][0] = x.x, v[u][1] = x.y, v[u][2] = x.z, v[u][3] = x.w;
+        v[u][4] = y.x, v[u][5] = y.y, v[u][6] = y.z, v[u][7] = y.w;
       }
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) add(st[u], v[u]);
+    for (int u = 0; u < 2; ++u) add(st[u].x, st[u].y, v[u]);
   }
-  __shared__ float2 st_s[kWarps], v_s[kWarps][32];
-  if (lane == 0) st_s[warp] = make_float2(m, l);
-  v_s[warp][lane] = make_float2(x, y);
+#pragma unroll
+  for (int x = 8; x < 32; x <<= 1) {  // the warp's four
+    float po[8];
+    const float pm = __shfl_xor_sync(0xffffffffu, m, x), pl = __shfl_xor_sync(0xffffffffu, l, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) po[i] = __shfl_xor_sync(0xffffffffu, o[i], x);
+    add(pm, pl, po);
+  }
+  __shared__ float2 st_s[kJoinWarps];
+  __shared__ float4 o_s[kJoinWarps][kHD / 4];
+  if (sub == 0) {
+    if (lane == 0) st_s[warp] = make_float2(m, l);
+    o_s[warp][d / 4] = make_float4(o[0], o[1], o[2], o[3]);
+    o_s[warp][d / 4 + 1] = make_float4(o[4], o[5], o[6], o[7]);
+  }
   __syncthreads();
-  if (warp) return;
-  for (int i = 1; i < kWarps; ++i) add(st_s[i], v_s[i][lane]);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  *reinterpret_cast<uint32_t*>(a.out + (long long)b * a.ldo + h * kHD + 2 * lane) = pack_bf16(x * inv, y * inv);
+  if (warp || sub) return;
+  for (int i = 1; i < warps; ++i) {
+    const float4 x = o_s[i][d / 4], y = o_s[i][d / 4 + 1];
+    const float po[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    add(st_s[i].x, st_s[i].y, po);
+  }
+  store_out8(a, b, h, d, o, l == 0.f ? 0.f : 1.f / l);
 }
 
 // ---------------------------------------------------------------------------
@@ -1291,7 +1347,7 @@ extern "C" int cdk_paged_gather(const CdkPagedCache* cache, int64_t B, const int
 namespace {
 inline int64_t prefix_bytes(int64_t B) { return ((B + 1) * 4 + 15) / 16 * 16; }
 
-template <bool FP8, int NT>
+template <bool FP8, int NT, bool WIDE>
 cudaError_t launch_attn(const AttnArgs& a, long long max_tiles, cudaStream_t st) {
   const long long items = (long long)a.B * a.pg.kv_heads;
   const int smem = AttnShared::bytes(a.group, FP8);
@@ -1301,26 +1357,27 @@ cudaError_t launch_attn(const AttnArgs& a, long long max_tiles, cudaStream_t st)
   if (e != cudaSuccess || dev < 0 || dev >= 64) return e != cudaSuccess ? e : cudaErrorInvalidDevice;
   if (!done[dev]) {
     const int most = AttnShared::bytes(kMaxGroup, FP8);
-    e = cudaFuncSetAttribute(paged_attn_item_kernel<FP8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    e = cudaFuncSetAttribute(paged_attn_item_kernel<FP8, NT, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(paged_attn_kernel<FP8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      e = cudaFuncSetAttribute(paged_attn_kernel<FP8, NT, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                (int)prefix_bytes(kMaxSeqs) + most);
     if (e != cudaSuccess) return e;
     done[dev] = true;
   }
   if (max_tiles <= kItemTiles) {
-    paged_attn_item_kernel<FP8, NT><<<(unsigned)items, kAttnThreads, smem, st>>>(a);
+    paged_attn_item_kernel<FP8, NT, WIDE><<<(unsigned)items, kAttnThreads, smem, st>>>(a);
     return cudaGetLastError();
   }
   // no more warps than tiles that the tables can hold: one tile is the smallest share
   const long long bound = max_tiles * items;
   const unsigned grid = (unsigned)(bound >= kAttnWarps ? kAttnBlocks : (bound + kWarps - 1) / kWarps);
-  paged_attn_kernel<FP8, NT><<<grid, kAttnThreads, (int)prefix_bytes(a.B) + smem, st>>>(a);
+  paged_attn_kernel<FP8, NT, WIDE><<<grid, kAttnThreads, (int)prefix_bytes(a.B) + smem, st>>>(a);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(items * a.group));
-  cfg.blockDim = dim3(128);
+  // few items have many results each (592 for one item): more warps then
+  cfg.blockDim = dim3(items >= 148 ? 128 : kJoinWarps * 32);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];  // set up while the first kernel drains; it waits for it before its first load
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1367,7 +1424,11 @@ extern "C" int cdk_paged_attn(const void* q, int64_t ldq, const CdkPagedCache* c
   a.stat = reinterpret_cast<float2*>(ws + prefix_bytes(B));
   a.part = reinterpret_cast<float*>(ws + prefix_bytes(B) + (int64_t)kSlots * a.group * 16);
   auto st = reinterpret_cast<cudaStream_t>(stream);
-  if (cache->dtype == 1)
-    return (int)(a.group <= 8 ? launch_attn<true, 1>(a, tiles, st) : launch_attn<true, 2>(a, tiles, st));
-  return (int)(a.group <= 8 ? launch_attn<false, 1>(a, tiles, st) : launch_attn<false, 2>(a, tiles, st));
+  // pages of 32 rows and more hold a tile whole (a kernel that takes both kinds needs
+  // registers that the loads in flight then miss: 64 x 0..2000 keys 52 us for 48)
+  const bool wide = a.pg.log_page >= 5;
+#define CDK_ATTN(FP8, NT) (int)(wide ? launch_attn<FP8, NT, true>(a, tiles, st) : launch_attn<FP8, NT, false>(a, tiles, st))
+  if (cache->dtype == 1) return a.group <= 8 ? CDK_ATTN(true, 1) : CDK_ATTN(true, 2);
+  return a.group <= 8 ? CDK_ATTN(false, 1) : CDK_ATTN(false, 2);
+#undef CDK_ATTN
 }
