@@ -288,35 +288,46 @@ __device__ __forceinline__ uint64_t best32(uint64_t a, uint64_t b, int lane) {
 }
 
 // Elements whose rank reaches T join the candidates (room for `most`; count goes on).
-constexpr int kCandidates = 512;
+// Where more reach it than there is room for -- of a warp's 32 maxima the 32nd is a
+// weak bound -- the k-th best of those that found room is a better one, and the
+// look is repeated with it, up to kLooks times.
+constexpr int kCandidates = 512, kLooks = 4;
+template <bool SHARED>  // by several warps: count is in shared memory; else it is the warp's own
 struct Candidates {
   uint64_t* list;
   int* count;
   int most;
   uint64_t T;
   float value;  // T's; T is the rank of an element, or 0: a NaN, below which nothing is
-  __device__ __forceinline__ void take(float x, int e) const {
-    const uint64_t key = rank_key(x, (uint32_t)e);
-    if (key < T) return;
-    const int at = atomicAdd(count, 1);
-    if (at < most) list[at] = key;
-  }
-  template <bool BF16>
-  __device__ __forceinline__ void take_vector(const Row<BF16>& row, int v, uint4 raw) const {
-    constexpr int N = Row<BF16>::N;
-    if (vector_max<BF16>(raw) < value) return;
-    float x[N];
-    Row<BF16>::values(raw, x);
+  __device__ __forceinline__ Candidates(uint64_t* l, int* c, int m, uint64_t T_)
+      : list(l), count(c), most(m), T(T_), value(key_value(T_)) {}
+  // Elements e + i, x[i], of every lane that has them; each lane's one by one.  A warp on
+  // its own counts by ballots (a shared atomic per candidate costs some 70 cycles each;
+  // 4000 rows of 3934 bf16 with 24 alternatives: 37 us, 24 so); the warps of a block
+  // have a few each.
+  template <int N>
+  __device__ __forceinline__ void take(const float (&x)[N], int e, bool have, int lane) const {
     uint32_t left = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) left |= x[i] < value ? 0u : 1u << i;
-    while (left) {  // one of them, mostly
+    if (!have) left = 0;
+    while (SHARED ? left != 0 : __any_sync(0xffffffffu, left != 0)) {
       const int i = __ffs(left) - 1;
-      left &= left - 1;
       float y = x[0];
 #pragma unroll
       for (int c = 1; c < N; ++c) y = i == c ? x[c] : y;
-      take(y, v * N - row.mis + i);
+      const uint64_t key = rank_key(y, (uint32_t)(e + i));
+      const bool in = left != 0 && key >= T;
+      left &= left - 1;
+      int at = most;
+      if (SHARED) {
+        if (in) at = atomicAdd(count, 1);
+      } else {
+        const uint32_t mask = __ballot_sync(0xffffffffu, in);
+        if (in) at = *count + __popc(mask & ((1u << lane) - 1));
+        *count += __popc(mask);
+      }
+      if (at < most) list[at] = key;
     }
   }
   // Second look at the shares of n threads (vectors v0 + owner, + STEP, ... below v1) by
@@ -324,19 +335,25 @@ struct Candidates {
   template <bool BF16, int STEP, int THREADS>
   __device__ __forceinline__ void take_shares(const Row<BF16>& row, int v0, int v1, const int* owners, int n,
                                               int tid) const {
-    const int per = (v1 - v0 + STEP - 1) / STEP, lg = per > 1 ? 32 - __clz(per - 1) : 0;
-    for (int i0 = tid; i0 < n << lg; i0 += 4 * THREADS) {
+    constexpr int N = Row<BF16>::N;
+    const int per = (v1 - v0 + STEP - 1) / STEP, lg = per > 1 ? 32 - __clz(per - 1) : 0, lane = tid & 31;
+    for (int i0 = tid - lane; i0 < n << lg; i0 += 4 * THREADS) {
       uint4 raw[4];
       int v[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const int i = i0 + u * THREADS;
+        const int i = i0 + lane + u * THREADS;
         v[u] = i < n << lg ? v0 + owners[i >> lg] + STEP * (i & ((1 << lg) - 1)) : v1;
-        if (v[u] < v1) raw[u] = row.load(v[u]);
+        raw[u] = v[u] < v1 ? row.load(v[u]) : make_uint4(0u, 0u, 0u, 0u);
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (v[u] < v1) take_vector(row, v[u], raw[u]);
+      for (int u = 0; u < 4; ++u) {
+        const bool have = v[u] < v1 && !(vector_max<BF16>(raw[u]) < value);
+        if (SHARED ? !have : !__any_sync(0xffffffffu, have)) continue;
+        float x[N];
+        Row<BF16>::values(raw[u], x);
+        take(x, v[u] * N - row.mis, have, lane);
+      }
     }
   }
 };
@@ -373,9 +390,9 @@ __device__ __forceinline__ void finish(const Args& a, const Row<BF16>& row, long
   }
 }
 
-// The k best of vectors [v0, v1) and the first n_edges edges by k passes of one
-// warp: for rows with a NaN, and where more candidates reach T than there is room
-// for (hundreds of the best logits in the share of k threads).
+// The k best of vectors [v0, v1) and, if asked, the edges by k passes of one warp: for
+// rows with a NaN, and where more candidates reach T than there is room for after
+// kLooks looks (thousands of the best logits, ascending, in the share of k threads).
 template <bool BF16>
 __device__ __noinline__ uint64_t slow_top(const Row<BF16>& row, int v0, int v1, bool edges, int k, int lane) {
   constexpr int N = Row<BF16>::N;
@@ -424,7 +441,7 @@ constexpr int kWarpCandidates = 160;  // the slow way is short here, and shared 
 template <bool BF16, bool TOP>
 __global__ void __launch_bounds__(kWarpsPerBlock * 32, TOP ? 4 : 5) token_stats_warp_kernel(const Args a) {
   __shared__ uint64_t cand_s[TOP ? kWarpsPerBlock : 1][TOP ? kWarpCandidates : 1];
-  __shared__ int count_s[kWarpsPerBlock], owners_s[TOP ? kWarpsPerBlock : 1][32];
+  __shared__ int owners_s[TOP ? kWarpsPerBlock : 1][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long r = (long long)blockIdx.x * kWarpsPerBlock + warp;
   if (r >= a.rows) return;
@@ -434,21 +451,27 @@ __global__ void __launch_bounds__(kWarpsPerBlock * 32, TOP ? 4 : 5) token_stats_
   const Stat st = join_warp(stream<BF16, 32, TOP>(row, v0, lane, v1, lane, a.entropy != nullptr, &key));
   if (TOP) {
     bool slow = st.s != st.s;
-    if (!slow) {
-      const uint64_t T = __shfl_sync(0xffffffffu, sort32(key, lane), a.k - 1);
+    uint64_t T = __shfl_sync(0xffffffffu, sort32(key, lane), a.k - 1);
+#pragma unroll 1
+    for (int look = 0; !slow; ++look) {
       const bool owner = key != 0 && key >= T;
       const uint32_t owners = __ballot_sync(0xffffffffu, owner);
       if (owner) owners_s[TOP ? warp : 0][__popc(owners & ((1u << lane) - 1))] = lane;
-      if (lane == 0) count_s[warp] = 0;
       __syncwarp();
-      const Candidates cand{cand_s[TOP ? warp : 0], &count_s[warp], kWarpCandidates, T, key_value(T)};
-      const int e = row.edge(lane);
-      if (owner && e >= 0) cand.take(row.at(e), e);
+      int n = 0;
+      const Candidates<false> cand(cand_s[TOP ? warp : 0], &n, kWarpCandidates, T);
+      const int e = owner ? row.edge(lane) : -1;
+      const float xe[1] = {e >= 0 ? row.at(e) : 0.f};
+      cand.take(xe, e, e >= 0, lane);
       cand.take_shares<BF16, 32, 32>(row, v0, v1, owners_s[TOP ? warp : 0], __popc(owners), lane);
       __syncwarp();
-      slow = count_s[warp] > kWarpCandidates;
+      top = best_of(cand_s[TOP ? warp : 0], min(n, kWarpCandidates), lane);
+      if (n <= kWarpCandidates) break;
+      T = __shfl_sync(0xffffffffu, top, a.k - 1);
+      slow = look == kLooks - 1;
+      __syncwarp();  // every lane has read the list
     }
-    top = slow ? slow_top<BF16>(row, v0, v1, true, a.k, lane) : best_of(cand_s[TOP ? warp : 0], count_s[warp], lane);
+    if (slow) top = slow_top<BF16>(row, v0, v1, true, a.k, lane);
   }
   finish<BF16>(a, row, r, st, lane, top);
 }
@@ -502,26 +525,38 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) token_stats_block_kerne
   uint64_t top = 0;
   if (TOP) {
     const bool broken = st.s != st.s;
+    bool slow = broken;
     if (!broken) {
 #pragma unroll 1
       for (int n = kRowWarps / 2; n > 0; n >>= 1) {  // the warps' lists, two and two
         if (warp < n) sh.lists[TOP ? warp : 0][lane] = best32(sh.lists[TOP ? warp : 0][lane], sh.lists[TOP ? warp + n : 0][lane], lane);
         __syncthreads();
       }
-      const uint64_t T = sh.lists[0][a.k - 1];
-      const Candidates cand{sh.cand, &sh.count, kCandidates, T, key_value(T)};
-      if (key != 0 && key >= T) {
-        sh.owners[atomicAdd(&sh.n_owners, 1)] = tid;  // at most k of them
-        const int e = edge >= 0 ? row.edge(edge) : -1;
-        if (e >= 0) cand.take(row.at(e), e);
+#pragma unroll 1
+      for (int look = 0;; ++look) {
+        const uint64_t T = sh.lists[0][a.k - 1];
+        const Candidates<true> cand(sh.cand, &sh.count, kCandidates, T);
+        const bool owner = key != 0 && key >= T;
+        if (owner) sh.owners[atomicAdd(&sh.n_owners, 1)] = tid;  // at most k of them
+        if (rank == 0 && warp == 0) {
+          const int e = owner ? row.edge(lane) : -1;
+          const float xe[1] = {e >= 0 ? row.at(e) : 0.f};
+          cand.take(xe, e, e >= 0, lane);
+        }
+        __syncthreads();
+        cand.take_shares<BF16, kThreads, kThreads>(row, v0, v1, sh.owners, sh.n_owners, tid);
+        __syncthreads();
+        const int n = sh.count;
+        if (warp == 0) top = best_of(sh.cand, min(n, kCandidates), lane);
+        slow = n > kCandidates;
+        if (!slow || look == kLooks - 1) break;
+        __syncthreads();  // every thread has read the count
+        if (warp == 0) sh.lists[0][lane] = top;
+        if (tid == 0) sh.n_owners = sh.count = 0;
+        __syncthreads();
       }
-      __syncthreads();
-      cand.take_shares<BF16, kThreads, kThreads>(row, v0, v1, sh.owners, sh.n_owners, tid);
-      __syncthreads();
     }
-    if (warp == 0)
-      top = broken || sh.count > kCandidates ? slow_top<BF16>(row, v0, v1, rank == 0, a.k, lane)
-                                             : best_of(sh.cand, sh.count, lane);
+    if (slow && warp == 0) top = slow_top<BF16>(row, v0, v1, rank == 0, a.k, lane);
   }
   if (blocks_per_row > 1) {
     if (TOP && warp == 0) sh.best[lane] = top;

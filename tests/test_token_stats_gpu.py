@@ -127,6 +127,30 @@ def test_alternatives(V, k, bf16):
     run(x, t, k)
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("V", [160, 480, 1924, 3934])
+def test_as_many_alternatives_as_lanes(V, bf16):
+    """Many rows of a warp each: the least of its lanes' maxima admits more candidates than there is room for in some."""
+    x, t, _, _ = inputs(2400, V, bf16, seed=V)
+    x[::3] = x[::3].sort(dim=1, descending=True)[0]
+    x[1::3] = 0.25
+    run(x, t, 32)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("descending", [False, True])
+@pytest.mark.parametrize("threads", [1, 3, 40])
+def test_best_logits_in_few_threads(threads, descending, bf16):
+    """The best are all in every 256th vector from a few on, in either order."""
+    V, n = 131072, 8 if bf16 else 4
+    x, t, _, _ = inputs(2, V, bf16, seed=threads)
+    part = x.view(2, V // (256 * n), 256, n)[:, :, :threads]
+    rise = torch.arange(part[0].numel(), device=DEV).view(part[0].shape) * 2.0 ** -6 + 20.0
+    part.copy_(rise.flip(0) if descending else rise)
+    run(x, t, 32)
+    run(x, t, 3)
+
+
 @pytest.mark.parametrize("R", [1, 2, 147, 149, 1000, 5000])
 def test_rows(R):
     x, t, dlp, dent = inputs(R, 131, seed=R)
