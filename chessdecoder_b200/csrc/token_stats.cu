@@ -13,13 +13,11 @@
 // it once.  The forward spends one ex2 and about eight other instructions per
 // logit, half (fp32) to most (bf16) of what an SM issues in the time that HBM takes.
 //
-// Alternatives.  Each thread's largest logit comes with its running maximum.  T,
-// the k-th largest of these (as a (value, index) rank), is a lower bound of the
-// k-th best of the row, and only the k threads that reach T can hold one of the
-// k best: their logits are read again (k of 32 or 256 threads' share), those that
-// reach T are gathered in shared memory -- k and a few -- and sorted by a warp.  So
-// the streaming pass has no work for the alternatives but to note in which of its
-// chunks a thread's maximum lay.
+// Alternatives.  T, the k-th largest of the threads' maxima (a warp's 32; a block's in
+// fours), is a lower bound of the k-th best logit, and only threads whose maximum
+// reaches T can hold one of the k best: their logits are read again, those that reach
+// T are gathered in shared memory -- k and a few -- and sorted by a warp.  So the
+// streaming pass has no work for the alternatives at all: its running maxima do.
 //
 // Measured on one B200 (device time, share of the copy rate): 16384 x 1924 fp32
 // forward 23.5 us (83%), with 5 alternatives 37 us (53%), gradient 41 us (95%); 509 x
@@ -156,22 +154,11 @@ __device__ __forceinline__ Stat join_warp(Stat a) {
 }
 
 // One thread's share of a row: vectors first + tid, first + tid + STEP, ... below
-// last and the edge with index `edge` (or none: -1).  TOP: key = rank of its largest element, 0
-// if it has none.
-template <bool BF16, int STEP, bool TOP>
-__device__ __forceinline__ Stat stream(const Row<BF16>& row, int first, int tid, int last, int edge,
-                                       bool want_t, uint64_t* key) {
+// last and the edge with index `edge` (or none: -1).
+template <bool BF16, int STEP>
+__device__ __forceinline__ Stat stream(const Row<BF16>& row, int first, int tid, int last, int edge, bool want_t) {
   constexpr int N = Row<BF16>::N;
   Stat st{kLowest, 0.f, 0.f};
-  float best = -INFINITY;  // this thread's largest element, in the chunk that begins at vector where
-  int where = first + tid;
-  auto rise = [&](float cm, int v) {
-    if (TOP && cm > best) {
-      best = cm;
-      where = v;
-    }
-    if (cm > st.m) st.rise(cm);
-  };
   auto add = [&](uint4 raw, float (&s2)[2], float (&t2)[2]) {
     float x[N];
     Row<BF16>::values(raw, x);
@@ -195,7 +182,6 @@ __device__ __forceinline__ Stat stream(const Row<BF16>& row, int first, int tid,
   }
 #pragma unroll 1
   while (more) {
-    const int v = first + tid;
     first += kUnroll * STEP;
     more = first + kUnroll * STEP <= last;
     uint4 next[kUnroll];
@@ -206,7 +192,7 @@ __device__ __forceinline__ Stat stream(const Row<BF16>& row, int first, int tid,
     float cm = vector_max<BF16>(raw[0]);
 #pragma unroll
     for (int u = 1; u < kUnroll; ++u) cm = fmaxf(cm, vector_max<BF16>(raw[u]));
-    rise(cm, v);
+    if (cm > st.m) st.rise(cm);
     float s2[2] = {0.f, 0.f}, t2[2] = {0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) add(raw[u], s2, t2);
@@ -224,7 +210,7 @@ __device__ __forceinline__ Stat stream(const Row<BF16>& row, int first, int tid,
 #pragma unroll
     for (int u = 1; u < kUnroll; ++u)
       if (v + u * STEP < last) cm = fmaxf(cm, vector_max<BF16>(raw[u]));
-    rise(cm, v);
+    if (cm > st.m) st.rise(cm);
     float s2[2] = {0.f, 0.f}, t2[2] = {0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
@@ -233,48 +219,33 @@ __device__ __forceinline__ Stat stream(const Row<BF16>& row, int first, int tid,
     st.t += t2[0] + t2[1];
   }
   const int e = edge >= 0 ? row.edge(edge) : -1;
-  float xe = -INFINITY;
-  if (e >= 0) {
-    xe = row.at(e);
-    st.add(xe);
-  }
-  if (TOP) {
-    // the first element that equals the maximum (a NaN makes s a NaN: ranked elsewhere)
-    uint64_t k = 0;
-    if (where < last) {
-      int at = 0;
-#pragma unroll
-      for (int u = kUnroll - 1; u >= 0; --u) {
-        const int w = where + u * STEP;
-        if (w >= last) continue;
-        float x[N];
-        Row<BF16>::values(row.load(w), x);
-#pragma unroll
-        for (int i = N - 1; i >= 0; --i)
-          if (x[i] == best) at = w * N + i;
-      }
-      k = rank_key(best, (uint32_t)(at - row.mis));
-    }
-    if (e >= 0) k = max(k, rank_key(xe, (uint32_t)e));
-    *key = k;
-  }
+  if (e >= 0) st.add(row.at(e));
   return st;
 }
 
+// Largest element of a share.  (It adds 1 to s.)
+__device__ __forceinline__ float largest(const Stat& st) { return st.s != 0.f ? st.m : -INFINITY; }
+
 // ---------------------------------------------------------------------------
-// Ranks in a warp: lane i holds one.
+// Ranks, or values, in a warp: lane i holds one.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ uint64_t exchange(uint64_t a, int o, bool keep_max) {
   const uint64_t b = __shfl_xor_sync(0xffffffffu, a, o);
   return (a > b) == keep_max ? a : b;
 }
+__device__ __forceinline__ float exchange(float a, int o, bool keep_max) {
+  const float b = __shfl_xor_sync(0xffffffffu, a, o);
+  return keep_max ? fmaxf(a, b) : fminf(a, b);
+}
 // bitonic sequence -> descending by lane
-__device__ __forceinline__ uint64_t bitonic_merge(uint64_t a, int lane) {
+template <typename T>
+__device__ __forceinline__ T bitonic_merge(T a, int lane) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) a = exchange(a, o, (lane & o) == 0);
   return a;
 }
-__device__ __forceinline__ uint64_t sort32(uint64_t a, int lane) {
+template <typename T>
+__device__ __forceinline__ T sort32(T a, int lane) {
 #pragma unroll
   for (int size = 2; size <= 16; size <<= 1)
 #pragma unroll
@@ -282,15 +253,31 @@ __device__ __forceinline__ uint64_t sort32(uint64_t a, int lane) {
   return bitonic_merge(a, lane);
 }
 // the 32 best of two descending lists, descending
-__device__ __forceinline__ uint64_t best32(uint64_t a, uint64_t b, int lane) {
-  const uint64_t r = __shfl_sync(0xffffffffu, b, 31 - lane);
+template <typename T>
+__device__ __forceinline__ T best32(T a, T b, int lane) {
+  const T r = __shfl_sync(0xffffffffu, b, 31 - lane);
   return bitonic_merge(a > r ? a : r, lane);
 }
 
-// Elements whose rank reaches T join the candidates (room for `most`; count goes on).
-// Where more reach it than there is room for -- of a warp's 32 maxima the 32nd is a
-// weak bound -- the k-th best of those that found room is a better one, and the
-// look is repeated with it, up to kLooks times.
+// Rank that bounds the k-th best from below, from the value of the k-th maximum.  Every
+// element of the value reaches it; where that is -inf (fewer than k maxima are above:
+// a masked row), only the first k elements, from index `first` on.
+__device__ __forceinline__ uint64_t bound(float value, int first, int k) {
+  return rank_key(value, value == -INFINITY ? (uint32_t)(first + k - 1) : 0xffffffffu);
+}
+
+// Whether a share with largest element `best` may hold a rank that reaches T: thread tid's
+// vectors begin with element first + tid * N, and the first 2 N threads have the edges.
+template <int N>
+__device__ __forceinline__ bool owns(uint64_t T, float best, int first, int tid) {
+  const float value = key_value(T);
+  return best > value || (best == value && (tid < 2 * N || (uint32_t)(first + tid * N) <= ~(uint32_t)T));
+}
+
+// Elements whose rank reaches T join the candidates, until there is no room: count is
+// above `most` then.  (Of a warp's 32 maxima the 32nd is a weak bound; in a row of equal
+// logits every element reaches it.)  The k-th best of those that found room is a better
+// bound, and the look is repeated with it, up to kLooks times.
 constexpr int kCandidates = 512, kLooks = 4;
 template <bool SHARED>  // by several warps: count is in shared memory; else it is the warp's own
 struct Candidates {
@@ -298,9 +285,12 @@ struct Candidates {
   int* count;
   int most;
   uint64_t T;
-  float value;  // T's; T is the rank of an element, or 0: a NaN, below which nothing is
+  float value;  // T's
   __device__ __forceinline__ Candidates(uint64_t* l, int* c, int m, uint64_t T_)
       : list(l), count(c), most(m), T(T_), value(key_value(T_)) {}
+  __device__ __forceinline__ bool full() const {  // the same in every lane of the warp
+    return SHARED ? __any_sync(0xffffffffu, *const_cast<volatile int*>(count) > most) : *count > most;
+  }
   // Elements e + i, x[i], of every lane that has them; each lane's one by one.  A warp on
   // its own counts by ballots (a shared atomic per candidate costs some 70 cycles each;
   // 4000 rows of 3934 bf16 with 24 alternatives: 37 us, 24 so); the warps of a block
@@ -321,7 +311,7 @@ struct Candidates {
       left &= left - 1;
       int at = most;
       if (SHARED) {
-        if (in) at = atomicAdd(count, 1);
+        if (in && (at = atomicAdd(count, 1)) >= most) break;
       } else {
         const uint32_t mask = __ballot_sync(0xffffffffu, in);
         if (in) at = *count + __popc(mask & ((1u << lane) - 1));
@@ -331,19 +321,24 @@ struct Candidates {
     }
   }
   // Second look at the shares of n threads (vectors v0 + owner, + STEP, ... below v1) by
-  // THREADS threads: 2^lg of them, the least power of two that covers a share, per owner.
-  template <bool BF16, int STEP, int THREADS>
-  __device__ __forceinline__ void take_shares(const Row<BF16>& row, int v0, int v1, const int* owners, int n,
+  // THREADS threads: 2^lg of them, the least power of two that covers a share, per
+  // owner.  Where every thread is one, in the row's order: equal logits (a mask's) leave
+  // no room then, and what found room has the low indices.
+  template <bool BF16, int STEP, int THREADS, typename Owner>
+  __device__ __forceinline__ void take_shares(const Row<BF16>& row, int v0, int v1, const Owner* owners, int n,
                                               int tid) const {
     constexpr int N = Row<BF16>::N;
     const int per = (v1 - v0 + STEP - 1) / STEP, lg = per > 1 ? 32 - __clz(per - 1) : 0, lane = tid & 31;
-    for (int i0 = tid - lane; i0 < n << lg; i0 += 4 * THREADS) {
+    const bool all = n == STEP;
+    const int slots = all ? v1 - v0 : n << lg;
+    for (int i0 = tid - lane; i0 < slots; i0 += 4 * THREADS) {
+      if (full()) return;
       uint4 raw[4];
       int v[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int i = i0 + lane + u * THREADS;
-        v[u] = i < n << lg ? v0 + owners[i >> lg] + STEP * (i & ((1 << lg) - 1)) : v1;
+        v[u] = i >= slots ? v1 : all ? v0 + i : v0 + owners[i >> lg] + STEP * (i & ((1 << lg) - 1));
         raw[u] = v[u] < v1 ? row.load(v[u]) : make_uint4(0u, 0u, 0u, 0u);
       }
 #pragma unroll
@@ -447,14 +442,16 @@ __global__ void __launch_bounds__(kWarpsPerBlock * 32, TOP ? 4 : 5) token_stats_
   if (r >= a.rows) return;
   const Row<BF16> row(a.logits, a.ldl, r, a.ncls);
   const int v0 = row.begin(), v1 = row.end();
-  uint64_t key = 0, top = 0;
-  const Stat st = join_warp(stream<BF16, 32, TOP>(row, v0, lane, v1, lane, a.entropy != nullptr, &key));
+  uint64_t top = 0;
+  Stat st = stream<BF16, 32>(row, v0, lane, v1, lane, a.entropy != nullptr);
+  const float best = largest(st);
+  st = join_warp(st);
   if (TOP) {
     bool slow = st.s != st.s;
-    uint64_t T = __shfl_sync(0xffffffffu, sort32(key, lane), a.k - 1);
+    uint64_t T = bound(__shfl_sync(0xffffffffu, sort32(best, lane), a.k - 1), 0, a.k);
 #pragma unroll 1
     for (int look = 0; !slow; ++look) {
-      const bool owner = key != 0 && key >= T;
+      const bool owner = owns<Row<BF16>::N>(T, best, 0, lane);
       const uint32_t owners = __ballot_sync(0xffffffffu, owner);
       if (owner) owners_s[TOP ? warp : 0][__popc(owners & ((1u << lane) - 1))] = lane;
       __syncwarp();
@@ -486,10 +483,11 @@ constexpr int kRowWarps = kThreads / 32;
 
 template <bool TOP>
 struct RowShared {
-  uint64_t lists[TOP ? kRowWarps : 1][32];
   uint64_t cand[TOP ? kCandidates : 1];
   uint64_t best[32];  // this block's best, descending
-  int owners[32];
+  uint64_t T;
+  float maxima[64];   // of four threads each
+  uint8_t owners[TOP ? kThreads : 1];
   int n_owners, count;
   Stat part[kRowWarps];
   Stat st;            // this block's
@@ -512,11 +510,17 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) token_stats_block_kerne
   const int begin = row.begin(), end = row.end();
   const int per_block = (end - begin + blocks_per_row - 1) / blocks_per_row;
   const int v0 = min(begin + rank * per_block, end), v1 = min(v0 + per_block, end);
+  const int first = rank == 0 ? 0 : v0 * Row<BF16>::N - row.mis;  // element
   const int edge = rank == 0 && warp == 0 ? lane : -1;  // the first warp of the first block has the edges
-  uint64_t key = 0;
-  Stat st = join_warp(stream<BF16, kThreads, TOP>(row, v0, tid, v1, edge, a.entropy != nullptr, &key));
+  Stat st = stream<BF16, kThreads>(row, v0, tid, v1, edge, a.entropy != nullptr);
+  const float best = largest(st);
+  if (TOP) {
+    float x = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
+    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+    if (lane % 4 == 0) sh.maxima[tid / 4] = x;
+  }
+  st = join_warp(st);
   if (lane == 0) sh.part[warp] = st;
-  if (TOP) sh.lists[TOP ? warp : 0][lane] = sort32(key, lane);
   if (tid == 0) sh.n_owners = sh.count = 0;
   __syncthreads();
   st = sh.part[0];
@@ -527,17 +531,20 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) token_stats_block_kerne
     const bool broken = st.s != st.s;
     bool slow = broken;
     if (!broken) {
-#pragma unroll 1
-      for (int n = kRowWarps / 2; n > 0; n >>= 1) {  // the warps' lists, two and two
-        if (warp < n) sh.lists[TOP ? warp : 0][lane] = best32(sh.lists[TOP ? warp : 0][lane], sh.lists[TOP ? warp + n : 0][lane], lane);
-        __syncthreads();
-      }
+      const float m0 = sh.maxima[lane], m1 = sh.maxima[lane + 32];  // every warp for itself: no barrier
+      const float order = a.k <= 16 ? sort32(fmaxf(m0, m1), lane) : best32(sort32(m0, lane), sort32(m1, lane), lane);
+      uint64_t T = bound(__shfl_sync(0xffffffffu, order, a.k - 1), first, a.k);
 #pragma unroll 1
       for (int look = 0;; ++look) {
-        const uint64_t T = sh.lists[0][a.k - 1];
         const Candidates<true> cand(sh.cand, &sh.count, kCandidates, T);
-        const bool owner = key != 0 && key >= T;
-        if (owner) sh.owners[atomicAdd(&sh.n_owners, 1)] = tid;  // at most k of them
+        const bool owner = owns<Row<BF16>::N>(T, best, first, tid);
+        const uint32_t owners = __ballot_sync(0xffffffffu, owner);
+        if (owners) {
+          int at = 0;
+          if (lane == 0) at = atomicAdd(&sh.n_owners, __popc(owners));
+          at = __shfl_sync(0xffffffffu, at, 0) + __popc(owners & ((1u << lane) - 1));
+          if (owner) sh.owners[at] = (uint8_t)tid;
+        }
         if (rank == 0 && warp == 0) {
           const int e = owner ? row.edge(lane) : -1;
           const float xe[1] = {e >= 0 ? row.at(e) : 0.f};
@@ -551,9 +558,10 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) token_stats_block_kerne
         slow = n > kCandidates;
         if (!slow || look == kLooks - 1) break;
         __syncthreads();  // every thread has read the count
-        if (warp == 0) sh.lists[0][lane] = top;
+        if (warp == 0 && lane == a.k - 1) sh.T = top;
         if (tid == 0) sh.n_owners = sh.count = 0;
         __syncthreads();
+        T = sh.T;
       }
     }
     if (slow && warp == 0) top = slow_top<BF16>(row, v0, v1, rank == 0, a.k, lane);

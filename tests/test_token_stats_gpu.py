@@ -138,6 +138,33 @@ def test_as_many_alternatives_as_lanes(V, bf16):
 
 
 @pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("V", [41, 1924, 20001, 131071])
+def test_alternatives_of_masked_and_equal_rows(V, bf16):
+    """Fewer logits than alternatives above the mask (-inf, the type's lowest, the lowest fp32), and rows of few values."""
+    dtype = torch.bfloat16 if bf16 else torch.float32
+    masks = [-math.inf, torch.finfo(dtype).min, -1e4]
+    x, t, _, _ = inputs(12, V, bf16, seed=V, pitch=3)
+    g = torch.Generator().manual_seed(V)
+    for r in range(9):
+        few = torch.randperm(V, generator=g)[:(0, 3, 31)[r // 3]].to(DEV)
+        keep = x[r, few].clone()
+        x[r] = masks[r % 3]
+        x[r, few] = keep
+    x[0, V // 2] = 1.0  # (a row of -inf alone has its test)
+    x[9] = 0.0
+    x[10] = torch.randint(0, 2, (V,), generator=g).to(DEV)
+    x[11] = torch.arange(V, device=DEV) // 7 % 50
+    for k in (1, 5, 20, 32):
+        lp, _, lse, ids, top, _ = run(x, t, k, check=False)
+        assert torch.equal(ids.cpu().long(), alternatives(x, k))
+        want = torch.log_softmax(x.cpu().double(), 1).gather(1, ids.cpu().long())
+        # 1e-3: ds <= (2 zbar + 72 + 131071 / 32) u < 3e-4 (zbar < 50), the other terms 4 u * 200;
+        # x - m is 0 in the rows of one value.
+        some = want > -1e4  # of the others the fp32 differences are as large as the mask
+        assert ((top.cpu() - want).abs() <= 1e-3)[some].all() and (top.cpu()[~some] <= -9e3).all()
+
+
+@pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("descending", [False, True])
 @pytest.mark.parametrize("threads", [1, 3, 40])
 def test_best_logits_in_few_threads(threads, descending, bf16):
