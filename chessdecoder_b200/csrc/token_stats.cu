@@ -320,16 +320,16 @@ struct Candidates {
       if (at < most) list[at] = key;
     }
   }
-  // Second look at the shares of n threads (vectors v0 + owner, + STEP, ... below v1) by
-  // THREADS threads: 2^lg of them, the least power of two that covers a share, per
-  // owner.  Where every thread is one, in the row's order: equal logits (a mask's) leave
+  // Second look at n shares, owner o's being vectors o % STEP, + STEP, ... of part o / STEP
+  // of [v0, v1), by THREADS threads: 2^lg of them, the least power of two that covers a share, per
+  // owner.  Where all shares are owners, in the row's order: equal logits (a mask's) leave
   // no room then, and what found room has the low indices.
-  template <bool BF16, int STEP, int THREADS, typename Owner>
-  __device__ __forceinline__ void take_shares(const Row<BF16>& row, int v0, int v1, const Owner* owners, int n,
-                                              int tid) const {
+  template <bool BF16, int STEP, int THREADS>
+  __device__ __forceinline__ void take_shares(const Row<BF16>& row, int v0, int v1, int part, const uint8_t* owners,
+                                              int n, int shares, int tid) const {
     constexpr int N = Row<BF16>::N;
-    const int per = (v1 - v0 + STEP - 1) / STEP, lg = per > 1 ? 32 - __clz(per - 1) : 0, lane = tid & 31;
-    const bool all = n == STEP;
+    const int per = (part + STEP - 1) / STEP, lg = per > 1 ? 32 - __clz(per - 1) : 0, lane = tid & 31;
+    const bool all = n == shares;
     const int slots = all ? v1 - v0 : n << lg;
     for (int i0 = tid - lane; i0 < slots; i0 += 4 * THREADS) {
       if (full()) return;
@@ -338,7 +338,13 @@ struct Candidates {
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int i = i0 + lane + u * THREADS;
-        v[u] = i >= slots ? v1 : all ? v0 + i : v0 + owners[i >> lg] + STEP * (i & ((1 << lg) - 1));
+        v[u] = v1;
+        if (i < slots && all) {
+          v[u] = v0 + i;
+        } else if (i < slots) {
+          const int o = owners[i >> lg], at = o % STEP + STEP * (i & ((1 << lg) - 1));  // in its part
+          if (at < part) v[u] = v0 + o / STEP * part + at;
+        }
         raw[u] = v[u] < v1 ? row.load(v[u]) : make_uint4(0u, 0u, 0u, 0u);
       }
 #pragma unroll
@@ -431,36 +437,60 @@ __device__ __forceinline__ uint64_t best_of(const uint64_t* cand, int n, int lan
 // Short rows: a warp per row.
 // ---------------------------------------------------------------------------
 constexpr int kWarpsPerBlock = 8;
+constexpr int kParts = 4;
 constexpr int kWarpCandidates = 160;  // the slow way is short here, and shared memory is warps
 
 template <bool BF16, bool TOP>
 __global__ void __launch_bounds__(kWarpsPerBlock * 32, TOP ? 4 : 5) token_stats_warp_kernel(const Args a) {
   __shared__ uint64_t cand_s[TOP ? kWarpsPerBlock : 1][TOP ? kWarpCandidates : 1];
-  __shared__ int owners_s[TOP ? kWarpsPerBlock : 1][32];
+  __shared__ float maxima_s[TOP ? kWarpsPerBlock : 1][32 * kParts];
+  __shared__ uint8_t owners_s[TOP ? kWarpsPerBlock : 1][32 * kParts];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long r = (long long)blockIdx.x * kWarpsPerBlock + warp;
   if (r >= a.rows) return;
   const Row<BF16> row(a.logits, a.ldl, r, a.ncls);
   const int v0 = row.begin(), v1 = row.end();
   uint64_t top = 0;
-  Stat st = stream<BF16, 32>(row, v0, lane, v1, lane, a.entropy != nullptr);
-  const float best = largest(st);
+  float* maxima = maxima_s[TOP ? warp : 0];
+  uint8_t* owners = owners_s[TOP ? warp : 0];
+  // A long row in 2 or 4 parts where many alternatives are asked: of 64 or 128 shares the
+  // k that are looked at again are less of the row, and T is tighter (8192 x 8000 bf16, 32
+  // alternatives: 109 us, 61 with 2 parts, 56 with 4; with 5: 37, 37, 43).
+  const int parts = !TOP || a.k <= 12 || v1 - v0 <= 128 ? 1 : v1 - v0 <= 768 ? 2 : 4;
+  const int part = (v1 - v0 + 128 * parts - 1) / (128 * parts) * 128;  // whole chunks
+  Stat st{kLowest, 0.f, 0.f};
+#pragma unroll 1
+  for (int p = 0; p < parts; ++p) {
+    const int p0 = min(v0 + p * part, v1);
+    const Stat x = stream<BF16, 32>(row, p0, lane, min(p0 + part, v1), p == 0 ? lane : -1, a.entropy != nullptr);
+    if (TOP) maxima[p * 32 + lane] = largest(x);
+    st = p == 0 ? x : join(st, x);
+  }
   st = join_warp(st);
   if (TOP) {
     bool slow = st.s != st.s;
-    uint64_t T = bound(__shfl_sync(0xffffffffu, sort32(best, lane), a.k - 1), 0, a.k);
+    float order = sort32(maxima[lane], lane);
+#pragma unroll 1
+    for (int p = 1; p < parts; ++p) order = best32(order, sort32(maxima[p * 32 + lane], lane), lane);
+    uint64_t T = bound(__shfl_sync(0xffffffffu, order, a.k - 1), 0, a.k);
 #pragma unroll 1
     for (int look = 0; !slow; ++look) {
-      const bool owner = owns<Row<BF16>::N>(T, best, 0, lane);
-      const uint32_t owners = __ballot_sync(0xffffffffu, owner);
-      if (owner) owners_s[TOP ? warp : 0][__popc(owners & ((1u << lane) - 1))] = lane;
+      int n_owners = 0;
+      bool owner = false;  // of part 0, where the edges are
+#pragma unroll 1
+      for (int p = parts - 1; p >= 0; --p) {
+        owner = owns<Row<BF16>::N>(T, maxima[p * 32 + lane], 0, p * part + lane);
+        const uint32_t mask = __ballot_sync(0xffffffffu, owner);
+        if (owner) owners[n_owners + __popc(mask & ((1u << lane) - 1))] = (uint8_t)(p * 32 + lane);
+        n_owners += __popc(mask);
+      }
       __syncwarp();
       int n = 0;
       const Candidates<false> cand(cand_s[TOP ? warp : 0], &n, kWarpCandidates, T);
       const int e = owner ? row.edge(lane) : -1;
       const float xe[1] = {e >= 0 ? row.at(e) : 0.f};
       cand.take(xe, e, e >= 0, lane);
-      cand.take_shares<BF16, 32, 32>(row, v0, v1, owners_s[TOP ? warp : 0], __popc(owners), lane);
+      cand.take_shares<BF16, 32, 32>(row, v0, v1, part, owners, n_owners, 32 * parts, lane);
       __syncwarp();
       top = best_of(cand_s[TOP ? warp : 0], min(n, kWarpCandidates), lane);
       if (n <= kWarpCandidates) break;
@@ -551,7 +581,7 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) token_stats_block_kerne
           cand.take(xe, e, e >= 0, lane);
         }
         __syncthreads();
-        cand.take_shares<BF16, kThreads, kThreads>(row, v0, v1, sh.owners, sh.n_owners, tid);
+        cand.take_shares<BF16, kThreads, kThreads>(row, v0, v1, v1 - v0, sh.owners, sh.n_owners, kThreads, tid);
         __syncthreads();
         const int n = sh.count;
         if (warp == 0) top = best_of(sh.cand, min(n, kCandidates), lane);
@@ -675,13 +705,16 @@ inline bool al(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>
 template <bool BF16, bool TOP>
 cudaError_t launch_fwd(const Args& a, cudaStream_t st) {
   const int n = BF16 ? 8 : 4;
-  // A warp per row up to 256 vectors, and up to 1024 where there are rows to fill the
-  // device with warps; beyond that a block per row, or a cluster of up to 8 that share
-  // it (two chunks each at least) while there are few blocks per SM: fewer than four
-  // (300 rows of 131071 fp32: 35 -> 29 us), or two with alternatives, since every block
-  // then selects its own (509 rows of 131071 bf16, 20 of them: 42 us, 49 with two blocks).
+  // A warp per row up to 256 vectors, and up to 2048 where there are rows to fill the
+  // device with warps (8192 x 8000 fp32 48 us, with 5 alternatives 63; a block per row 54
+  // and 92: its parts wait for one another at each step of the selection; beyond, few
+  // warps have rows that are too long: 2400 x 32003 bf16 43 us, 35); else a block per
+  // row, or a cluster of up to 8 that share it (two chunks each at least) while there are
+  // few blocks per SM: fewer than four (300 rows of 131071 fp32: 35 -> 29 us), or two with
+  // alternatives, since every block then selects its own (509 rows of 131071 bf16, 20 of
+  // them: 42 us, 49 with two blocks).
   const long long vectors = (a.ncls + n - 1) / n;
-  if (vectors <= 8 * 32 || (vectors <= 32 * 32 && a.rows >= 148 * 16)) {
+  if (vectors <= 8 * 32 || (vectors <= 64 * 32 && a.rows >= 148 * 16)) {
     const long long blocks = (a.rows + kWarpsPerBlock - 1) / kWarpsPerBlock;
     token_stats_warp_kernel<BF16, TOP><<<(unsigned)blocks, kWarpsPerBlock * 32, 0, st>>>(a);
     return cudaGetLastError();

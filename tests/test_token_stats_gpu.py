@@ -138,6 +138,26 @@ def test_as_many_alternatives_as_lanes(V, bf16):
 
 
 @pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("V", [1029, 3999, 8003, 16001])
+def test_many_long_rows(V, bf16):
+    """Rows in one, two and four parts of a warp, equal and masked ones among them."""
+    R = 2400
+    x, t, _, _ = inputs(R, V, bf16, seed=V, pitch=1)
+    x[7::11] = -math.inf
+    x[7::11, V // 3] = 2.0
+    x[8::11] = -1e4
+    x[9::11, :40] = 30.0
+    order = x.float().sort(dim=1, descending=True, stable=True)[1]
+    want = reference(x[:33], t[:33])
+    for k in (1, 12, 13, 32):
+        lp, ent, lse, ids, top, _ = run(x, t, k, check=False)
+        assert torch.equal(ids.long(), order[:, :k])
+        assert ((lp[:33].cpu() - want["lp"]).abs() <= want["lp_tol"])[want["lp"] > -math.inf].all()
+        assert ((ent[:33].cpu() - want["ent"]).abs() <= want["ent_tol"]).all()
+        assert ((lse[:33].cpu() - want["lse"]).abs() <= want["lse_tol"]).all()
+
+
+@pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("V", [41, 1924, 20001, 131071])
 def test_alternatives_of_masked_and_equal_rows(V, bf16):
     """Fewer logits than alternatives above the mask (-inf, the type's lowest, the lowest fp32), and rows of few values."""
