@@ -13,17 +13,19 @@
 // it once.  The forward spends one ex2 and about eight other instructions per
 // logit, half (fp32) to most (bf16) of what an SM issues in the time that HBM takes.
 //
-// Alternatives.  T, the k-th largest of the threads' maxima (a warp's 32; a block's in
-// fours), is a lower bound of the k-th best logit, and only threads whose maximum
-// reaches T can hold one of the k best: their logits are read again, those that reach
-// T are gathered in shared memory -- k and a few -- and sorted by a warp.  So the
-// streaming pass has no work for the alternatives at all: its running maxima do.
+// Alternatives.  A thread notes the maximum of each of up to four parts of its vectors.
+// T, the k-th largest of the threads' maxima (or parts' of them), is a lower bound of
+// the k-th best logit, and only a share (of a thread and part) whose maximum reaches T
+// can hold one of the k best: these few are read again, the logits that reach T are
+// gathered in shared memory -- k and a few -- and sorted by a warp.  So the streaming
+// pass has next to no work for the alternatives.
 //
 // Measured on one B200 (device time, share of the copy rate): 16384 x 1924 fp32
-// forward 23.5 us (83%), with 5 alternatives 37 us (53%), gradient 41 us (95%); 509 x
-// 131071 bf16 forward 32 us (64%), with 20 alternatives 40 us (52%: selecting takes
-// each block about 4 us at its end, when its neighbours do the same), gradient 43 us
-// (96%); 300 x 131071 fp32 forward 28.6 us (85%).
+// forward 24 us (82%), with 5 alternatives 36 us (54%), gradient 41 us (95%); 8192 x 8000
+// fp32 forward 45 us (89%), with 5 alternatives 53 us (76%); 509 x 131071 bf16 forward
+// 32 us (65%), with 20 alternatives 36 us (58%: selecting takes each block about 3 us
+// at its end, when its neighbours do the same), gradient 43 us (96%); 300 x 131071
+// fp32 forward 29 us (84%).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -154,11 +156,22 @@ __device__ __forceinline__ Stat join_warp(Stat a) {
 }
 
 // One thread's share of a row: vectors first + tid, first + tid + STEP, ... below
-// last and the edge with index `edge` (or none: -1).
-template <bool BF16, int STEP>
-__device__ __forceinline__ Stat stream(const Row<BF16>& row, int first, int tid, int last, int edge, bool want_t) {
+// last and the edge with index `edge` (or none: -1).  PARTS > 0: the largest of its
+// vectors' elements in each part of [first, last), parts of `part` chunks (of kUnroll
+// vectors a thread), goes to maxima[p * STEP + tid], and that of all to best.  PARTS *
+// part is above the chunks that every thread has whole.
+template <bool BF16, int STEP, int PARTS>
+__device__ __forceinline__ Stat stream(const Row<BF16>& row, int first, int tid, int last, int edge, bool want_t,
+                                       int part, float* maxima, float* best) {
   constexpr int N = Row<BF16>::N;
   Stat st{kLowest, 0.f, 0.f};
+  float most = -INFINITY;  // in this part
+  int p = 0, left = part;
+  if (PARTS) *best = -INFINITY;
+  auto rise = [&](float cm) {
+    if (PARTS) most = fmaxf(most, cm);
+    if (cm > st.m) st.rise(cm);
+  };
   auto add = [&](uint4 raw, float (&s2)[2], float (&t2)[2]) {
     float x[N];
     Row<BF16>::values(raw, x);
@@ -192,7 +205,7 @@ __device__ __forceinline__ Stat stream(const Row<BF16>& row, int first, int tid,
     float cm = vector_max<BF16>(raw[0]);
 #pragma unroll
     for (int u = 1; u < kUnroll; ++u) cm = fmaxf(cm, vector_max<BF16>(raw[u]));
-    if (cm > st.m) st.rise(cm);
+    rise(cm);
     float s2[2] = {0.f, 0.f}, t2[2] = {0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) add(raw[u], s2, t2);
@@ -200,6 +213,12 @@ __device__ __forceinline__ Stat stream(const Row<BF16>& row, int first, int tid,
     st.t += t2[0] + t2[1];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) raw[u] = next[u];
+    if (PARTS && --left == 0) {
+      maxima[p++ * STEP + tid] = most;
+      *best = fmaxf(*best, most);
+      most = -INFINITY;
+      left = part;
+    }
   }
   const int v = first + tid;
   if (v < last) {  // what is left: a vector at least
@@ -210,7 +229,7 @@ __device__ __forceinline__ Stat stream(const Row<BF16>& row, int first, int tid,
 #pragma unroll
     for (int u = 1; u < kUnroll; ++u)
       if (v + u * STEP < last) cm = fmaxf(cm, vector_max<BF16>(raw[u]));
-    if (cm > st.m) st.rise(cm);
+    rise(cm);
     float s2[2] = {0.f, 0.f}, t2[2] = {0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
@@ -220,11 +239,12 @@ __device__ __forceinline__ Stat stream(const Row<BF16>& row, int first, int tid,
   }
   const int e = edge >= 0 ? row.edge(edge) : -1;
   if (e >= 0) st.add(row.at(e));
+  if (PARTS) {
+    maxima[p * STEP + tid] = most;
+    *best = fmaxf(*best, most);
+  }
   return st;
 }
-
-// Largest element of a share.  (It adds 1 to s.)
-__device__ __forceinline__ float largest(const Stat& st) { return st.s != 0.f ? st.m : -INFINITY; }
 
 // ---------------------------------------------------------------------------
 // Ranks, or values, in a warp: lane i holds one.
@@ -266,12 +286,11 @@ __device__ __forceinline__ uint64_t bound(float value, int first, int k) {
   return rank_key(value, value == -INFINITY ? (uint32_t)(first + k - 1) : 0xffffffffu);
 }
 
-// Whether a share with largest element `best` may hold a rank that reaches T: thread tid's
-// vectors begin with element first + tid * N, and the first 2 N threads have the edges.
-template <int N>
-__device__ __forceinline__ bool owns(uint64_t T, float best, int first, int tid) {
+// Whether a share whose vectors begin with element `first`, `best` the largest, may hold
+// a rank that reaches T.
+__device__ __forceinline__ bool owns(uint64_t T, float best, uint32_t first) {
   const float value = key_value(T);
-  return best > value || (best == value && (tid < 2 * N || (uint32_t)(first + tid * N) <= ~(uint32_t)T));
+  return best > value || (best == value && first <= ~(uint32_t)T);
 }
 
 // Elements whose rank reaches T join the candidates, until there is no room: count is
@@ -325,7 +344,7 @@ struct Candidates {
   // owner.  Where all shares are owners, in the row's order: equal logits (a mask's) leave
   // no room then, and what found room has the low indices.
   template <bool BF16, int STEP, int THREADS>
-  __device__ __forceinline__ void take_shares(const Row<BF16>& row, int v0, int v1, int part, const uint8_t* owners,
+  __device__ __forceinline__ void take_shares(const Row<BF16>& row, int v0, int v1, int part, const uint16_t* owners,
                                               int n, int shares, int tid) const {
     constexpr int N = Row<BF16>::N;
     const int per = (part + STEP - 1) / STEP, lg = per > 1 ? 32 - __clz(per - 1) : 0, lane = tid & 31;
@@ -437,60 +456,73 @@ __device__ __forceinline__ uint64_t best_of(const uint64_t* cand, int n, int lan
 // Short rows: a warp per row.
 // ---------------------------------------------------------------------------
 constexpr int kWarpsPerBlock = 8;
-constexpr int kParts = 4;
 constexpr int kWarpCandidates = 160;  // the slow way is short here, and shared memory is warps
+
+// Parts of a row whose shares are looked at again apart: of 4 x 32 shares (or 4 x 256)
+// those that can hold one of the best are little of the row.
+constexpr int kParts = 4;
+struct Parts {
+  int chunks, vectors;  // of one
+  int n;                // those that are not empty
+  __device__ __forceinline__ Parts(int vectors_, int step) {
+    const int whole = vectors_ / (step * kUnroll);
+    chunks = whole / kParts + 1;
+    vectors = chunks * step * kUnroll;
+    n = whole / chunks + 1;
+  }
+};
 
 template <bool BF16, bool TOP>
 __global__ void __launch_bounds__(kWarpsPerBlock * 32, TOP ? 4 : 5) token_stats_warp_kernel(const Args a) {
+  constexpr int N = Row<BF16>::N;
   __shared__ uint64_t cand_s[TOP ? kWarpsPerBlock : 1][TOP ? kWarpCandidates : 1];
-  __shared__ float maxima_s[TOP ? kWarpsPerBlock : 1][32 * kParts];
-  __shared__ uint8_t owners_s[TOP ? kWarpsPerBlock : 1][32 * kParts];
+  __shared__ float maxima_s[TOP ? kWarpsPerBlock : 1][TOP ? kParts * 32 : 1];
+  __shared__ uint16_t owners_s[TOP ? kWarpsPerBlock : 1][TOP ? kParts * 32 : 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long r = (long long)blockIdx.x * kWarpsPerBlock + warp;
   if (r >= a.rows) return;
   const Row<BF16> row(a.logits, a.ldl, r, a.ncls);
   const int v0 = row.begin(), v1 = row.end();
-  uint64_t top = 0;
+  const Parts parts(v1 - v0, 32);
   float* maxima = maxima_s[TOP ? warp : 0];
-  uint8_t* owners = owners_s[TOP ? warp : 0];
-  // A long row in 2 or 4 parts where many alternatives are asked: of 64 or 128 shares the
-  // k that are looked at again are less of the row, and T is tighter (8192 x 8000 bf16, 32
-  // alternatives: 109 us, 61 with 2 parts, 56 with 4; with 5: 37, 37, 43).
-  const int parts = !TOP || a.k <= 12 || v1 - v0 <= 128 ? 1 : v1 - v0 <= 768 ? 2 : 4;
-  const int part = (v1 - v0 + 128 * parts - 1) / (128 * parts) * 128;  // whole chunks
-  Stat st{kLowest, 0.f, 0.f};
-#pragma unroll 1
-  for (int p = 0; p < parts; ++p) {
-    const int p0 = min(v0 + p * part, v1);
-    const Stat x = stream<BF16, 32>(row, p0, lane, min(p0 + part, v1), p == 0 ? lane : -1, a.entropy != nullptr);
-    if (TOP) maxima[p * 32 + lane] = largest(x);
-    st = p == 0 ? x : join(st, x);
-  }
-  st = join_warp(st);
+  uint16_t* owners = owners_s[TOP ? warp : 0];
+  float best;  // of this lane
+  const Stat st = join_warp(
+      stream<BF16, 32, TOP ? kParts : 0>(row, v0, lane, v1, lane, a.entropy != nullptr, parts.chunks, maxima, &best));
+  uint64_t top = 0;
   if (TOP) {
     bool slow = st.s != st.s;
-    float order = sort32(maxima[lane], lane);
+    // the k-th of 32 maxima, or 64 or 128 where k is near that: the 32nd of 32 admits 130 of a row, of 128 37
+    const int lists = min(a.k <= 12 ? 1 : a.k <= 24 ? 2 : 4, parts.n);
+    float order = -INFINITY;
+    if (lists == 1) {
+      order = sort32(best, lane);
+    } else {
 #pragma unroll 1
-    for (int p = 1; p < parts; ++p) order = best32(order, sort32(maxima[p * 32 + lane], lane), lane);
+      for (int i = 0; i < lists; ++i) {
+        float x = -INFINITY;
+        for (int p = i; p < parts.n; p += lists) x = fmaxf(x, maxima[p * 32 + lane]);
+        order = best32(order, sort32(x, lane), lane);
+      }
+    }
     uint64_t T = bound(__shfl_sync(0xffffffffu, order, a.k - 1), 0, a.k);
 #pragma unroll 1
     for (int look = 0; !slow; ++look) {
       int n_owners = 0;
-      bool owner = false;  // of part 0, where the edges are
 #pragma unroll 1
-      for (int p = parts - 1; p >= 0; --p) {
-        owner = owns<Row<BF16>::N>(T, maxima[p * 32 + lane], 0, p * part + lane);
+      for (int p = 0; p < parts.n; ++p) {
+        const bool owner = owns(T, maxima[p * 32 + lane], (uint32_t)(p * parts.vectors + lane) * N);
         const uint32_t mask = __ballot_sync(0xffffffffu, owner);
-        if (owner) owners[n_owners + __popc(mask & ((1u << lane) - 1))] = (uint8_t)(p * 32 + lane);
+        if (owner) owners[n_owners + __popc(mask & ((1u << lane) - 1))] = (uint16_t)(p * 32 + lane);
         n_owners += __popc(mask);
       }
       __syncwarp();
       int n = 0;
       const Candidates<false> cand(cand_s[TOP ? warp : 0], &n, kWarpCandidates, T);
-      const int e = owner ? row.edge(lane) : -1;
+      const int e = row.edge(lane);
       const float xe[1] = {e >= 0 ? row.at(e) : 0.f};
       cand.take(xe, e, e >= 0, lane);
-      cand.take_shares<BF16, 32, 32>(row, v0, v1, part, owners, n_owners, 32 * parts, lane);
+      cand.take_shares<BF16, 32, 32>(row, v0, v1, parts.vectors, owners, n_owners, 32 * parts.n, lane);
       __syncwarp();
       top = best_of(cand_s[TOP ? warp : 0], min(n, kWarpCandidates), lane);
       if (n <= kWarpCandidates) break;
@@ -504,22 +536,22 @@ __global__ void __launch_bounds__(kWarpsPerBlock * 32, TOP ? 4 : 5) token_stats_
 }
 
 // ---------------------------------------------------------------------------
-// Long rows: a block of 256 threads per row, or a cluster of blocks that share
+// Long rows: a block of 256 or 128 threads per row, or a cluster of blocks that share
 // the row's vectors; the blocks' (m, s, t) and best lists are joined by the first
 // of them through distributed shared memory.
 // ---------------------------------------------------------------------------
 constexpr int kThreads = 256;
-constexpr int kRowWarps = kThreads / 32;
 
-template <bool TOP>
+template <bool TOP, int THREADS>
 struct RowShared {
   uint64_t cand[TOP ? kCandidates : 1];
   uint64_t best[32];  // this block's best, descending
   uint64_t T;
-  float maxima[64];   // of four threads each
-  uint8_t owners[TOP ? kThreads : 1];
+  float maxima[64];   // of THREADS / 64 threads each
+  float shares[TOP ? kParts * THREADS : 1];
+  uint16_t owners[TOP ? kParts * THREADS : 1];
   int n_owners, count;
-  Stat part[kRowWarps];
+  Stat part[THREADS / 32];
   Stat st;            // this block's
 };
 
@@ -530,9 +562,9 @@ __device__ __forceinline__ const T* remote(const T* p, uint32_t rank) {
   return reinterpret_cast<const T*>(q);
 }
 
-template <bool BF16, bool TOP>
-__global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) token_stats_block_kernel(const Args a, int blocks_per_row) {
-  __shared__ RowShared<TOP> sh;
+template <bool BF16, bool TOP, int THREADS>
+__global__ void __launch_bounds__(THREADS, (TOP ? 4 : 5) * kThreads / THREADS) token_stats_block_kernel(const Args a, int blocks_per_row) {
+  __shared__ RowShared<TOP, THREADS> sh;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long r = blockIdx.x / blocks_per_row;
   const int rank = (int)(blockIdx.x % blocks_per_row);
@@ -542,12 +574,16 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) token_stats_block_kerne
   const int v0 = min(begin + rank * per_block, end), v1 = min(v0 + per_block, end);
   const int first = rank == 0 ? 0 : v0 * Row<BF16>::N - row.mis;  // element
   const int edge = rank == 0 && warp == 0 ? lane : -1;  // the first warp of the first block has the edges
-  Stat st = stream<BF16, kThreads>(row, v0, tid, v1, edge, a.entropy != nullptr);
-  const float best = largest(st);
+  const Parts parts(v1 - v0, THREADS);
+  float best;  // of this thread
+  Stat st = stream<BF16, THREADS, TOP ? kParts : 0>(row, v0, tid, v1, edge, a.entropy != nullptr, parts.chunks,
+                                                    sh.shares, &best);
   if (TOP) {
-    float x = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
-    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-    if (lane % 4 == 0) sh.maxima[tid / 4] = x;
+    constexpr int kGroup = THREADS / 64;
+    float x = best;
+#pragma unroll
+    for (int o = 1; o < kGroup; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+    if (lane % kGroup == 0) sh.maxima[tid / kGroup] = x;
   }
   st = join_warp(st);
   if (lane == 0) sh.part[warp] = st;
@@ -555,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) token_stats_block_kerne
   __syncthreads();
   st = sh.part[0];
 #pragma unroll
-  for (int w = 1; w < kRowWarps; ++w) st = join(st, sh.part[w]);  // the same order in every thread
+  for (int w = 1; w < THREADS / 32; ++w) st = join(st, sh.part[w]);  // the same order in every thread
   uint64_t top = 0;
   if (TOP) {
     const bool broken = st.s != st.s;
@@ -567,21 +603,27 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) token_stats_block_kerne
 #pragma unroll 1
       for (int look = 0;; ++look) {
         const Candidates<true> cand(sh.cand, &sh.count, kCandidates, T);
-        const bool owner = owns<Row<BF16>::N>(T, best, first, tid);
-        const uint32_t owners = __ballot_sync(0xffffffffu, owner);
-        if (owners) {
-          int at = 0;
-          if (lane == 0) at = atomicAdd(&sh.n_owners, __popc(owners));
-          at = __shfl_sync(0xffffffffu, at, 0) + __popc(owners & ((1u << lane) - 1));
-          if (owner) sh.owners[at] = (uint8_t)tid;
+        if (__any_sync(0xffffffffu, best >= cand.value)) {
+#pragma unroll 1
+          for (int p = 0; p < parts.n; ++p) {
+            const bool owner =
+                owns(T, sh.shares[p * THREADS + tid], first + (uint32_t)(p * parts.vectors + tid) * Row<BF16>::N);
+            const uint32_t owners = __ballot_sync(0xffffffffu, owner);
+            if (owners == 0) continue;
+            int at = 0;
+            if (lane == 0) at = atomicAdd(&sh.n_owners, __popc(owners));
+            at = __shfl_sync(0xffffffffu, at, 0) + __popc(owners & ((1u << lane) - 1));
+            if (owner) sh.owners[at] = (uint16_t)(p * THREADS + tid);
+          }
         }
         if (rank == 0 && warp == 0) {
-          const int e = owner ? row.edge(lane) : -1;
+          const int e = row.edge(lane);
           const float xe[1] = {e >= 0 ? row.at(e) : 0.f};
           cand.take(xe, e, e >= 0, lane);
         }
         __syncthreads();
-        cand.take_shares<BF16, kThreads, kThreads>(row, v0, v1, v1 - v0, sh.owners, sh.n_owners, kThreads, tid);
+        cand.take_shares<BF16, THREADS, THREADS>(row, v0, v1, parts.vectors, sh.owners, sh.n_owners,
+                                                   THREADS * parts.n, tid);
         __syncthreads();
         const int n = sh.count;
         if (warp == 0) top = best_of(sh.cand, min(n, kCandidates), lane);
@@ -602,7 +644,7 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) token_stats_block_kerne
     cluster_sync();
     if (rank == 0 && warp == 0) {
       for (int c = 1; c < blocks_per_row; ++c) {
-        const RowShared<TOP>* o = remote(&sh, (uint32_t)c);
+        const RowShared<TOP, THREADS>* o = remote(&sh, (uint32_t)c);
         st = join(st, Stat{o->st.m, o->st.s, o->st.t});
         if (TOP) top = best32(top, o->best[lane], lane);
       }
@@ -706,7 +748,7 @@ template <bool BF16, bool TOP>
 cudaError_t launch_fwd(const Args& a, cudaStream_t st) {
   const int n = BF16 ? 8 : 4;
   // A warp per row up to 256 vectors, and up to 2048 where there are rows to fill the
-  // device with warps (8192 x 8000 fp32 48 us, with 5 alternatives 63; a block per row 54
+  // device with warps (8192 x 8000 fp32 45 us, with 5 alternatives 53; a block per row 54
   // and 92: its parts wait for one another at each step of the selection; beyond, few
   // warps have rows that are too long: 2400 x 32003 bf16 43 us, 35); else a block per
   // row, or a cluster of up to 8 that share it (two chunks each at least) while there are
@@ -722,9 +764,13 @@ cudaError_t launch_fwd(const Args& a, cudaStream_t st) {
   int c = 1;
   while (c < 8 && a.rows * c < (TOP ? 2 : 4) * 148 && vectors >= 2 * (2 * c) * kThreads * kUnroll) c *= 2;
   if (a.rows * c > 0x7fffffffll) return cudaErrorInvalidValue;
+  // Half the threads where rows are not very long and fill the device all the same: more
+  // rows at a time on an SM, so that one selects while others stream (8192 x 32003 bf16
+  // 102 -> 91 us, with 5 alternatives 150 -> 116; 1300 x 131071 with 20: 79, 90).
+  const bool small = c == 1 && vectors <= 8192 && a.rows >= (vectors <= 2048 ? 2 : 4) * 148;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.rows * c));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(small ? kThreads / 2 : kThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -732,7 +778,9 @@ cudaError_t launch_fwd(const Args& a, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = c > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, token_stats_block_kernel<BF16, TOP>, (const Args)a, c);
+  return cudaLaunchKernelEx(
+      &cfg, small ? token_stats_block_kernel<BF16, TOP, kThreads / 2> : token_stats_block_kernel<BF16, TOP, kThreads>,
+      (const Args)a, c);
 }
 
 }  // namespace

@@ -138,10 +138,9 @@ def test_as_many_alternatives_as_lanes(V, bf16):
 
 
 @pytest.mark.parametrize("bf16", [False, True])
-@pytest.mark.parametrize("V", [1029, 3999, 8003, 16001])
-def test_many_long_rows(V, bf16):
-    """Rows in one, two and four parts of a warp, equal and masked ones among them."""
-    R = 2400
+@pytest.mark.parametrize("R,V", [(2400, 1029), (2400, 3999), (2400, 8003), (2400, 16001), (600, 20001), (600, 33001)])
+def test_many_long_rows(R, V, bf16):
+    """A warp's rows in one part and more, a block's with fewer and more threads, equal and masked ones among them."""
     x, t, _, _ = inputs(R, V, bf16, seed=V, pitch=1)
     x[7::11] = -math.inf
     x[7::11, V // 3] = 2.0
