@@ -342,8 +342,8 @@ __global__ void __launch_bounds__(256)
 // below 2^8), so that most tiles need no exchange between lanes and no rescaling.
 //
 // Work.  The keys of one (sequence, kv head) item are cut into tiles of 32.
-// Where the tables hold few tiles per item, a block takes an item,
-// its four warps a quarter of the tiles each.  Otherwise the tiles of all items,
+// Where the tables hold few tiles per item (warps_per_item), a block takes an item, its
+// warps a part of the tiles each, or a warp does.  Otherwise the tiles of all items,
 // in the order (sequence, head, tile), are dealt to the grid's warps in equal
 // contiguous runs, whatever the lengths; an item counts kSetup tiles more than it
 // has, for what it costs a warp to begin one.  A warp that holds a whole item writes
@@ -385,11 +385,6 @@ constexpr int kAttnWarps = kAttnBlocks * kWarps;
 constexpr int kSlots = 2 * kAttnWarps;
 constexpr float kNoScore = -3.0e38f;  // m before the first key
 constexpr float kSlack = 8.f;
-// Tiles per item up to which a block takes an item: the second kernel's launch
-// and the deal's search cost more than a warp's few tiles in a row (64 x 512 keys:
-// 25 us; the deal takes 30 for 64 x 520; one game of 137 keys: 4.1 us and 6.8).
-constexpr int kItemTiles = 16;
-
 // What beginning an item costs a warp, in tiles of the deal: its table, queries and
 // first rows come one after the other.  (64 sequences of 0 .. 2000 keys: 72 us
 // without, 59 with 1, 50 with 2, 51 with 3 -- a warp that is dealt fourteen items of
@@ -976,14 +971,32 @@ struct AttnShared {
     const int results = (group * (kHD * 4 + 8) + 15) / 16 * 16;
     return fp8 && results < kStages * kStageBytes ? kStages * kStageBytes : results;
   }
-  static __host__ __device__ constexpr int bytes(int group, bool fp8) { return kWarps * region_bytes(group, fp8) + 112; }
+  static __host__ __device__ constexpr int bytes(int group, bool fp8, int n_warps = kWarps) {
+    return n_warps * region_bytes(group, fp8) + 112;
+  }
 };
 static_assert(kMaxGroup * (kHD * 4 + 8) <= kStages * kStageBytes, "a warp's results fit its ring");
+
+// The output of an item from the state of the warp that had all of it.
+template <int NT>
+__device__ __forceinline__ void store_item(const AttnArgs& a, const Acc<NT>& acc, int b, int kvh, int lane) {
+  const int g = lane >> 2, t4 = lane & 3;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int hq = n * 8 + 2 * t4 + c;
+      if (hq >= a.group) continue;
+      float v[8];
+      acc.dims(n, c, v);
+      store_out8(a, b, kvh * a.group + hq, 8 * g, v, acc.l[n][c] == 0.f ? 0.f : 1.f / acc.l[n][c]);
+    }
+}
 
 // A block whose warps all worked on one item (a warp without tiles has an empty
 // state): their sum goes to the output, or to workspace slot `slot` when other
 // blocks share the item.
-template <int NT>
+template <int NT, int W>
 __device__ __forceinline__ void merge_block(const AttnArgs& a, const AttnShared& sh, const Acc<NT>& acc, int b, int kvh,
                                             bool whole, int slot) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
@@ -1002,13 +1015,13 @@ __device__ __forceinline__ void merge_block(const AttnArgs& a, const AttnShared&
       if (g == 0) sh.stat(warp, hq) = make_float2(acc.m[n][c], acc.l[n][c]);
     }
   __syncthreads();
-  for (int i = tid; i < a.group * (kHD / 8); i += kAttnThreads) {
+  for (int i = tid; i < a.group * (kHD / 8); i += W * 32) {
     const int hq = i / (kHD / 8), d = (i % (kHD / 8)) * 8;
     float m = kNoScore, l = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sh.stat(w, hq).x);
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+#pragma unroll 4
+    for (int w = 0; w < W; ++w) m = fmaxf(m, sh.stat(w, hq).x);
+#pragma unroll 4
+    for (int w = 0; w < W; ++w) {
       const float f = ex2(sh.stat(w, hq).x - m);
       l += sh.stat(w, hq).y * f;
 #pragma unroll
@@ -1026,22 +1039,26 @@ __device__ __forceinline__ void merge_block(const AttnArgs& a, const AttnShared&
   }
 }
 
-// A block per (sequence, kv head).
-template <bool FP8, int NT, bool WIDE>
-__global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 3) paged_attn_item_kernel(const AttnArgs a) {
+// SPLIT warps per (sequence, kv head): a block of them, or a warp of a block of four.
+template <bool FP8, int NT, bool WIDE, int SPLIT>
+__global__ void __launch_bounds__(SPLIT > 4 ? SPLIT * 32 : kAttnThreads, SPLIT > 4 ? 3 - NT : 5 - NT)
+    paged_attn_item_kernel(const AttnArgs a) {
   extern __shared__ __align__(16) char smem[];
   const AttnShared sh(smem, a.group, FP8);
-  char* ring = sh.of(threadIdx.x >> 5);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int b = blockIdx.x / a.pg.kv_heads, kvh = blockIdx.x - b * a.pg.kv_heads;
-  const int len = length_of(a, b, kvh == 0 && threadIdx.x == 0);
-  const int tiles = (len + kTK - 1) / kTK, per = (tiles + kWarps - 1) / kWarps;
-  const int ta = min(warp * per, tiles), tb = min(ta + per, tiles);
+  char* ring = sh.of(warp);
+  const int item = SPLIT == 1 ? (int)blockIdx.x * kWarps + warp : (int)blockIdx.x;
+  if (SPLIT == 1 && item >= a.B * a.pg.kv_heads) return;
+  const int b = item / a.pg.kv_heads, kvh = item - b * a.pg.kv_heads;
+  const int len = length_of(a, b, kvh == 0 && (SPLIT == 1 ? lane : (int)threadIdx.x) == 0);
+  const int tiles = (len + kTK - 1) / kTK, per = (tiles + SPLIT - 1) / SPLIT;
+  const int ta = SPLIT == 1 ? 0 : min(warp * per, tiles), tb = min(ta + per, tiles);
   Acc<NT> acc;
   acc.clear();
   if (ta < tb) attend<FP8, NT, WIDE>(a, b, kvh, ta, tb, len, lane, ring, acc);
   acc.sum_lanes();
-  merge_block<NT>(a, sh, acc, b, kvh, true, 0);  // len 0: l = 0, zeros
+  if (SPLIT == 1) store_item<NT>(a, acc, b, kvh, lane);  // len 0: l = 0, zeros
+  else merge_block<NT, SPLIT>(a, sh, acc, b, kvh, true, 0);
 }
 
 // Shares [f, f + chunk) of the deal for warp w = f / chunk; see the join for the slots.
@@ -1122,7 +1139,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 3) paged_attn_kern
     acc.clear();
     if (f < f_end && ta < tb) attend<FP8, NT, WIDE>(a, bi.b, bi.kvh, ta, tb, length_of(a, bi.b, false), lane, ring, acc);
     acc.sum_lanes();
-    merge_block<NT>(a, sh, acc, bi.b, bi.kvh, block_f == bi.first && block_end == bi.first + bi.n, 2 * (int)w0);
+    merge_block<NT, kWarps>(a, sh, acc, bi.b, bi.kvh, block_f == bi.first && block_end == bi.first + bi.n, 2 * (int)w0);
     return;
   }
   while (f < f_end) {
@@ -1135,7 +1152,10 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 3) paged_attn_kern
     acc.clear();
     attend<FP8, NT, WIDE>(a, it.b, it.kvh, ta, tb, length_of(a, it.b, false), lane, ring, acc);
     acc.sum_lanes();
-    const bool whole = ta == 0 && tb == it.n - kSetup;
+    if (ta == 0 && tb == it.n - kSetup) {
+      store_item<NT>(a, acc, it.b, it.kvh, lane);
+      continue;
+    }
     const int slot = 2 * (int)w + (ta == 0 ? 1 : 0);
     const int g = lane >> 2, t4 = lane & 3;
 #pragma unroll
@@ -1146,15 +1166,11 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 3) paged_attn_kern
         if (hq >= a.group) continue;
         float v[8];
         acc.dims(n, c, v);
-        if (whole) {
-          store_out8(a, it.b, it.kvh * a.group + hq, 8 * g, v, acc.l[n][c] == 0.f ? 0.f : 1.f / acc.l[n][c]);
-        } else {
-          const int at = slot * a.group + hq;
-          float4* dst = reinterpret_cast<float4*>(a.part + at * kHD + 8 * g);
-          dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-          dst[1] = make_float4(v[4], v[5], v[6], v[7]);
-          if (g == 0) a.stat[at] = make_float2(acc.m[n][c], acc.l[n][c]);
-        }
+        const int at = slot * a.group + hq;
+        float4* dst = reinterpret_cast<float4*>(a.part + at * kHD + 8 * g);
+        dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+        dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+        if (g == 0) a.stat[at] = make_float2(acc.m[n][c], acc.l[n][c]);
       }
   }
 }
@@ -1347,6 +1363,23 @@ extern "C" int cdk_paged_gather(const CdkPagedCache* cache, int64_t B, const int
 namespace {
 inline int64_t prefix_bytes(int64_t B) { return ((B + 1) * 4 + 15) / 16 * 16; }
 
+// Warps that share an item of at most max_tiles tiles, or 0: the deal.  The deal's cost
+// beside the keys -- its search, the partial results, the second launch -- is some 5 us
+// and grows with the items; a block per item leaves SMs idle at the end while the
+// longest is read.  So a block takes an item up to 32 tiles (300 x 1000 keys of 2 heads:
+// 35 us both ways, 150 x 1000: 18 and 22), and longer ones where items are many and
+// the end is little of the whole (1600 x 1 .. 4000 keys of 2 heads: 252 us, 270 by the
+// deal; 64 x 1 .. 2000 of 16: 53, 49).  Eight warps while every block of that size is
+// resident at once (72 x 1000 of 2 heads: 11.8 us, 14.4 with four, 16.0 by the deal); a
+// warp of its own where blocks would be many and short (1600 x 32 of 2 heads: 9.9, 17.4).
+constexpr int kMany = 8;
+inline int warps_per_item(long long items, long long max_tiles, int group) {
+  if (items > kAttnBlocks && max_tiles <= (items >= 2 * kAttnBlocks ? 8 : 2)) return 1;
+  if (items <= (group <= 8 ? 2 : 1) * 148 && max_tiles > 4 && max_tiles <= 32) return kMany;
+  const long long most = items / 18;
+  return max_tiles <= (most < 32 ? 32 : most > 256 ? 256 : most) ? kWarps : 0;
+}
+
 template <bool FP8, int NT, bool WIDE>
 cudaError_t launch_attn(const AttnArgs& a, long long max_tiles, cudaStream_t st) {
   const long long items = (long long)a.B * a.pg.kv_heads;
@@ -1356,18 +1389,27 @@ cudaError_t launch_attn(const AttnArgs& a, long long max_tiles, cudaStream_t st)
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess || dev < 0 || dev >= 64) return e != cudaSuccess ? e : cudaErrorInvalidDevice;
   if (!done[dev]) {
-    const int most = AttnShared::bytes(kMaxGroup, FP8);
-    e = cudaFuncSetAttribute(paged_attn_item_kernel<FP8, NT, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(paged_attn_kernel<FP8, NT, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)prefix_bytes(kMaxSeqs) + most);
+    auto allow = [&](const void* f, int bytes) {
+      if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    };
+    allow((const void*)paged_attn_item_kernel<FP8, NT, WIDE, 1>, AttnShared::bytes(kMaxGroup, FP8));
+    allow((const void*)paged_attn_item_kernel<FP8, NT, WIDE, kWarps>, AttnShared::bytes(kMaxGroup, FP8));
+    allow((const void*)paged_attn_item_kernel<FP8, NT, WIDE, kMany>, AttnShared::bytes(kMaxGroup, FP8, kMany));
+    allow((const void*)paged_attn_kernel<FP8, NT, WIDE>, (int)prefix_bytes(kMaxSeqs) + AttnShared::bytes(kMaxGroup, FP8));
     if (e != cudaSuccess) return e;
     done[dev] = true;
   }
-  if (max_tiles <= kItemTiles) {
-    paged_attn_item_kernel<FP8, NT, WIDE><<<(unsigned)items, kAttnThreads, smem, st>>>(a);
-    return cudaGetLastError();
+  const int split = warps_per_item(items, max_tiles, a.group);
+  if (split == 1) {
+    const unsigned blocks = (unsigned)((items + kWarps - 1) / kWarps);
+    paged_attn_item_kernel<FP8, NT, WIDE, 1><<<blocks, kAttnThreads, smem, st>>>(a);
+  } else if (split == kWarps) {
+    paged_attn_item_kernel<FP8, NT, WIDE, kWarps><<<(unsigned)items, kAttnThreads, smem, st>>>(a);
+  } else if (split == kMany) {
+    paged_attn_item_kernel<FP8, NT, WIDE, kMany>
+        <<<(unsigned)items, kMany * 32, AttnShared::bytes(a.group, FP8, kMany), st>>>(a);
   }
+  if (split) return cudaGetLastError();
   // no more warps than tiles that the tables can hold: one tile is the smallest share
   const long long bound = max_tiles * items;
   const unsigned grid = (unsigned)(bound >= kAttnWarps ? kAttnBlocks : (bound + kWarps - 1) / kWarps);
@@ -1376,8 +1418,12 @@ cudaError_t launch_attn(const AttnArgs& a, long long max_tiles, cudaStream_t st)
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(items * a.group));
-  // few items have many results each (592 for one item): more warps then
-  cfg.blockDim = dim3(items >= 148 ? 128 : kJoinWarps * 32);
+  // eight results in flight per warp; an item has one from each block inside it, and of
+  // the warps of the blocks at its ends (592 of one long item, 12 of 23 tiles)
+  const long long results = (max_tiles < kAttnWarps ? max_tiles : kAttnWarps) / kWarps + 6;
+  const long long warps = (results + 7) / 8, most = items >= 148 ? 4 : kJoinWarps;
+  const int join = (int)(warps < most ? warps : most);
+  cfg.blockDim = dim3(join * 32);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];  // set up while the first kernel drains; it waits for it before its first load
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1392,7 +1438,7 @@ extern "C" int64_t cdk_paged_attn_workspace(int64_t B, int64_t H, int64_t kv_hea
   if (B < 0 || B > kMaxSeqs || H <= 0 || H > 65536 || kv_heads <= 0 || H % kv_heads || H / kv_heads > kMaxGroup ||
       max_keys < 0)
     return -1;
-  if (max_keys <= (int64_t)kItemTiles * kTK) return 0;
+  if (max_keys < (1ll << 31) && warps_per_item(B * kv_heads, (max_keys + kTK - 1) / kTK, (int)(H / kv_heads))) return 0;
   return prefix_bytes(B) + (int64_t)kSlots * (H / kv_heads) * (16 + kHD * 4);
 }
 

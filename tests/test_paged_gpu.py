@@ -234,6 +234,18 @@ def test_attn_uneven_batches(lens, fp8):
     run_attn(lens, 4, 2, 64, fp8, seed=len(lens))
 
 
+# a warp per item; eight; four, with one to many waves of blocks; the deal
+WAYS = [[i * 7 % 61 for i in range(320)], [i * 37 % 257 for i in range(640)], [700, 0, 33, 1000, 129],
+        [i * 331 % 1001 for i in range(160)], [0, 1, 1500, 40, 3000], [i * 331 % 1201 for i in range(150)]]
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("H,p", [(2, 16), (16, 64), (18, 16), (32, 32)])
+@pytest.mark.parametrize("lens", WAYS, ids=["warp", "warp8", "eight", "four", "deal", "deal150"])
+def test_attn_ways(lens, H, p, fp8):
+    run_attn(lens, H, 2, p, fp8, seed=H)
+
+
 @pytest.mark.parametrize("fp8", [False, True])
 def test_attn_sharp_and_flat_scores(fp8):
     for scale in (0.0, 1.0, -2.0, 8.0):
