@@ -370,12 +370,12 @@ __global__ void __launch_bounds__(256)
 // sum of the w_j alone reaches 2^(8 - e_j); e_j below -96 counts as -96 for m (a
 // row of zeros has the smallest scale), which only values below 448 * 2^-96 feel.
 //
-// Measured on one B200 (16 heads, device time, both kernels): bf16, 256 sequences of
-// up to 4095 keys 334 us (2.15 GB: the copy rate), 64 of up to 2000 48 us (85%),
-// 64 x 512 (an item per block) 25 us (83%); e4m3, 256 x 2000 176 us (94%), 6 of up to
+// Measured on one B200 (16 heads, device time, join and all): bf16, 256 sequences of up to
+// 4095 keys 319 us (2.15 GB: the copy rate; 334 by the deal), 64 of up to 2000 49 us
+// (84%), 64 x 512 25 us (82%); e4m3, 256 x 2000 163 us (101%; 177 by the deal), 6 of up to
 // 65536 with groups of 8 heads 27 us (62%: of the 10 us over the floor about 5 pass
 // before the first rows arrive -- launch, lengths, table, rows -- and 2 in the join).
-// Pages of 16 rows: 256 sequences of up to 4000 keys 338 us bf16 (96%), 188 e4m3 (88%).
+// Pages of 16 rows: 256 sequences of up to 4000 keys 336 us bf16 (97%), 174 e4m3 (95%).
 // ---------------------------------------------------------------------------
 constexpr int kTK = 32;             // keys per tile
 constexpr int kAttnThreads = 128;   // 4 warps; 128 registers: 4 blocks per SM
@@ -1372,11 +1372,13 @@ inline int64_t prefix_bytes(int64_t B) { return ((B + 1) * 4 + 15) / 16 * 16; }
 // deal; 64 x 1 .. 2000 of 16: 53, 49).  Eight warps while every block of that size is
 // resident at once (72 x 1000 of 2 heads: 11.8 us, 14.4 with four, 16.0 by the deal); a
 // warp of its own where blocks would be many and short (1600 x 32 of 2 heads: 9.9, 17.4).
+// The tiles of bf16 pages below 32 rows take a warp twice as long, so that the end is
+// more (256 x 1 .. 4000 keys of 16 heads on pages of 16: 361 us, 338 by the deal).
 constexpr int kMany = 8;
-inline int warps_per_item(long long items, long long max_tiles, int group) {
-  if (items > kAttnBlocks && max_tiles <= (items >= 2 * kAttnBlocks ? 8 : 2)) return 1;
+inline int warps_per_item(long long items, long long max_tiles, int group, bool fp8, bool wide) {
+  if (items > kAttnBlocks && max_tiles <= (items < 2 * kAttnBlocks ? 2 : fp8 ? 8 : 4)) return 1;
   if (items <= (group <= 8 ? 2 : 1) * 148 && max_tiles > 4 && max_tiles <= 32) return kMany;
-  const long long most = items / 18;
+  const long long most = fp8 || wide ? items / 18 : 0;
   return max_tiles <= (most < 32 ? 32 : most > 256 ? 256 : most) ? kWarps : 0;
 }
 
@@ -1399,7 +1401,7 @@ cudaError_t launch_attn(const AttnArgs& a, long long max_tiles, cudaStream_t st)
     if (e != cudaSuccess) return e;
     done[dev] = true;
   }
-  const int split = warps_per_item(items, max_tiles, a.group);
+  const int split = warps_per_item(items, max_tiles, a.group, FP8, WIDE);
   if (split == 1) {
     const unsigned blocks = (unsigned)((items + kWarps - 1) / kWarps);
     paged_attn_item_kernel<FP8, NT, WIDE, 1><<<blocks, kAttnThreads, smem, st>>>(a);
@@ -1438,7 +1440,9 @@ extern "C" int64_t cdk_paged_attn_workspace(int64_t B, int64_t H, int64_t kv_hea
   if (B < 0 || B > kMaxSeqs || H <= 0 || H > 65536 || kv_heads <= 0 || H % kv_heads || H / kv_heads > kMaxGroup ||
       max_keys < 0)
     return -1;
-  if (max_keys < (1ll << 31) && warps_per_item(B * kv_heads, (max_keys + kTK - 1) / kTK, (int)(H / kv_heads))) return 0;
+  // whatever the pages are: the smaller set of those that need none
+  if (max_keys < (1ll << 31) && warps_per_item(B * kv_heads, (max_keys + kTK - 1) / kTK, (int)(H / kv_heads), false, false))
+    return 0;
   return prefix_bytes(B) + (int64_t)kSlots * (H / kv_heads) * (16 + kHD * 4);
 }
 

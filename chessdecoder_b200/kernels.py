@@ -862,7 +862,7 @@ def paged_attn(q, k_pages, v_pages, table, lens, out, *, k_scale=None, v_scale=N
     _call("paged_attn", lib().cdk_paged_attn, dev, q.data_ptr(), ldq,
           _cache_arg(k_pages, v_pages, k_scale, v_scale, table, fields), B, H, lens.data_ptr(), out.data_ptr(), ldo,
           scale, workspace.data_ptr() if need else None, need)
-    _count(2 if need else 1)  # the item kernel, or the deal and the join
+    _count(2 if need else 1)  # the item kernel, or (where a workspace is needed, mostly) the deal and the join
 
 
 # ---------------------------------------------------------------------------
