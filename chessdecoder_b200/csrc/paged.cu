@@ -158,7 +158,7 @@ __device__ __forceinline__ uint2 quantise8(const float (&x)[8], int* byte) {
 }
 
 template <bool F32, bool FP8>
-__global__ void __launch_bounds__(256, 4)
+__global__ void __launch_bounds__(128, 8)  // (a block's warps end at different times: 256 threads 2% longer)
     paged_append_kernel(const void* __restrict__ qkv, long long ldq, const int32_t* __restrict__ pos,
                         const float* __restrict__ rope, long long rope_len, unsigned S_new, int H, Pages pg,
                         const int32_t* __restrict__ start, const int32_t* __restrict__ num_new,
@@ -1324,11 +1324,11 @@ extern "C" int cdk_paged_append(const void* qkv, int64_t ldq, int qkv_f32, const
   long long parts = (148 * 16 + tokens - 1) / tokens;
   if (parts > (most + 3) / 4) parts = (most + 3) / 4;
   if (tokens * parts > 0xfffffff0ll) parts = 1;
-  const long long blocks = (tokens * parts + 7) / 8;
+  const long long blocks = (tokens * parts + 3) / 4;
   auto* st = reinterpret_cast<cudaStream_t>(stream);
   auto* qo = reinterpret_cast<__nv_bfloat16*>(q_out);
 #define CDK_APPEND(F32, FP8)                                                                                     \
-  paged_append_kernel<F32, FP8><<<(unsigned)blocks, 256, 0, st>>>(qkv, ldq, pos, rope, rope_len, (unsigned)S_new,   \
+  paged_append_kernel<F32, FP8><<<(unsigned)blocks, 128, 0, st>>>(qkv, ldq, pos, rope, rope_len, (unsigned)S_new,   \
                                                                   (int)H, pg, start, num_new, qo, ldo,               \
                                                                   (unsigned)tokens, (unsigned)parts)
   if (cache->dtype == 1) {
