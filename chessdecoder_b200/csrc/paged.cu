@@ -80,10 +80,11 @@ __device__ __forceinline__ int page_of(const Pages& p, long long b, long long j)
 // add), so that a quantised code does not depend on how a compiler contracts
 // them.  Bound by HBM: one read of qkv, one write of each row.  Measured on one
 // B200 (16 + 16 + 16 heads): 18,200 fp32 tokens rotated into bf16 pages 54 us, 97%
-// of the copy rate, into e4m3 pages 49 us (94%); bf16 rows into e4m3 pages 24 us
-// (73%: fewer bytes for the same instructions).  A lane per eight values with all
+// of the copy rate, into e4m3 pages 49 us (94%); bf16 rows into e4m3 pages 23 us
+// (74%: fewer bytes for the same instructions).  A lane per eight values with all
 // indices its own took 70 us there; a warp per token whose row loads came after
-// the place was looked up 35, before it 27; keys and values together 24.
+// the place was looked up 35, before it 27; keys and values together 24, blocks of 128
+// threads 23.
 // ---------------------------------------------------------------------------
 // Eight values of a row as loaded, and as numbers.
 template <bool F32>
