@@ -165,7 +165,10 @@ def token_logprobs(logits: Tensor, target: Tensor, k: int) -> Tuple[Tensor, Tens
     """(lp, entropy, lse [...], top_ids int32, top_lp [..., k]) of logits
     [..., V] (fp32 or bf16) and targets [...]: lp = log_softmax(logits)[target],
     0 where the target is outside the classes (padding).  lp and entropy carry
-    gradients; k <= min(32, V), 0: no alternatives."""
+    gradients; k <= min(32, V), 0: no alternatives.  Forward and backward may be
+    captured into a CUDA graph while no eager autograd graph of the same leaves
+    lives (its accumulation belongs to the stream of the eager pass, which a
+    capture may not touch)."""
     x, t = _stat_rows(logits, target)
     n, lead = x.shape[0], logits.shape[:-1]
     lp, ent, lse = (torch.empty(n, device=x.device) for _ in range(3))
