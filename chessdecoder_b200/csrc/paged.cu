@@ -518,7 +518,8 @@ template <int NT>
 __device__ __forceinline__ void follow(Acc<NT>& acc, const float (&mx)[NT][2]) {
   bool pass = false;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) pass |= mx[n][0] > acc.m[n][0] + kSlack || mx[n][1] > acc.m[n][1] + kSlack;
+  for (int n = 0; n < NT; ++n)  // (by the difference: m + kSlack rounds up where a step of m is 16)
+    pass |= mx[n][0] - acc.m[n][0] > kSlack || mx[n][1] - acc.m[n][1] > kSlack;
   if (!__any_sync(0xffffffffu, pass)) return;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
