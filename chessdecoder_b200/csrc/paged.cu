@@ -367,16 +367,19 @@ __global__ void __launch_bounds__(256)
 // that they add no error beside the output's rounding.  e4m3 pages: codes are
 // exact in fp16; q is scaled to fp16 by a power of two per head.  The products
 // with the values take w_j 2^e_j, e_j the value row's scale, so that m has to
-// follow s_j + e_j: weights then fit fp16 (2^-11) whatever the scales are.  The
-// sum of the w_j alone reaches 2^(8 - e_j); e_j below -96 counts as -96 for m (a
-// row of zeros has the smallest scale), which only values below 448 * 2^-96 feel.
+// follow s_j + e_j: weights then fit fp16 whatever the scales are, and are split
+// like the others into two fp16 (2^-22 of w, and 2^-32 of the largest).  The sum
+// of the w_j alone reaches 2^(15 - e_j); e_j below -88 counts as -88 for m (a row
+// of zeros has the smallest scale), which only values below 448 * 2^-88 feel.
+// Scores beyond 2^24 do not resolve s_j + e_j: such a weight may overflow.
 //
 // Measured on one B200 (16 heads, device time, join and all): bf16, 256 sequences of up to
 // 4095 keys 319 us (2.15 GB: the copy rate; 334 by the deal), 64 of up to 2000 49 us
-// (84%), 64 x 512 25 us (82%); e4m3, 256 x 2000 163 us (101%; 177 by the deal), 6 of up to
-// 65536 with groups of 8 heads 27 us (62%: of the 10 us over the floor about 5 pass
-// before the first rows arrive -- launch, lengths, table, rows -- and 2 in the join).
-// Pages of 16 rows: 256 sequences of up to 4000 keys 336 us bf16 (97%), 174 e4m3 (95%).
+// (84%), 64 x 512 25 us (82%); e4m3, 256 x 2000 166 us (99%; 163 with weights in one
+// fp16), 6 of up to 65536 with groups of 8 heads 27 us (62%: of the 10 us over the floor
+// about 5 pass before the first rows arrive -- launch, lengths, table, rows -- and 2 in
+// the join).  Pages of 16 rows: 256 sequences of up to 4000 keys 336 us bf16 (97%), 181
+// e4m3 (91%; 174).
 // ---------------------------------------------------------------------------
 constexpr int kTK = 32;             // keys per tile
 constexpr int kAttnThreads = 128;   // 4 warps; 128 registers: 4 blocks per SM
@@ -386,6 +389,10 @@ constexpr int kAttnWarps = kAttnBlocks * kWarps;
 constexpr int kSlots = 2 * kAttnWarps;
 constexpr float kNoScore = -3.0e38f;  // m before the first key
 constexpr float kSlack = 8.f;
+// e4m3 pages: how far below the largest s_j + e_j m is put, so that weights reach 2^15 at
+// most, 2^7 at least, and their two fp16 parts leave 2^-32 of the largest.
+constexpr float kLift = 7.f;
+constexpr float kLowScale = -88.f;  // smallest e_j that m follows
 // What beginning an item costs a warp, in tiles of the deal: its table, queries and
 // first rows come one after the other.  (64 sequences of 0 .. 2000 keys: 72 us
 // without, 59 with 1, 50 with 2, 51 with 3 -- a warp that is dealt fourteen items of
@@ -512,14 +519,14 @@ __device__ __forceinline__ uint32_t mask_of_tile(const AttnArgs& a, int tile, in
   return mask;
 }
 
-// The reference follows the scores of a tile where one passes it; mx: this lane's
-// largest per column.
+// The reference follows the scores of a tile where one passes it, and stays `lift` below
+// them; mx: this lane's largest per column.
 template <int NT>
-__device__ __forceinline__ void follow(Acc<NT>& acc, const float (&mx)[NT][2]) {
+__device__ __forceinline__ void follow(Acc<NT>& acc, const float (&mx)[NT][2], float lift) {
   bool pass = false;
 #pragma unroll
   for (int n = 0; n < NT; ++n)  // (by the difference: m + kSlack rounds up where a step of m is 16)
-    pass |= mx[n][0] - acc.m[n][0] > kSlack || mx[n][1] - acc.m[n][1] > kSlack;
+    pass |= mx[n][0] - acc.m[n][0] > kSlack + lift || mx[n][1] - acc.m[n][1] > kSlack + lift;
   if (!__any_sync(0xffffffffu, pass)) return;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
@@ -529,7 +536,7 @@ __device__ __forceinline__ void follow(Acc<NT>& acc, const float (&mx)[NT][2]) {
       x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
       x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
       x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-      x = fmaxf(x, acc.m[n][c]);
+      x = fmaxf(x - lift, acc.m[n][c]);
       const float al = ex2(acc.m[n][c] - x);
       acc.m[n][c] = x;
       acc.l[n][c] *= al;
@@ -684,7 +691,7 @@ __device__ __forceinline__ void attend_bf16(const AttnArgs& a, int b, int kvh, i
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int c = 0; c < 2; ++c) mx[n][c] = fmaxf(fmaxf(s[n][0][c], s[n][1][c]), fmaxf(s[n][2][c], s[n][3][c]));
-    follow<NT>(acc, mx);
+    follow<NT>(acc, mx, 0.f);
 
     // weights of keys (16 jj + g, + 8) for heads 2 t4, 2 t4 + 1, as the B operand: high and low parts
     uint32_t ph[NT][2][2], pl[NT][2][2];
@@ -898,17 +905,17 @@ __device__ __forceinline__ void attend_e4m3(const AttnArgs& a, int b, int kvh, i
     for (int n = 0; n < NT; ++n) mx[n][0] = mx[n][1] = -INFINITY;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const float e = fmaxf((float)((int)(__float_as_uint(vs[r]) >> 23) - 127), -96.f);
+      const float e = fmaxf((float)((int)(__float_as_uint(vs[r]) >> 23) - 127), kLowScale);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         mx[n][0] = fmaxf(mx[n][0], s[n][r][0] + e);
         mx[n][1] = fmaxf(mx[n][1], s[n][r][1] + e);
       }
     }
-    follow<NT>(acc, mx);
+    follow<NT>(acc, mx, kLift);
 
-    // weights with the value scales, as the B operand
-    uint32_t pb[NT][2][2];
+    // weights with the value scales, as the B operand: high and low parts
+    uint32_t ph[NT][2][2], pl[NT][2][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -916,7 +923,11 @@ __device__ __forceinline__ void attend_e4m3(const AttnArgs& a, int b, int kvh, i
         const float p0 = ex2(s[n][r][0] - acc.m[n][0]), p1 = ex2(s[n][r][1] - acc.m[n][1]);
         acc.l[n][0] += p0;
         acc.l[n][1] += p1;
-        pb[n][r >> 1][r & 1] = transpose8x8(pack_f16(p0 * vs[r], p1 * vs[r]));
+        const float w0 = p0 * vs[r], w1 = p1 * vs[r];
+        const uint32_t hi = pack_f16(w0, w1);
+        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+        ph[n][r >> 1][r & 1] = transpose8x8(hi);
+        pl[n][r >> 1][r & 1] = transpose8x8(pack_f16(w0 - back.x, w1 - back.y));
       }
 
     // O^T += V^T P^T; bytes of two keys interleaved first: one permute gives two dims of both
@@ -935,7 +946,10 @@ __device__ __forceinline__ void attend_e4m3(const AttnArgs& a, int b, int kvh, i
         e4m3x4_h(lo, af[0], af[1]);
         e4m3x4_h(hi, af[2], af[3]);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma_f16_16816(acc.o[n][i], af, pb[n][jj][0], pb[n][jj][1]);
+        for (int n = 0; n < NT; ++n) {
+          mma_f16_16816(acc.o[n][i], af, ph[n][jj][0], ph[n][jj][1]);
+          mma_f16_16816(acc.o[n][i], af, pl[n][jj][0], pl[n][jj][1]);
+        }
       }
     }
     mask = mask1, mask1 = mask2;

@@ -62,3 +62,54 @@ def test_scores_one_step_apart(more, fp8):
     w = 2.0 ** (16 * more)
     want = (n - 1 - 2 * w) / (n - 1 + w)
     assert ((got - want).abs() <= (2.0 ** -8 + n * 2.0 ** -24) * abs(want)).all(), got[0, 0]
+
+
+# Scores with one product each: exact but for the scale's rounding, its product and the
+# difference to the reference, 2 * 3 * 2^-24 |s| + 2^-24 |s - m| with |s| <= 8 and |s - m| <= 24
+# in base 2, so 2^-18 of a weight at most; the exponential 2^-22; sums of 64 terms 2^-18; a
+# weight in two bf16 2^-17 (in two fp16 2^-22).
+WEIGHTS = {fp8: 2.0 ** -18 + 2.0 ** -22 + 2.0 ** -18 + 2.0 ** (-22 if fp8 else -17) for fp8 in (False, True)}
+
+
+def held_to_the_weights(got, s, v, fp8):
+    """got [H, 64] against softmax(s [H, n]) @ v with values of magnitude 1: the output's
+    own rounding and WEIGHTS.  One rounding of the weights to the products' type is
+    outside that somewhere."""
+    w = torch.exp(s - s.amax(-1, keepdim=True))
+    want = (w @ v.double()) / w.sum(-1, keepdim=True)
+    tol = 2.0 ** -8 * want.abs() + WEIGHTS[fp8]
+    once = w.float().to(torch.float16 if fp8 else torch.bfloat16).double()
+    assert (((once @ v.double()) / w.sum(-1, keepdim=True) - want).abs() > 1.5 * tol).any()
+    assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("H", [1, 7, 12])
+@pytest.mark.parametrize("p", [8, 16, 64])
+def test_weights_that_nearly_cancel(p, H, fp8):
+    """Values of +-1 whose weighted sum is next to nothing: what the weights lose shows."""
+    g = torch.Generator().manual_seed(100 * H + p)
+    n = 64
+    q, k = torch.zeros(H, D), torch.zeros(n, D)
+    q[:, 0] = torch.rand(1, generator=g).add(0.5).to(torch.bfloat16).float()
+    k[:, 0] = torch.randint(-16, 17, (n,), generator=g) / 8.0
+    s = q[:, :1].double() * k[:, 0].double() * 1.1
+    w = torch.softmax(s, -1).mean(0)
+    v, left = torch.zeros(n, D), torch.zeros(D, dtype=torch.float64)
+    for i, j in enumerate(w.argsort(descending=True).tolist()):  # at random, then against what is left
+        side = torch.randint(0, 2, (D,), generator=g) * 2.0 - 1 if i < 12 else torch.where(left > 0, -1.0, 1.0)
+        v[j], left = side, left + side.double() * w[j]
+    held_to_the_weights(attend(q, k, v, fp8, p=p, scale=1.1), s, v, fp8)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_many_equal_weights_beside_a_large_one(fp8):
+    """Two tiles of one key with weight 1 and 31 with r 2^-5 each, r next to the middle
+    between two numbers of the products' type, so that all round the same way."""
+    r = 1 + 0.98 * (2.0 ** -11 if fp8 else 2.0 ** -8)
+    scale = (5 - math.log2(r)) * math.log(2)
+    q, k, v = torch.zeros(1, D), torch.zeros(64, D), -torch.ones(64, D)
+    q[0, 0] = 1.0
+    k[:, 0] = -1.0
+    k[::32, 0], v[::32] = 0.0, 1.0
+    held_to_the_weights(attend(q, k, v, fp8, scale=scale), k[:, 0].double()[None] * scale, v, fp8)
