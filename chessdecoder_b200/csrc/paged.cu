@@ -37,11 +37,11 @@ __device__ __forceinline__ float2 e4m3x2_f(uint32_t w) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
-// Value of a scale byte: 2^(e - 127).  Bytes 1..254 are exponent fields; byte 0
-// (never written here) is the subnormal 2^-127 and 255 a NaN, as in e8m0.
-__device__ __forceinline__ float scale_of(uint32_t e) {
-  return e == 0 ? __uint_as_float(0x00400000u) : e == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float(e << 23);
-}
+// Value of a scale byte: 2^(e - 127), as the upper 16 bits of an fp32.  Bytes 1..254 are
+// exponent fields; byte 0 (never written here) is the subnormal 2^-127 and 255 a NaN, as
+// in e8m0.
+__device__ __forceinline__ uint32_t scale16_of(uint32_t e) { return e == 0 ? 0x0040u : e == 255 ? 0x7fc0u : e << 7; }
+__device__ __forceinline__ float scale_of(uint32_t e) { return __uint_as_float(scale16_of(e) << 16); }
 
 // The pages of one call, as the kernels see them.
 struct Pages {
@@ -820,7 +820,7 @@ __device__ __forceinline__ void attend_e4m3(const AttnArgs& a, int b, int kvh, i
   }
   int page = page_of_key(a, trow, ta + 2, tb, len, lane);
   int stage = 0;
-  uint32_t sc = sk | (sv << 8);  // scale bytes of this tile, key | value << 8
+  uint32_t sc = scale16_of(sk) | (scale16_of(sv) << 16);  // scales of this tile, key and value
 
   // queries as the B operand: head 8 n + g, 16 dims from 16 t4, scaled to fp16
   uint32_t qf[NT][8];
@@ -884,8 +884,8 @@ __device__ __forceinline__ void attend_e4m3(const AttnArgs& a, int b, int kvh, i
       for (int h = 0; h < 2; ++h) {
         const int r = 2 * i + h;
         const uint32_t x = __shfl_sync(0xffffffffu, sc, g + 8 * r);
-        const float ks = __uint_as_float((x & 0xffu) << 23);
-        vs[r] = __uint_as_float((x & 0xff00u) << 15);
+        const float ks = __uint_as_float(x << 16);
+        vs[r] = __uint_as_float(x & 0xffff0000u);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -953,7 +953,7 @@ __device__ __forceinline__ void attend_e4m3(const AttnArgs& a, int b, int kvh, i
       }
     }
     mask = mask1, mask1 = mask2;
-    sc = sk1 | (sv1 << 8);  // loaded a tile ago
+    sc = scale16_of(sk1) | (scale16_of(sv1) << 16);  // loaded a tile ago
     sk1 = sk2, sv1 = sv2;
     stage = stage == kStages - 1 ? 0 : stage + 1;
   }

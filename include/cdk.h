@@ -415,9 +415,9 @@ int cdk_mish_bf16(const float* z, int64_t ldz, int64_t rows, int64_t cols, void*
  *             [num_pages][kv_heads][page_size][64], ld_page elements from page
  *             to page (a multiple of 8 for bf16, 16 for e4m3; 16-byte aligned
  *             base)
- *   k_scale, v_scale   dtype 1: one byte e, 1 .. 254, per row, [num_pages][kv_heads]
+ *   k_scale, v_scale   dtype 1: one byte e per row (e8m0), [num_pages][kv_heads]
  *             [page_size], ld_scale bytes from page to page; the row stands for
- *             code * 2^(e - 127).  dtype 0: unused.
+ *             code * 2^(e - 127), for e = 255 for NaNs.  dtype 0: unused.
  *   table     int32 [B][width], row pitch ldt: row j of sequence b is row
  *             j % page_size of page table[b][j / page_size].
  * A table entry outside [0, num_pages) that a call has to follow, or a row at or
@@ -469,7 +469,8 @@ int cdk_paged_gather(const CdkPagedCache* cache, int64_t B, const int32_t* lens,
  * h / (H / kv_heads) (H a multiple of kv_heads, at most 16 query heads each).
  * q, out bf16 [B, H * 64] with pitches ldq, ldo (multiples of 8, 16-byte aligned
  * bases).  lens[b] == 0 gives zeros.  e4m3 pages: scores (in base 2) below 2^24
- * in magnitude, or a weight may overflow.  B <= 16384.  workspace:
+ * in magnitude, or a weight may overflow; values below 448 * 2^-88 lose bits to
+ * the weights' range.  B <= 16384.  workspace:
  * cdk_paged_attn_workspace bytes for tables that hold max_keys = width * page_size
  * keys (0 bytes where short tables need none), 16-byte aligned, not shared by
  * calls that can overlap; nothing in it needs clearing or is kept between calls. */

@@ -113,3 +113,38 @@ def test_many_equal_weights_beside_a_large_one(fp8):
     k[:, 0] = -1.0
     k[::32, 0], v[::32] = 0.0, 1.0
     held_to_the_weights(attend(q, k, v, fp8, scale=scale), k[:, 0].double()[None] * scale, v, fp8)
+
+
+@pytest.mark.parametrize("p", [8, 16, 64])
+def test_the_smallest_scale(p):
+    """Keys at scale byte 0 (2^-127) under queries of 2^122: ordinary scores, products
+    of four numbers each (as WEIGHTS has them, to 2^-17 with three more); values at byte 0
+    beside others."""
+    n = 64
+    q, k, v = torch.zeros(2, D), torch.zeros(n, D), torch.ones(n, D)
+    q[:, 0] = torch.tensor([2.0 ** 122, -1.5 * 2.0 ** 122])
+    k[:, 0] = torch.arange(n) % 9.0 * 8 - 32
+    v[1::2] = -1.75
+    byte = torch.full((n,), 127)
+    byte[::5] = 0
+    got = attend(q, k, v, True, p=p, kbyte=0, vbyte=byte)
+    w = torch.softmax(q[:, :1].double() * 2.0 ** -127 * k[:, 0].double(), -1)
+    seen = v.double() * torch.pow(2.0, byte.double() - 127)[:, None]
+    assert ((got - w @ seen).abs() <= 2.0 ** -8 * (w @ seen).abs() + 2.0 ** -16 * (w @ seen.abs())).all()
+
+
+@pytest.mark.parametrize("which", ["key", "value"])
+def test_a_scale_that_is_not_a_number(which):
+    """Scale byte 255: the row is NaNs, as in the read-back, and so is what attends to it."""
+    n = 70
+    byte = torch.full((n,), 127)
+    byte[66] = 255
+    kw = dict(kbyte=byte) if which == "key" else dict(vbyte=byte)
+    assert attend(torch.ones(3, D), torch.ones(n, D), torch.ones(n, D), True, **kw).isnan().all()
+    out = torch.zeros(1, 1, 32, D, dtype=torch.bfloat16, device=DEV)
+    pool = torch.ones(1, 1, 32, D, device=DEV).to(torch.float8_e4m3fn)
+    s = torch.full((1, 1, 32), 127, dtype=torch.uint8, device=DEV)
+    s[0, 0, 3], s[0, 0, 4] = 255, 0
+    K.paged_gather(pool, pool, torch.zeros(1, 1, dtype=torch.int32, device=DEV),
+                   torch.tensor([32], dtype=torch.int32, device=DEV), out, out.clone(), k_scale=s, v_scale=s)
+    assert out[0, 0, 3].isnan().all() and (out[0, 0, 4] == 2.0 ** -127).all() and (out[0, 0, 5:] == 1).all()
