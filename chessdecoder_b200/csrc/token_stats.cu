@@ -55,10 +55,10 @@ __device__ __forceinline__ float ex2(float x) {
 // Order of the alternatives as one integer: larger value first, then smaller
 // index.  The float's bits are mapped to an unsigned integer that orders like the
 // value (-0 as +0, NaN above +inf); the index enters inverted.  0 is below every
-// rank.
+// rank, ~0 above.
 __device__ __forceinline__ uint64_t rank_key(float x, uint32_t j) {
   uint32_t u = __float_as_uint(x + 0.f);
-  if (x != x) u = 0x7fffffffu;
+  if (x != x) u = 0x7fc00000u;
   u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
   return ((uint64_t)u << 32) | (uint32_t)~j;
 }
