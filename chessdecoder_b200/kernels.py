@@ -895,10 +895,8 @@ def _stats_plan(logits, target32, lp, entropy, lse, top_ids, top_lp, ncls):
         k = top_ids[1][1] if len(top_ids[1]) == 2 else -1
         if not 0 <= k <= min(MAX_TOP, ncls) or top_ids[:2] != (torch.int32, (rows, k)) \
                 or top_lp[:2] != (torch.float32, (rows, k)) \
-                or any(s[2] != (k, 1) for s in (top_ids, top_lp) if rows > 1 and k > 1):
+                or any((k > 1 and s[2][1] != 1) or (rows > 1 and k > 0 and s[2][0] != k) for s in (top_ids, top_lp)):
             _refuse(op, f"top_ids / top_lp must be contiguous int32 / fp32 [{rows}, k], k <= min({MAX_TOP}, classes)")
-        if k == 1 and rows > 1 and (top_ids[2][0] != 1 or top_lp[2][0] != 1):
-            _refuse(op, "top_ids / top_lp must be contiguous")
     return _on(op, logits, target32, lp, entropy, lse, top_ids, top_lp), rows, ncls, ldl, dt, k
 
 

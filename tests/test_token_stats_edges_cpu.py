@@ -1,0 +1,38 @@
+"""Arguments of the token statistics that are refused or converted, without a GPU."""
+import pytest
+import torch
+
+from chessdecoder_b200 import kernels as K
+
+
+def _top(rows, k, dtype, kind):
+    if kind == "spread":  # a step between the columns
+        return torch.zeros(rows, 2 * k, dtype=dtype)[:, ::2]
+    if kind == "tail":  # the last of them at the end of the storage
+        return torch.zeros(rows, 3 * k, dtype=dtype)[:, 2::3]
+    return torch.zeros(k, rows + 1, dtype=dtype).t()[:rows]
+
+
+@pytest.mark.parametrize("rows,k,kind", [(r, k, kind) for r, k in ((1, 2), (1, 5), (3, 2), (3, 1))
+                                         for kind in ("spread", "tail", "turned") if k > 1 or kind != "turned"])
+@pytest.mark.parametrize("which", ["top_ids", "top_lp"])
+def test_alternatives_that_are_not_contiguous_are_refused(which, kind, rows, k):
+    """One row too: the kernel writes k neighbours, which a view with a step does not own."""
+    dtypes = dict(top_ids=torch.int32, top_lp=torch.float32)
+    kw = {n: torch.zeros(rows, k, dtype=d) for n, d in dtypes.items()}
+    kw[which] = _top(rows, k, dtypes[which], kind)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        K.token_logprobs(torch.zeros(rows, 10), torch.zeros(rows, dtype=torch.int32), torch.zeros(rows), **kw)
+
+
+@pytest.mark.parametrize("rows,k", [(1, 1), (1, 4), (3, 1), (3, 4), (3, 0)])
+def test_contiguous_alternatives_are_taken(rows, k):
+    """Views of one row or column whose strides do not matter pass the check (and stop at the device's)."""
+    ids, top = torch.zeros(rows, 9, dtype=torch.int32), torch.zeros(rows, 9)
+    pairs = [(torch.zeros(rows, k, dtype=torch.int32), torch.zeros(rows, k))]
+    if rows == 1:
+        pairs.append((ids[:, 2:2 + k], top[:, 2:2 + k]))
+    for i, t in pairs:
+        with pytest.raises(RuntimeError, match="need CUDA tensors"):
+            K.token_logprobs(torch.zeros(rows, 10), torch.zeros(rows, dtype=torch.int32), torch.zeros(rows), top_ids=i,
+                             top_lp=t)
