@@ -145,19 +145,25 @@ soft_bucket_ce.register_autograd(_sb_bwd, setup_context=_sb_setup)
 # ---------------------------------------------------------------------------
 
 
+_TARGETS = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8, torch.bool)
+
+
 def _stat_rows(logits: Tensor, target: Tensor):
-    """(rows [n, V] with unit inner stride, int32 targets [n]); a target outside
-    the classes, of whatever magnitude, becomes -100."""
+    """(rows [n, V] with unit inner stride, int32 targets [n]); an int64 target
+    outside the classes, of whatever magnitude, becomes -100 (the other types
+    fit int32, and the kernel tells)."""
     V = logits.shape[-1]
     if logits.dtype not in (torch.float32, torch.bfloat16):
         raise ValueError("cdk::token_logprobs needs fp32 or bf16 logits")
-    if target.shape != logits.shape[:-1] or target.is_floating_point():
+    if target.shape != logits.shape[:-1] or target.dtype not in _TARGETS:
         raise ValueError(f"cdk::token_logprobs needs integer targets {tuple(logits.shape[:-1])}")
     x = logits.detach().reshape(-1, V)
     if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < V):
         x = x.contiguous()
     t = target.reshape(-1)
-    return x, torch.where((t >= 0) & (t < V), t, -100).to(torch.int32)
+    if t.dtype == torch.int64:
+        t = torch.where((t >= 0) & (t < V), t, -100)
+    return x, t.to(torch.int32).contiguous()
 
 
 @torch.library.custom_op("cdk::token_logprobs", mutates_args=())

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from chessdecoder_b200 import kernels as K
+from chessdecoder_b200.ops import _stat_rows
 
 
 def _top(rows, k, dtype, kind):
@@ -36,3 +37,26 @@ def test_contiguous_alternatives_are_taken(rows, k):
         with pytest.raises(RuntimeError, match="need CUDA tensors"):
             K.token_logprobs(torch.zeros(rows, 10), torch.zeros(rows, dtype=torch.int32), torch.zeros(rows), top_ids=i,
                              top_lp=t)
+
+
+@pytest.mark.parametrize("V", [100, 200, 1924, 70000])
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8, torch.bool])
+def test_targets_of_every_integer_type_keep_their_meaning(dtype, V):
+    """Targets inside the classes stay, those outside stay outside, whatever the type holds."""
+    low, high = (0, 1) if dtype == torch.bool else (torch.iinfo(dtype).min, torch.iinfo(dtype).max)
+    given = [v for v in (0, 1, 99, 100, 127, 156, 200, 250, 255, 1923, 32767, 69999, 2 ** 31 - 1, 2 ** 32 + 5, 2 ** 40,
+                         -1, -100, -128, -2 ** 31, -2 ** 40) if low <= v <= high]
+    t = torch.tensor(given, dtype=dtype)
+    got = _stat_rows(torch.zeros(len(given), V), t)[1]
+    assert got.dtype == torch.int32
+    for v, g in zip(given, got.tolist()):
+        assert g == v if 0 <= v < V else not 0 <= g < V, (v, g)
+    wide = torch.stack([t, t], 1)  # every second one of a wider tensor
+    assert torch.equal(_stat_rows(torch.zeros(len(given), V), wide[:, 0])[1], got)
+    assert _stat_rows(torch.zeros(len(given), V), wide[:, 0])[1].is_contiguous()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.complex64, torch.uint16, torch.uint64])
+def test_targets_of_other_types_are_refused(dtype):
+    with pytest.raises(ValueError, match="integer targets"):
+        _stat_rows(torch.zeros(3, 10), torch.zeros(3, dtype=dtype))
