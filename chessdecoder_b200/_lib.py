@@ -117,6 +117,9 @@ SIGNATURES = {
     "cdk_paged_attn": (_int, [_vp, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _f32, _vp, _i64, _vp]),
     "cdk_token_logprobs": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
     "cdk_token_logprobs_bwd": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "cdk_token_logprobs_split": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "cdk_token_logprobs_bwd_split": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64,
+                                            _vp]),
 }
 
 _lib = None

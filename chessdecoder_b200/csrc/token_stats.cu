@@ -6,6 +6,8 @@
 // With m = max x, s = sum e^(x - m), t = sum e^(x - m) (x - m):
 //   L = m + log s,  lp = x_target - L,  entropy = log s - t / s
 //   dx_j = g (1[j = target] - p_j) - h p_j (log p_j + entropy)
+// L alone is off by half a step of it, which would be a relative error of every p_j of
+// the row, so the gradient takes what its rounding lost as well.
 // (m, s, t) of two parts of a row join as  a_i = e^(m_i - m):  s = sum a_i s_i,
 // t = sum a_i (t_i + s_i (m_i - m)).
 //
@@ -386,6 +388,7 @@ struct Args {
   float* lp;
   float* entropy;
   float* lse;
+  float* lse_low;
   int32_t* top_ids;
   float* top_lp;
   int k;
@@ -402,7 +405,12 @@ __device__ __forceinline__ void finish(const Args& a, const Row<BF16>& row, long
     const int tg = a.target[r];
     a.lp[r] = (tg < 0 || tg >= a.ncls) ? 0.f : none ? -INFINITY : (row.at(tg) - st.m) - ls;
     if (a.entropy) a.entropy[r] = none ? 0.f : ls - st.t / st.s;
-    if (a.lse) a.lse[r] = none ? -INFINITY : st.m + ls;
+    const float L = none ? -INFINITY : st.m + ls;
+    if (a.lse) a.lse[r] = L;
+    if (a.lse_low) {  // the rest of the sum, exactly: the parts of m and log s that L holds taken from them
+      const float of_m = L - ls, of_ls = L - of_m;
+      a.lse_low[r] = none ? 0.f : (st.m - of_m) + (ls - of_ls);
+    }
   }
   if (lane < a.k) {
     a.top_ids[r * a.k + lane] = (int32_t)~(uint32_t)top;
@@ -664,8 +672,8 @@ constexpr int kSlab = 32 * kUnroll * 4;
 template <bool BF16>
 __global__ void __launch_bounds__(256)
     token_stats_bwd_kernel(const void* logits, long long ldl, int ncls, const int32_t* __restrict__ target,
-                           const float* __restrict__ lse, const float* __restrict__ entropy,
-                           const float* __restrict__ dlp, const float* __restrict__ dentropy, void* dlogits,
+                           const float* __restrict__ lse, const float* __restrict__ lse_low,
+                           const float* __restrict__ entropy, const float* __restrict__ dlp, const float* __restrict__ dentropy, void* dlogits,
                            long long ldd, unsigned units, unsigned slabs) {
   constexpr int N = Row<BF16>::N, kElt = Row<BF16>::kElt;
   const int lane = threadIdx.x & 31;
@@ -676,14 +684,14 @@ __global__ void __launch_bounds__(256)
   const int tg = target[r];
   const float g = dlp && tg >= 0 && tg < ncls ? dlp[r] : 0.f;
   const float h = dentropy ? dentropy[r] : 0.f;
-  const float L = lse[r], H = dentropy ? entropy[r] : 0.f;
+  const float L = lse[r], low = lse_low ? lse_low[r] : 0.f, H = dentropy ? entropy[r] : 0.f;
   const bool zero = L == -INFINITY || (g == 0.f && h == 0.f && L == L);  // nothing to read
   char* out = reinterpret_cast<char*>(dlogits) + (long long)r * ldd * kElt;
-  // -p (g + h (log p + H)) = p (nc + nh log p)
-  const float nh = -h, nc = -fmaf(h, H, g);
+  // with z = x - L, log p = z - low:  -p (g + h (log p + H)) = p (nc + nh z)
+  const float nh = -h, nc = -fmaf(h, H - low, g), l2 = -low * kLog2e;
   auto grad = [&](float x, int e) {
     if (zero) return 0.f;
-    const float z = x - L, d = ex2(z * kLog2e) * fmaf(nh, fmaxf(z, kFar), nc);
+    const float z = x - L, d = ex2(fmaf(z, kLog2e, l2)) * fmaf(nh, fmaxf(z, kFar), nc);
     return e == tg ? d + g : d;  // (a target outside the classes has g = 0)
   };
   auto put = [&](int e, float d) {
@@ -718,7 +726,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           const float z = d[i] - L;
-          d[i] = ex2(z * kLog2e) * fmaf(nh, fmaxf(z, kFar), nc);
+          d[i] = ex2(fmaf(z, kLog2e, l2)) * fmaf(nh, fmaxf(z, kFar), nc);
         }
         if ((unsigned)(tg - e0) < (unsigned)N) {
 #pragma unroll
@@ -785,9 +793,9 @@ cudaError_t launch_fwd(const Args& a, cudaStream_t st) {
 
 }  // namespace
 
-extern "C" int cdk_token_logprobs(const void* logits, int dtype, int64_t ldl, int64_t rows, int64_t ncls,
-                                  const int32_t* target, float* lp, float* entropy, float* lse, int32_t* top_ids,
-                                  float* top_lp, int64_t k, void* stream) {
+extern "C" int cdk_token_logprobs_split(const void* logits, int dtype, int64_t ldl, int64_t rows, int64_t ncls,
+                                        const int32_t* target, float* lp, float* entropy, float* lse, float* lse_low,
+                                        int32_t* top_ids, float* top_lp, int64_t k, void* stream) {
   if (rows == 0) return 0;
   if (!logits || !target || !lp || rows < 0 || rows > 0x7fffffff) return -1;
   if (dtype != 0 && dtype != 1) return -2;
@@ -796,15 +804,23 @@ extern "C" int cdk_token_logprobs(const void* logits, int dtype, int64_t ldl, in
   if (!top_ids != !top_lp) return -5;
   if (!top_ids) k = 0;
   if (k < 0 || k > kMaxTop || k > ncls) return -6;
-  const Args a{logits, ldl, rows, (int)ncls, target, lp, entropy, lse, top_ids, top_lp, (int)k};
+  const Args a{logits, ldl, rows, (int)ncls, target, lp, entropy, lse, lse_low, top_ids, top_lp, (int)k};
   auto* st = reinterpret_cast<cudaStream_t>(stream);
   if (k) return (int)(dtype ? launch_fwd<true, true>(a, st) : launch_fwd<false, true>(a, st));
   return (int)(dtype ? launch_fwd<true, false>(a, st) : launch_fwd<false, false>(a, st));
 }
 
-extern "C" int cdk_token_logprobs_bwd(const void* logits, int dtype, int64_t ldl, int64_t rows, int64_t ncls,
-                                      const int32_t* target, const float* lse, const float* entropy, const float* dlp,
-                                      const float* dentropy, void* dlogits, int64_t ldd, void* stream) {
+extern "C" int cdk_token_logprobs(const void* logits, int dtype, int64_t ldl, int64_t rows, int64_t ncls,
+                                  const int32_t* target, float* lp, float* entropy, float* lse, int32_t* top_ids,
+                                  float* top_lp, int64_t k, void* stream) {
+  return cdk_token_logprobs_split(logits, dtype, ldl, rows, ncls, target, lp, entropy, lse, nullptr, top_ids, top_lp, k,
+                                  stream);
+}
+
+extern "C" int cdk_token_logprobs_bwd_split(const void* logits, int dtype, int64_t ldl, int64_t rows, int64_t ncls,
+                                            const int32_t* target, const float* lse, const float* lse_low,
+                                            const float* entropy, const float* dlp, const float* dentropy,
+                                            void* dlogits, int64_t ldd, void* stream) {
   if (rows == 0) return 0;
   if (!logits || !target || !lse || !dlogits || rows < 0 || rows > 0x7fffffff) return -1;
   if (dtype != 0 && dtype != 1) return -2;
@@ -818,10 +834,17 @@ extern "C" int cdk_token_logprobs_bwd(const void* logits, int dtype, int64_t ldl
   const unsigned units = (unsigned)(rows * slabs), blocks = (units + 7) / 8;
   auto* st = reinterpret_cast<cudaStream_t>(stream);
   if (dtype)
-    token_stats_bwd_kernel<true><<<blocks, 256, 0, st>>>(logits, ldl, (int)ncls, target, lse, entropy, dlp, dentropy,
-                                                         dlogits, ldd, units, (unsigned)slabs);
+    token_stats_bwd_kernel<true><<<blocks, 256, 0, st>>>(logits, ldl, (int)ncls, target, lse, lse_low, entropy, dlp,
+                                                         dentropy, dlogits, ldd, units, (unsigned)slabs);
   else
-    token_stats_bwd_kernel<false><<<blocks, 256, 0, st>>>(logits, ldl, (int)ncls, target, lse, entropy, dlp, dentropy,
-                                                          dlogits, ldd, units, (unsigned)slabs);
+    token_stats_bwd_kernel<false><<<blocks, 256, 0, st>>>(logits, ldl, (int)ncls, target, lse, lse_low, entropy, dlp,
+                                                          dentropy, dlogits, ldd, units, (unsigned)slabs);
   return (int)cudaGetLastError();
+}
+
+extern "C" int cdk_token_logprobs_bwd(const void* logits, int dtype, int64_t ldl, int64_t rows, int64_t ncls,
+                                      const int32_t* target, const float* lse, const float* entropy, const float* dlp,
+                                      const float* dentropy, void* dlogits, int64_t ldd, void* stream) {
+  return cdk_token_logprobs_bwd_split(logits, dtype, ldl, rows, ncls, target, lse, nullptr, entropy, dlp, dentropy,
+                                      dlogits, ldd, stream);
 }

@@ -883,10 +883,10 @@ def _logits_plan(op, logits, target32, ncls):
 
 
 @functools.lru_cache(maxsize=1024)
-def _stats_plan(logits, target32, lp, entropy, lse, top_ids, top_lp, ncls):
+def _stats_plan(logits, target32, lp, entropy, lse, lse_low, top_ids, top_lp, ncls):
     op = "token_logprobs"
     rows, ncls, ldl, dt = _logits_plan(op, logits, target32, ncls)
-    for name, lay in (("lp", lp), ("entropy", entropy), ("lse", lse)):
+    for name, lay in (("lp", lp), ("entropy", entropy), ("lse", lse), ("lse_low", lse_low)):
         _vec(op, name, lay, torch.float32, rows)
     if (top_ids is None) != (top_lp is None):
         _refuse(op, "top_ids and top_lp go together")
@@ -897,47 +897,51 @@ def _stats_plan(logits, target32, lp, entropy, lse, top_ids, top_lp, ncls):
                 or top_lp[:2] != (torch.float32, (rows, k)) \
                 or any((k > 1 and s[2][1] != 1) or (rows > 1 and k > 0 and s[2][0] != k) for s in (top_ids, top_lp)):
             _refuse(op, f"top_ids / top_lp must be contiguous int32 / fp32 [{rows}, k], k <= min({MAX_TOP}, classes)")
-    return _on(op, logits, target32, lp, entropy, lse, top_ids, top_lp), rows, ncls, ldl, dt, k
+    return _on(op, logits, target32, lp, entropy, lse, lse_low, top_ids, top_lp), rows, ncls, ldl, dt, k
 
 
 @_timed("token_logprobs")
-def token_logprobs(logits, target32, lp, *, entropy=None, lse=None, top_ids=None, top_lp=None, ncls=None):
+def token_logprobs(logits, target32, lp, *, entropy=None, lse=None, lse_low=None, top_ids=None, top_lp=None, ncls=None):
     """Per row: lp = log_softmax(logits)[target] (0 for a target outside
-    [0, ncls)), and where given the entropy, the log-sum-exp and the k best
-    classes (top_ids int32 [rows, k], top_lp fp32 [rows, k], k <= 32; equal
-    logits in order of their index).  fp32 outputs."""
+    [0, ncls)), and where given the entropy, the log-sum-exp (lse_low: what its
+    rounding to fp32 lost, for the gradient) and the k best classes (top_ids
+    int32 [rows, k], top_lp fp32 [rows, k], k <= 32; equal logits in order of
+    their index).  fp32 outputs."""
     dev, rows, ncls, ldl, dt, k = _stats_plan(_lay(logits), _lay(target32), _lay(lp), _lay(entropy), _lay(lse),
-                                              _lay(top_ids), _lay(top_lp), ncls)
+                                              _lay(lse_low), _lay(top_ids), _lay(top_lp), ncls)
     if rows == 0:
         return
-    _call("token_logprobs", lib().cdk_token_logprobs, dev, logits.data_ptr(), dt, ldl, rows, ncls,
-          target32.data_ptr(), lp.data_ptr(), _ptr(entropy), _ptr(lse), _ptr(top_ids) if k else None,
+    _call("token_logprobs", lib().cdk_token_logprobs_split, dev, logits.data_ptr(), dt, ldl, rows, ncls,
+          target32.data_ptr(), lp.data_ptr(), _ptr(entropy), _ptr(lse), _ptr(lse_low), _ptr(top_ids) if k else None,
           _ptr(top_lp) if k else None, k)
     _count(1)
 
 
 @functools.lru_cache(maxsize=1024)
-def _stats_bwd_plan(logits, target32, lse, entropy, dlp, dentropy, dlogits, ncls):
+def _stats_bwd_plan(logits, target32, lse, lse_low, entropy, dlp, dentropy, dlogits, ncls):
     op = "token_logprobs_bwd"
     rows, ncls, ldl, dt = _logits_plan(op, logits, target32, ncls)
     if dentropy is not None and entropy is None:
         _refuse(op, "dentropy needs the forward's entropy")
-    for name, lay in (("lse", lse), ("entropy", entropy), ("dlp", dlp), ("dentropy", dentropy)):
+    for name, lay in (("lse", lse), ("lse_low", lse_low), ("entropy", entropy), ("dlp", dlp), ("dentropy", dentropy)):
         _vec(op, name, lay, torch.float32, rows)
     ldd = _rows2d(op, "dlogits", dlogits, (logits[0],), rows, ncls)
-    return _on(op, logits, target32, lse, entropy, dlp, dentropy, dlogits), rows, ncls, ldl, dt, ldd
+    return _on(op, logits, target32, lse, lse_low, entropy, dlp, dentropy, dlogits), rows, ncls, ldl, dt, ldd
 
 
 @_timed("token_logprobs_bwd")
-def token_logprobs_bwd(logits, target32, lse, entropy, dlp, dentropy, dlogits, *, ncls=None):
+def token_logprobs_bwd(logits, target32, lse, entropy, dlp, dentropy, dlogits, *, lse_low=None, ncls=None):
     """dlogits = dlp * (onehot(target) - p) - dentropy * p * (log p + entropy)
     from the forward's lse and entropy; dlp / dentropy fp32 [rows], either may be
-    None (zero; entropy is then not needed for dentropy None).  dlogits has the
-    logits' type and may be the same tensor."""
-    dev, rows, ncls, ldl, dt, ldd = _stats_bwd_plan(_lay(logits), _lay(target32), _lay(lse), _lay(entropy), _lay(dlp),
-                                                    _lay(dentropy), _lay(dlogits), ncls)
+    None (zero; entropy is then not needed for dentropy None).  Without the
+    forward's lse_low every p of a row is off by what lse's rounding lost, up to
+    2^-24 |lse| of itself.  dlogits has the logits' type and may be the same
+    tensor."""
+    dev, rows, ncls, ldl, dt, ldd = _stats_bwd_plan(_lay(logits), _lay(target32), _lay(lse), _lay(lse_low),
+                                                    _lay(entropy), _lay(dlp), _lay(dentropy), _lay(dlogits), ncls)
     if rows == 0:
         return
-    _call("token_logprobs_bwd", lib().cdk_token_logprobs_bwd, dev, logits.data_ptr(), dt, ldl, rows, ncls,
-          target32.data_ptr(), lse.data_ptr(), _ptr(entropy), _ptr(dlp), _ptr(dentropy), dlogits.data_ptr(), ldd)
+    _call("token_logprobs_bwd", lib().cdk_token_logprobs_bwd_split, dev, logits.data_ptr(), dt, ldl, rows, ncls,
+          target32.data_ptr(), lse.data_ptr(), _ptr(lse_low), _ptr(entropy), _ptr(dlp), _ptr(dentropy),
+          dlogits.data_ptr(), ldd)
     _count(1)

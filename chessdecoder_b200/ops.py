@@ -150,7 +150,7 @@ _TARGETS = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8, torc
 
 def _stat_rows(logits: Tensor, target: Tensor):
     """(rows [n, V] with unit inner stride, int32 targets [n]); an int64 target
-    outside the classes, of whatever magnitude, becomes -100 (the other types
+    outside the classes, of whatever magnitude, becomes -1 or V (the other types
     fit int32, and the kernel tells)."""
     V = logits.shape[-1]
     if logits.dtype not in (torch.float32, torch.bfloat16):
@@ -162,11 +162,64 @@ def _stat_rows(logits: Tensor, target: Tensor):
         x = x.contiguous()
     t = target.reshape(-1)
     if t.dtype == torch.int64:
-        t = torch.where((t >= 0) & (t < V), t, -100)
+        t = t.clamp(-1, V)
     return x, t.to(torch.int32).contiguous()
 
 
-@torch.library.custom_op("cdk::token_logprobs", mutates_args=())
+@torch.library.custom_op("cdk::token_logprobs_forward", mutates_args=())
+def token_logprobs_forward(logits: Tensor, target: Tensor,
+                           k: int) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """The outputs of cdk::token_logprobs, and before the alternatives what the
+    rounding of lse to fp32 lost (the gradient needs both)."""
+    x, t = _stat_rows(logits, target)
+    n, lead = x.shape[0], logits.shape[:-1]
+    lp, ent, lse, low = (torch.empty(n, device=x.device) for _ in range(4))
+    ids = torch.empty(n, k, dtype=torch.int32, device=x.device)
+    top = torch.empty(n, k, device=x.device)
+    K.token_logprobs(x, t, lp, entropy=ent, lse=lse, lse_low=low, top_ids=ids, top_lp=top)
+    return lp.view(lead), ent.view(lead), lse.view(lead), low.view(lead), ids.view(*lead, k), top.view(*lead, k)
+
+
+@token_logprobs_forward.register_fake
+def _(logits, target, k):
+    lead = logits.shape[:-1]
+    f = logits.new_empty(lead, dtype=torch.float32)
+    return (f, torch.empty_like(f), torch.empty_like(f), torch.empty_like(f),
+            logits.new_empty(*lead, k, dtype=torch.int32), logits.new_empty(*lead, k, dtype=torch.float32))
+
+
+@torch.library.custom_op("cdk::token_logprobs_backward", mutates_args=())
+def token_logprobs_backward(logits: Tensor, target: Tensor, lse: Tensor, entropy: Tensor, dlp: Optional[Tensor],
+                            dentropy: Optional[Tensor], lse_low: Optional[Tensor] = None) -> Tensor:
+    """d(logits), in their shape and type, from the gradients of lp and entropy."""
+    x, t = _stat_rows(logits, target)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    g, h = (None if d is None else d.to(torch.float32).reshape(-1).contiguous() for d in (dlp, dentropy))
+    K.token_logprobs_bwd(x, t, lse.reshape(-1), entropy.reshape(-1), g, h, dx,
+                         lse_low=None if lse_low is None else lse_low.reshape(-1))
+    return dx.view(logits.shape)
+
+
+@token_logprobs_backward.register_fake
+def _(logits, target, lse, entropy, dlp, dentropy, lse_low=None):
+    return logits.new_empty(logits.shape)
+
+
+def _stats_setup(ctx, inputs, output):
+    logits, target, _ = inputs
+    _, ent, lse, low, ids, top = output
+    ctx.save_for_backward(logits, target, lse, ent, low)
+    ctx.mark_non_differentiable(lse, low, ids, top)
+
+
+def _stats_bwd(ctx, dlp, dentropy, *_):
+    logits, target, lse, ent, low = ctx.saved_tensors
+    return torch.ops.cdk.token_logprobs_backward(logits, target, lse, ent, dlp, dentropy, low), None, None
+
+
+token_logprobs_forward.register_autograd(_stats_bwd, setup_context=_stats_setup)
+
+
 def token_logprobs(logits: Tensor, target: Tensor, k: int) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
     """(lp, entropy, lse [...], top_ids int32, top_lp [..., k]) of logits
     [..., V] (fp32 or bf16) and targets [...]: lp = log_softmax(logits)[target],
@@ -175,52 +228,13 @@ def token_logprobs(logits: Tensor, target: Tensor, k: int) -> Tuple[Tensor, Tens
     captured into a CUDA graph while no eager autograd graph of the same leaves
     lives (its accumulation belongs to the stream of the eager pass, which a
     capture may not touch)."""
-    x, t = _stat_rows(logits, target)
-    n, lead = x.shape[0], logits.shape[:-1]
-    lp, ent, lse = (torch.empty(n, device=x.device) for _ in range(3))
-    ids = torch.empty(n, k, dtype=torch.int32, device=x.device)
-    top = torch.empty(n, k, device=x.device)
-    K.token_logprobs(x, t, lp, entropy=ent, lse=lse, top_ids=ids, top_lp=top)
-    return lp.view(lead), ent.view(lead), lse.view(lead), ids.view(*lead, k), top.view(*lead, k)
+    lp, ent, lse, _, ids, top = torch.ops.cdk.token_logprobs_forward(logits, target, k)
+    return lp, ent, lse, ids, top
 
 
-@token_logprobs.register_fake
-def _(logits, target, k):
-    lead = logits.shape[:-1]
-    f = logits.new_empty(lead, dtype=torch.float32)
-    return (f, torch.empty_like(f), torch.empty_like(f), logits.new_empty(*lead, k, dtype=torch.int32),
-            logits.new_empty(*lead, k, dtype=torch.float32))
-
-
-@torch.library.custom_op("cdk::token_logprobs_backward", mutates_args=())
-def token_logprobs_backward(logits: Tensor, target: Tensor, lse: Tensor, entropy: Tensor, dlp: Optional[Tensor],
-                            dentropy: Optional[Tensor]) -> Tensor:
-    """d(logits), in their shape and type, from the gradients of lp and entropy."""
-    x, t = _stat_rows(logits, target)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    g, h = (None if d is None else d.to(torch.float32).reshape(-1).contiguous() for d in (dlp, dentropy))
-    K.token_logprobs_bwd(x, t, lse.reshape(-1), entropy.reshape(-1), g, h, dx)
-    return dx.view(logits.shape)
-
-
-@token_logprobs_backward.register_fake
-def _(logits, target, lse, entropy, dlp, dentropy):
-    return logits.new_empty(logits.shape)
-
-
-def _stats_setup(ctx, inputs, output):
-    logits, target, _ = inputs
-    _, ent, lse, ids, top = output
-    ctx.save_for_backward(logits, target, lse, ent)
-    ctx.mark_non_differentiable(lse, ids, top)
-
-
-def _stats_bwd(ctx, dlp, dentropy, *_):
-    logits, target, lse, ent = ctx.saved_tensors
-    return torch.ops.cdk.token_logprobs_backward(logits, target, lse, ent, dlp, dentropy), None, None
-
-
-token_logprobs.register_autograd(_stats_bwd, setup_context=_stats_setup)
+_LIB = torch.library.Library("cdk", "FRAGMENT")
+_LIB.define("token_logprobs(Tensor logits, Tensor target, SymInt k) -> (Tensor, Tensor, Tensor, Tensor, Tensor)")
+_LIB.impl("token_logprobs", token_logprobs, "CompositeImplicitAutograd")
 
 # ---------------------------------------------------------------------------
 # Backbone

@@ -491,6 +491,11 @@ int cdk_paged_attn(const void* q, int64_t ldq, const CdkPagedCache* cache, int64
  * or +inf has lse, lp, entropy and top_lp NaN (NaN ranks above every number).
  * ncls < 2^31 - 32.
  *
+ * The log-sum-exp as one fp32 is off by up to half a step of it, and with it every
+ * p_j of a gradient: by 3e-5 of itself where logits are near 1000.  The _split forms
+ * write and take what the rounding lost beside it (lse + lse_low is the sum of the
+ * row's maximum and the logarithm exactly; lse_low may be NULL: not wanted, and 0).
+ *
  * Backward: dlogits_j = g (1[j = target] - p_j) - h p_j (log p_j + entropy) with
  * g = dlp[r] (taken as 0 for a target outside [0, ncls)), h = dentropy[r];
  * either may be NULL (= 0).  Rows whose lse is -inf get zeros.  dlogits has the
@@ -501,6 +506,12 @@ int cdk_token_logprobs(const void* logits, int dtype, int64_t ldl, int64_t rows,
 int cdk_token_logprobs_bwd(const void* logits, int dtype, int64_t ldl, int64_t rows, int64_t ncls,
                            const int32_t* target, const float* lse, const float* entropy, const float* dlp,
                            const float* dentropy, void* dlogits, int64_t ldd, void* stream);
+int cdk_token_logprobs_split(const void* logits, int dtype, int64_t ldl, int64_t rows, int64_t ncls,
+                             const int32_t* target, float* lp, float* entropy, float* lse, float* lse_low,
+                             int32_t* top_ids, float* top_lp, int64_t k, void* stream);
+int cdk_token_logprobs_bwd_split(const void* logits, int dtype, int64_t ldl, int64_t rows, int64_t ncls,
+                                 const int32_t* target, const float* lse, const float* lse_low, const float* entropy,
+                                 const float* dlp, const float* dentropy, void* dlogits, int64_t ldd, void* stream);
 
 #ifdef __cplusplus
 }

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from chessdecoder_b200 import _lib
 from chessdecoder_b200 import kernels as K
 from chessdecoder_b200.ops import _stat_rows
 
@@ -60,3 +61,32 @@ def test_targets_of_every_integer_type_keep_their_meaning(dtype, V):
 def test_targets_of_other_types_are_refused(dtype):
     with pytest.raises(ValueError, match="integer targets"):
         _stat_rows(torch.zeros(3, 10), torch.zeros(3, dtype=dtype))
+
+
+def test_the_second_part_of_the_sum_is_checked_like_the_first():
+    x, t, f = torch.zeros(3, 10), torch.zeros(3, dtype=torch.int32), torch.zeros(3)
+    for bad in (torch.zeros(2), torch.zeros(3, dtype=torch.float64), torch.zeros(6)[::2]):
+        with pytest.raises(RuntimeError, match="lse_low"):
+            K.token_logprobs(x, t, f, lse_low=bad)
+        with pytest.raises(RuntimeError, match="lse_low"):
+            K.token_logprobs_bwd(x, t, f, f, f, f, x, lse_low=bad)
+    lib = _lib.load()  # the addresses are never followed: the host refuses before it launches
+    f = lambda x=64, V=10, R=3: lib.cdk_token_logprobs_split(  # noqa: E731
+        x, 0, 10, R, V, 64, 64, None, None, 64, None, None, 0, None)
+    b = lambda dx=128, lse=64, R=3: lib.cdk_token_logprobs_bwd_split(  # noqa: E731
+        64, 0, 10, R, 10, 64, lse, 64, 64, 64, 64, dx, 10, None)
+    assert f(x=None) == -1 and f(V=11) == -3 and f(R=0) == 0
+    assert b(dx=None) == -1 and b(lse=None) == -1 and b(dx=130) == -4 and b(R=0) == 0
+
+
+def test_op_has_five_outputs_and_is_the_forward_with_both_parts():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        x = torch.empty(3, 50, device="cuda", requires_grad=True)
+        out = torch.ops.cdk.token_logprobs(x, torch.empty(3, dtype=torch.long, device="cuda"), 2)
+        both = torch.ops.cdk.token_logprobs_forward(x, torch.empty(3, dtype=torch.long, device="cuda"), 2)
+        assert len(out) == 5 and len(both) == 6
+        assert [o.requires_grad for o in both] == [True, True, False, False, False, False]
+        dx = torch.ops.cdk.token_logprobs_backward(x, torch.empty(3, dtype=torch.long, device="cuda"), both[2], both[1],
+                                                   both[0], None, both[3])
+        assert dx.shape == x.shape

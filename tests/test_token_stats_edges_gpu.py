@@ -7,6 +7,8 @@ import torch
 
 from chessdecoder_b200 import kernels as K
 
+from test_token_stats_gpu import U, reference
+
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
 
@@ -47,3 +49,57 @@ def test_nan_comes_first_wherever_it_is(V, bf16):
         K.token_logprobs(x, t, lp, entropy=ent, lse=lse, top_ids=ids, top_lp=top)
         assert torch.equal(ids.cpu().long(), best(x, k)), (ids.cpu(), best(x, k))
         assert top.isnan().all() and lp.isnan().all() and ent.isnan().all() and lse.isnan().all()
+
+
+def grid(R, V, seed):
+    """fp32 logits on a grid of 2^-6, so that a shift by a whole number is exact."""
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn(R, V, generator=g) * 3 * 64).round() / 64
+    t = torch.randint(0, V, (R,), generator=g)
+    t[1] = -100
+    dlp, dent = torch.randn(2, R, generator=g)
+    return x, t.to(torch.int32).to(DEV), dlp.to(DEV), dent.to(DEV)
+
+
+@pytest.mark.parametrize("shift", [0, 100, -1000, 10000, 100000])
+@pytest.mark.parametrize("V", [41, 1924, 20001])
+def test_gradient_of_rows_far_from_zero(V, shift):
+    """A constant added to a row changes no probability: the gradient keeps the bound of
+    the row whose maximum is 0 (tests/test_token_stats_gpu.py; log s and x - m are what it
+    is computed from), through the op and through the kernels, and sums to as little."""
+    import chessdecoder_b200.ops  # noqa: F401
+    x, t, dlp, dent = grid(8, V, V)
+    want = reference(x - x.amax(1, keepdim=True), t, dlp, dent)
+    x = (x + shift).to(DEV)
+    lp, ent, lse, low = (torch.empty(8, device=DEV) for _ in range(4))
+    K.token_logprobs(x, t, lp, entropy=ent, lse=lse, lse_low=low)
+    dx = torch.empty_like(x)
+    K.token_logprobs_bwd(x, t, lse, ent, dlp, dent, dx, lse_low=low)
+    tol = want["dx_tol"] + U * (want["dx"].abs() + want["dx_tol"]) + 2.0 ** -126
+    off = (dx.cpu().double() - want["dx"]).abs()
+    assert (off <= tol).all(), (off / tol).max()
+    assert (dx.cpu().double().sum(1).abs() <= tol.sum(1)).all()
+    exact = x.cpu().double().logsumexp(1)
+    assert ((lse.cpu().double() + low.cpu().double() - exact).abs() <= want["lse_tol"]).all()
+    assert torch.equal(lse, (lse.double() + low.double()).float())
+    y = x.clone().requires_grad_(True)
+    a, b, c, _, _ = torch.ops.cdk.token_logprobs(y, t.long(), 0)
+    assert torch.equal(a, lp) and torch.equal(b, ent) and torch.equal(c, lse)
+    torch.autograd.backward([a, b], [dlp, dent])
+    assert torch.equal(y.grad, dx)
+
+
+def test_lse_low_of_rows_without_a_sum():
+    """Nothing above -inf: 0 beside -inf, and a gradient of zeros; NaN and +inf: NaN."""
+    x = torch.full((3, 50), -math.inf, device=DEV)
+    x[1, 7], x[2, 7] = math.nan, math.inf
+    t = torch.zeros(3, dtype=torch.int32, device=DEV)
+    lp, ent, lse, low = (torch.full((3,), 5.0, device=DEV) for _ in range(4))
+    K.token_logprobs(x, t, lp, entropy=ent, lse=lse, lse_low=low)
+    assert lse[0] == -math.inf and low[0] == 0 and lse[1:].isnan().all() and low[1:].isnan().all()
+    dx = torch.full_like(x, 5.0)
+    K.token_logprobs_bwd(x, t, lse, ent, torch.ones(3, device=DEV), torch.ones(3, device=DEV), dx, lse_low=low)
+    assert (dx[0] == 0).all() and dx[1:].isnan().all()
+    one = torch.empty(3, device=DEV)
+    K.token_logprobs(x, t, lp, lse_low=one)  # alone
+    assert torch.equal(one.nan_to_num(9), low.nan_to_num(9))
