@@ -135,6 +135,9 @@ class _Backbone:
         cfg, st = self.cfg, self.store
         T, E, nf = ids.numel(), cfg.embed_dim, cfg.num_fourier_freq
         dev = self.device
+        if ov.numel() < T or om_u8.numel() != T:  # the kernels go by the tokens and the mask alone
+            raise ValueError(f"{T} tokens need as many override values and mask entries, "
+                             f"got {ov.numel()} and {om_u8.numel()}")
         rows = self._arange32(T)
         ones = torch.ones(T, dtype=torch.uint8, device=dev)
         fvals = torch.empty(T, device=dev)
@@ -288,6 +291,8 @@ class BatchedBackbone(_Backbone):
         T = B * S
         ids = ids.to(device=dev, dtype=torch.int64).reshape(-1).contiguous()
         pos32 = pos.to(device=dev, dtype=torch.int32).reshape(-1).contiguous()
+        if pos32.numel() < T:
+            raise ValueError(f"{T} tokens need as many positions, got {pos32.numel()}")
         ov = (torch.zeros(T, device=dev) if ov is None else
               ov.to(device=dev, dtype=torch.float32).reshape(-1).contiguous())
         om_u8 = (torch.zeros(T, dtype=torch.uint8, device=dev) if om is None else _u8(om, dev).reshape(-1))

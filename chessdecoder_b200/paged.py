@@ -122,6 +122,12 @@ class PagedKVCache:
             self.lens[torch.tensor(seqs, device=self.device)] = 0
 
 
+def _check_overrides(ids, ov, om):
+    for name, t in (("ov", ov), ("om", om)):
+        if t is not None and t.numel() != ids.numel():
+            raise ValueError(f"{name} must have a value for each of the {ids.numel()} tokens, has {t.numel()}")
+
+
 def _flags(active, B):
     if active is None:
         return [1] * B
@@ -174,6 +180,7 @@ class PagedBackbone(_Backbone):
             num_real.tolist() if torch.is_tensor(num_real) else num_real)]
         if len(real) != B or any(n < 0 or n > S for n in real):
             raise ValueError(f"num_real must be {B} counts of 0 .. {S}")
+        _check_overrides(ids, ov, om)
         for b, n in enumerate(real):
             if n and c._len[b]:
                 raise ValueError(f"prefill needs an empty sequence; {b} holds {c._len[b]} tokens")
@@ -246,6 +253,7 @@ class PagedBackbone(_Backbone):
         result is then a static buffer, valid until the next step."""
         if tuple(ids.shape) != (self.B, 1):
             raise ValueError(f"a step takes ids [{self.B}, 1]")
+        _check_overrides(ids, ov, om)
         flags = _flags(active, self.B)
         self._begin(flags, 1)
         if self._step is None or not self.use_graphs:
