@@ -109,6 +109,13 @@ class PagedKVCache:
         for b, n in enumerate(new):
             self._len[b] += n
 
+    def settle(self, lengths: Sequence[int]):
+        """Both lengths as they were before a call that raised on its way: it may
+        have moved the device's, and the rows that it wrote behind them count no
+        more."""
+        self._len = list(lengths)
+        self.lens.copy_(torch.tensor(self._len, dtype=torch.int32))
+
     def release(self, seqs):
         """Empties sequences: their pages are free, their length is 0."""
         seqs = [int(b) for b in seqs]
@@ -141,7 +148,8 @@ class PagedBackbone(_Backbone):
     """The dense ChessDecoder's KV-cache backbone over a PagedKVCache (causal
     attention).  ``batch_size`` sequences of up to ``max_seq_len`` tokens share
     ``num_pages`` pages (default: enough for all of them at full length);
-    ``kv_dtype``: torch.bfloat16 or torch.float8_e4m3fn."""
+    ``kv_dtype``: torch.bfloat16 or torch.float8_e4m3fn.  A prefill, step or
+    generate that raises leaves every sequence with the tokens that it had."""
 
     def __init__(self, cfg=None, batch_size: int = 1, max_seq_len: Optional[int] = None, num_pages: Optional[int] = None,
                  page_size: int = 64, kv_dtype=torch.bfloat16, **kw):
@@ -187,7 +195,18 @@ class PagedBackbone(_Backbone):
         if S == 0:
             return torch.empty(B, 0, self.cfg.embed_dim, device=self.device)
         c.reserve(real)
-        dev, E, H = self.device, self.cfg.embed_dim, self.cfg.num_heads
+        before = c.lengths
+        try:
+            h = self._prompts(ids, real, ov, om)
+            c.advance(real)
+        except BaseException:
+            c.settle(before)
+            raise
+        return h
+
+    def _prompts(self, ids, real, ov, om):
+        B, S = ids.shape
+        c, dev, E, H = self.cache, self.device, self.cfg.embed_dim, self.cfg.num_heads
         T = B * S
         count = torch.tensor(real, dtype=torch.int32, device=dev)
         c.start.copy_(c.lens)
@@ -208,9 +227,7 @@ class PagedBackbone(_Backbone):
             K.paged_gather(lens=seen, k_out=k_rows, v_out=v_rows, **pool)
             K.attn_fwd(qkv16, ao, lse, B, B, S, H)
 
-        h = self._layers_forward(x, B, S, attend)
-        c.advance(real)
-        return h
+        return self._layers_forward(x, B, S, attend)
 
     def _embed_rows(self, ids, ov, om):
         dev, T = self.device, ids.numel()
@@ -256,15 +273,20 @@ class PagedBackbone(_Backbone):
         _check_overrides(ids, ov, om)
         flags = _flags(active, self.B)
         self._begin(flags, 1)
-        if self._step is None or not self.use_graphs:
-            h = self._step_body(ids, ov, om)  # eager: every lazy set-up happens outside capture
-            if self.use_graphs:
-                self._step = "warm"
-        else:
-            if self._step == "warm":
-                self._step = _Captured(self)
-            h = self._step.replay(self, ids, ov, om)
-        self.cache.advance(flags)
+        before = self.cache.lengths
+        try:
+            if self._step is None or not self.use_graphs:
+                h = self._step_body(ids, ov, om)  # eager: every lazy set-up happens outside capture
+                if self.use_graphs:
+                    self._step = "warm"
+            else:
+                if self._step == "warm":
+                    self._step = _Captured(self)
+                h = self._step.replay(self, ids, ov, om)
+            self.cache.advance(flags)
+        except BaseException:
+            self.cache.settle(before)
+            raise
         return h
 
     # -- generation ------------------------------------------------------------
@@ -290,18 +312,23 @@ class PagedBackbone(_Backbone):
         out = st.outputs(n_steps)
         if n_steps == 0:
             return out
-        self._begin(flags, n_steps)
         st.ids.copy_(ids.reshape(B, 1))
+        self._begin(flags, n_steps)
         st.seed.fill_(int(seed) & 0x7FFFFFFFFFFFFFFF)
         st.counter.zero_()
-        for i in range(n_steps):
-            if i == 0 or not self.use_graphs:
-                st.body(self)  # eager: every lazy set-up happens outside capture
-            else:
-                st.replay(self)
-            for name, rows in out.items():
-                rows[i].copy_(getattr(st, name).view_as(rows[i]))
-            self.cache.advance(flags)
+        before = self.cache.lengths
+        try:
+            for i in range(n_steps):
+                if i == 0 or not self.use_graphs:
+                    st.body(self)  # eager: every lazy set-up happens outside capture
+                else:
+                    st.replay(self)
+                for name, rows in out.items():
+                    rows[i].copy_(getattr(st, name).view_as(rows[i]))
+                self.cache.advance(flags)
+        except BaseException:
+            self.cache.settle(before)
+            raise
         return out
 
 
@@ -387,14 +414,14 @@ class _GenLoop:
 
     def replay(self, bb: PagedBackbone):
         if self.graph is None:
-            self.graph = torch.cuda.CUDAGraph()
+            graph = torch.cuda.CUDAGraph()
             torch.cuda.synchronize(bb.device)
             n0 = K.LAUNCHES[0]
-            with torch.cuda.graph(self.graph):
+            with torch.cuda.graph(graph):
                 self.body(bb)
             self.n_launch = K.LAUNCHES[0] - n0
             K.LAUNCHES[0] = n0
-            self.out16 = bb.last_hidden16
+            self.graph, self.out16 = graph, bb.last_hidden16
         self.graph.replay()
         K.LAUNCHES[0] += self.n_launch
         bb.last_hidden16 = self.out16

@@ -71,3 +71,102 @@ def test_the_right_sizes_reach_the_kernels():
             BatchedBackbone(ModelConfig(**CFG), B, 32, device="cpu").causal_probe(IDS, torch.arange(S).repeat(B, 1), ov, om)
     with pytest.raises(MemoryError):
         paged().step(IDS[:, :1], torch.zeros(B), torch.zeros(B, 1))
+
+
+def _passes(monkeypatch, bb):
+    """The pass without its kernels, for the bookkeeping around it."""
+    monkeypatch.setattr(bb, "_embed", lambda ids, ov, om: torch.zeros(ids.numel(), bb.cfg.embed_dim))
+    monkeypatch.setattr(bb, "_layers_forward", lambda x, b, s, attend: x.view(b, s, -1))
+
+
+def _books(bb):
+    c = bb.cache
+    return c.lengths, c.lens.tolist(), c.start.tolist(), c.table.tolist(), sorted(c._free), c._held
+
+
+@pytest.mark.parametrize("error", [MemoryError, KeyboardInterrupt])
+@pytest.mark.parametrize("times", [1, 3])
+def test_a_call_that_fails_leaves_the_lengths(monkeypatch, times, error):
+    """The device's lengths are moved before the pass; a pass that raises (memory that
+    runs out is the ordinary way) must not leave them so: what follows is what a
+    backbone without the failure does."""
+    def reached(*a, **kw):
+        raise error
+    monkeypatch.setattr(K, "fourier_features", reached)
+    bb, fresh = paged(), paged()
+    tok = IDS[:, :1]
+
+    def fail(call):
+        before = _books(bb)[:2]
+        for _ in range(times):
+            with pytest.raises(error):
+                call()
+            assert _books(bb)[:2] == before
+    fail(lambda: bb.prefill(IDS, [S, S - 1]))
+    with monkeypatch.context() as m:
+        for b in (bb, fresh):
+            _passes(m, b)
+            b.prefill(IDS, [S, S - 1])
+        assert _books(bb) == _books(fresh) and bb.cache.lens.tolist() == [S, S - 1]
+        # a replaced prompt while the other sequence keeps its tokens
+        for b in (bb, fresh):
+            b.release([1])
+    fail(lambda: bb.prefill(IDS, [0, 3]))
+    fail(lambda: bb.step(tok, active=[True, False]))
+    fail(lambda: bb.generate(tok, 4, active=[True, False]))
+    with monkeypatch.context() as m:
+        for b in (bb, fresh):
+            _passes(m, b)
+            b.prefill(IDS, [0, 3])
+            b.step(tok, active=[True, False])
+            b.step(tok)
+        assert _books(bb)[:5] == _books(fresh)[:5] and bb.cache.lens.tolist() == [S + 2, 4]
+
+
+def test_a_generation_that_fails_on_its_way_counts_for_nothing(monkeypatch):
+    bb = paged()
+    _passes(monkeypatch, bb)
+    bb.prefill(IDS, [S, 2])
+    left = [2]
+
+    def body(self, b):
+        b._step_body(self.ids, None, None)
+        left[0] -= 1
+        if left[0] < 0:
+            raise MemoryError
+    from chessdecoder_b200 import paged as P
+    monkeypatch.setattr(P._GenLoop, "body", body)
+    with pytest.raises(MemoryError):
+        bb.generate(IDS[:, :1], 6)
+    assert bb.lengths == bb.cache.lens.tolist() == [S, 2]
+    with pytest.raises(RuntimeError):
+        bb.generate(IDS, 6)  # not one token per sequence: refused before pages are taken
+    assert bb.cache.free_pages == 2
+
+
+def test_a_call_that_is_cut_short_by_its_capture_can_be_made_again(monkeypatch):
+    """A capture that raises leaves no half-made graph behind to be replayed."""
+    from chessdecoder_b200 import paged as P
+    bb = paged()
+    st = P._GenLoop(bb, "board_head", None, 0.0, 0)
+
+    class Graph:
+        def replay(self):
+            raise AssertionError("replayed before it was captured")
+
+    class Capture:
+        def __init__(self, graph):
+            pass
+
+        def __enter__(self):
+            pass
+
+        def __exit__(self, *a):
+            return False
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", Graph)
+    monkeypatch.setattr(torch.cuda, "graph", Capture)
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda dev=None: None)
+    for _ in range(2):
+        with pytest.raises(MemoryError):
+            st.replay(bb)
+        assert st.graph is None

@@ -1,0 +1,67 @@
+"""PagedBackbone around its calls: what a failed one leaves behind, and that a
+backbone ends with its last reference.  Hidden states are held to the tolerance of
+tests/test_paged_backbone_gpu.py between two backbones of the same weights."""
+import pytest
+import torch
+
+from chessdecoder_b200 import kernels as K
+from chessdecoder_b200.engine import ModelConfig
+from chessdecoder_b200.paged import PagedBackbone
+
+from test_paged_backbone_gpu import near, weights
+
+pytestmark = pytest.mark.gpu
+CFG = dict(num_layers=2)
+
+
+@pytest.fixture(autouse=True)
+def _no_device_error():
+    K.get_error()
+    yield
+    assert K.get_error() == 0
+
+
+@pytest.mark.parametrize("use_graphs", [True, False])
+def test_what_follows_a_failed_call(monkeypatch, use_graphs):
+    """Prompts, steps and a generation that raise half-way, some of their kernels
+    launched: the next calls answer as on a backbone that never failed."""
+    cfg = ModelConfig(**CFG)
+    sd = weights(cfg, 5, head=30.0)
+    bb, ok = (PagedBackbone(cfg, 3, 64, page_size=16, state_dict=sd, use_graphs=use_graphs) for _ in range(2))
+    g = torch.Generator().manual_seed(1)
+    ids = torch.randint(0, cfg.vocab_size, (3, 40), generator=g)
+    tok = torch.randint(0, cfg.vocab_size, (3, 1), generator=g)
+    real = [12, 40, 3]
+
+    def fail(name, after, call):
+        calls, fn = [0], getattr(K, name)
+
+        def cut(*a, **k):
+            calls[0] += 1
+            if calls[0] > after:
+                raise MemoryError
+            return fn(*a, **k)
+        before = bb.lengths
+        with monkeypatch.context() as m:
+            m.setattr(K, name, cut)
+            with pytest.raises(MemoryError):
+                call()
+        assert bb.lengths == bb.cache.lens.tolist() == before
+
+    fail("attn_fwd", 1, lambda: bb.prefill(ids, real))
+    fail("fourier_features", 0, lambda: bb.prefill(ids, real))
+    a, b = bb.prefill(ids, real), ok.prefill(ids, real)
+    for i, n in enumerate(real):
+        near(a[i, :n], b[i, :n].cpu(), ("prompt", i))
+    fail("paged_attn", 1, lambda: bb.step(tok))
+    near(bb.step(tok), ok.step(tok).cpu(), "step")
+    if use_graphs:
+        fail("paged_attn", 1, lambda: bb.step(tok))  # within the capture
+    near(bb.step(tok, active=[1, 0, 1]), ok.step(tok, active=[1, 0, 1]).cpu(), "second step")
+    near(bb.step(tok), ok.step(tok).cpu(), "third step")
+    fail("head_select", 1, lambda: bb.generate(tok, 5))  # the second step, within the capture or not
+    assert bb.lengths == bb.cache.lens.tolist() == ok.lengths == [15, 42, 6]
+    x, y = (c.generate(tok, 4, top_k=3) for c in (bb, ok))
+    # the first choice is of one hidden state; the logits' scale is the head's
+    assert (x["top_log_probs"][0] - y["top_log_probs"][0]).abs().max() < 6e-2 * y["top_log_probs"][0].abs().max() + 0.1
+    assert bb.lengths == bb.cache.lens.tolist() == ok.lengths
