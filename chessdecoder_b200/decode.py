@@ -204,6 +204,10 @@ class _Backbone:
         self.last_hidden16 = h16.view(B, S, E)
         return h32.view(B, S, E)
 
+    def _last_rows(self):
+        """bf16 hidden states [B, E] of the last position of the latest call."""
+        return self.last_hidden16[:, -1, :]
+
     # -- value heads (evalWlHead / evalDHead, batched_engine.cpp:151-180) -------
     def value_head(self, name: str = "wl_head", h16=None, temperature: float = 0.0, seed: int = 0):
         """WL or D value head on hidden states h16 [B, E] bf16 (default: the
@@ -215,7 +219,7 @@ class _Backbone:
             raise ValueError("value heads are wl_head and d_head")
         st, cfg, dev = self.store, self.cfg, self.device
         if h16 is None:
-            h16 = self.last_hidden16[:, -1, :]
+            h16 = self._last_rows()
         B = h16.shape[0]
         hv, nb = cfg.value_hidden_size, cfg.n_buckets
         z = torch.empty(B, hv, device=dev)

@@ -164,6 +164,7 @@ class PagedBackbone(_Backbone):
         self.cache = PagedKVCache(self.cfg.num_layers, num_pages, self.B, self.max_len, H, page_size, dtype, self.device)
         self._ws = None  # attention workspace, one for every step: they run one after the other
         self._step = None
+        self._ends = None  # the last token's row of each sequence, after prompts of different lengths
 
     @property
     def lengths(self):
@@ -172,6 +173,13 @@ class PagedBackbone(_Backbone):
     def release(self, seqs):
         """Empties sequences, so that prefill can begin others in their place."""
         self.cache.release(seqs)
+
+    def _last_rows(self):
+        """... and after prompts the row of each one's last token, not of the padding
+        behind it.  (A sequence that took no token in the call has none.)"""
+        if self._ends is None:
+            return super()._last_rows()
+        return self.last_hidden16[torch.arange(self.B, device=self.device), self._ends]
 
     # -- prompts -------------------------------------------------------------
     def prefill(self, ids, num_real=None, ov=None, om=None):
@@ -198,6 +206,7 @@ class PagedBackbone(_Backbone):
         before = c.lengths
         try:
             h = self._prompts(ids, real, ov, om)
+            self._ends = None if min(real) == S else torch.tensor([max(n - 1, 0) for n in real], device=self.device)
             c.advance(real)
         except BaseException:
             c.settle(before)
@@ -283,6 +292,7 @@ class PagedBackbone(_Backbone):
                 if self._step == "warm":
                     self._step = _Captured(self)
                 h = self._step.replay(self, ids, ov, om)
+            self._ends = None
             self.cache.advance(flags)
         except BaseException:
             self.cache.settle(before)
@@ -325,6 +335,7 @@ class PagedBackbone(_Backbone):
                     st.replay(self)
                 for name, rows in out.items():
                     rows[i].copy_(getattr(st, name).view_as(rows[i]))
+                self._ends = None
                 self.cache.advance(flags)
         except BaseException:
             self.cache.settle(before)

@@ -170,3 +170,28 @@ def test_a_call_that_is_cut_short_by_its_capture_can_be_made_again(monkeypatch):
         with pytest.raises(MemoryError):
             st.replay(bb)
         assert st.graph is None
+
+
+def test_the_last_rows_are_each_sequences_own(monkeypatch):
+    """value_head's default rows: a prompt's last token, not the padding behind it."""
+    bb = paged()
+
+    def run(x, b, s, attend):
+        bb.last_hidden16 = torch.arange(float(b * s)).view(b, s, 1).to(torch.bfloat16)
+        return bb.last_hidden16.float()
+    monkeypatch.setattr(bb, "_embed", lambda ids, ov, om: None)
+    monkeypatch.setattr(bb, "_layers_forward", run)
+    rows = lambda: bb._last_rows().flatten().tolist()  # noqa: E731
+    bb.prefill(IDS, [2, S])
+    assert rows() == [1, S + S - 1]
+    bb.release([0])
+    bb.prefill(IDS, [4, 0])
+    assert rows()[0] == 3
+    bb.step(IDS[:, :1])
+    assert rows() == [0, 1]
+    bb.release([0, 1])
+    bb.prefill(IDS)
+    assert rows() == [S - 1, 2 * S - 1]
+    bb.release([0, 1])
+    bb.prefill(IDS, torch.tensor([1, 1]))
+    assert rows() == [0, S]

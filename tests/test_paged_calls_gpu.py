@@ -65,3 +65,18 @@ def test_what_follows_a_failed_call(monkeypatch, use_graphs):
     # the first choice is of one hidden state; the logits' scale is the head's
     assert (x["top_log_probs"][0] - y["top_log_probs"][0]).abs().max() < 6e-2 * y["top_log_probs"][0].abs().max() + 0.1
     assert bb.lengths == bb.cache.lens.tolist() == ok.lengths
+
+
+def test_value_heads_after_prompts_of_different_lengths():
+    """By default on the last token of each prompt: what its own hidden state gives."""
+    cfg = ModelConfig(**CFG)
+    bb = PagedBackbone(cfg, 3, 32, page_size=16, state_dict=weights(cfg, 2))
+    ids = torch.randint(0, cfg.vocab_size, (3, 9), generator=torch.Generator().manual_seed(3))
+    real = [9, 2, 5]
+    bb.prefill(ids, real)
+    mine = torch.stack([bb.last_hidden16[b, n - 1] for b, n in enumerate(real)])
+    for head in ("wl_head", "d_head"):
+        for got, want in zip(bb.value_head(head), bb.value_head(head, h16=mine)):
+            assert torch.equal(got, want)
+    bb.step(ids[:, :1])
+    assert torch.equal(bb.value_head("wl_head")[3], bb.value_head("wl_head", h16=bb.last_hidden16[:, 0])[3])
