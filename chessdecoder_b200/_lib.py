@@ -114,6 +114,7 @@ SIGNATURES = {
                                 _vp, _i64, _vp]),
     "cdk_paged_gather": (_int, [_vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp]),
     "cdk_paged_attn_workspace": (_i64, [_i64, _i64, _i64, _i64]),
+    "cdk_paged_attn_launches": (_int, [_vp, _i64, _i64]),
     "cdk_paged_attn": (_int, [_vp, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _f32, _vp, _i64, _vp]),
     "cdk_token_logprobs": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
     "cdk_token_logprobs_bwd": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),

@@ -1391,6 +1391,7 @@ inline int64_t prefix_bytes(int64_t B) { return ((B + 1) * 4 + 15) / 16 * 16; }
 // The tiles of bf16 pages below 32 rows take a warp twice as long, so that the end is
 // more (256 x 1 .. 4000 keys of 16 heads on pages of 16: 361 us, 338 by the deal).
 constexpr int kMany = 8;
+constexpr int kWideLog = 5;  // pages of 32 rows and more hold a tile whole
 inline int warps_per_item(long long items, long long max_tiles, int group, bool fp8, bool wide) {
   if (items > kAttnBlocks && max_tiles <= (items < 2 * kAttnBlocks ? 2 : fp8 ? 8 : 4)) return 1;
   if (items <= (group <= 8 ? 2 : 1) * 148 && max_tiles > 4 && max_tiles <= 32) return kMany;
@@ -1462,6 +1463,15 @@ extern "C" int64_t cdk_paged_attn_workspace(int64_t B, int64_t H, int64_t kv_hea
   return prefix_bytes(B) + (int64_t)kSlots * (H / kv_heads) * (16 + kHD * 4);
 }
 
+extern "C" int cdk_paged_attn_launches(const CdkPagedCache* cache, int64_t B, int64_t H) {
+  if (B == 0) return 0;
+  Pages pg;
+  if (const int rc = take_pages(cache, &pg)) return rc;
+  if (B < 0 || B > kMaxSeqs || H <= 0 || H > 65536 || H % pg.kv_heads || H / pg.kv_heads > kMaxGroup) return -11;
+  const int64_t tiles = ((pg.width << pg.log_page) + kTK - 1) / kTK;
+  return warps_per_item(B * pg.kv_heads, tiles, (int)(H / pg.kv_heads), cache->dtype == 1, pg.log_page >= kWideLog) ? 1 : 2;
+}
+
 extern "C" int cdk_paged_attn(const void* q, int64_t ldq, const CdkPagedCache* cache, int64_t B, int64_t H,
                               const int32_t* lens, void* out, int64_t ldo, float scale, void* workspace,
                               int64_t workspace_bytes, void* stream) {
@@ -1492,7 +1502,7 @@ extern "C" int cdk_paged_attn(const void* q, int64_t ldq, const CdkPagedCache* c
   auto st = reinterpret_cast<cudaStream_t>(stream);
   // pages of 32 rows and more hold a tile whole (a kernel that takes both kinds needs
   // registers that the loads in flight then miss: 64 x 0..2000 keys 52 us for 48)
-  const bool wide = a.pg.log_page >= 5;
+  const bool wide = a.pg.log_page >= kWideLog;
 #define CDK_ATTN(FP8, NT) (int)(wide ? launch_attn<FP8, NT, true>(a, tiles, st) : launch_attn<FP8, NT, false>(a, tiles, st))
   if (cache->dtype == 1) return a.group <= 8 ? CDK_ATTN(true, 1) : CDK_ATTN(true, 2);
   return a.group <= 8 ? CDK_ATTN(false, 1) : CDK_ATTN(false, 2);

@@ -842,7 +842,10 @@ def _attn_plan(k, v, table, ks, vs, q, lens, out, workspace):
     if need and workspace is not None and (workspace[0] != torch.uint8 or len(workspace[1]) != 1 or workspace[2] != (1,)
                                   or workspace[1][0] < need):
         _refuse(op, f"workspace must be contiguous uint8 of at least {need} bytes")
-    return _on(op, k, v, table, ks, vs, q, lens, out, workspace), fields, B, cols // 64, ldq, ldo, need
+    dev = _on(op, k, v, table, ks, vs, q, lens, out, workspace)
+    # (the count goes by the sizes alone: any aligned address stands for the tensors)
+    count = lib().cdk_paged_attn_launches(_lib.PAGED_CACHE.pack(*[256] * 5, *fields), B, cols // 64)
+    return dev, fields, B, cols // 64, ldq, ldo, need, count
 
 
 @_timed("paged_attn")
@@ -852,7 +855,7 @@ def paged_attn(q, k_pages, v_pages, table, lens, out, *, k_scale=None, v_scale=N
     (grouped queries).  A sequence of length 0 gets zeros.  workspace (uint8,
     paged_attn_workspace bytes): allocated here when not given; a given one must
     not be shared by calls that can overlap."""
-    dev, fields, B, H, ldq, ldo, need = _attn_plan(
+    dev, fields, B, H, ldq, ldo, need, count = _attn_plan(
         _lay(k_pages), _lay(v_pages), _lay(table), _lay(k_scale), _lay(v_scale), _lay(q), _lay(lens), _lay(out),
         _lay(workspace))
     if B == 0:
@@ -862,7 +865,7 @@ def paged_attn(q, k_pages, v_pages, table, lens, out, *, k_scale=None, v_scale=N
     _call("paged_attn", lib().cdk_paged_attn, dev, q.data_ptr(), ldq,
           _cache_arg(k_pages, v_pages, k_scale, v_scale, table, fields), B, H, lens.data_ptr(), out.data_ptr(), ldo,
           scale, workspace.data_ptr() if need else None, need)
-    _count(2 if need else 1)  # the item kernel, or (where a workspace is needed, mostly) the deal and the join
+    _count(count)
 
 
 # ---------------------------------------------------------------------------

@@ -475,6 +475,8 @@ int cdk_paged_gather(const CdkPagedCache* cache, int64_t B, const int32_t* lens,
  * keys (0 bytes where short tables need none), 16-byte aligned, not shared by
  * calls that can overlap; nothing in it needs clearing or is kept between calls. */
 int64_t cdk_paged_attn_workspace(int64_t B, int64_t H, int64_t kv_heads, int64_t max_keys);
+/* Kernels that cdk_paged_attn launches for these sizes: 1, or 2 where partial results are joined. */
+int cdk_paged_attn_launches(const CdkPagedCache* cache, int64_t B, int64_t H);
 int cdk_paged_attn(const void* q, int64_t ldq, const CdkPagedCache* cache, int64_t B, int64_t H, const int32_t* lens,
                    void* out, int64_t ldo, float scale, void* workspace, int64_t workspace_bytes, void* stream);
 

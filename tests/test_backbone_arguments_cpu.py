@@ -195,3 +195,27 @@ def test_the_last_rows_are_each_sequences_own(monkeypatch):
     bb.release([0, 1])
     bb.prefill(IDS, torch.tensor([1, 1]))
     assert rows() == [0, S]
+
+
+def test_attention_launches_go_with_the_workspace():
+    """No workspace, one kernel; and what the C entry refuses."""
+    from chessdecoder_b200 import _lib
+    lib = _lib.load()
+
+    def cache(page_size=64, width=10, kv_heads=2, dtype=0, **kw):
+        row = kv_heads * page_size
+        c = dict(k=256, v=256, k_scale=256, v_scale=256, table=256, ldt=width, width=width, num_pages=4,
+                 ld_page=row * 64, ld_scale=row, kv_heads=kv_heads, page_size=page_size, dtype=dtype, reserved=0)
+        return _lib.PAGED_CACHE.pack(*{**c, **kw}.values())
+    seen = set()
+    for b in (1, 5, 64, 300, 700, 1600, 16384):
+        for width in (1, 4, 16, 63, 128, 400):
+            for p in (16, 32, 64):
+                for dtype in (0, 1):
+                    n = lib.cdk_paged_attn_launches(cache(p, width, dtype=dtype), b, 4)
+                    need = lib.cdk_paged_attn_workspace(b, 4, 2, width * p)
+                    assert n == 1 if need == 0 else n in (1, 2)
+                    seen.add((n, need > 0))
+    assert seen == {(1, False), (1, True), (2, True)}
+    assert lib.cdk_paged_attn_launches(cache(), 0, 4) == 0 and lib.cdk_paged_attn_launches(cache(), 3, 5) == -11
+    assert lib.cdk_paged_attn_launches(cache(page_size=12), 3, 4) == -4 and lib.cdk_paged_attn_launches(None, 3, 4) == -1

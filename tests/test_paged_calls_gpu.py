@@ -80,3 +80,24 @@ def test_value_heads_after_prompts_of_different_lengths():
             assert torch.equal(got, want)
     bb.step(ids[:, :1])
     assert torch.equal(bb.value_head("wl_head")[3], bb.value_head("wl_head", h16=bb.last_hidden16[:, 0])[3])
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("p", [16, 32, 64])
+@pytest.mark.parametrize("B,Hkv,keys", [(1, 16, 137), (3, 2, 3000), (64, 16, 2000), (150, 2, 1500), (700, 2, 60),
+                                        (700, 2, 200), (1600, 2, 4000), (2, 1, 0)])
+def test_launches_are_counted_as_they_are(B, Hkv, keys, p, fp8):
+    """One kernel where items are whole, two where partial results are joined: those
+    write the workspace, the others leave it as it was, also where one is given."""
+    width = -(-keys // p)  # the way goes by the table's size: sequences of 200 keys on the same pages
+    n = max(min(width, 4), 1)
+    table = (torch.arange(width, dtype=torch.int32, device="cuda") % n).repeat(B, 1)
+    pool = torch.zeros(n, Hkv, p, 64, dtype=torch.uint8 if fp8 else torch.bfloat16, device="cuda")
+    pool = pool.view(torch.float8_e4m3fn) if fp8 else pool
+    s = torch.full((n, Hkv, p), 127, dtype=torch.uint8, device="cuda") if fp8 else None
+    q = torch.zeros(B, Hkv * 64, dtype=torch.bfloat16, device="cuda")
+    lens = torch.full((B,), min(keys, 200), dtype=torch.int32, device="cuda")
+    ws = torch.full((K.paged_attn_workspace(B, Hkv, Hkv),), 0x5A, dtype=torch.uint8, device="cuda")
+    before = K.LAUNCHES[0]
+    K.paged_attn(q, pool, pool, table, lens, torch.empty_like(q), k_scale=s, v_scale=s, workspace=ws)
+    assert K.LAUNCHES[0] - before == 1 + int((ws != 0x5A).any())
