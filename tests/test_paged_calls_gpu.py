@@ -1,6 +1,9 @@
 """PagedBackbone around its calls: what a failed one leaves behind, and that a
 backbone ends with its last reference.  Hidden states are held to the tolerance of
 tests/test_paged_backbone_gpu.py between two backbones of the same weights."""
+import gc
+import weakref
+
 import pytest
 import torch
 
@@ -101,3 +104,24 @@ def test_launches_are_counted_as_they_are(B, Hkv, keys, p, fp8):
     before = K.LAUNCHES[0]
     K.paged_attn(q, pool, pool, table, lens, torch.empty_like(q), k_scale=s, v_scale=s, workspace=ws)
     assert K.LAUNCHES[0] - before == 1 + int((ws != 0x5A).any())
+
+
+def test_a_backbone_ends_with_its_last_reference():
+    """What it keeps of its graphs does not point back at it: a collection that came
+    later could end a graph while another is being captured."""
+    cfg = ModelConfig(**CFG)
+    bb = PagedBackbone(cfg, 2, 32, page_size=16, state_dict=weights(cfg, 2))
+    tok = torch.zeros(2, 1, dtype=torch.long)
+    bb.prefill(torch.zeros(2, 5, dtype=torch.long), [5, 2])
+    for _ in range(3):
+        bb.step(tok)
+    bb.generate(tok, 4, top_k=2)
+    assert bb._step is not None and all(st.graph is not None for st in bb._gen.values())
+    ends = [weakref.ref(x) for x in (bb, bb.cache, bb._step, *bb._gen.values())]
+    gc.collect()
+    gc.disable()
+    try:
+        del bb
+        assert [r() for r in ends] == [None] * len(ends)
+    finally:
+        gc.enable()
