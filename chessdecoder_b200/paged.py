@@ -120,6 +120,9 @@ class PagedKVCache:
         """Empties sequences: their pages are free, their length is 0."""
         seqs = [int(b) for b in seqs]
         for b in seqs:
+            if not -self.max_seqs <= b < self.max_seqs:
+                raise IndexError(f"no sequence {b} of {self.max_seqs}")
+        for b in seqs:
             held = self._held[b]
             self._free.extend(reversed(self._table[b, :held].tolist()))
             self._table[b] = -1

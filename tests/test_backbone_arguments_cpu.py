@@ -8,7 +8,7 @@ from chessdecoder_b200 import engine
 from chessdecoder_b200 import kernels as K
 from chessdecoder_b200.decode import BatchedBackbone
 from chessdecoder_b200.engine import ModelConfig
-from chessdecoder_b200.paged import PagedBackbone
+from chessdecoder_b200.paged import PagedBackbone, PagedKVCache
 
 CFG = dict(num_layers=1)
 B, S = 2, 5
@@ -219,3 +219,18 @@ def test_attention_launches_go_with_the_workspace():
     assert seen == {(1, False), (1, True), (2, True)}
     assert lib.cdk_paged_attn_launches(cache(), 0, 4) == 0 and lib.cdk_paged_attn_launches(cache(), 3, 5) == -11
     assert lib.cdk_paged_attn_launches(cache(page_size=12), 3, 4) == -4 and lib.cdk_paged_attn_launches(None, 3, 4) == -1
+
+
+@pytest.mark.parametrize("seqs", [[0, 7], [2, -4], [1, 0, 3], [3]])
+def test_releasing_a_sequence_that_is_not_there_releases_none(seqs):
+    """The host's books and the device's table and lengths say the same afterwards."""
+    c = PagedKVCache(1, 8, 3, 16, 1, page_size=4, device="cpu")
+    c.reserve([4, 5, 4])
+    c.advance([4, 5, 4])
+    c.lens.copy_(torch.tensor([4, 5, 4]))
+    before = (c.lengths, c.lens.tolist(), c.table.tolist(), c.free_pages)
+    with pytest.raises(IndexError):
+        c.release(seqs)
+    assert (c.lengths, c.lens.tolist(), c.table.tolist(), c.free_pages) == before
+    c.release([-1, 0, 0])
+    assert c.lengths == c.lens.tolist() == [0, 5, 0] and c.free_pages == 6 and torch.equal(c.table, c._table)
