@@ -80,8 +80,9 @@ __device__ __forceinline__ int page_of(const Pages& p, long long b, long long j)
 // add), so that a quantised code does not depend on how a compiler contracts
 // them.  Bound by HBM: one read of qkv, one write of each row.  Measured on one
 // B200 (16 + 16 + 16 heads): 18,200 fp32 tokens rotated into bf16 pages 54 us, 97%
-// of the copy rate, into e4m3 pages 49 us (94%); bf16 rows into e4m3 pages 23 us
-// (74%: fewer bytes for the same instructions).  A lane per eight values with all
+// of the copy rate, into e4m3 pages 49 us (95%); bf16 rows into e4m3 pages 23 us
+// (74%, 57% of the issue slots: a warp loads its next heads after it has stored the
+// present ones, and meanwhile has nothing in flight).  A lane per eight values with all
 // indices its own took 70 us there; a warp per token whose row loads came after
 // the place was looked up 35, before it 27; keys and values together 24, blocks of 128
 // threads 23.
@@ -376,13 +377,20 @@ __global__ void __launch_bounds__(256)
 // Measured on one B200 (16 heads, device time, join and all): bf16, 256 sequences of up to
 // 4095 keys 319 us (2.15 GB: the copy rate; 334 by the deal), 64 of up to 2000 49 us
 // (84%), 64 x 512 25 us (82%); e4m3, 256 x 2000 166 us (99%; 163 with weights in one
-// fp16), 6 of up to 65536 with groups of 8 heads 27 us (62%: of the 10 us over the floor
+// fp16), 6 of up to 65536 with groups of 8 heads 27 us (61%: of the 11 us over the floor
 // about 5 pass before the first rows arrive -- launch, lengths, table, rows -- and 2 in
-// the join).  Pages of 16 rows: 256 sequences of up to 4000 keys 336 us bf16 (97%), 181
-// e4m3 (91%; 174).
+// the join; the loop leaves half of the issue slots free, four warps to a scheduler
+// waiting for their loads).  Pages of 16 rows: 256 sequences of up to 4000 keys 337 us
+// bf16 (96%), 180 e4m3 (92%; 174).  Groups of 9 to 16 heads, 16 x 9001..20000 keys x 4 kv
+// heads: 69 us bf16 (52%), 51 e4m3 (36%).
 // ---------------------------------------------------------------------------
 constexpr int kTK = 32;             // keys per tile
-constexpr int kAttnThreads = 128;   // 4 warps; 128 registers: 4 blocks per SM
+// 4 warps.  Groups of up to 8 heads: 128 registers, 4 blocks per SM (bf16 kernels spill 20 to
+// 116 bytes, e4m3 none); on e4m3 pages with more than some 1700 sequences the deal's prefix
+// beside the rings leaves shared memory for 3.  Larger groups: up to 168 registers, 3 blocks
+// (bf16 spills up to 72 bytes).  The deal is cut for 4 all the same: where 3 fit, a quarter of
+// its blocks start when others end.
+constexpr int kAttnThreads = 128;
 constexpr int kWarps = kAttnThreads / 32;
 constexpr int kAttnBlocks = 148 * 4;
 constexpr int kAttnWarps = kAttnBlocks * kWarps;

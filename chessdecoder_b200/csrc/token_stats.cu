@@ -23,8 +23,8 @@
 // pass has next to no work for the alternatives.
 //
 // Measured on one B200 (device time, share of the copy rate): 16384 x 1924 fp32
-// forward 24 us (82%), with 5 alternatives 36 us (54%), gradient 41 us (95%); 8192 x 8000
-// fp32 forward 45 us (89%), with 5 alternatives 53 us (76%); 509 x 131071 bf16 forward
+// forward 23 us (84%), with 5 alternatives 36 us (54%), gradient 41 us (95%); 8192 x 8000
+// fp32 forward 46 us (88%), with 5 alternatives 53 us (77%); 509 x 131071 bf16 forward
 // 32 us (65%), with 20 alternatives 36 us (58%: selecting takes each block about 3 us
 // at its end, when its neighbours do the same), gradient 43 us (96%); 300 x 131071
 // fp32 forward 29 us (84%).

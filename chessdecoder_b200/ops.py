@@ -12,7 +12,8 @@ around nothing: every op has a fake impl) see ordinary operators.
 * ``cdk::token_logprobs(logits, target, k) -> (lp, entropy, lse, top_ids,
   top_lp)`` -- log-probabilities of given tokens with the entropy and the k best
   alternatives (rl/log_probs.py:58-101 is the first of them); lp and entropy are
-  differentiable.
+  differentiable.  It is ``cdk::token_logprobs_forward`` without the second part
+  of lse that the gradient takes.
 * ``cdk::backbone_fwd(...) -> (h, handle)`` and ``cdk::backbone_bwd_(handle,
   dh, grad)`` -- embedding + Fourier injection, every layer and the final
   norm (model.py:143-187).  The forward keeps its activations on the device

@@ -469,8 +469,8 @@ int cdk_paged_gather(const CdkPagedCache* cache, int64_t B, const int32_t* lens,
  * h / (H / kv_heads) (H a multiple of kv_heads, at most 16 query heads each).
  * q, out bf16 [B, H * 64] with pitches ldq, ldo (multiples of 8, 16-byte aligned
  * bases).  lens[b] == 0 gives zeros.  e4m3 pages: scores (in base 2) below 2^24
- * in magnitude, or a weight may overflow; values below 448 * 2^-88 lose bits to
- * the weights' range.  B <= 16384.  workspace:
+ * in magnitude, or a weight may overflow; values below 448 * 2^-88 or above 2^120
+ * lose bits to the weights' range.  B <= 16384.  workspace:
  * cdk_paged_attn_workspace bytes for tables that hold max_keys = width * page_size
  * keys (0 bytes where short tables need none), 16-byte aligned, not shared by
  * calls that can overlap; nothing in it needs clearing or is kept between calls. */
