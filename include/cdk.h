@@ -445,7 +445,8 @@ typedef struct CdkPagedCache {
 /* cdk_paged_append: rows t = b * S_new + s of qkv (fp32 or bf16; q | k | v with
  * H, kv_heads and kv_heads heads of 64, pitch ldq elements, 16-byte aligned
  * rows).  With rope ([rope_len][32][2] = (cos, sin)), q and k are rotated at
- * positions pos[t].  q goes to q_out (bf16, pitch ldo; NULL: not wanted), k and
+ * positions pos[t]; one outside [0, rope_len) sets the index error bit and its
+ * token is skipped, q_out and cache alike.  q goes to q_out (bf16, pitch ldo; NULL: not wanted), k and
  * v to row start[b] + s of sequence b, as bf16 or quantised: with a = max|x| of
  * the 64 values, e = the least integer >= -126 with a <= 448 * 2^e, code =
  * e4m3(x * 2^-e) (round to nearest even), scale byte e + 127.  Scaling by a
